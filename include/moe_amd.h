@@ -395,6 +395,45 @@ int moe_amd_gather_backward_add(const void* d_xs, const int32_t* slot, const int
                                 const void* addend, int64_t T, int K, int E, int H, int dtype,
                                 void* d_x, void* stream);
 
+/* --------------------------------------------- the layer for a few tokens */
+
+/* The expert layer for up to MOE_FEW_MAX_TOKENS tokens, forward only: the
+ * decode step of a served model, bound by reading each routed expert's weights
+ * once.  Two entry points: the experts with the routing given (the arguments
+ * of transformers/integrations/moe.py:377-382; topk_weights [T,K] fp32 or
+ * bf16), and the whole layer with its router
+ * (src/models/modeling_qwen3_moe.py:266-289, src/models/router.py:103-152).
+ * dtype BF16 or F32 is that of hidden_states [T,H], router_weight [E,H],
+ * gate_up_proj, down_proj and out [T,H]; sums are fp32, act = silu(gate) * up
+ * is rounded to dtype, each output once; the routing weights stay fp32.  Ids
+ * outside [0,E) contribute nothing; an expert may be listed twice.  Results
+ * do not depend on timing.
+ *
+ * The router: MOE_ROUTER_SOFTMAX as moe_amd_router_softmax_topk on logits of
+ * dtype (offset_or_bias: the logit offset [E] or NULL), MOE_ROUTER_SIGMOID as
+ * moe_amd_router_sigmoid_topk on fp32 logits (offset_or_bias: the expert bias
+ * or NULL).  topk_weights [T,K] fp32 and topk_index [T,K] (either may be NULL)
+ * receive the routing.
+ *
+ * T <= 64, K <= 16, E <= 4096, H and I multiples of 64 up to 65536 (else
+ * MOE_ERR_UNSUPPORTED, MOE_ERR_ARG).  The workspace
+ * (moe_amd_few_workspace_size bytes, 0 for a refused shape) needs no
+ * preparation and keeps nothing between calls; calls that may overlap need one
+ * each. */
+enum { MOE_FEW_MAX_TOKENS = 64, MOE_FEW_MAX_TOP_K = 16 };
+enum { MOE_ROUTER_SOFTMAX = 0, MOE_ROUTER_SIGMOID = 1 };
+size_t moe_amd_few_workspace_size(int64_t T, int E, int K, int H, int I, int dtype);
+int moe_amd_experts_few(const void* hidden_states, const int64_t* topk_index,
+                        const void* topk_weights, int weights_dtype, const void* gate_up_proj,
+                        const void* down_proj, int64_t T, int K, int E, int H, int I, int dtype,
+                        void* workspace, size_t workspace_bytes, void* out, void* stream);
+int moe_amd_moe_layer_few(const void* hidden_states, const void* router_weight,
+                          const void* gate_up_proj, const void* down_proj, int64_t T, int K, int E,
+                          int H, int I, int dtype, int router, const float* offset_or_bias,
+                          int renormalize, float scaling_factor, int num_groups, int group_topk,
+                          void* workspace, size_t workspace_bytes, float* topk_weights,
+                          int64_t* topk_index, void* out, void* stream);
+
 /* ---------------------------------------------------- routing consumers */
 
 /* One pass over a layer's router probabilities probs [T,E] (fp32 or bf16):

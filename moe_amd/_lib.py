@@ -83,6 +83,12 @@ SIGNATURES: dict[str, tuple] = {
     "moe_amd_weight_grad_reduce": (_i, [_p, _i, _p, _p, _i64, _i, _i, _p, _i, _p]),
     "moe_amd_gather_backward": (_i, [_p, _p, _p, _i64, _i, _i, _i, _i, _p, _p]),
     "moe_amd_gather_backward_add": (_i, [_p, _p, _p, _p, _i64, _i, _i, _i, _i, _p, _p]),
+    "moe_amd_few_workspace_size": (_sz, [_i64, _i, _i, _i, _i, _i]),
+    "moe_amd_experts_few": (
+        _i, [_p, _p, _p, _i, _p, _p, _i64, _i, _i, _i, _i, _i, _p, _sz, _p, _p]),
+    "moe_amd_moe_layer_few": (
+        _i, [_p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _i, _f, _i, _i, _p, _sz, _p, _p,
+             _p, _p]),
     "moe_amd_topk_stats_workspace_size": (_sz, [_i64, _i]),
     "moe_amd_topk_stats": (_i, [_p, _i, _p, _i64, _i, _i, _p, _sz, _p, _p, _p, _p]),
     "moe_amd_seq_stats_workspace_size": (_sz, [_i64, _i, _i]),

@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from . import library  # noqa: F401  (registers the moe_amd:: ops)
+from . import few, library  # noqa: F401  (library registers the moe_amd:: ops)
 
 
 def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
@@ -66,7 +66,13 @@ def _check_module(self) -> None:
 def mi355x_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                            top_k_weights: torch.Tensor) -> torch.Tensor:
     """ExpertsInterface entry ("mi355x"), drop-in for grouped_mm_experts_forward
-    (transformers/integrations/moe.py:377-478)."""
+    (transformers/integrations/moe.py:377-478).  A bank with a ``few_tokens``
+    attribute runs the few-token experts up to that many tokens where no
+    gradient is wanted (``hf.install(model, few_tokens=...)`` sets it)."""
     _check_module(self)
+    if few.wanted(getattr(self, "few_tokens", 0), hidden_states, top_k_weights,
+                  self.gate_up_proj, self.down_proj):
+        return few.experts_forward_few(hidden_states, top_k_index, top_k_weights,
+                                       self.gate_up_proj, self.down_proj)
     return experts_forward(hidden_states, top_k_index, top_k_weights, self.gate_up_proj,
                            self.down_proj)

@@ -45,10 +45,24 @@ def swap_routers(model: nn.Module) -> int:
     return n
 
 
-def install(model: nn.Module, routers: bool = True, experts: bool = True) -> nn.Module:
+def expert_banks(model: nn.Module) -> list[nn.Module]:
+    """The modules that hold an expert bank (gate_up_proj and down_proj)."""
+    return [m for m in model.modules()
+            if hasattr(m, "gate_up_proj") and hasattr(m, "down_proj")
+            and getattr(m.gate_up_proj, "ndim", 0) == 3]
+
+
+def install(model: nn.Module, routers: bool = True, experts: bool = True,
+            few_tokens: int = 0) -> nn.Module:
+    """Swaps the routers and selects the "mi355x" experts.  ``few_tokens``
+    (with ``experts``): calls of at most that many tokens (up to
+    ``moe_amd.few.MAX_TOKENS``) that want no gradient run the few-token
+    experts."""
     register()
     if routers:
         swap_routers(model)
     if experts:
         model.set_experts_implementation(EXPERTS_KEY)
+        for bank in expert_banks(model):
+            bank.few_tokens = int(few_tokens)
     return model

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import library  # registers the moe_amd:: ops
+from . import few, library  # library registers the moe_amd:: ops
 from .experts import experts_forward
 from .router import gating_linear, linear_sigmoid_topk, sigmoid_topk, softmax_topk
 
@@ -89,7 +89,13 @@ class _Bank(nn.Module):
 
 class SparseMoeBlock(nn.Module):
     """Stand-alone MoE block: [B,S,H] (or [T,H]) -> same shape.  The last
-    router outputs are kept in ``router_logits`` / ``topk_index``."""
+    router outputs are kept in ``router_logits`` / ``topk_index``.
+
+    Up to ``few_tokens`` tokens without a gradient run the few-token layer
+    (``moe_amd.few``; 0, the default: never), which computes no router_logits:
+    they are None then."""
+
+    few_tokens = 0
 
     def __init__(self, hidden_size: int, num_experts: int, top_k: int, intermediate_size: int,
                  router: str = "softmax", norm_topk_prob: bool = True):
@@ -107,6 +113,15 @@ class SparseMoeBlock(nn.Module):
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         shape = hidden_states.shape
         flat = hidden_states.reshape(-1, shape[-1])
+        if few.wanted(self.few_tokens, flat, *self.parameters()):
+            sig = self.router == "sigmoid"
+            out, _, self.topk_index = few.moe_layer_few(
+                flat, self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj,
+                self.top_k, router=self.router, renormalize=self.norm_topk_prob,
+                logit_offset=None if sig else self.logit_offset,
+                expert_bias=self.expert_bias if sig else None, return_routing=True)
+            self.router_logits = None
+            return out.reshape(shape)
         out, probs, _, idx = moe_layer(
             flat, self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj, self.top_k,
             router=self.router, renormalize=self.norm_topk_prob, logit_offset=self.logit_offset,

@@ -18,6 +18,8 @@ differentiable piece of the MI355X path, each a functional op in namespace
   linear_sigmoid_topk            its fp32 gating linear and the router in one
                                  kernel (backward: sigmoid_topk_backward, then
                                  router_linear_backward)
+  experts_few / moe_layer_few    the experts, and the layer, for a few tokens
+                                 (forward only)
 
 A forward op returns, besides its results, the tensors its backward needs
 (the routing plan, gate_up), so that setup_context saves only op outputs; the
@@ -698,3 +700,36 @@ def _layer_backward(ctx, d_out, d_probs, d_w, *unused):
 
 torch.library.register_autograd(f"{_LIB}::moe_layer_fwd", _layer_backward,
                                 setup_context=_layer_setup)
+
+
+# ------------------------------------------------------- few tokens (forward)
+
+@torch.library.custom_op(f"{_LIB}::experts_few", mutates_args=())
+def experts_few(x: Tensor, topk_index: Tensor, topk_weights: Tensor, gate_up_proj: Tensor,
+                down_proj: Tensor) -> Tensor:
+    """The experts for a few tokens, routing given; no autograd formula."""
+    return ops.experts_few(x, topk_index, topk_weights, gate_up_proj, down_proj)
+
+
+@experts_few.register_fake
+def _(x, topk_index, topk_weights, gate_up_proj, down_proj):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{_LIB}::moe_layer_few", mutates_args=())
+def moe_layer_few(x: Tensor, w_router: Tensor, gate_up_proj: Tensor, down_proj: Tensor,
+                  top_k: int, router: str, renormalize: bool, logit_offset: Optional[Tensor],
+                  expert_bias: Optional[Tensor], scaling_factor: Optional[float],
+                  num_groups: Optional[int], group_topk: Optional[int]
+                  ) -> tuple[Tensor, Tensor, Tensor]:
+    """(out, weights fp32, index) of the layer for a few tokens; no autograd formula."""
+    return ops.moe_layer_few(x, w_router, gate_up_proj, down_proj, top_k, router, renormalize,
+                             logit_offset, expert_bias, scaling_factor, num_groups, group_topk)
+
+
+@moe_layer_few.register_fake
+def _(x, w_router, gate_up_proj, down_proj, top_k, router, renormalize, logit_offset, expert_bias,
+      scaling_factor, num_groups, group_topk):
+    T = x.shape[0]
+    return (x.new_empty(x.shape), x.new_empty(T, top_k, dtype=torch.float32),
+            x.new_empty(T, top_k, dtype=torch.int64))

@@ -71,8 +71,8 @@ def on_tensor_device(fn):
     return run
 
 
-def _call(name: str, *args) -> None:
-    if torch.cuda.is_current_stream_capturing():
+def _call(name: str, *args, capturable: bool = False) -> None:
+    if not capturable and torch.cuda.is_current_stream_capturing():
         # A test that captured the layer's fwd+bwd with torch.cuda.graph
         # ended the process with a segmentation fault inside the end of the
         # capture (no GPU fault); until that is understood, refuse capture.
@@ -753,3 +753,103 @@ def gather_backward(dxs, plan: RoutingPlan, addend: torch.Tensor | None = None) 
               plan.offsets.data_ptr(), addend.data_ptr(), T, K, E, H, _dtype_code(dxs.dtype),
               dx.data_ptr(), _stream(dxs))
     return dx
+
+
+# -------------------------------------------------- the layer for few tokens
+
+FEW_MAX_TOKENS = 64
+FEW_MAX_TOP_K = 16
+_ROUTERS = {"softmax": 0, "sigmoid": 1}
+
+
+def _few_inputs(name: str, x, gate_up_proj, down_proj, K: int):
+    """(E, H, I) of a few-token call after checking its shapes and types."""
+    if x.dim() != 2 or gate_up_proj.dim() != 3 or down_proj.dim() != 3:
+        raise ValueError(f"{name}: hidden_states must be [T, H], gate_up_proj [E, 2I, H] and "
+                         "down_proj [E, H, I]")
+    E, I2, H = gate_up_proj.shape
+    if tuple(down_proj.shape) != (E, H, I2 // 2) or I2 % 2 or x.shape[1] != H:
+        raise ValueError(f"{name}: shape mismatch: hidden {tuple(x.shape)}, gate_up_proj "
+                         f"{tuple(gate_up_proj.shape)}, down_proj {tuple(down_proj.shape)}")
+    if not (x.dtype == gate_up_proj.dtype == down_proj.dtype):
+        raise TypeError(f"{name}: hidden states and weights of dtypes {x.dtype}, "
+                        f"{gate_up_proj.dtype}, {down_proj.dtype}")
+    if x.shape[0] > FEW_MAX_TOKENS or K > FEW_MAX_TOP_K:
+        raise RuntimeError(f"{name}: {x.shape[0]} tokens with top-{K}; it takes at most "
+                           f"{FEW_MAX_TOKENS} and {FEW_MAX_TOP_K}")
+    return E, H, I2 // 2
+
+
+def _few_workspace(x, E, K, H, I) -> torch.Tensor:
+    n = _lib.load().moe_amd_few_workspace_size(x.shape[0], E, K, H, I, _dtype_code(x.dtype))
+    return torch.empty(max(int(n), 16), device=x.device, dtype=torch.uint8)
+
+
+@on_tensor_device
+def experts_few(x: torch.Tensor, topk_index: torch.Tensor, topk_weights: torch.Tensor,
+                gate_up_proj: torch.Tensor, down_proj: torch.Tensor) -> torch.Tensor:
+    """out [T,H] of the experts for at most FEW_MAX_TOKENS tokens with the
+    routing given (weights fp32 or bf16); forward only.  May be captured in a
+    HIP graph."""
+    _need_cuda(x, topk_index, topk_weights, gate_up_proj, down_proj)
+    if topk_index.dim() != 2 or topk_index.shape != topk_weights.shape \
+            or topk_index.shape[0] != x.shape[0]:
+        raise ValueError("experts_few: topk_index / topk_weights must both be [T, K]")
+    T, K = topk_index.shape
+    E, H, I = _few_inputs("experts_few", x, gate_up_proj, down_proj, K)
+    x, gate_up_proj, down_proj = _contig(x), _contig(gate_up_proj), _contig(down_proj)
+    topk_index = _contig(topk_index.to(torch.int64))
+    topk_weights = _contig(topk_weights)
+    ws = _few_workspace(x, E, K, H, I)
+    out = torch.empty(T, H, device=x.device, dtype=x.dtype)
+    _call("moe_amd_experts_few", x.data_ptr(), topk_index.data_ptr(), topk_weights.data_ptr(),
+          _dtype_code(topk_weights.dtype), gate_up_proj.data_ptr(), down_proj.data_ptr(), T, K, E,
+          H, I, _dtype_code(x.dtype), ws.data_ptr(), ws.numel(), out.data_ptr(), _stream(x),
+          capturable=True)
+    return out
+
+
+@on_tensor_device
+def moe_layer_few(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tensor,
+                  down_proj: torch.Tensor, top_k: int, router: str = "softmax",
+                  renormalize: bool = True, logit_offset: torch.Tensor | None = None,
+                  expert_bias: torch.Tensor | None = None, scaling_factor: float | None = None,
+                  num_groups: int | None = None, group_topk: int | None = None,
+                  return_routing: bool = True):
+    """Router and experts for at most FEW_MAX_TOKENS tokens; forward only.
+    (out [T,H], weights fp32 [T,K], index int64 [T,K]), or out alone without
+    return_routing.  May be captured in a HIP graph."""
+    name = "moe_layer_few"
+    if router not in _ROUTERS:
+        raise ValueError(f"unknown router {router!r}")
+    if (logit_offset is not None and router != "softmax") or \
+            (expert_bias is not None and router != "sigmoid"):
+        raise ValueError(f"{name}: logit_offset is the softmax router's, expert_bias the "
+                         "sigmoid router's")
+    extra = logit_offset if router == "softmax" else expert_bias
+    _need_cuda(x, w_router, gate_up_proj, down_proj, extra)
+    K = int(top_k)
+    E, H, I = _few_inputs(name, x, gate_up_proj, down_proj, K)
+    if tuple(w_router.shape) != (E, H) or w_router.dtype != x.dtype:
+        raise ValueError(f"{name}: router weight {tuple(w_router.shape)} {w_router.dtype}, "
+                         f"expected {(E, H)} {x.dtype}")
+    if extra is not None:
+        if tuple(extra.shape) != (E,):
+            raise ValueError(f"{name}: offset or bias {tuple(extra.shape)}, expected {(E,)}")
+        extra = _contig(extra.to(torch.float32))
+    x, w_router = _contig(x), _contig(w_router)
+    gate_up_proj, down_proj = _contig(gate_up_proj), _contig(down_proj)
+    T = x.shape[0]
+    grouped = num_groups is not None and group_topk is not None
+    ws = _few_workspace(x, E, K, H, I)
+    out = torch.empty(T, H, device=x.device, dtype=x.dtype)
+    w = idx = None
+    if return_routing:
+        w = torch.empty(T, K, device=x.device, dtype=torch.float32)
+        idx = torch.empty(T, K, device=x.device, dtype=torch.int64)
+    _call("moe_amd_moe_layer_few", x.data_ptr(), w_router.data_ptr(), gate_up_proj.data_ptr(),
+          down_proj.data_ptr(), T, K, E, H, I, _dtype_code(x.dtype), _ROUTERS[router],
+          _ptr(extra), int(renormalize), float(scaling_factor or 0.0),
+          int(num_groups) if grouped else 0, int(group_topk) if grouped else 0, ws.data_ptr(),
+          ws.numel(), _ptr(w), _ptr(idx), out.data_ptr(), _stream(x), capturable=True)
+    return (out, w, idx) if return_routing else out

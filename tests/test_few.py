@@ -1,0 +1,100 @@
+"""The few-token layer without a GPU: refusals of its C entry points and of
+the Python functions, the workspace size, and the form a block chooses."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from moe_amd import _lib, few, hf, ops
+from moe_amd.layer import SparseMoeBlock
+
+
+def _ws(T=4, E=8, K=2, H=128, I=64, dtype=1):
+    return _lib.load().moe_amd_few_workspace_size(T, E, K, H, I, dtype)
+
+
+def test_workspace_size_and_refused_shapes(built_lib):
+    assert _ws() > 0
+    assert _ws(T=64, K=16) > _ws(T=1, K=16)
+    assert _ws(dtype=0) > _ws(dtype=1)
+    for bad in (dict(T=65), dict(T=-1), dict(K=17), dict(K=0), dict(E=0), dict(E=4097),
+                dict(H=96), dict(I=32), dict(H=0), dict(dtype=2), dict(H=1 << 17)):
+        assert _ws(**bad) == 0, bad
+
+
+@pytest.mark.parametrize("change,status,text", [
+    (dict(T=65), "MOE_ERR_UNSUPPORTED", "64 tokens"),
+    (dict(K=17), "MOE_ERR_UNSUPPORTED", "top-16"),
+    (dict(E=5000), "MOE_ERR_UNSUPPORTED", "4096 experts"),
+    (dict(H=100), "MOE_ERR_ARG", "multiples of 64"),
+    (dict(dtype=3), "MOE_ERR_DTYPE", "neither bf16 nor fp32"),
+    (dict(wdtype=5), "MOE_ERR_DTYPE", "weights dtype"),
+    (dict(x=None), "MOE_ERR_ARG", "null pointer"),
+    (dict(ws_bytes=100), "MOE_ERR_WORKSPACE", "needs"),
+    (dict(x=8), "MOE_ERR_ALIGN", "16-byte aligned"),
+])
+def test_experts_few_refuses(built_lib, change, status, text):
+    a = dict(T=4, E=8, K=2, H=128, I=64, dtype=1, wdtype=0, x=4096, ws_bytes=1 << 30)
+    a.update(change)
+    with pytest.raises(RuntimeError, match=f"{status}.*{text}"):
+        _lib.call("moe_amd_experts_few", a["x"], 4096, 4096, a["wdtype"], 4096, 4096, a["T"],
+                  a["K"], a["E"], a["H"], a["I"], a["dtype"], 4096, a["ws_bytes"], 4096, None)
+
+
+@pytest.mark.parametrize("change,status,text", [
+    (dict(router=2), "MOE_ERR_ARG", "router 2"),
+    (dict(K=9), "MOE_ERR_ARG", "K=9"),
+    (dict(groups=3), "MOE_ERR_ARG", "bad grouping"),
+    (dict(router=0, groups=2), "MOE_ERR_ARG", "bad grouping"),
+    (dict(groups=4, gtopk=1), "MOE_ERR_ARG", "bad grouping"),
+    (dict(ws=None), "MOE_ERR_WORKSPACE", "workspace"),
+])
+def test_moe_layer_few_refuses(built_lib, change, status, text):
+    a = dict(T=4, E=8, K=4, H=128, I=64, router=1, groups=0, gtopk=0, ws=4096)
+    a.update(change)
+    with pytest.raises(RuntimeError, match=f"{status}.*{text}"):
+        _lib.call("moe_amd_moe_layer_few", 4096, 4096, 4096, 4096, a["T"], a["K"], a["E"], a["H"],
+                  a["I"], 1, a["router"], None, 1, 0.0, a["groups"], a["gtopk"], a["ws"], 1 << 30,
+                  None, None, 4096, None)
+
+
+def test_no_tokens_is_no_call(built_lib):
+    # nothing is read or launched: the pointers may be null
+    _lib.call("moe_amd_experts_few", None, None, None, 0, None, None, 0, 2, 8, 128, 64, 1, None, 0,
+              None, None)
+
+
+def _inputs(T=4, E=8, K=2, H=128, I=64):
+    return (torch.zeros(T, H), torch.zeros(T, K, dtype=torch.int64), torch.zeros(T, K),
+            torch.zeros(E, 2 * I, H), torch.zeros(E, H, I))
+
+
+def test_cpu_tensors_and_gradients_are_refused():
+    x, idx, w, w1, w2 = _inputs()
+    with pytest.raises(RuntimeError, match="GPU only"):
+        few.experts_forward_few(x, idx, w, w1, w2)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        few.moe_layer_few(x, torch.zeros(8, 128), w1, w2, 2)
+    w1.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="forward only"):
+        few.experts_forward_few(x, idx, w, w1, w2)
+    with pytest.raises(RuntimeError, match="forward only"):
+        few.moe_layer_few(x, torch.zeros(8, 128), w1, w2, 2)
+
+
+def test_a_block_takes_the_few_token_form_only_without_gradients():
+    x = torch.zeros(4, 8)
+    p = torch.nn.Parameter(torch.zeros(3))
+    with torch.no_grad():
+        assert few.wanted(4, x, p) and few.wanted(1000, x, p)
+        assert not few.wanted(0, x, p) and not few.wanted(3, x, p)
+        assert not few.wanted(64, torch.zeros(0, 8), p)
+        assert not few.wanted(1000, torch.zeros(65, 8), p)
+    assert not few.wanted(4, x, p)
+    assert few.wanted(4, x, p.detach())
+
+
+def test_install_sets_the_banks(monkeypatch):
+    block = SparseMoeBlock(64, 4, 2, 64)
+    assert hf.expert_banks(block) == [block.experts]
+    assert few.MAX_TOKENS == ops.FEW_MAX_TOKENS == 64
