@@ -32,6 +32,7 @@ constexpr int kFewExperts = 4096;
 constexpr int kFewRows = kFewTokens * kFewTopK;
 constexpr int kWaves = 8;        // waves per workgroup of the GEMV kernels
 constexpr int kPlanWaves = 16;
+constexpr int kRouteWaves = 4;   // tokens per workgroup of the routing
 constexpr int kGroup = 4;        // experts per workgroup of the down kernel
 constexpr int kParts = kWaves / kGroup;  // waves that split one expert's contraction there
 
@@ -48,13 +49,13 @@ struct FewArgs {
   int T, E, K, H, I;
   float* logits;           // workspace from here on
   float* w;                // [S]
-  int* hdr;                // [0] active experts
+  int* hdr;                // [0] active experts, [1] finished routing workgroups
   int* arrived;            // [H/16] finished groups of the down kernel's column slices
   int4* list;              // {expert, first row, rows, 0} of the active experts
   int* rows;               // flat entries s = t*K + k by active expert, ascending
   void* act;               // [S,I] by flat entry
   float* y;                // [S,H]
-  int* real;               // [S] whether the entry names an expert
+  int* real;               // [S] the entry's expert, negative for padding
   float* out_w;            // routing out (may be null)
   int64_t* out_idx;
   void* out;
@@ -83,9 +84,15 @@ template <> struct Mma<float> {
 };
 
 __device__ __forceinline__ u32x4 ld16(const char* p) { return *(const u32x4*)p; }
-// Weights are read once: no other workgroup finds them in a cache.
-__device__ __forceinline__ u32x4 ld16_nt(const char* p) {
+#ifndef FEW_NT
+#define FEW_NT 0
+#endif
+__device__ __forceinline__ u32x4 ld16_w(const char* p) {
+#if FEW_NT
   return __builtin_nontemporal_load((const u32x4*)p);
+#else
+  return *(const u32x4*)p;
+#endif
 }
 
 template <typename T> __device__ __forceinline__ float few_round(float v) {
@@ -93,8 +100,40 @@ template <typename T> __device__ __forceinline__ float few_round(float v) {
   return v;
 }
 
+// The counters that workgroups of later launches finish by.
+__device__ __forceinline__ void clear_counters(const FewArgs& p) {
+  if (threadIdx.x == 0) p.hdr[1] = 0;
+  for (int i = threadIdx.x; i < p.H / 16; i += blockDim.x) p.arrived[i] = 0;
+}
+
+// What one workgroup leaves for another of the same launch: written through to
+// and read from the memory that all XCDs share, so that no cache has to be
+// written back or invalidated.  A workgroup counts itself as arrived once its
+// writes are there; the last one to arrive reads everybody's.
+__device__ __forceinline__ void put_shared(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get_shared(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put_shared(int* p, int v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ int get_shared(const int* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool last_to_arrive(int* counter, int of, int* box) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's writes are there
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *box = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1;
+  __syncthreads();
+  return *box;
+}
+
 // ---------------------------------------------------------------- logits
-// Workgroup: 16 experts, all tokens; the eight waves split H.
+// Workgroup: 16 experts and 16 tokens; the eight waves split H.  The first one
+// clears the counters of the launches behind it.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
   __shared__ f32x4 red[kWaves][64];
@@ -105,24 +144,23 @@ __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
   const int s0 = wid * ns / kWaves, s1 = (wid + 1) * ns / kWaves;
   const int64_t ld = (int64_t)p.H * sizeof(T);
   const char* a = (const char*)p.wr + (int64_t)min(e0 + n, p.E - 1) * ld + g * 16;
-  for (int t0 = 0; t0 < p.T; t0 += 16) {
-    const char* b = (const char*)p.x + (int64_t)min(t0 + n, p.T - 1) * ld + g * 16;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int t0 = blockIdx.y * 16;
+  const char* b = (const char*)p.x + (int64_t)min(t0 + n, p.T - 1) * ld + g * 16;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-    for (int s = s0; s < s1; ++s) acc = Mma<T>::step(ld16(a + s * 64), ld16(b + s * 64), acc);
-    __syncthreads();
-    red[wid][lane] = acc;
-    __syncthreads();
-    if (threadIdx.x < 256) {
-      const int e = threadIdx.x & 15, t = threadIdx.x >> 4;
-      double v = 0;
+  for (int s = s0; s < s1; ++s) acc = Mma<T>::step(ld16(a + s * 64), ld16(b + s * 64), acc);
+  red[wid][lane] = acc;
+  if (blockIdx.x == 0 && blockIdx.y == 0) clear_counters(p);
+  __syncthreads();
+  if (threadIdx.x < 256) {
+    const int e = threadIdx.x & 15, t = threadIdx.x >> 4;
+    double v = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) v += (double)red[w][(e >> 2) * 16 + t][e & 3];
-      if (t0 + t < p.T && e0 + e < p.E) {
-        const float f = (float)v;
-        // the softmax router's logits have x's type, as the model's linear returns them
-        p.logits[(int64_t)(t0 + t) * p.E + e0 + e] = p.sigmoid ? f : few_round<T>(f);
-      }
+    for (int w = 0; w < kWaves; ++w) v += (double)red[w][(e >> 2) * 16 + t][e & 3];
+    if (t0 + t < p.T && e0 + e < p.E) {
+      const float f = (float)v;
+      // the softmax router's logits have x's type, as the model's linear returns them
+      p.logits[(int64_t)(t0 + t) * p.E + e0 + e] = p.sigmoid ? f : few_round<T>(f);
     }
   }
 }
@@ -219,42 +257,55 @@ __device__ void route_token(const FewArgs& p, const float* logits, int lane, flo
   wk = dsk_weight(wk, ssum, p.renorm, p.scaling, 0);
 }
 
-// One workgroup: the tokens' top-K (from the logits, or as given), then the
-// active experts and their rows.  Every entry counts the entries of its expert
+// The tokens' top-K, one token a wave, four a workgroup; the last workgroup to
+// finish lists the active experts and their rows.  With the routing given there
+// is one workgroup, which lists.  Every entry counts the entries of its expert
 // and those before it by reading all ids from LDS (S <= 1024).
 template <int NV>
 __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
   __shared__ __attribute__((aligned(16))) int ids[kFewRows];
   __shared__ int row0_of[kFewRows];
   __shared__ int2 wsum[kPlanWaves];
+  __shared__ int box;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S = p.T * p.K;
   if (p.wr) {
-    for (int t = wid; t < p.T; t += kPlanWaves) {
+    const int t = blockIdx.x * kRouteWaves + wid;
+    if (wid < kRouteWaves && t < p.T) {
       float wk;
       int ek;
       route_token<NV>(p, p.logits + (int64_t)t * p.E, lane, wk, ek);
       if (lane < p.K) {
         const int s = t * p.K + lane;
-        ids[s] = ek;
+        put_shared(&p.real[s], ek);
         p.w[s] = wk;
         if (p.out_w) p.out_w[s] = wk;
         if (p.out_idx) p.out_idx[s] = ek;
       }
     }
-  } else if (tid < S) {
-    const int64_t e = p.ids[tid];
-    ids[tid] = e >= 0 && e < p.E ? (int)e : -1;
-    p.w[tid] = p.weights_bf16 ? bf2f(((const bf16*)p.weights)[tid])
-                              : ((const float*)p.weights)[tid];
+    if (gridDim.x > 1) {
+      if (!last_to_arrive(&p.hdr[1], gridDim.x, &box)) return;
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
+    if (tid < S) ids[tid] = get_shared(&p.real[tid]);
+  } else {
+    if (tid < S) {
+      const int64_t e = p.ids[tid];
+      ids[tid] = e >= 0 && e < p.E ? (int)e : -1;
+      p.real[tid] = ids[tid];
+      p.w[tid] = p.weights_bf16 ? bf2f(((const bf16*)p.weights)[tid])
+                                : ((const float*)p.weights)[tid];
+    }
+    clear_counters(p);
   }
   for (int i = S + tid; i < kFewRows; i += 64 * kPlanWaves) ids[i] = -1;
-  for (int i = tid; i < p.H / 16; i += 64 * kPlanWaves) p.arrived[i] = 0;
   __syncthreads();
   const int e = ids[tid];
   int rank = 0, cnt = 0, first = S;
-  for (int i = 0; i < S; i += 4) {
+  for (int i = 0; i < S && wid * 64 < S; i += 4) {
     const int4 q = *(const int4*)&ids[i];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -293,15 +344,15 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
   }
   __syncthreads();
   if (e >= 0) p.rows[row0_of[first] + rank] = tid;
-  if (tid < S) p.real[tid] = e >= 0;
   if (tid == 0) p.hdr[0] = all.x;
 }
 
 // ------------------------------------------------------- gate/up + SwiGLU
 // Workgroup: 16 features of one active expert; the waves split H, CH steps of
-// gate and up rows in flight each.
+// gate and up rows in flight each.  An expert with more than 16 rows reads its
+// weights again for the next 16, from L2.
 template <typename T, int CH>
-__global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
+__global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) {
   __shared__ f32x4 red[kWaves][2][64];
   const int nsl = p.I / 16;
   const int slot = blockIdx.x / nsl, f0 = (blockIdx.x % nsl) * 16;
@@ -314,59 +365,44 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   const int64_t ld = (int64_t)p.H * sizeof(T);
   const char* wg = (const char*)p.w1 + ((int64_t)info.x * 2 * p.I + f0 + n) * ld + g * 16;
   const char* wu = wg + (int64_t)p.I * ld;
-  for (int rg = 0; rg < info.z; rg += 64) {
+  for (int rg = 0; rg < info.z; rg += 16) {
     const int left = info.z - rg;
-    const char* xr[4];
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int r = min(m * 16 + n, left - 1);
-      xr[m] = (const char*)p.x + (int64_t)(p.rows[info.y + rg + r] / p.K) * ld + g * 16;
-    }
-    f32x4 ag[4], au[4];
-#pragma unroll
-    for (int m = 0; m < 4; ++m) ag[m] = au[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const char* xr = (const char*)p.x +
+                     (int64_t)(p.rows[info.y + rg + min(n, left - 1)] / p.K) * ld + g * 16;
+    f32x4 ag = {0.f, 0.f, 0.f, 0.f}, au = ag;
     for (int sb = s0; sb < s1; sb += CH) {
-      u32x4 a[CH], b[CH];
+      u32x4 a[CH], b[CH], c[CH];
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int s = min(sb + i, s1 - 1);
-        a[i] = ld16_nt(wg + s * 64);
-        b[i] = ld16_nt(wu + s * 64);
+        a[i] = ld16_w(wg + s * 64);
+        b[i] = ld16_w(wu + s * 64);
       }
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        if (m * 16 >= left) break;
-        u32x4 c[CH];
+      for (int i = 0; i < CH; ++i) c[i] = ld16(xr + min(sb + i, s1 - 1) * 64);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) c[i] = ld16(xr[m] + min(sb + i, s1 - 1) * 64);
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-          if (sb + i < s1) {
-            ag[m] = Mma<T>::step(a[i], c[i], ag[m]);
-            au[m] = Mma<T>::step(b[i], c[i], au[m]);
-          }
+      for (int i = 0; i < CH; ++i) {
+        if (sb + i < s1) {
+          ag = Mma<T>::step(a[i], c[i], ag);
+          au = Mma<T>::step(b[i], c[i], au);
         }
       }
     }
+    if (rg) __syncthreads();
+    red[wid][0][lane] = ag;
+    red[wid][1][lane] = au;
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      const int f = threadIdx.x & 15, r = threadIdx.x >> 4, l = (f >> 2) * 16 + r;
+      if (r < left) {
+        float gs = 0.f, us = 0.f;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      if (m * 16 >= left) break;
-      __syncthreads();
-      red[wid][0][lane] = ag[m];
-      red[wid][1][lane] = au[m];
-      __syncthreads();
-      if (threadIdx.x < 256) {
-        const int f = threadIdx.x & 15, r = threadIdx.x >> 4, l = (f >> 2) * 16 + r;
-        if (m * 16 + r < left) {
-          float gs = 0.f, us = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWaves; ++w) {
-            gs += red[w][0][l][f & 3];
-            us += red[w][1][l][f & 3];
-          }
-          const int s = p.rows[info.y + rg + m * 16 + r];
-          ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
+        for (int w = 0; w < kWaves; ++w) {
+          gs += red[w][0][l][f & 3];
+          us += red[w][1][l][f & 3];
         }
+        const int s = p.rows[info.y + rg + r];
+        ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
       }
     }
   }
@@ -377,9 +413,9 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
 // an expert.  y rows go to the workspace; the workgroup that finishes a column
 // slice's last group sums them with the routing weights, in k order.
 template <typename T, int CH>
-__global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
+__global__ __launch_bounds__(64 * kWaves, 4) void few_down_kernel(FewArgs p) {
   __shared__ f32x4 red[kWaves][64];
-  __shared__ int s_last;
+  __shared__ int box;
   const int nh = p.H / 16;
   const int hs = blockIdx.x % nh, grp = blockIdx.x / nh, h0 = hs * 16;
   const int nact = p.hdr[0];
@@ -398,72 +434,45 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
   const int s0 = part * ns / kParts, s1 = (part + 1) * ns / kParts;
   const int64_t ld = (int64_t)p.I * sizeof(T);
   const char* wd = (const char*)p.w2 + ((int64_t)info.x * p.H + h0 + n) * ld + g * 16;
-  for (int rg = 0; rg < most; rg += 64) {
+  for (int rg = 0; rg < most; rg += 16) {
     const int left = info.z - rg;
-    f32x4 acc[4];
-#pragma unroll
-    for (int m = 0; m < 4; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (left > 0) {
-      const char* ar[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int r = min(m * 16 + n, left - 1);
-        ar[m] = (const char*)p.act + (int64_t)p.rows[info.y + rg + r] * ld + g * 16;
-      }
+      const char* ar =
+          (const char*)p.act + (int64_t)p.rows[info.y + rg + min(n, left - 1)] * ld + g * 16;
       for (int sb = s0; sb < s1; sb += CH) {
-        u32x4 a[CH];
+        u32x4 a[CH], c[CH];
 #pragma unroll
-        for (int i = 0; i < CH; ++i) a[i] = ld16_nt(wd + min(sb + i, s1 - 1) * 64);
+        for (int i = 0; i < CH; ++i) a[i] = ld16_w(wd + min(sb + i, s1 - 1) * 64);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          if (m * 16 >= left) break;
-          u32x4 c[CH];
+        for (int i = 0; i < CH; ++i) c[i] = ld16(ar + min(sb + i, s1 - 1) * 64);
 #pragma unroll
-          for (int i = 0; i < CH; ++i) c[i] = ld16(ar[m] + min(sb + i, s1 - 1) * 64);
-#pragma unroll
-          for (int i = 0; i < CH; ++i)
-            if (sb + i < s1) acc[m] = Mma<T>::step(a[i], c[i], acc[m]);
-        }
+        for (int i = 0; i < CH; ++i)
+          if (sb + i < s1) acc = Mma<T>::step(a[i], c[i], acc);
       }
     }
+    if (rg) __syncthreads();
+    red[wid][lane] = acc;
+    __syncthreads();
+    for (int v = tid; v < kGroup * 256; v += 64 * kWaves) {
+      const int q = v >> 8, h = v & 15, r = (v >> 4) & 15, l = (h >> 2) * 16 + r;
+      if (grp * kGroup + q >= nact) continue;
+      const int4 iq = p.list[grp * kGroup + q];
+      if (rg + r >= iq.z) continue;
+      float sum = 0.f;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      if (rg + m * 16 >= most) break;
-      __syncthreads();
-      red[wid][lane] = acc[m];
-      __syncthreads();
-      for (int v = tid; v < kGroup * 256; v += 64 * kWaves) {
-        const int q = v >> 8, h = v & 15, r = (v >> 4) & 15, l = (h >> 2) * 16 + r;
-        if (grp * kGroup + q >= nact) continue;
-        const int4 iq = p.list[grp * kGroup + q];
-        const int row = rg + m * 16 + r;
-        if (row >= iq.z) continue;
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < kParts; ++w) sum += red[q * kParts + w][l][h & 3];
-        p.y[(int64_t)p.rows[iq.y + row] * p.H + h0 + h] = sum;
-      }
+      for (int w = 0; w < kParts; ++w) sum += red[q * kParts + w][l][h & 3];
+      put_shared(&p.y[(int64_t)p.rows[iq.y + rg + r] * p.H + h0 + h], sum);
     }
   }
   // the slice's last group combines
-  if (ngrp > 1) {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
-    __syncthreads();
-    if (tid == 0)
-      s_last = __hip_atomic_fetch_add(&p.arrived[hs], 1, __ATOMIC_RELAXED,
-                                      __HIP_MEMORY_SCOPE_AGENT) == ngrp - 1;
-    __syncthreads();
-    if (!s_last) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  } else {
-    __syncthreads();
-  }
+  if (!last_to_arrive(&p.arrived[hs], ngrp, &box)) return;
   const int h = h0 + (tid & 15);
   for (int t = tid >> 4; t < p.T; t += 4 * kWaves) {
     float o = 0.f;
     for (int k = 0; k < p.K; ++k) {
       const int s = t * p.K + k;
-      if (p.real[s]) o = fmaf(p.w[s], p.y[(int64_t)s * p.H + h], o);
+      if (p.real[s] >= 0) o = fmaf(p.w[s], get_shared(&p.y[(int64_t)s * p.H + h]), o);
     }
     ((T*)p.out)[(int64_t)t * p.H + h] = (T)o;
   }
@@ -514,15 +523,16 @@ int few_check(int64_t T, int K, int E, int H, int I, int dtype, const char* who)
 template <typename T>
 void few_launch(FewArgs& p, hipStream_t st) {
   const int S = p.T * p.K, slots = S < p.E ? S : p.E;
-  if (p.wr) few_logits_kernel<T><<<(p.E + 15) / 16, 64 * kWaves, 0, st>>>(p);
+  if (p.wr) few_logits_kernel<T><<<dim3((p.E + 15) / 16, (p.T + 15) / 16), 64 * kWaves, 0, st>>>(p);
   const int nv = p.wr ? (p.E + 63) / 64 : 1;
-  if (nv <= 1) few_plan_kernel<1><<<1, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 2) few_plan_kernel<2><<<1, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 4) few_plan_kernel<4><<<1, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 8) few_plan_kernel<8><<<1, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 16) few_plan_kernel<16><<<1, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 32) few_plan_kernel<32><<<1, 64 * kPlanWaves, 0, st>>>(p);
-  else few_plan_kernel<64><<<1, 64 * kPlanWaves, 0, st>>>(p);
+  const int nr = p.wr ? (p.T + kRouteWaves - 1) / kRouteWaves : 1;
+  if (nv <= 1) few_plan_kernel<1><<<nr, 64 * kPlanWaves, 0, st>>>(p);
+  else if (nv <= 2) few_plan_kernel<2><<<nr, 64 * kPlanWaves, 0, st>>>(p);
+  else if (nv <= 4) few_plan_kernel<4><<<nr, 64 * kPlanWaves, 0, st>>>(p);
+  else if (nv <= 8) few_plan_kernel<8><<<nr, 64 * kPlanWaves, 0, st>>>(p);
+  else if (nv <= 16) few_plan_kernel<16><<<nr, 64 * kPlanWaves, 0, st>>>(p);
+  else if (nv <= 32) few_plan_kernel<32><<<nr, 64 * kPlanWaves, 0, st>>>(p);
+  else few_plan_kernel<64><<<nr, 64 * kPlanWaves, 0, st>>>(p);
   few_gate_up_kernel<T, 8><<<slots * (p.I / 16), 64 * kWaves, 0, st>>>(p);
   few_down_kernel<T, 12>
       <<<(slots + kGroup - 1) / kGroup * (p.H / 16), 64 * kWaves, 0, st>>>(p);
