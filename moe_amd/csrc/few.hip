@@ -32,9 +32,14 @@ constexpr int kFewExperts = 4096;
 constexpr int kFewRows = kFewTokens * kFewTopK;
 constexpr int kWaves = 8;        // waves per workgroup of the GEMV kernels
 constexpr int kPlanWaves = 16;
-constexpr int kRouteWaves = 4;   // tokens per workgroup of the routing
-constexpr int kGroup = 4;        // experts per workgroup of the down kernel
-constexpr int kParts = kWaves / kGroup;  // waves that split one expert's contraction there
+#ifndef FEW_DGRID
+#define FEW_DGRID 512
+#endif
+#ifndef FEW_DCH
+#define FEW_DCH 8
+#endif
+constexpr int kDownGrid = FEW_DGRID;
+constexpr int kLdsRows = 128;    // routed rows whose y the down kernel keeps in LDS
 
 struct FewArgs {
   const void* x;           // [T,H]
@@ -84,16 +89,6 @@ template <> struct Mma<float> {
 };
 
 __device__ __forceinline__ u32x4 ld16(const char* p) { return *(const u32x4*)p; }
-#ifndef FEW_NT
-#define FEW_NT 0
-#endif
-__device__ __forceinline__ u32x4 ld16_w(const char* p) {
-#if FEW_NT
-  return __builtin_nontemporal_load((const u32x4*)p);
-#else
-  return *(const u32x4*)p;
-#endif
-}
 
 template <typename T> __device__ __forceinline__ float few_round(float v) {
   if constexpr (sizeof(T) == 2) return round_bf(v);
@@ -147,8 +142,18 @@ __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
   const int t0 = blockIdx.y * 16;
   const char* b = (const char*)p.x + (int64_t)min(t0 + n, p.T - 1) * ld + g * 16;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = s0; s < s1; ++s) acc = Mma<T>::step(ld16(a + s * 64), ld16(b + s * 64), acc);
+  for (int sb = s0; sb < s1; sb += 8) {
+    u32x4 va[8], vb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = min(sb + i, s1 - 1);
+      va[i] = ld16(a + s * 64);
+      vb[i] = ld16(b + s * 64);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (sb + i < s1) acc = Mma<T>::step(va[i], vb[i], acc);
+  }
   red[wid][lane] = acc;
   if (blockIdx.x == 0 && blockIdx.y == 0) clear_counters(p);
   __syncthreads();
@@ -257,40 +262,40 @@ __device__ void route_token(const FewArgs& p, const float* logits, int lane, flo
   wk = dsk_weight(wk, ssum, p.renorm, p.scaling, 0);
 }
 
-// The tokens' top-K, one token a wave, four a workgroup; the last workgroup to
-// finish lists the active experts and their rows.  With the routing given there
-// is one workgroup, which lists.  Every entry counts the entries of its expert
-// and those before it by reading all ids from LDS (S <= 1024).
+// The tokens' top-K, one token a wave; the last workgroup to finish lists the
+// active experts and their rows.  With the routing given there is one
+// workgroup, which lists.  An entry's place among its expert's rows: a wave's
+// 64 entries find their peers by one readlane per entry, then the waves add
+// their counts to the expert's in LDS one after the other.
 template <int NV>
 __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
-  __shared__ __attribute__((aligned(16))) int ids[kFewRows];
-  __shared__ int row0_of[kFewRows];
+  __shared__ int ids[kFewRows];
+  __shared__ int count[kFewExperts];   // rows of an expert, then its first row
   __shared__ int2 wsum[kPlanWaves];
   __shared__ int box;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S = p.T * p.K;
   if (p.wr) {
-    const int t = blockIdx.x * kRouteWaves + wid;
-    if (wid < kRouteWaves && t < p.T) {
+    const int t = blockIdx.x * kPlanWaves + wid;
+    const bool one = gridDim.x == 1;
+    if (t < p.T) {
       float wk;
       int ek;
       route_token<NV>(p, p.logits + (int64_t)t * p.E, lane, wk, ek);
       if (lane < p.K) {
         const int s = t * p.K + lane;
+        if (one) ids[s] = ek;
         put_shared(&p.real[s], ek);
         p.w[s] = wk;
         if (p.out_w) p.out_w[s] = wk;
         if (p.out_idx) p.out_idx[s] = ek;
       }
     }
-    if (gridDim.x > 1) {
+    if (!one) {
       if (!last_to_arrive(&p.hdr[1], gridDim.x, &box)) return;
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+      if (tid < S) ids[tid] = get_shared(&p.real[tid]);
     }
-    if (tid < S) ids[tid] = get_shared(&p.real[tid]);
   } else {
     if (tid < S) {
       const int64_t e = p.ids[tid];
@@ -301,26 +306,33 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
     }
     clear_counters(p);
   }
-  for (int i = S + tid; i < kFewRows; i += 64 * kPlanWaves) ids[i] = -1;
+  for (int i = tid; i < p.E; i += 64 * kPlanWaves) count[i] = 0;
   __syncthreads();
-  const int e = ids[tid];
-  int rank = 0, cnt = 0, first = S;
-  for (int i = 0; i < S && wid * 64 < S; i += 4) {
-    const int4 q = *(const int4*)&ids[i];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int o = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
-      if (o == e) {
-        ++cnt;
-        rank += i + j < tid;
-        first = min(first, i + j);
-      }
+  const int e = tid < S ? ids[tid] : -1;
+  // peers: the entries of this wave with the same expert
+  int before = 0, peers = 0;
+  const int nw = (S + 63) >> 6;
+  if (wid < nw) {
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) {
+      const bool same = __builtin_amdgcn_readlane(e, i) == e;
+      peers += same;
+      before += same && i < lane;
     }
   }
+  int rank = before;
+  for (int w = 0; w < nw; ++w) {
+    if (wid == w && e >= 0) {
+      rank += count[e];
+      __builtin_amdgcn_wave_barrier();
+      if (before == 0) count[e] += peers;
+    }
+    __syncthreads();
+  }
   const bool lead = e >= 0 && rank == 0;
+  const int cnt = lead ? count[e] : 0;
   // exclusive prefixes over the leaders: their number and their rows
-  int2 v = lead ? make_int2(1, cnt) : make_int2(0, 0);
-  int2 inc = v;
+  int2 inc = make_int2(lead, cnt);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int a = __shfl_up(inc.x, o, 64), b = __shfl_up(inc.y, o, 64);
@@ -332,18 +344,18 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
   if (lane == 63) wsum[wid] = inc;
   __syncthreads();
   int2 base = make_int2(0, 0), all = make_int2(0, 0);
-  for (int w = 0; w < kPlanWaves; ++w) {
+  for (int w = 0; w < nw; ++w) {
     if (w == wid) base = all;
     all.x += wsum[w].x;
     all.y += wsum[w].y;
   }
   if (lead) {
-    const int at = base.x + inc.x - 1, r0 = base.y + inc.y - cnt;
-    p.list[at] = make_int4(e, r0, cnt, 0);
-    row0_of[tid] = r0;
+    const int r0 = base.y + inc.y - cnt;
+    p.list[base.x + inc.x - 1] = make_int4(e, r0, cnt, 0);
+    count[e] = r0;
   }
   __syncthreads();
-  if (e >= 0) p.rows[row0_of[first] + rank] = tid;
+  if (e >= 0) p.rows[count[e] + rank] = tid;
   if (tid == 0) p.hdr[0] = all.x;
 }
 
@@ -356,8 +368,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) 
   __shared__ f32x4 red[kWaves][2][64];
   const int nsl = p.I / 16;
   const int slot = blockIdx.x / nsl, f0 = (blockIdx.x % nsl) * 16;
-  if (slot >= p.hdr[0]) return;
-  const int4 info = p.list[slot];
+  const int nact = p.hdr[0];
+  const int4 info = p.list[slot];  // a slot past the active experts holds anything
+  if (slot >= nact) return;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ns = p.H / Mma<T>::kStep;
@@ -375,8 +388,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) 
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int s = min(sb + i, s1 - 1);
-        a[i] = ld16_w(wg + s * 64);
-        b[i] = ld16_w(wu + s * 64);
+        a[i] = ld16(wg + s * 64);
+        b[i] = ld16(wu + s * 64);
       }
 #pragma unroll
       for (int i = 0; i < CH; ++i) c[i] = ld16(xr + min(sb + i, s1 - 1) * 64);
@@ -409,72 +422,125 @@ __global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) 
 }
 
 // --------------------------------------------------------- down + combine
-// Workgroup: 16 columns of the output and kGroup active experts, kParts waves
-// an expert.  y rows go to the workspace; the workgroup that finishes a column
-// slice's last group sums them with the routing weights, in k order.
+// Workgroup: 16 columns of the output and a share (one of gridDim.x / (H / 16))
+// of the active experts, a wave for each of them in turn.  A wave needs no other
+// one: it reads 16 rows of an expert's weights, CH steps at a time and the next
+// CH before it multiplies these, and leaves the y of the expert's rows in the
+// workspace (LDS where the workgroup has all experts of at most kLdsRows rows).
+// The last workgroup of a column slice sums y with the routing weights, in k
+// order.
 template <typename T, int CH>
-__global__ __launch_bounds__(64 * kWaves, 4) void few_down_kernel(FewArgs p) {
-  __shared__ f32x4 red[kWaves][64];
+__global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
+  __shared__ int4 s_list[kFewRows];
+  __shared__ int s_rows[kFewRows];
+  __shared__ float s_y[kLdsRows][16];
   __shared__ int box;
-  const int nh = p.H / 16;
-  const int hs = blockIdx.x % nh, grp = blockIdx.x / nh, h0 = hs * 16;
-  const int nact = p.hdr[0];
-  const int ngrp = max(1, (nact + kGroup - 1) / kGroup);
-  if (grp >= ngrp) return;
+  const int nh = p.H / 16, share = gridDim.x / nh;
+  const int hs = blockIdx.x % nh, h0 = hs * 16, sh = blockIdx.x / nh;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = wid / kParts, part = wid % kParts;
-  int most = 0;
-#pragma unroll
-  for (int q = 0; q < kGroup; ++q)
-    if (grp * kGroup + q < nact) most = max(most, p.list[grp * kGroup + q].z);
-  int4 info = make_int4(0, 0, 0, 0);
-  if (grp * kGroup + j < nact) info = p.list[grp * kGroup + j];
+  const int S = p.T * p.K;
+  const bool in_lds = share == 1 && S <= kLdsRows;
+  const int stride = share * kWaves;
+  // this workgroup's experts are list[sh * kWaves + wave + i * stride]
+  const int nact = p.hdr[0];
+  for (int i = tid; i < S; i += 64 * kWaves) s_rows[i] = p.rows[i];
+  for (int i = tid; (i / kWaves) * stride < S; i += 64 * kWaves) {
+    const int q = (i / kWaves) * stride + sh * kWaves + i % kWaves;
+    if (q < S) s_list[i] = p.list[q];
+  }
+  __syncthreads();
   const int ns = p.I / Mma<T>::kStep;
-  const int s0 = part * ns / kParts, s1 = (part + 1) * ns / kParts;
   const int64_t ld = (int64_t)p.I * sizeof(T);
-  const char* wd = (const char*)p.w2 + ((int64_t)info.x * p.H + h0 + n) * ld + g * 16;
-  for (int rg = 0; rg < most; rg += 16) {
-    const int left = info.z - rg;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (left > 0) {
-      const char* ar =
-          (const char*)p.act + (int64_t)p.rows[info.y + rg + min(n, left - 1)] * ld + g * 16;
-      for (int sb = s0; sb < s1; sb += CH) {
-        u32x4 a[CH], c[CH];
+  struct Pos {
+    int i, rg, sb;
+    bool more;
+    int4 info;
+    const char *w, *a;
+  };
+  auto start = [&](Pos& c) {  // expert c.i of the wave
+    c.more = c.i * stride + sh * kWaves + wid < nact;
+    if (!c.more) return;
+    c.info = s_list[c.i * kWaves + wid];
+    c.w = (const char*)p.w2 + ((int64_t)c.info.x * p.H + h0 + n) * ld + g * 16;
+  };
+  auto rows = [&](Pos& c) {
+    c.a = (const char*)p.act +
+          (int64_t)s_rows[c.info.y + c.rg + min(n, c.info.z - c.rg - 1)] * ld + g * 16;
+  };
+  auto next = [&](Pos c) {
+    c.sb += CH;
+    if (c.sb < ns) return c;
+    c.sb = 0;
+    c.rg += 16;
+    if (c.rg >= c.info.z) {
+      c.rg = 0;
+      ++c.i;
+      start(c);
+    }
+    if (c.more) rows(c);
+    return c;
+  };
+  auto load = [&](const Pos& c, u32x4 (&a)[CH], u32x4 (&b)[CH]) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) a[i] = ld16_w(wd + min(sb + i, s1 - 1) * 64);
+    for (int i = 0; i < CH; ++i) a[i] = ld16(c.w + min(c.sb + i, ns - 1) * 64);
 #pragma unroll
-        for (int i = 0; i < CH; ++i) c[i] = ld16(ar + min(sb + i, s1 - 1) * 64);
+    for (int i = 0; i < CH; ++i) b[i] = ld16(c.a + min(c.sb + i, ns - 1) * 64);
+  };
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto step = [&](const Pos& c, const u32x4 (&a)[CH], const u32x4 (&b)[CH]) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
-          if (sb + i < s1) acc = Mma<T>::step(a[i], c[i], acc);
+    for (int i = 0; i < CH; ++i)
+      if (c.sb + i < ns) acc = Mma<T>::step(a[i], b[i], acc);
+    if (c.sb + CH < ns) return;
+    if (n < c.info.z - c.rg) {
+      const int s = s_rows[c.info.y + c.rg + n];
+      if (in_lds) {
+        *(f32x4*)&s_y[s][g * 4] = acc;
+      } else {
+        float* y = p.y + (int64_t)s * p.H + h0 + g * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put_shared(y + i, acc[i]);
       }
     }
-    if (rg) __syncthreads();
-    red[wid][lane] = acc;
-    __syncthreads();
-    for (int v = tid; v < kGroup * 256; v += 64 * kWaves) {
-      const int q = v >> 8, h = v & 15, r = (v >> 4) & 15, l = (h >> 2) * 16 + r;
-      if (grp * kGroup + q >= nact) continue;
-      const int4 iq = p.list[grp * kGroup + q];
-      if (rg + r >= iq.z) continue;
-      float sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kParts; ++w) sum += red[q * kParts + w][l][h & 3];
-      put_shared(&p.y[(int64_t)p.rows[iq.y + rg + r] * p.H + h0 + h], sum);
+    acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  };
+  Pos c{};
+  start(c);
+  if (c.more) {
+    u32x4 a0[CH], b0[CH], a1[CH], b1[CH];
+    rows(c);
+    load(c, a0, b0);
+    while (true) {
+      Pos d = next(c);
+      if (d.more) load(d, a1, b1);
+      step(c, a0, b0);
+      if (!d.more) break;
+      c = next(d);
+      if (c.more) load(c, a0, b0);
+      step(d, a1, b1);
+      if (!c.more) break;
     }
   }
-  // the slice's last group combines
-  if (!last_to_arrive(&p.arrived[hs], ngrp, &box)) return;
-  const int h = h0 + (tid & 15);
+  if (in_lds) __syncthreads();
+  else if (!last_to_arrive(&p.arrived[hs], share, &box)) return;
+  const int h = tid & 15;
   for (int t = tid >> 4; t < p.T; t += 4 * kWaves) {
     float o = 0.f;
-    for (int k = 0; k < p.K; ++k) {
-      const int s = t * p.K + k;
-      if (p.real[s] >= 0) o = fmaf(p.w[s], get_shared(&p.y[(int64_t)s * p.H + h]), o);
+    for (int k0 = 0; k0 < p.K; k0 += 8) {
+      float y[8], w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int s = t * p.K + min(k0 + k, p.K - 1);
+        const bool real = k0 + k < p.K && p.real[s] >= 0;
+        w[k] = real ? p.w[s] : 0.f;
+        y[k] = 0.f;
+        if (real) y[k] = in_lds ? s_y[s][h] : get_shared(&p.y[(int64_t)s * p.H + h0 + h]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o = fmaf(w[k], y[k], o);
     }
-    ((T*)p.out)[(int64_t)t * p.H + h] = (T)o;
+    ((T*)p.out)[(int64_t)t * p.H + h0 + h] = (T)o;
   }
 }
 
@@ -525,7 +591,7 @@ void few_launch(FewArgs& p, hipStream_t st) {
   const int S = p.T * p.K, slots = S < p.E ? S : p.E;
   if (p.wr) few_logits_kernel<T><<<dim3((p.E + 15) / 16, (p.T + 15) / 16), 64 * kWaves, 0, st>>>(p);
   const int nv = p.wr ? (p.E + 63) / 64 : 1;
-  const int nr = p.wr ? (p.T + kRouteWaves - 1) / kRouteWaves : 1;
+  const int nr = p.wr ? (p.T + kPlanWaves - 1) / kPlanWaves : 1;
   if (nv <= 1) few_plan_kernel<1><<<nr, 64 * kPlanWaves, 0, st>>>(p);
   else if (nv <= 2) few_plan_kernel<2><<<nr, 64 * kPlanWaves, 0, st>>>(p);
   else if (nv <= 4) few_plan_kernel<4><<<nr, 64 * kPlanWaves, 0, st>>>(p);
@@ -534,8 +600,12 @@ void few_launch(FewArgs& p, hipStream_t st) {
   else if (nv <= 32) few_plan_kernel<32><<<nr, 64 * kPlanWaves, 0, st>>>(p);
   else few_plan_kernel<64><<<nr, 64 * kPlanWaves, 0, st>>>(p);
   few_gate_up_kernel<T, 8><<<slots * (p.I / 16), 64 * kWaves, 0, st>>>(p);
-  few_down_kernel<T, 12>
-      <<<(slots + kGroup - 1) / kGroup * (p.H / 16), 64 * kWaves, 0, st>>>(p);
+  const int nh = p.H / 16;
+  int share = kDownGrid / nh;
+  const int most = (slots + kWaves - 1) / kWaves;
+  if (share > most) share = most;
+  if (share < 1) share = 1;
+  few_down_kernel<T, FEW_DCH><<<nh * share, 64 * kWaves, 0, st>>>(p);
 }
 
 int few_run(FewArgs& p, int dtype, void* workspace, size_t workspace_bytes, hipStream_t st,
