@@ -35,9 +35,6 @@ constexpr int kPlanWaves = 16;
 #ifndef FEW_DGRID
 #define FEW_DGRID 512
 #endif
-#ifndef FEW_DCH
-#define FEW_DCH 8
-#endif
 constexpr int kDownGrid = FEW_DGRID;
 constexpr int kLdsRows = 128;    // routed rows whose y the down kernel keeps in LDS
 
@@ -88,7 +85,21 @@ template <> struct Mma<float> {
   }
 };
 
-__device__ __forceinline__ u32x4 ld16(const char* p) { return *(const u32x4*)p; }
+// 16 bytes of a row of a wave-uniform base: the lane's part of the address has
+// 32 bits and a step's is an immediate, which keeps a chunk of loads short (a
+// workgroup of these kernels runs each instruction once or twice, so fetching
+// them is part of its time).
+__device__ __forceinline__ u32x4 ld16(const char* base, uint32_t lane_off, int imm = 0) {
+  return *(const u32x4*)(base + lane_off + imm);
+}
+
+// f(chunk length, first step) over the steps [s, end): chunks of CH, then the
+// rest in halves.
+template <int CH, typename F>
+__device__ __forceinline__ void chunks(int s, int end, F&& f) {
+  for (; s + CH <= end; s += CH) f(std::integral_constant<int, CH>{}, s);
+  if constexpr (CH > 1) chunks<CH / 2>(s, end, f);
+}
 
 template <typename T> __device__ __forceinline__ float few_round(float v) {
   if constexpr (sizeof(T) == 2) return round_bf(v);
@@ -101,15 +112,18 @@ __device__ __forceinline__ void clear_counters(const FewArgs& p) {
   for (int i = threadIdx.x; i < p.H / 16; i += blockDim.x) p.arrived[i] = 0;
 }
 
+// The sc1 bit of a buffer access: device scope.
+constexpr int kDeviceScope = 16;
+
 // What one workgroup leaves for another of the same launch: written through to
 // and read from the memory that all XCDs share, so that no cache has to be
 // written back or invalidated.  A workgroup counts itself as arrived once its
 // writes are there; the last one to arrive reads everybody's.
-__device__ __forceinline__ void put_shared(float* p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ void put_shared(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, off, 0, kDeviceScope);
 }
-__device__ __forceinline__ float get_shared(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ __forceinline__ float get_shared(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kDeviceScope));
 }
 __device__ __forceinline__ void put_shared(int* p, int v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -138,22 +152,23 @@ __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
   const int ns = p.H / Mma<T>::kStep;
   const int s0 = wid * ns / kWaves, s1 = (wid + 1) * ns / kWaves;
   const int64_t ld = (int64_t)p.H * sizeof(T);
-  const char* a = (const char*)p.wr + (int64_t)min(e0 + n, p.E - 1) * ld + g * 16;
+  const uint32_t ao = (uint32_t)(min(e0 + n, p.E - 1) - e0) * (uint32_t)ld + g * 16;
   const int t0 = blockIdx.y * 16;
-  const char* b = (const char*)p.x + (int64_t)min(t0 + n, p.T - 1) * ld + g * 16;
+  const uint32_t bo = (uint32_t)min(t0 + n, p.T - 1) * (uint32_t)ld + g * 16;
+  const char* a = (const char*)p.wr + e0 * ld;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int sb = s0; sb < s1; sb += 8) {
-    u32x4 va[8], vb[8];
+  auto chunk = [&](auto ch, int s) {
+    constexpr int CH = decltype(ch)::value;
+    const char *as = a + s * 64, *bs = (const char*)p.x + s * 64;
+    u32x4 va[CH], vb[CH];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int s = min(sb + i, s1 - 1);
-      va[i] = ld16(a + s * 64);
-      vb[i] = ld16(b + s * 64);
-    }
+    for (int i = 0; i < CH; ++i) va[i] = ld16(as, ao, i * 64);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (sb + i < s1) acc = Mma<T>::step(va[i], vb[i], acc);
-  }
+    for (int i = 0; i < CH; ++i) vb[i] = ld16(bs, bo, i * 64);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) acc = Mma<T>::step(va[i], vb[i], acc);
+  };
+  chunks<8>(s0, s1, chunk);
   red[wid][lane] = acc;
   if (blockIdx.x == 0 && blockIdx.y == 0) clear_counters(p);
   __syncthreads();
@@ -376,31 +391,31 @@ __global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) 
   const int ns = p.H / Mma<T>::kStep;
   const int s0 = wid * ns / kWaves, s1 = (wid + 1) * ns / kWaves;
   const int64_t ld = (int64_t)p.H * sizeof(T);
-  const char* wg = (const char*)p.w1 + ((int64_t)info.x * 2 * p.I + f0 + n) * ld + g * 16;
+  const char* wg = (const char*)p.w1 + ((int64_t)info.x * 2 * p.I + f0) * ld;
   const char* wu = wg + (int64_t)p.I * ld;
+  const uint32_t wo = (uint32_t)n * (uint32_t)ld + g * 16;
   for (int rg = 0; rg < info.z; rg += 16) {
     const int left = info.z - rg;
-    const char* xr = (const char*)p.x +
-                     (int64_t)(p.rows[info.y + rg + min(n, left - 1)] / p.K) * ld + g * 16;
+    const uint32_t xo =
+        (uint32_t)(p.rows[info.y + rg + min(n, left - 1)] / p.K) * (uint32_t)ld + g * 16;
     f32x4 ag = {0.f, 0.f, 0.f, 0.f}, au = ag;
-    for (int sb = s0; sb < s1; sb += CH) {
-      u32x4 a[CH], b[CH], c[CH];
+    chunks<CH>(s0, s1, [&](auto ch, int s) {
+      constexpr int C = decltype(ch)::value;
+      const char *gs = wg + s * 64, *us = wu + s * 64, *xs = (const char*)p.x + s * 64;
+      u32x4 a[C], b[C], c[C];
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int s = min(sb + i, s1 - 1);
-        a[i] = ld16(wg + s * 64);
-        b[i] = ld16(wu + s * 64);
+      for (int i = 0; i < C; ++i) {
+        a[i] = ld16(gs, wo, i * 64);
+        b[i] = ld16(us, wo, i * 64);
       }
 #pragma unroll
-      for (int i = 0; i < CH; ++i) c[i] = ld16(xr + min(sb + i, s1 - 1) * 64);
+      for (int i = 0; i < C; ++i) c[i] = ld16(xs, xo, i * 64);
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        if (sb + i < s1) {
-          ag = Mma<T>::step(a[i], c[i], ag);
-          au = Mma<T>::step(b[i], c[i], au);
-        }
+      for (int i = 0; i < C; ++i) {
+        ag = Mma<T>::step(a[i], c[i], ag);
+        au = Mma<T>::step(b[i], c[i], au);
       }
-    }
+    });
     if (rg) __syncthreads();
     red[wid][0][lane] = ag;
     red[wid][1][lane] = au;
@@ -433,6 +448,8 @@ template <typename T, int CH>
 __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
   __shared__ int4 s_list[kFewRows];
   __shared__ int s_rows[kFewRows];
+  __shared__ float s_w[kFewRows];
+  __shared__ uint64_t s_real[kFewRows / 64];
   __shared__ float s_y[kLdsRows][16];
   __shared__ int box;
   const int nh = p.H / 16, share = gridDim.x / nh;
@@ -444,33 +461,45 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
   const int stride = share * kWaves;
   // this workgroup's experts are list[sh * kWaves + wave + i * stride]
   const int nact = p.hdr[0];
-  for (int i = tid; i < S; i += 64 * kWaves) s_rows[i] = p.rows[i];
+  for (int i0 = 0; i0 < S; i0 += 64 * kWaves) {
+    const int i = i0 + tid;
+    if (i < S) {
+      s_rows[i] = p.rows[i];
+      s_w[i] = p.w[i];
+    }
+    const uint64_t real = __ballot(i < S && p.real[i] >= 0);
+    if (lane == 0 && i < S) s_real[i >> 6] = real;
+  }
   for (int i = tid; (i / kWaves) * stride < S; i += 64 * kWaves) {
     const int q = (i / kWaves) * stride + sh * kWaves + i % kWaves;
     if (q < S) s_list[i] = p.list[q];
   }
   __syncthreads();
+  const auto y_rows = make_rsrc(p.y, (uint32_t)S * p.H * 4);
   const int ns = p.I / Mma<T>::kStep;
   const int64_t ld = (int64_t)p.I * sizeof(T);
   struct Pos {
     int i, rg, sb;
     bool more;
     int4 info;
-    const char *w, *a;
+    const char* w;
+    uint32_t a;
   };
+  const uint32_t wo = (uint32_t)n * (uint32_t)ld + g * 16;
   auto start = [&](Pos& c) {  // expert c.i of the wave
     c.more = c.i * stride + sh * kWaves + wid < nact;
     if (!c.more) return;
     c.info = s_list[c.i * kWaves + wid];
-    c.w = (const char*)p.w2 + ((int64_t)c.info.x * p.H + h0 + n) * ld + g * 16;
+    c.w = (const char*)p.w2 + ((int64_t)c.info.x * p.H + h0) * ld;
   };
   auto rows = [&](Pos& c) {
-    c.a = (const char*)p.act +
-          (int64_t)s_rows[c.info.y + c.rg + min(n, c.info.z - c.rg - 1)] * ld + g * 16;
+    c.a = (uint32_t)s_rows[c.info.y + c.rg + min(n, c.info.z - c.rg - 1)] * (uint32_t)ld + g * 16;
   };
-  auto next = [&](Pos c) {
-    c.sb += CH;
-    if (c.sb < ns) return c;
+  auto next = [&](Pos c) {  // without one: more false, the addresses as they were
+    if (c.sb + CH < ns) {
+      c.sb += CH;
+      return c;
+    }
     c.sb = 0;
     c.rg += 16;
     if (c.rg >= c.info.z) {
@@ -481,26 +510,34 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
     if (c.more) rows(c);
     return c;
   };
+  // The last chunk of a contraction that CH does not divide starts earlier: its
+  // first steps are the previous chunk's and are passed over.
   auto load = [&](const Pos& c, u32x4 (&a)[CH], u32x4 (&b)[CH]) {
+    const int sb = max(0, min(c.sb, ns - CH));
+    const char *ws = c.w + sb * 64, *as = (const char*)p.act + sb * 64;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) a[i] = ld16(c.w + min(c.sb + i, ns - 1) * 64);
+    for (int i = 0; i < CH; ++i) a[i] = ld16(ws, wo, i * 64);
 #pragma unroll
-    for (int i = 0; i < CH; ++i) b[i] = ld16(c.a + min(c.sb + i, ns - 1) * 64);
+    for (int i = 0; i < CH; ++i) b[i] = ld16(as, c.a, i * 64);
   };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   auto step = [&](const Pos& c, const u32x4 (&a)[CH], const u32x4 (&b)[CH]) {
+    const int skip = c.sb - max(0, min(c.sb, ns - CH));
+    if (skip == 0) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
-      if (c.sb + i < ns) acc = Mma<T>::step(a[i], b[i], acc);
+      for (int i = 0; i < CH; ++i) acc = Mma<T>::step(a[i], b[i], acc);
+    } else {
+#pragma unroll
+      for (int i = 1; i < CH; ++i)
+        if (i >= skip) acc = Mma<T>::step(a[i], b[i], acc);
+    }
     if (c.sb + CH < ns) return;
     if (n < c.info.z - c.rg) {
       const int s = s_rows[c.info.y + c.rg + n];
       if (in_lds) {
         *(f32x4*)&s_y[s][g * 4] = acc;
       } else {
-        float* y = p.y + (int64_t)s * p.H + h0 + g * 4;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put_shared(y + i, acc[i]);
+        put_shared(y_rows, ((uint32_t)s * p.H + h0 + g * 4) * 4, acc);
       }
     }
     acc = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -511,13 +548,15 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
     u32x4 a0[CH], b0[CH], a1[CH], b1[CH];
     rows(c);
     load(c, a0, b0);
+    // Past the wave's last expert the last addresses are loaded again, unused:
+    // with a branch around the loads the compiler waits for all of them.
     while (true) {
-      Pos d = next(c);
-      if (d.more) load(d, a1, b1);
+      const Pos d = next(c);
+      load(d, a1, b1);
       step(c, a0, b0);
       if (!d.more) break;
       c = next(d);
-      if (c.more) load(c, a0, b0);
+      load(c, a0, b0);
       step(d, a1, b1);
       if (!c.more) break;
     }
@@ -532,10 +571,10 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int s = t * p.K + min(k0 + k, p.K - 1);
-        const bool real = k0 + k < p.K && p.real[s] >= 0;
-        w[k] = real ? p.w[s] : 0.f;
+        const bool real = k0 + k < p.K && (s_real[s >> 6] >> (s & 63) & 1);
+        w[k] = real ? s_w[s] : 0.f;
         y[k] = 0.f;
-        if (real) y[k] = in_lds ? s_y[s][h] : get_shared(&p.y[(int64_t)s * p.H + h0 + h]);
+        if (real) y[k] = in_lds ? s_y[s][h] : get_shared(y_rows, ((uint32_t)s * p.H + h0 + h) * 4);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) o = fmaf(w[k], y[k], o);
@@ -605,7 +644,11 @@ void few_launch(FewArgs& p, hipStream_t st) {
   const int most = (slots + kWaves - 1) / kWaves;
   if (share > most) share = most;
   if (share < 1) share = 1;
-  few_down_kernel<T, FEW_DCH><<<nh * share, 64 * kWaves, 0, st>>>(p);
+  // a chunk no longer than the contraction: weights past an expert's rows are not read
+  const int ns = p.I / Mma<T>::kStep;
+  if (ns >= 8) few_down_kernel<T, 8><<<nh * share, 64 * kWaves, 0, st>>>(p);
+  else if (ns >= 4) few_down_kernel<T, 4><<<nh * share, 64 * kWaves, 0, st>>>(p);
+  else few_down_kernel<T, 2><<<nh * share, 64 * kWaves, 0, st>>>(p);
 }
 
 int few_run(FewArgs& p, int dtype, void* workspace, size_t workspace_bytes, hipStream_t st,
