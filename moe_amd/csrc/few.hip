@@ -32,11 +32,7 @@ constexpr int kFewExperts = 4096;
 constexpr int kFewRows = kFewTokens * kFewTopK;
 constexpr int kWaves = 8;        // waves per workgroup of the GEMV kernels
 constexpr int kPlanWaves = 16;
-#ifndef FEW_DGRID
-#define FEW_DGRID 512
-#endif
-constexpr int kDownGrid = FEW_DGRID;
-constexpr int kLdsRows = 128;    // routed rows whose y the down kernel keeps in LDS
+constexpr int kMaxLds = kFewRows * (16 + 64 + 12);  // of the down kernel
 
 struct FewArgs {
   const void* x;           // [T,H]
@@ -52,11 +48,9 @@ struct FewArgs {
   float* logits;           // workspace from here on
   float* w;                // [S]
   int* hdr;                // [0] active experts, [1] finished routing workgroups
-  int* arrived;            // [H/16] finished groups of the down kernel's column slices
   int4* list;              // {expert, first row, rows, 0} of the active experts
   int* rows;               // flat entries s = t*K + k by active expert, ascending
   void* act;               // [S,I] by flat entry
-  float* y;                // [S,H]
   int* real;               // [S] the entry's expert, negative for padding
   float* out_w;            // routing out (may be null)
   int64_t* out_idx;
@@ -109,22 +103,12 @@ template <typename T> __device__ __forceinline__ float few_round(float v) {
 // The counters that workgroups of later launches finish by.
 __device__ __forceinline__ void clear_counters(const FewArgs& p) {
   if (threadIdx.x == 0) p.hdr[1] = 0;
-  for (int i = threadIdx.x; i < p.H / 16; i += blockDim.x) p.arrived[i] = 0;
 }
-
-// The sc1 bit of a buffer access: device scope.
-constexpr int kDeviceScope = 16;
 
 // What one workgroup leaves for another of the same launch: written through to
 // and read from the memory that all XCDs share, so that no cache has to be
 // written back or invalidated.  A workgroup counts itself as arrived once its
 // writes are there; the last one to arrive reads everybody's.
-__device__ __forceinline__ void put_shared(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 v) {
-  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, off, 0, kDeviceScope);
-}
-__device__ __forceinline__ float get_shared(__amdgpu_buffer_rsrc_t r, uint32_t off) {
-  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, off, 0, kDeviceScope));
-}
 __device__ __forceinline__ void put_shared(int* p, int v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -186,17 +170,51 @@ __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
 }
 
 // ------------------------------------------------------- routing and plan
-// The largest key of the wave below thr (0: none).
+// The order of wave_topk.h's rank_key in 32 bits, by value alone; 0 is below
+// every value.
+__device__ __forceinline__ uint32_t value_key(float v) { return (uint32_t)(rank_key(v, 0) >> 32); }
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return key_value((uint64_t)key << 32);
+}
+
+// Takes the largest key (entry j*64 + lane in slot j) out and returns it and
+// its entry, the lowest of equal ones: the value by DPP, its holder by ballots.
+// (64-bit keys that hold the index too need four times the instructions.)
 template <int NV>
-__device__ __forceinline__ uint64_t wave_next_key(const uint64_t (&key)[NV], uint64_t thr) {
-  const uint64_t b = group_max_key<16>(lane_next_key<NV>(key, thr));
-  uint64_t w = readlane_u64(b, 0);
+__device__ __forceinline__ uint32_t take_largest(uint32_t (&key)[NV], int lane, int& entry) {
+  uint32_t m = key[0];
 #pragma unroll
-  for (int r = 16; r < 64; r += 16) {
-    const uint64_t o = readlane_u64(b, r);
-    w = o > w ? o : w;
+  for (int j = 1; j < NV; ++j) m = max(m, key[j]);
+  m = group_max_key<16>(m);
+  m = max(max((uint32_t)__builtin_amdgcn_readlane(m, 0), (uint32_t)__builtin_amdgcn_readlane(m, 16)),
+          max((uint32_t)__builtin_amdgcn_readlane(m, 32), (uint32_t)__builtin_amdgcn_readlane(m, 48)));
+  entry = 0;
+  bool found = false;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const uint64_t here = __ballot(key[j] == m);
+    if (!found && here) {
+      const int l = __builtin_ctzll(here);
+      entry = j * 64 + l;
+      if (lane == l) key[j] = 0;
+      found = true;
+    }
   }
-  return w;
+  return m;
+}
+
+// The K largest in order: lane k < K gets the k-th entry and its key.
+template <int NV>
+__device__ __forceinline__ void take_topk(uint32_t (&key)[NV], int lane, int K, int& my_e,
+                                          uint32_t& my_key) {
+  my_e = 0;
+  my_key = 0;
+  for (int k = 0; k < K; ++k) {
+    int e;
+    const uint32_t m = take_largest<NV>(key, lane, e);
+    my_e = lane == k ? e : my_e;
+    my_key = lane == k ? m : my_key;
+  }
 }
 
 // One token on one wave: lane k < K gets its k-th expert and weight.  The
@@ -204,7 +222,7 @@ __device__ __forceinline__ uint64_t wave_next_key(const uint64_t (&key)[NV], uin
 template <int NV>
 __device__ void route_token(const FewArgs& p, const float* logits, int lane, float& wk, int& ek) {
   const int E = p.E, K = p.K;
-  uint64_t key[NV], kk;
+  uint32_t key[NV], kk;
   if (!p.sigmoid) {
     float v[NV];
     bool nan_here = false;
@@ -228,48 +246,46 @@ __device__ void route_token(const FewArgs& p, const float* logits, int lane, flo
     for (int j = 0; j < NV; ++j) {
       const int e = j * 64 + lane;
       s += e < E ? expf(v[j] - m) : 0.f;
-      key[j] = e < E ? rank_key(v[j], e) : 0ull;
+      key[j] = e < E ? value_key(v[j]) : 0u;
     }
     s = wave_sum(s);
-    ek = wave_topk_keys<NV>(key, lane, K, kk);
-    wk = lane < K ? expf(key_value(kk) - m) / s : 0.f;
+    take_topk<NV>(key, lane, K, ek, kk);
+    wk = lane < K ? expf(value_of(kk) - m) / s : 0.f;
     if (p.renorm) wk = wk / wave_sum(wk);
     return;
   }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int e = j * 64 + lane;
-    key[j] = e < E ? rank_key(sigmoidf_(logits[e]) + (p.offset ? p.offset[e] : 0.f), e) : 0ull;
+    key[j] = e < E ? value_key(sigmoidf_(logits[e]) + (p.offset ? p.offset[e] : 0.f)) : 0u;
   }
   if (p.ngroups > 0) {
     // groups scored by the sum of their K / gtopk best biased scores, gtopk kept
     const int eg = E / p.ngroups, per = K / p.gtopk;
     float gv = -INFINITY;
     for (int q = 0; q < p.ngroups; ++q) {
-      uint64_t gk[NV];
+      uint32_t gk[NV];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) gk[j] = (j * 64 + lane) / eg == q ? key[j] : 0ull;
+      for (int j = 0; j < NV; ++j) gk[j] = (j * 64 + lane) / eg == q ? key[j] : 0u;
       float acc = 0.f;
-      uint64_t thr = ~0ull;
-      for (int r = 0; r < per; ++r) {
-        thr = wave_next_key<NV>(gk, thr);
-        acc += key_value(thr);
-      }
+      int e;
+      for (int r = 0; r < per; ++r) acc += value_of(take_largest<NV>(gk, lane, e));
       gv = lane == q ? acc : gv;
     }
-    uint64_t gkey[1] = {lane < p.ngroups ? rank_key(gv, lane) : 0ull};
-    uint64_t keep = 0, thr = ~0ull;
+    uint32_t gkey[1] = {lane < p.ngroups ? value_key(gv) : 0u};
+    uint64_t keep = 0;
     for (int q = 0; q < p.gtopk; ++q) {
-      thr = wave_next_key<1>(gkey, thr);
-      keep |= 1ull << key_index(thr);
+      int e;
+      take_largest<1>(gkey, lane, e);
+      keep |= 1ull << e;
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int e = j * 64 + lane;
-      if (e < E && !((keep >> (e / eg)) & 1ull)) key[j] = 0ull;
+      if (e < E && !((keep >> (e / eg)) & 1ull)) key[j] = 0u;
     }
   }
-  ek = wave_topk_keys<NV>(key, lane, K, kk);
+  take_topk<NV>(key, lane, K, ek, kk);
   wk = lane < K ? sigmoidf_(logits[ek]) : 0.f;
   float ssum = 0.f;
   if (p.renorm)
@@ -375,14 +391,17 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 }
 
 // ------------------------------------------------------- gate/up + SwiGLU
-// Workgroup: 16 features of one active expert; the waves split H, CH steps of
-// gate and up rows in flight each.  An expert with more than 16 rows reads its
-// weights again for the next 16, from L2.
+// Workgroup: 8 features of one active expert, their gate and up rows being the
+// 16 rows of the A operand; the waves split H, CH steps in flight each.  An
+// expert with more than 16 rows reads its weights again for the next 16, from
+// L2.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
+// dealt to all of them in small pieces: with 16 features a workgroup one token
+// (K = 8, I = 768) has 384 for 256 CUs.
 template <typename T, int CH>
-__global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) {
-  __shared__ f32x4 red[kWaves][2][64];
-  const int nsl = p.I / 16;
-  const int slot = blockIdx.x / nsl, f0 = (blockIdx.x % nsl) * 16;
+__global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
+  __shared__ f32x4 red[kWaves][64];
+  const int nsl = p.I / 8;
+  const int slot = blockIdx.x / nsl, f0 = (blockIdx.x % nsl) * 8;
   const int nact = p.hdr[0];
   const int4 info = p.list[slot];  // a slot past the active experts holds anything
   if (slot >= nact) return;
@@ -391,43 +410,35 @@ __global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) 
   const int ns = p.H / Mma<T>::kStep;
   const int s0 = wid * ns / kWaves, s1 = (wid + 1) * ns / kWaves;
   const int64_t ld = (int64_t)p.H * sizeof(T);
-  const char* wg = (const char*)p.w1 + ((int64_t)info.x * 2 * p.I + f0) * ld;
-  const char* wu = wg + (int64_t)p.I * ld;
-  const uint32_t wo = (uint32_t)n * (uint32_t)ld + g * 16;
+  const char* w = (const char*)p.w1 +
+                  ((int64_t)info.x * 2 * p.I + f0 + (n & 7) + (n >> 3) * p.I) * ld + g * 16;
   for (int rg = 0; rg < info.z; rg += 16) {
     const int left = info.z - rg;
     const uint32_t xo =
         (uint32_t)(p.rows[info.y + rg + min(n, left - 1)] / p.K) * (uint32_t)ld + g * 16;
-    f32x4 ag = {0.f, 0.f, 0.f, 0.f}, au = ag;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     chunks<CH>(s0, s1, [&](auto ch, int s) {
       constexpr int C = decltype(ch)::value;
-      const char *gs = wg + s * 64, *us = wu + s * 64, *xs = (const char*)p.x + s * 64;
-      u32x4 a[C], b[C], c[C];
+      const char *ws = w + s * 64, *xs = (const char*)p.x + s * 64;
+      u32x4 a[C], c[C];
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        a[i] = ld16(gs, wo, i * 64);
-        b[i] = ld16(us, wo, i * 64);
-      }
+      for (int i = 0; i < C; ++i) a[i] = ld16(ws, 0, i * 64);
 #pragma unroll
       for (int i = 0; i < C; ++i) c[i] = ld16(xs, xo, i * 64);
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        ag = Mma<T>::step(a[i], c[i], ag);
-        au = Mma<T>::step(b[i], c[i], au);
-      }
+      for (int i = 0; i < C; ++i) acc = Mma<T>::step(a[i], c[i], acc);
     });
     if (rg) __syncthreads();
-    red[wid][0][lane] = ag;
-    red[wid][1][lane] = au;
+    red[wid][lane] = acc;
     __syncthreads();
-    if (threadIdx.x < 256) {
-      const int f = threadIdx.x & 15, r = threadIdx.x >> 4, l = (f >> 2) * 16 + r;
+    if (threadIdx.x < 128) {
+      const int f = threadIdx.x & 7, r = threadIdx.x >> 3, l = (f >> 2) * 16 + r;
       if (r < left) {
         float gs = 0.f, us = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          gs += red[w][0][l][f & 3];
-          us += red[w][1][l][f & 3];
+        for (int q = 0; q < kWaves; ++q) {
+          gs += red[q][l][f & 3];
+          us += red[q][l + 32][f & 3];
         }
         const int s = p.rows[info.y + rg + r];
         ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
@@ -437,63 +448,54 @@ __global__ __launch_bounds__(64 * kWaves, 4) void few_gate_up_kernel(FewArgs p) 
 }
 
 // --------------------------------------------------------- down + combine
-// Workgroup: 16 columns of the output and a share (one of gridDim.x / (H / 16))
-// of the active experts, a wave for each of them in turn.  A wave needs no other
-// one: it reads 16 rows of an expert's weights, CH steps at a time and the next
-// CH before it multiplies these, and leaves the y of the expert's rows in the
-// workspace (LDS where the workgroup has all experts of at most kLdsRows rows).
-// The last workgroup of a column slice sums y with the routing weights, in k
-// order.
+// Workgroup: C = 16 / parts columns of the output and every active expert, a
+// wave for each of them in turn.  `parts` makes the column slices about as many
+// as CUs: the A operand's 16 rows are C columns' weights for each of `parts`
+// pieces of the contraction, B's 16 columns C of the expert's rows for each of
+// them, and the blocks of the product where the pieces match are added.
+// A wave needs no other one: it reads CH steps and the next CH before it
+// multiplies these, and leaves y in LDS, where the workgroup then sums it with
+// the routing weights, in k order.
 template <typename T, int CH>
-__global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
-  __shared__ int4 s_list[kFewRows];
-  __shared__ int s_rows[kFewRows];
-  __shared__ float s_w[kFewRows];
-  __shared__ uint64_t s_real[kFewRows / 64];
-  __shared__ float s_y[kLdsRows][16];
-  __shared__ int box;
-  const int nh = p.H / 16, share = gridDim.x / nh;
-  const int hs = blockIdx.x % nh, h0 = hs * 16, sh = blockIdx.x / nh;
+__global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int parts) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int S = p.T * p.K, C = 16 / parts;
+  int4* s_list = (int4*)lds;
+  float* s_y = (float*)(s_list + S);   // [S][C]
+  int* s_rows = (int*)(s_y + S * C);
+  float* s_w = (float*)(s_rows + S);
+  int* s_real = (int*)(s_w + S);
+  const int h0 = blockIdx.x * C;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int S = p.T * p.K;
-  const bool in_lds = share == 1 && S <= kLdsRows;
-  const int stride = share * kWaves;
-  // this workgroup's experts are list[sh * kWaves + wave + i * stride]
   const int nact = p.hdr[0];
-  for (int i0 = 0; i0 < S; i0 += 64 * kWaves) {
-    const int i = i0 + tid;
-    if (i < S) {
-      s_rows[i] = p.rows[i];
-      s_w[i] = p.w[i];
-    }
-    const uint64_t real = __ballot(i < S && p.real[i] >= 0);
-    if (lane == 0 && i < S) s_real[i >> 6] = real;
-  }
-  for (int i = tid; (i / kWaves) * stride < S; i += 64 * kWaves) {
-    const int q = (i / kWaves) * stride + sh * kWaves + i % kWaves;
-    if (q < S) s_list[i] = p.list[q];
+  for (int i = tid; i < S; i += 64 * kWaves) {
+    s_list[i] = p.list[i];  // past the active experts: anything
+    s_rows[i] = p.rows[i];
+    s_w[i] = p.w[i];
+    s_real[i] = p.real[i];
   }
   __syncthreads();
-  const auto y_rows = make_rsrc(p.y, (uint32_t)S * p.H * 4);
-  const int ns = p.I / Mma<T>::kStep;
+  const int ns = p.I / Mma<T>::kStep / parts;
   const int64_t ld = (int64_t)p.I * sizeof(T);
   struct Pos {
-    int i, rg, sb;
+    int q, rg, sb;
     bool more;
     int4 info;
     const char* w;
     uint32_t a;
   };
-  const uint32_t wo = (uint32_t)n * (uint32_t)ld + g * 16;
-  auto start = [&](Pos& c) {  // expert c.i of the wave
-    c.more = c.i * stride + sh * kWaves + wid < nact;
+  const int nc = n % C;
+  const uint32_t piece = n / C * ns * 64 + g * 16;
+  const uint32_t wo = (uint32_t)nc * (uint32_t)ld + piece;
+  auto start = [&](Pos& c) {
+    c.more = c.q < nact;
     if (!c.more) return;
-    c.info = s_list[c.i * kWaves + wid];
+    c.info = s_list[c.q];
     c.w = (const char*)p.w2 + ((int64_t)c.info.x * p.H + h0) * ld;
   };
   auto rows = [&](Pos& c) {
-    c.a = (uint32_t)s_rows[c.info.y + c.rg + min(n, c.info.z - c.rg - 1)] * (uint32_t)ld + g * 16;
+    c.a = (uint32_t)s_rows[c.info.y + c.rg + min(nc, c.info.z - c.rg - 1)] * (uint32_t)ld + piece;
   };
   auto next = [&](Pos c) {  // without one: more false, the addresses as they were
     if (c.sb + CH < ns) {
@@ -501,10 +503,10 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
       return c;
     }
     c.sb = 0;
-    c.rg += 16;
+    c.rg += C;
     if (c.rg >= c.info.z) {
       c.rg = 0;
-      ++c.i;
+      c.q += kWaves;
       start(c);
     }
     if (c.more) rows(c);
@@ -513,7 +515,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
   // The last chunk of a contraction that CH does not divide starts earlier: its
   // first steps are the previous chunk's and are passed over.
   auto load = [&](const Pos& c, u32x4 (&a)[CH], u32x4 (&b)[CH]) {
-    const int sb = max(0, min(c.sb, ns - CH));
+    const int sb = min(c.sb, ns - CH);
     const char *ws = c.w + sb * 64, *as = (const char*)p.act + sb * 64;
 #pragma unroll
     for (int i = 0; i < CH; ++i) a[i] = ld16(ws, wo, i * 64);
@@ -522,7 +524,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
   };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   auto step = [&](const Pos& c, const u32x4 (&a)[CH], const u32x4 (&b)[CH]) {
-    const int skip = c.sb - max(0, min(c.sb, ns - CH));
+    const int skip = c.sb - min(c.sb, ns - CH);
     if (skip == 0) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) acc = Mma<T>::step(a[i], b[i], acc);
@@ -532,17 +534,18 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
         if (i >= skip) acc = Mma<T>::step(a[i], b[i], acc);
     }
     if (c.sb + CH < ns) return;
-    if (n < c.info.z - c.rg) {
-      const int s = s_rows[c.info.y + c.rg + n];
-      if (in_lds) {
-        *(f32x4*)&s_y[s][g * 4] = acc;
-      } else {
-        put_shared(y_rows, ((uint32_t)s * p.H + h0 + g * 4) * 4, acc);
-      }
-    }
+    // lane (n, g) holds rows 4g .. 4g+3 of column n: the block of piece f starts
+    // 16 (C/4) + C = 5C lanes after that of piece f - 1
+    f32x4 y = acc;
+    for (int f = 1; f < parts; ++f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] += __shfl(acc[i], lane + 5 * C * f, 64);
+    if (n < C && 4 * g < C && n < c.info.z - c.rg)
+      *(f32x4*)&s_y[s_rows[c.info.y + c.rg + n] * C + 4 * g] = y;
     acc = f32x4{0.f, 0.f, 0.f, 0.f};
   };
   Pos c{};
+  c.q = wid;
   start(c);
   if (c.more) {
     u32x4 a0[CH], b0[CH], a1[CH], b1[CH];
@@ -561,33 +564,21 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p) {
       if (!c.more) break;
     }
   }
-  if (in_lds) __syncthreads();
-  else if (!last_to_arrive(&p.arrived[hs], share, &box)) return;
-  const int h = tid & 15;
-  for (int t = tid >> 4; t < p.T; t += 4 * kWaves) {
+  __syncthreads();
+  for (int v = tid; v < p.T * C; v += 64 * kWaves) {
+    const int t = v / C, h = v % C;
     float o = 0.f;
-    for (int k0 = 0; k0 < p.K; k0 += 8) {
-      float y[8], w[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int s = t * p.K + min(k0 + k, p.K - 1);
-        const bool real = k0 + k < p.K && (s_real[s >> 6] >> (s & 63) & 1);
-        w[k] = real ? s_w[s] : 0.f;
-        y[k] = 0.f;
-        if (real) y[k] = in_lds ? s_y[s][h] : get_shared(y_rows, ((uint32_t)s * p.H + h0 + h) * 4);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) o = fmaf(w[k], y[k], o);
-    }
+    for (int s = t * p.K; s < (t + 1) * p.K; ++s)
+      if (s_real[s] >= 0) o = fmaf(s_w[s], s_y[s * C + h], o);
     ((T*)p.out)[(int64_t)t * p.H + h0 + h] = (T)o;
   }
 }
 
 // ------------------------------------------------------------------- host
 struct FewLayout {
-  size_t logits, w, hdr, arrived, list, rows, real, act, y, bytes;
+  size_t logits, w, hdr, list, rows, real, act, bytes;
 };
-FewLayout few_layout(int T, int E, int K, int H, int I, int elem) {
+FewLayout few_layout(int T, int E, int K, int I, int elem) {
   const size_t S = (size_t)T * K;
   FewLayout l{};
   size_t at = 0;
@@ -597,14 +588,12 @@ FewLayout few_layout(int T, int E, int K, int H, int I, int elem) {
     return o;
   };
   l.hdr = take(256);
-  l.arrived = take((size_t)(H / 16) * 4);
   l.w = take(S * 4);
   l.rows = take(S * 4);
   l.real = take(S * 4);
   l.list = take(S * 16);
   l.logits = take((size_t)T * E * 4);
   l.act = take(S * I * elem);
-  l.y = take(S * H * 4);
   l.bytes = at;
   return l;
 }
@@ -626,7 +615,7 @@ int few_check(int64_t T, int K, int E, int H, int I, int dtype, const char* who)
 }
 
 template <typename T>
-void few_launch(FewArgs& p, hipStream_t st) {
+hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   const int S = p.T * p.K, slots = S < p.E ? S : p.E;
   if (p.wr) few_logits_kernel<T><<<dim3((p.E + 15) / 16, (p.T + 15) / 16), 64 * kWaves, 0, st>>>(p);
   const int nv = p.wr ? (p.E + 63) / 64 : 1;
@@ -638,38 +627,56 @@ void few_launch(FewArgs& p, hipStream_t st) {
   else if (nv <= 16) few_plan_kernel<16><<<nr, 64 * kPlanWaves, 0, st>>>(p);
   else if (nv <= 32) few_plan_kernel<32><<<nr, 64 * kPlanWaves, 0, st>>>(p);
   else few_plan_kernel<64><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  few_gate_up_kernel<T, 8><<<slots * (p.I / 16), 64 * kWaves, 0, st>>>(p);
-  const int nh = p.H / 16;
-  int share = kDownGrid / nh;
-  const int most = (slots + kWaves - 1) / kWaves;
-  if (share > most) share = most;
-  if (share < 1) share = 1;
-  // a chunk no longer than the contraction: weights past an expert's rows are not read
-  const int ns = p.I / Mma<T>::kStep;
-  if (ns >= 8) few_down_kernel<T, 8><<<nh * share, 64 * kWaves, 0, st>>>(p);
-  else if (ns >= 4) few_down_kernel<T, 4><<<nh * share, 64 * kWaves, 0, st>>>(p);
-  else few_down_kernel<T, 2><<<nh * share, 64 * kWaves, 0, st>>>(p);
+  few_gate_up_kernel<T, 8><<<slots * (p.I / 8), 64 * kWaves, 0, st>>>(p);
+  // column slices of 16 / parts: about one for every CU
+  int parts = p.H / 16 >= 256 ? 1 : p.H / 8 >= 256 ? 2 : 4;
+  const int steps = p.I / Mma<T>::kStep;
+  while (steps % parts) parts /= 2;
+  const int ns = steps / parts;
+  const int lds = S * (16 + 64 / parts + 12);
+  // the chunk of the fewest rounds and steps read twice; never more steps than
+  // there are, as a step past the end is another row's or nobody's
+  int ch = 1;
+  const auto cost = [&](int c) { return (ns + c - 1) / c * (c + 2); };
+  for (int c : {2, 4, 6, 8})
+    if (c <= ns && cost(c) <= cost(ch)) ch = c;
+  auto down = [&](auto c) -> hipError_t {
+    static std::atomic<int> done[64];
+    constexpr int CH = decltype(c)::value;
+    const void* f = (const void*)few_down_kernel<T, CH>;
+    if (lds > 65536) {
+      const hipError_t err = set_dynamic_lds_once(done, f, kMaxLds);
+      if (err != hipSuccess) return err;
+    }
+    few_down_kernel<T, CH><<<p.H * parts / 16, 64 * kWaves, lds, st>>>(p, parts);
+    return hipSuccess;
+  };
+  if (ch == 8) return down(std::integral_constant<int, 8>{});
+  if (ch == 6) return down(std::integral_constant<int, 6>{});
+  if (ch == 4) return down(std::integral_constant<int, 4>{});
+  if (ch == 2) return down(std::integral_constant<int, 2>{});
+  return down(std::integral_constant<int, 1>{});
 }
 
 int few_run(FewArgs& p, int dtype, void* workspace, size_t workspace_bytes, hipStream_t st,
             const char* who) {
-  const FewLayout l = few_layout(p.T, p.E, p.K, p.H, p.I, dtype == MOE_DTYPE_BF16 ? 2 : 4);
+  const FewLayout l = few_layout(p.T, p.E, p.K, p.I, dtype == MOE_DTYPE_BF16 ? 2 : 4);
   MOE_REQUIRE(workspace && workspace_bytes >= l.bytes, MOE_ERR_WORKSPACE,
               "%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, l.bytes);
   MOE_REQUIRE(al16(p.x) && al16(p.wr) && al16(p.w1) && al16(p.w2) && al16(workspace),
               MOE_ERR_ALIGN, "%s: pointers must be 16-byte aligned", who);
   char* ws = (char*)workspace;
   p.hdr = (int*)(ws + l.hdr);
-  p.arrived = (int*)(ws + l.arrived);
   p.w = (float*)(ws + l.w);
   p.rows = (int*)(ws + l.rows);
   p.real = (int*)(ws + l.real);
   p.list = (int4*)(ws + l.list);
   p.logits = (float*)(ws + l.logits);
   p.act = ws + l.act;
-  p.y = (float*)(ws + l.y);
-  if (dtype == MOE_DTYPE_BF16) few_launch<bf16>(p, st);
-  else few_launch<float>(p, st);
+  const hipError_t err =
+      dtype == MOE_DTYPE_BF16 ? few_launch<bf16>(p, st) : few_launch<float>(p, st);
+  MOE_REQUIRE(err == hipSuccess, MOE_ERR_HIP, "%s: HIP error %d (%s)", who, (int)err,
+              hipGetErrorString(err));
   return check_launch(who);
 }
 
@@ -680,7 +687,7 @@ using namespace moe;
 
 extern "C" size_t moe_amd_few_workspace_size(int64_t T, int E, int K, int H, int I, int dtype) {
   if (few_check(T, K, E, H, I, dtype, "few_workspace_size") != MOE_OK) return 0;
-  return few_layout((int)T, E, K, H, I, dtype == MOE_DTYPE_BF16 ? 2 : 4).bytes;
+  return few_layout((int)T, E, K, I, dtype == MOE_DTYPE_BF16 ? 2 : 4).bytes;
 }
 
 extern "C" int moe_amd_experts_few(const void* hidden_states, const int64_t* topk_index,
