@@ -100,11 +100,6 @@ template <typename T> __device__ __forceinline__ float few_round(float v) {
   return v;
 }
 
-// The counters that workgroups of later launches finish by.
-__device__ __forceinline__ void clear_counters(const FewArgs& p) {
-  if (threadIdx.x == 0) p.hdr[1] = 0;
-}
-
 // What one workgroup leaves for another of the same launch: written through to
 // and read from the memory that all XCDs share, so that no cache has to be
 // written back or invalidated.  A workgroup counts itself as arrived once its
@@ -126,7 +121,7 @@ __device__ __forceinline__ bool last_to_arrive(int* counter, int of, int* box) {
 
 // ---------------------------------------------------------------- logits
 // Workgroup: 16 experts and 16 tokens; the eight waves split H.  The first one
-// clears the counters of the launches behind it.
+// clears the counter that the routing workgroups finish by.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
   __shared__ f32x4 red[kWaves][64];
@@ -154,7 +149,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
   };
   chunks<8>(s0, s1, chunk);
   red[wid][lane] = acc;
-  if (blockIdx.x == 0 && blockIdx.y == 0) clear_counters(p);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.hdr[1] = 0;
   __syncthreads();
   if (threadIdx.x < 256) {
     const int e = threadIdx.x & 15, t = threadIdx.x >> 4;
@@ -293,101 +288,70 @@ __device__ void route_token(const FewArgs& p, const float* logits, int lane, flo
   wk = dsk_weight(wk, ssum, p.renorm, p.scaling, 0);
 }
 
+// Routes token t on one wave and leaves its entries for later launches.
+template <int NV>
+__device__ __forceinline__ void route_and_store(const FewArgs& p, int t, int lane, int& ek) {
+  float wk;
+  route_token<NV>(p, p.logits + (int64_t)t * p.E, lane, wk, ek);
+  if (lane < p.K) {
+    const int s = t * p.K + lane;
+    put_shared(&p.real[s], ek);
+    p.w[s] = wk;
+    if (p.out_w) p.out_w[s] = wk;
+    if (p.out_idx) p.out_idx[s] = ek;
+  }
+}
+
 // The tokens' top-K, one token a wave; the last workgroup to finish lists the
 // active experts and their rows.  With the routing given there is one
-// workgroup, which lists.  An entry's place among its expert's rows: a wave's
-// 64 entries find their peers by one readlane per entry, then the waves add
-// their counts to the expert's in LDS one after the other.
+// workgroup, which lists.  Places in the list and among an expert's rows are
+// taken with LDS atomics: their order may differ from call to call, which no
+// result depends on (rows are computed apart, and combined by their number).
 template <int NV>
 __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
-  __shared__ int ids[kFewRows];
   __shared__ int count[kFewExperts];   // rows of an expert, then its first row
-  __shared__ int2 wsum[kPlanWaves];
-  __shared__ int box;
+  __shared__ int ids[kFewRows];
+  __shared__ int total, box;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int S = p.T * p.K;
+  for (int i = tid; i < p.E; i += blockDim.x) count[i] = 0;
+  if (tid == 0) total = 0;
+  int e = -1;
   if (p.wr) {
     const int t = blockIdx.x * kPlanWaves + wid;
     const bool one = gridDim.x == 1;
     if (t < p.T) {
-      float wk;
       int ek;
-      route_token<NV>(p, p.logits + (int64_t)t * p.E, lane, wk, ek);
-      if (lane < p.K) {
-        const int s = t * p.K + lane;
-        if (one) ids[s] = ek;
-        put_shared(&p.real[s], ek);
-        p.w[s] = wk;
-        if (p.out_w) p.out_w[s] = wk;
-        if (p.out_idx) p.out_idx[s] = ek;
-      }
+      route_and_store<NV>(p, t, lane, ek);
+      if (one && lane < p.K) ids[t * p.K + lane] = ek;
     }
-    if (!one) {
-      if (!last_to_arrive(&p.hdr[1], gridDim.x, &box)) return;
-      if (tid < S) ids[tid] = get_shared(&p.real[tid]);
-    }
+    if (!one && !last_to_arrive(&p.hdr[1], gridDim.x, &box)) return;
+    __syncthreads();
+    if (tid < S) e = one ? ids[tid] : get_shared(&p.real[tid]);
   } else {
     if (tid < S) {
-      const int64_t e = p.ids[tid];
-      ids[tid] = e >= 0 && e < p.E ? (int)e : -1;
-      p.real[tid] = ids[tid];
+      const int64_t id = p.ids[tid];
+      if (id >= 0 && id < p.E) e = (int)id;
+      p.real[tid] = e;
       p.w[tid] = p.weights_bf16 ? bf2f(((const bf16*)p.weights)[tid])
                                 : ((const float*)p.weights)[tid];
     }
-    clear_counters(p);
-  }
-  for (int i = tid; i < p.E; i += 64 * kPlanWaves) count[i] = 0;
-  __syncthreads();
-  const int e = tid < S ? ids[tid] : -1;
-  // peers: the entries of this wave with the same expert
-  int before = 0, peers = 0;
-  const int nw = (S + 63) >> 6;
-  if (wid < nw) {
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) {
-      const bool same = __builtin_amdgcn_readlane(e, i) == e;
-      peers += same;
-      before += same && i < lane;
-    }
-  }
-  int rank = before;
-  for (int w = 0; w < nw; ++w) {
-    if (wid == w && e >= 0) {
-      rank += count[e];
-      __builtin_amdgcn_wave_barrier();
-      if (before == 0) count[e] += peers;
-    }
     __syncthreads();
   }
+  const int rank = e >= 0 ? atomicAdd(&count[e], 1) : 0;
+  __syncthreads();
   const bool lead = e >= 0 && rank == 0;
   const int cnt = lead ? count[e] : 0;
-  // exclusive prefixes over the leaders: their number and their rows
-  int2 inc = make_int2(lead, cnt);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int a = __shfl_up(inc.x, o, 64), b = __shfl_up(inc.y, o, 64);
-    if (lane >= o) {
-      inc.x += a;
-      inc.y += b;
-    }
-  }
-  if (lane == 63) wsum[wid] = inc;
   __syncthreads();
-  int2 base = make_int2(0, 0), all = make_int2(0, 0);
-  for (int w = 0; w < nw; ++w) {
-    if (w == wid) base = all;
-    all.x += wsum[w].x;
-    all.y += wsum[w].y;
-  }
   if (lead) {
-    const int r0 = base.y + inc.y - cnt;
-    p.list[base.x + inc.x - 1] = make_int4(e, r0, cnt, 0);
-    count[e] = r0;
+    const int at = atomicAdd(&total, 1 << 16 | cnt);  // experts and rows before it
+    p.list[at >> 16] = make_int4(e, at & 0xffff, cnt, 0);
+    count[e] = at & 0xffff;
   }
   __syncthreads();
   if (e >= 0) p.rows[count[e] + rank] = tid;
-  if (tid == 0) p.hdr[0] = all.x;
+  if (tid == 0) p.hdr[0] = total >> 16;
 }
 
 // ------------------------------------------------------- gate/up + SwiGLU
@@ -397,16 +361,40 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 // L2.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
 // dealt to all of them in small pieces: with 16 features a workgroup one token
 // (K = 8, I = 768) has 384 for 256 CUs.
-template <typename T, int CH>
+// NV > 0: one token, routed by every workgroup for itself; slot k is its k-th
+// expert, and the first workgroup leaves the plan for the down kernel.
+template <typename T, int CH, int NV>
 __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   __shared__ f32x4 red[kWaves][64];
+  __shared__ int s_e;
   const int nsl = p.I / 8;
   const int slot = blockIdx.x / nsl, f0 = (blockIdx.x % nsl) * 8;
-  const int nact = p.hdr[0];
-  const int4 info = p.list[slot];  // a slot past the active experts holds anything
-  if (slot >= nact) return;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int4 info;
+  if constexpr (NV > 0) {
+    if (wid == 0) {
+      int ek;
+      if (blockIdx.x == 0) {
+        route_and_store<NV>(p, 0, lane, ek);
+        if (lane < p.K) {
+          p.list[lane] = make_int4(ek, lane, 1, 0);
+          p.rows[lane] = lane;
+        }
+        if (lane == 0) p.hdr[0] = p.K;
+      } else {
+        float wk;
+        route_token<NV>(p, p.logits, lane, wk, ek);
+      }
+      if (lane == slot) s_e = ek;
+    }
+    __syncthreads();
+    info = make_int4(__builtin_amdgcn_readfirstlane(s_e), 0, 1, 0);
+  } else {
+    const int nact = p.hdr[0];
+    info = p.list[slot];  // a slot past the active experts holds anything
+    if (slot >= nact) return;
+  }
   const int ns = p.H / Mma<T>::kStep;
   const int s0 = wid * ns / kWaves, s1 = (wid + 1) * ns / kWaves;
   const int64_t ld = (int64_t)p.H * sizeof(T);
@@ -414,8 +402,8 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
                   ((int64_t)info.x * 2 * p.I + f0 + (n & 7) + (n >> 3) * p.I) * ld + g * 16;
   for (int rg = 0; rg < info.z; rg += 16) {
     const int left = info.z - rg;
-    const uint32_t xo =
-        (uint32_t)(p.rows[info.y + rg + min(n, left - 1)] / p.K) * (uint32_t)ld + g * 16;
+    const int token = NV > 0 ? 0 : p.rows[info.y + rg + min(n, left - 1)] / p.K;
+    const uint32_t xo = (uint32_t)token * (uint32_t)ld + g * 16;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     chunks<CH>(s0, s1, [&](auto ch, int s) {
       constexpr int C = decltype(ch)::value;
@@ -440,7 +428,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
           gs += red[q][l][f & 3];
           us += red[q][l + 32][f & 3];
         }
-        const int s = p.rows[info.y + rg + r];
+        const int s = NV > 0 ? slot : p.rows[info.y + rg + r];
         ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
       }
     }
@@ -448,8 +436,10 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
 }
 
 // --------------------------------------------------------- down + combine
-// Workgroup: C = 16 / parts columns of the output and every active expert, a
-// wave for each of them in turn.  `parts` makes the column slices about as many
+// Workgroup: C = 16 / parts columns of the output and every active expert; a
+// wave takes the next one when it is done with its own (the oldest waves get
+// their loads first: with a fixed share each, they end after half of the time
+// and the rest finishes with too few loads in flight).  `parts` makes the column slices about as many
 // as CUs: the A operand's 16 rows are C columns' weights for each of `parts`
 // pieces of the contraction, B's 16 columns C of the expert's rows for each of
 // them, and the blocks of the product where the pieces match are added.
@@ -465,6 +455,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
   int* s_rows = (int*)(s_y + S * C);
   float* s_w = (float*)(s_rows + S);
   int* s_real = (int*)(s_w + S);
+  __shared__ int s_next;
   const int h0 = blockIdx.x * C;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -475,6 +466,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
     s_w[i] = p.w[i];
     s_real[i] = p.real[i];
   }
+  if (tid == 0) s_next = kWaves;
   __syncthreads();
   const int ns = p.I / Mma<T>::kStep / parts;
   const int64_t ld = (int64_t)p.I * sizeof(T);
@@ -506,7 +498,9 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
     c.rg += C;
     if (c.rg >= c.info.z) {
       c.rg = 0;
-      c.q += kWaves;
+      int q = 0;
+      if (lane == 0) q = atomicAdd(&s_next, 1);
+      c.q = __builtin_amdgcn_readfirstlane(q);
       start(c);
     }
     if (c.more) rows(c);
@@ -568,8 +562,19 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
   for (int v = tid; v < p.T * C; v += 64 * kWaves) {
     const int t = v / C, h = v % C;
     float o = 0.f;
-    for (int s = t * p.K; s < (t + 1) * p.K; ++s)
-      if (s_real[s] >= 0) o = fmaf(s_w[s], s_y[s * C + h], o);
+    for (int k0 = 0; k0 < p.K; k0 += 8) {
+      float w[8], y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int s = t * p.K + min(k0 + k, p.K - 1);
+        const bool real = k0 + k < p.K && s_real[s] >= 0;
+        w[k] = s_w[s];
+        y[k] = s_y[s * C + h];
+        if (!real) w[k] = y[k] = 0.f;  // padding's y was never written
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o = fmaf(w[k], y[k], o);
+    }
     ((T*)p.out)[(int64_t)t * p.H + h0 + h] = (T)o;
   }
 }
@@ -618,16 +623,28 @@ template <typename T>
 hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   const int S = p.T * p.K, slots = S < p.E ? S : p.E;
   if (p.wr) few_logits_kernel<T><<<dim3((p.E + 15) / 16, (p.T + 15) / 16), 64 * kWaves, 0, st>>>(p);
+  const bool single = p.wr && p.T == 1;
+  const auto plan = [&](auto nv) {
+    constexpr int NV = decltype(nv)::value;
+    if (single) {
+      few_gate_up_kernel<T, 8, NV><<<slots * (p.I / 8), 64 * kWaves, 0, st>>>(p);
+      return;
+    }
+    // a wave for every 64 entries, and for each of the tokens that it routes
+    const int nr = p.wr ? (p.T + kPlanWaves - 1) / kPlanWaves : 1;
+    const int tokens = p.wr ? (p.T < kPlanWaves ? p.T : kPlanWaves) : 1;
+    const int entries = (S + 63) / 64;
+    few_plan_kernel<NV><<<nr, 64 * (tokens > entries ? tokens : entries), 0, st>>>(p);
+    few_gate_up_kernel<T, 8, 0><<<slots * (p.I / 8), 64 * kWaves, 0, st>>>(p);
+  };
   const int nv = p.wr ? (p.E + 63) / 64 : 1;
-  const int nr = p.wr ? (p.T + kPlanWaves - 1) / kPlanWaves : 1;
-  if (nv <= 1) few_plan_kernel<1><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 2) few_plan_kernel<2><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 4) few_plan_kernel<4><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 8) few_plan_kernel<8><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 16) few_plan_kernel<16><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  else if (nv <= 32) few_plan_kernel<32><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  else few_plan_kernel<64><<<nr, 64 * kPlanWaves, 0, st>>>(p);
-  few_gate_up_kernel<T, 8><<<slots * (p.I / 8), 64 * kWaves, 0, st>>>(p);
+  if (nv <= 1) plan(std::integral_constant<int, 1>{});
+  else if (nv <= 2) plan(std::integral_constant<int, 2>{});
+  else if (nv <= 4) plan(std::integral_constant<int, 4>{});
+  else if (nv <= 8) plan(std::integral_constant<int, 8>{});
+  else if (nv <= 16) plan(std::integral_constant<int, 16>{});
+  else if (nv <= 32) plan(std::integral_constant<int, 32>{});
+  else plan(std::integral_constant<int, 64>{});
   // column slices of 16 / parts: about one for every CU
   int parts = p.H / 16 >= 256 ? 1 : p.H / 8 >= 256 ? 2 : 4;
   const int steps = p.I / Mma<T>::kStep;
