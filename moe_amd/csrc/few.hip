@@ -172,87 +172,131 @@ __device__ __forceinline__ float value_of(uint32_t key) {
   return key_value((uint64_t)key << 32);
 }
 
-// Takes the largest key (entry j*64 + lane in slot j) out and returns it and
-// its entry, the lowest of equal ones: the value by DPP, its holder by ballots.
-// (64-bit keys that hold the index too need four times the instructions.)
-template <int NV>
-__device__ __forceinline__ uint32_t take_largest(uint32_t (&key)[NV], int lane, int& entry) {
-  uint32_t m = key[0];
+// The waves that route one token: one, which holds entry j*64 + lane of its
+// experts in slot j, or (BLOCK) all of a workgroup's kPlanWaves, wave w holding
+// the experts from w * chunk on.  They share the largest keys of their parts
+// through LDS, in two places by turns, so that a round needs one barrier.
+struct RouteShared {
+  uint32_t key[2][kPlanWaves];
+  float part[2][kPlanWaves];
+  int entry[64];
+};
+template <int NV, bool BLOCK>
+struct Router {
+  RouteShared* sh;
+  int lane, wid, base, count, turn = 0;
+
+  __device__ __forceinline__ Router(RouteShared* sh_, int E, int wid_, int lane_)
+      : sh(sh_), lane(lane_), wid(wid_) {
+    const int chunk = BLOCK ? (E + kPlanWaves - 1) / kPlanWaves : E;
+    base = BLOCK ? wid * chunk : 0;
+    count = min(chunk, E - base);  // none, or fewer, of a last wave's
+  }
+  __device__ __forceinline__ bool has(int j) const { return j * 64 + lane < count; }
+  __device__ __forceinline__ int expert(int j) const { return base + j * 64 + lane; }
+
+  // Over all entries: whether any, maximum, sum.
+  __device__ __forceinline__ bool any(bool v) {
+    if constexpr (BLOCK) return all_max(v ? 1.f : 0.f) > 0.f;
+    return __ballot(v) != 0;
+  }
+  __device__ __forceinline__ float all_max(float v) {
+    v = group_max<16>(v);
+    v = fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
+    if constexpr (BLOCK) v = group_max<16>(exchange(v));
+    return v;
+  }
+  __device__ __forceinline__ float all_sum(float v) {
+    v = group_sum<16>(v);
+    v = (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+    if constexpr (BLOCK) v = group_sum<16>(exchange(v));
+    return v;
+  }
+  static __device__ __forceinline__ float lane_of(float v, int l) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l));
+  }
+  __device__ __forceinline__ float exchange(float v) {  // wave (lane % 16)'s v
+    float* at = sh->part[turn ^= 1];
+    if (lane == 0) at[wid] = v;
+    __syncthreads();
+    return at[lane & 15];
+  }
+
+  // Takes the largest key out and returns it: the value by DPP, its holder (of
+  // equal ones the lowest expert) by ballots.  (64-bit keys that hold the index
+  // too need four times the instructions.)  `entry`, in its holder's wave alone
+  // where BLOCK: the expert, else negative.
+  __device__ __forceinline__ uint32_t take(uint32_t (&key)[NV], int& entry) {
+    uint32_t m = key[0];
 #pragma unroll
-  for (int j = 1; j < NV; ++j) m = max(m, key[j]);
-  m = group_max_key<16>(m);
-  m = max(max((uint32_t)__builtin_amdgcn_readlane(m, 0), (uint32_t)__builtin_amdgcn_readlane(m, 16)),
-          max((uint32_t)__builtin_amdgcn_readlane(m, 32), (uint32_t)__builtin_amdgcn_readlane(m, 48)));
-  entry = 0;
-  bool found = false;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const uint64_t here = __ballot(key[j] == m);
-    if (!found && here) {
-      const int l = __builtin_ctzll(here);
-      entry = j * 64 + l;
-      if (lane == l) key[j] = 0;
-      found = true;
+    for (int j = 1; j < NV; ++j) m = max(m, key[j]);
+    m = group_max_key<16>(m);
+    m = max(max((uint32_t)__builtin_amdgcn_readlane(m, 0),
+                (uint32_t)__builtin_amdgcn_readlane(m, 16)),
+            max((uint32_t)__builtin_amdgcn_readlane(m, 32),
+                (uint32_t)__builtin_amdgcn_readlane(m, 48)));
+    entry = -1;
+    if constexpr (BLOCK) {
+      uint32_t* at = sh->key[turn ^= 1];
+      if (lane == 0) at[wid] = m;
+      __syncthreads();
+      const uint32_t other = at[lane & 15];
+      m = __builtin_amdgcn_readfirstlane(group_max_key<16>(other));
+      if (__builtin_ctzll(__ballot(other == m)) != wid) return m;
     }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const uint64_t here = __ballot(key[j] == m);
+      if (entry < 0 && here) {
+        const int l = __builtin_ctzll(here);
+        entry = base + j * 64 + l;
+        if (lane == l) key[j] = 0;
+      }
+    }
+    return m;
   }
-  return m;
-}
+};
 
-// The K largest in order: lane k < K gets the k-th entry and its key.
-template <int NV>
-__device__ __forceinline__ void take_topk(uint32_t (&key)[NV], int lane, int K, int& my_e,
-                                          uint32_t& my_key) {
-  my_e = 0;
-  my_key = 0;
-  for (int k = 0; k < K; ++k) {
-    int e;
-    const uint32_t m = take_largest<NV>(key, lane, e);
-    my_e = lane == k ? e : my_e;
-    my_key = lane == k ? m : my_key;
-  }
-}
-
-// One token on one wave: lane k < K gets its k-th expert and weight.  The
-// selections and the arithmetic are those of the router kernels.
-template <int NV>
-__device__ void route_token(const FewArgs& p, const float* logits, int lane, float& wk, int& ek) {
+// One token: lane k < K gets its k-th expert and weight (of every wave that
+// routes it).  The selections and the arithmetic are those of the router
+// kernels.
+template <int NV, bool BLOCK>
+__device__ __forceinline__ void route_token(const FewArgs& p, const float* logits,
+                                            RouteShared* sh, int wid, int lane, float& wk,
+                                            int& ek) {
   const int E = p.E, K = p.K;
-  uint32_t key[NV], kk;
+  Router<NV, BLOCK> r(sh, E, wid, lane);
+  uint32_t key[NV];
+  float m = 0.f, s = 0.f;
   if (!p.sigmoid) {
     float v[NV];
     bool nan_here = false;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int e = j * 64 + lane;
-      v[j] = e < E ? logits[e] + (p.offset ? p.offset[e] : 0.f) : -INFINITY;
+      v[j] = r.has(j) ? logits[r.expert(j)] + (p.offset ? p.offset[r.expert(j)] : 0.f) : -INFINITY;
       nan_here |= v[j] != v[j];
     }
-    if (__ballot(nan_here)) {  // every prob of the row is NaN: they rank by index
+    if (r.any(nan_here)) {  // every prob of the row is NaN: they rank by index
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (j * 64 + lane < E) v[j] = __builtin_nanf("");
+        if (r.has(j)) v[j] = __builtin_nanf("");
     }
-    float m = -INFINITY;
+    m = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; ++j) m = fmaxf(m, v[j]);
-    m = wave_max(m);
-    float s = 0.f;
+    m = r.all_max(m);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int e = j * 64 + lane;
-      s += e < E ? expf(v[j] - m) : 0.f;
-      key[j] = e < E ? value_key(v[j]) : 0u;
+      s += r.has(j) ? expf(v[j] - m) : 0.f;
+      key[j] = r.has(j) ? value_key(v[j]) : 0u;
     }
-    s = wave_sum(s);
-    take_topk<NV>(key, lane, K, ek, kk);
-    wk = lane < K ? expf(value_of(kk) - m) / s : 0.f;
-    if (p.renorm) wk = wk / wave_sum(wk);
-    return;
-  }
+    s = r.all_sum(s);
+  } else {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int e = j * 64 + lane;
-    key[j] = e < E ? value_key(sigmoidf_(logits[e]) + (p.offset ? p.offset[e] : 0.f)) : 0u;
+    for (int j = 0; j < NV; ++j)
+      key[j] = r.has(j) ? value_key(sigmoidf_(logits[r.expert(j)]) +
+                                    (p.offset ? p.offset[r.expert(j)] : 0.f))
+                        : 0u;
   }
   if (p.ngroups > 0) {
     // groups scored by the sum of their K / gtopk best biased scores, gtopk kept
@@ -261,54 +305,71 @@ __device__ void route_token(const FewArgs& p, const float* logits, int lane, flo
     for (int q = 0; q < p.ngroups; ++q) {
       uint32_t gk[NV];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) gk[j] = (j * 64 + lane) / eg == q ? key[j] : 0u;
+      for (int j = 0; j < NV; ++j) gk[j] = r.expert(j) / eg == q ? key[j] : 0u;
       float acc = 0.f;
       int e;
-      for (int r = 0; r < per; ++r) acc += value_of(take_largest<NV>(gk, lane, e));
+      for (int i = 0; i < per; ++i) acc += value_of(r.take(gk, e));
       gv = lane == q ? acc : gv;
     }
     uint32_t gkey[1] = {lane < p.ngroups ? value_key(gv) : 0u};
+    Router<1, false> groups(sh, 64, 0, lane);  // every wave for itself
     uint64_t keep = 0;
     for (int q = 0; q < p.gtopk; ++q) {
       int e;
-      take_largest<1>(gkey, lane, e);
+      groups.take(gkey, e);
       keep |= 1ull << e;
     }
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int e = j * 64 + lane;
-      if (e < E && !((keep >> (e / eg)) & 1ull)) key[j] = 0u;
+    for (int j = 0; j < NV; ++j)
+      if (r.has(j) && !((keep >> (r.expert(j) / eg)) & 1ull)) key[j] = 0u;
+  }
+  uint32_t kk = 0;
+  ek = 0;
+  for (int k = 0; k < K; ++k) {
+    int e;
+    const uint32_t top = r.take(key, e);
+    kk = lane == k ? top : kk;
+    if constexpr (BLOCK) {
+      if (e >= 0 && lane == 0) sh->entry[k] = e;
+    } else {
+      ek = lane == k ? e : ek;
     }
   }
-  take_topk<NV>(key, lane, K, ek, kk);
-  wk = lane < K ? sigmoidf_(logits[ek]) : 0.f;
-  float ssum = 0.f;
-  if (p.renorm)
-    for (int k = 0; k < K; ++k) ssum += __shfl(wk, k, 64);
-  wk = dsk_weight(wk, ssum, p.renorm, p.scaling, 0);
-}
-
-// Routes token t on one wave and leaves its entries for later launches.
-template <int NV>
-__device__ __forceinline__ void route_and_store(const FewArgs& p, int t, int lane, int& ek) {
-  float wk;
-  route_token<NV>(p, p.logits + (int64_t)t * p.E, lane, wk, ek);
-  if (lane < p.K) {
-    const int s = t * p.K + lane;
-    put_shared(&p.real[s], ek);
-    p.w[s] = wk;
-    if (p.out_w) p.out_w[s] = wk;
-    if (p.out_idx) p.out_idx[s] = ek;
+  if constexpr (BLOCK) {
+    __syncthreads();
+    ek = lane < K ? sh->entry[lane] : 0;
+  }
+  if (!p.sigmoid) {
+    wk = lane < K ? expf(value_of(kk) - m) / s : 0.f;
+    if (p.renorm) wk = wk / group_sum<16>(wk);  // K <= 16: the other rows of lanes divide by 0
+  } else {
+    wk = lane < K ? sigmoidf_(logits[ek]) : 0.f;
+    float ssum = 0.f;
+    if (p.renorm)
+      for (int k = 0; k < K; ++k) ssum += __shfl(wk, k, 64);
+    wk = dsk_weight(wk, ssum, p.renorm, p.scaling, 0);
   }
 }
 
-// The tokens' top-K, one token a wave; the last workgroup to finish lists the
-// active experts and their rows.  With the routing given there is one
-// workgroup, which lists.  Places in the list and among an expert's rows are
-// taken with LDS atomics: their order may differ from call to call, which no
-// result depends on (rows are computed apart, and combined by their number).
-template <int NV>
+// Leaves token t's routing, held by lanes 0 .. K-1, for later launches.
+__device__ __forceinline__ void store_route(const FewArgs& p, int t, int lane, float wk, int ek) {
+  if (lane >= p.K) return;
+  const int s = t * p.K + lane;
+  put_shared(&p.real[s], ek);
+  p.w[s] = wk;
+  if (p.out_w) p.out_w[s] = wk;
+  if (p.out_idx) p.out_idx[s] = ek;
+}
+
+// The tokens' top-K, one token a wave or (BLOCK) a workgroup; the last
+// workgroup to finish lists the active experts and their rows.  With the
+// routing given there is one workgroup, which lists.  Places in the list and
+// among an expert's rows are taken with LDS atomics: their order may differ
+// from call to call, which no result depends on (rows are computed apart, and
+// combined by their number).
+template <int NV, bool BLOCK>
 __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
+  __shared__ RouteShared sh;
   __shared__ int count[kFewExperts];   // rows of an expert, then its first row
   __shared__ int ids[kFewRows];
   __shared__ int total, box;
@@ -319,12 +380,16 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
   if (tid == 0) total = 0;
   int e = -1;
   if (p.wr) {
-    const int t = blockIdx.x * kPlanWaves + wid;
+    const int t = BLOCK ? blockIdx.x : blockIdx.x * kPlanWaves + wid;
     const bool one = gridDim.x == 1;
-    if (t < p.T) {
+    if (t < p.T) {  // uniform over the workgroup where BLOCK
+      float wk;
       int ek;
-      route_and_store<NV>(p, t, lane, ek);
-      if (one && lane < p.K) ids[t * p.K + lane] = ek;
+      route_token<NV, BLOCK>(p, p.logits + (int64_t)t * p.E, &sh, wid, lane, wk, ek);
+      if (!BLOCK || wid == 0) {
+        store_route(p, t, lane, wk, ek);
+        if (one && lane < p.K) ids[t * p.K + lane] = ek;
+      }
     }
     if (!one && !last_to_arrive(&p.hdr[1], gridDim.x, &box)) return;
     __syncthreads();
@@ -374,19 +439,18 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   int4 info;
   if constexpr (NV > 0) {
     if (wid == 0) {
+      float wk;
       int ek;
+      route_token<NV, false>(p, p.logits, nullptr, 0, lane, wk, ek);
+      if (lane == slot) s_e = ek;
       if (blockIdx.x == 0) {
-        route_and_store<NV>(p, 0, lane, ek);
+        store_route(p, 0, lane, wk, ek);
         if (lane < p.K) {
           p.list[lane] = make_int4(ek, lane, 1, 0);
           p.rows[lane] = lane;
         }
         if (lane == 0) p.hdr[0] = p.K;
-      } else {
-        float wk;
-        route_token<NV>(p, p.logits, lane, wk, ek);
       }
-      if (lane == slot) s_e = ek;
     }
     __syncthreads();
     info = make_int4(__builtin_amdgcn_readfirstlane(s_e), 0, 1, 0);
@@ -623,28 +687,31 @@ template <typename T>
 hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   const int S = p.T * p.K, slots = S < p.E ? S : p.E;
   if (p.wr) few_logits_kernel<T><<<dim3((p.E + 15) / 16, (p.T + 15) / 16), 64 * kWaves, 0, st>>>(p);
-  const bool single = p.wr && p.T == 1;
+  // One wave routes a token of up to 256 experts, a workgroup one of more (with
+  // 28 entries a lane, one wave took 46 us for each of 64 tokens, E = 1792).
+  const bool wide = p.wr && p.E > 256;
+  const int threads = 64 * kWaves, gu_grid = slots * (p.I / 8);
   const auto plan = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
-    if (single) {
-      few_gate_up_kernel<T, 8, NV><<<slots * (p.I / 8), 64 * kWaves, 0, st>>>(p);
+    if (p.wr && p.T == 1 && !wide) {
+      few_gate_up_kernel<T, 8, NV><<<gu_grid, threads, 0, st>>>(p);
       return;
     }
-    // a wave for every 64 entries, and for each of the tokens that it routes
-    const int nr = p.wr ? (p.T + kPlanWaves - 1) / kPlanWaves : 1;
-    const int tokens = p.wr ? (p.T < kPlanWaves ? p.T : kPlanWaves) : 1;
-    const int entries = (S + 63) / 64;
-    few_plan_kernel<NV><<<nr, 64 * (tokens > entries ? tokens : entries), 0, st>>>(p);
-    few_gate_up_kernel<T, 8, 0><<<slots * (p.I / 8), 64 * kWaves, 0, st>>>(p);
+    if (wide) {
+      few_plan_kernel<NV, true><<<p.T, 64 * kPlanWaves, 0, st>>>(p);
+    } else {
+      // a wave for every 64 entries, and for each of the tokens that it routes
+      const int nr = p.wr ? (p.T + kPlanWaves - 1) / kPlanWaves : 1;
+      const int tokens = p.wr ? (p.T < kPlanWaves ? p.T : kPlanWaves) : 1;
+      const int entries = (S + 63) / 64;
+      few_plan_kernel<NV, false><<<nr, 64 * (tokens > entries ? tokens : entries), 0, st>>>(p);
+    }
+    few_gate_up_kernel<T, 8, 0><<<gu_grid, threads, 0, st>>>(p);
   };
-  const int nv = p.wr ? (p.E + 63) / 64 : 1;
-  if (nv <= 1) plan(std::integral_constant<int, 1>{});
-  else if (nv <= 2) plan(std::integral_constant<int, 2>{});
-  else if (nv <= 4) plan(std::integral_constant<int, 4>{});
-  else if (nv <= 8) plan(std::integral_constant<int, 8>{});
-  else if (nv <= 16) plan(std::integral_constant<int, 16>{});
-  else if (nv <= 32) plan(std::integral_constant<int, 32>{});
-  else plan(std::integral_constant<int, 64>{});
+  const int part = wide ? (p.E + kPlanWaves - 1) / kPlanWaves : p.wr ? p.E : 1;
+  if (part <= 64) plan(std::integral_constant<int, 1>{});
+  else if (part <= 128) plan(std::integral_constant<int, 2>{});
+  else plan(std::integral_constant<int, 4>{});
   // column slices of 16 / parts: about one for every CU
   int parts = p.H / 16 >= 256 ? 1 : p.H / 8 >= 256 ? 2 : 4;
   const int steps = p.I / Mma<T>::kStep;
