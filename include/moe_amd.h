@@ -395,6 +395,39 @@ int moe_amd_gather_backward_add(const void* d_xs, const int32_t* slot, const int
                                 const void* addend, int64_t T, int K, int E, int H, int dtype,
                                 void* d_x, void* stream);
 
+/* ----------------------------------------------- activations in 8 bits */
+
+/* For 64 consecutive values v of a row (its last block may be shorter) a power
+ * of two s and the integers q = rint(v / s), halves to even: s is the smallest
+ * power of two >= 2^-126 with max|v| <= 127 s.  What is restored, q * s, is
+ * exact in bf16 and fp32.  q int8 [rows, cols], scale [rows, ceil(cols / 64)]
+ * bytes: s's biased exponent, or 255 for a block with a value that is not
+ * finite, which is restored as NaN whole.  No counterpart in the reference. */
+int moe_amd_pack8(const void* x, int dtype, int64_t rows, int64_t cols, void* q, void* scale,
+                  void* stream);
+int moe_amd_unpack8(const void* q, const void* scale, int64_t rows, int64_t cols, void* x,
+                    int dtype, void* stream);
+
+/* moe_amd_gemm_gate_up_swiglu and moe_amd_gemm_down_backward_dx_fused with
+ * gate_up kept in 8 bits between them, packed and restored inside the two
+ * (bf16 only): the values of moe_amd_pack8 on the bf16 gate_up, with the bytes
+ * of eight gate features beside those of the same up features: gate_up_q
+ * [S][I/8][gate 8, up 8], gate_up_scale [S][I/64][gate, up], both 16-byte
+ * aligned.  Rows of sentinels are not written.  act_out is
+ * moe_amd_gemm_gate_up_swiglu's, and the backward's results are
+ * moe_amd_gemm_down_backward_dx_fused's on the restored gate_up, bit for bit. */
+int moe_amd_gemm_gate_up_swiglu_pack8(const void* hidden_states, const int32_t* row_src, int top_k,
+                                      const int32_t* offsets, const void* tile_plan,
+                                      const void* gate_up_proj, int64_t T, int64_t S, int E, int H,
+                                      int I, int dtype, void* gate_up_q, void* gate_up_scale,
+                                      void* act_out, void* stream);
+int moe_amd_gemm_down_backward_dx_fused_pack8(
+    const void* d_out, const int32_t* row_src, int top_k, const int32_t* offsets,
+    const void* tile_plan, const void* down_proj, const void* gate_up_q,
+    const void* gate_up_scale, const void* topk_weights, int weights_dtype, int64_t T, int64_t S,
+    int E, int H, int I, int dtype, void* d_gate_up, void* act_w, float* dw_partials,
+    void* stream);
+
 /* --------------------------------------------- the layer for a few tokens */
 
 /* The expert layer for up to MOE_FEW_MAX_TOKENS tokens, forward only: the

@@ -83,6 +83,13 @@ SIGNATURES: dict[str, tuple] = {
     "moe_amd_weight_grad_reduce": (_i, [_p, _i, _p, _p, _i64, _i, _i, _p, _i, _p]),
     "moe_amd_gather_backward": (_i, [_p, _p, _p, _i64, _i, _i, _i, _i, _p, _p]),
     "moe_amd_gather_backward_add": (_i, [_p, _p, _p, _p, _i64, _i, _i, _i, _i, _p, _p]),
+    "moe_amd_pack8": (_i, [_p, _i, _i64, _i64, _p, _p, _p]),
+    "moe_amd_unpack8": (_i, [_p, _p, _i64, _i64, _p, _i, _p]),
+    "moe_amd_gemm_gate_up_swiglu_pack8": (
+        _i, [_p, _p, _i, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p, _p, _p, _p]),
+    "moe_amd_gemm_down_backward_dx_fused_pack8": (
+        _i, [_p, _p, _i, _p, _p, _p, _p, _p, _p, _i, _i64, _i64, _i, _i, _i, _i, _p, _p, _p,
+             _p]),
     "moe_amd_few_workspace_size": (_sz, [_i64, _i, _i, _i, _i, _i]),
     "moe_amd_experts_few": (
         _i, [_p, _p, _p, _i, _p, _p, _i64, _i, _i, _i, _i, _i, _p, _sz, _p, _p]),

@@ -61,6 +61,7 @@
 
 #include "common.h"
 #include "gemm_f32.h"
+#include "pack8.h"
 #include "router_group.h"
 
 namespace moe {
@@ -138,6 +139,8 @@ struct GemmArgs {
   const int* xorder;
   const int* xnz;        // ... of which the first xnz[x] have rows
   int accumulate;        // G1DW/G2DWG: out[e] += dW[e] in place, experts without rows untouched
+  uint8_t* q8;           // PACK: gate_up in 8 bits [S][I/8][gate 8 | up 8] (G1F writes, G2DXF
+  uint8_t* q8_scale;     //   reads) and its scale bytes [S][I/64][gate, up]
 };
 
 // Eight bf16 pairs added as torch adds two bf16 tensors: in fp32, then
@@ -213,8 +216,11 @@ __device__ __forceinline__ float fast_sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
 }
 
-template <int MODE, int BR>
+// PACK: G1F saves gate_up packed to 8 bits (pack8.h), G2DXF reads it so; the
+// same tile, main loop and number of stores otherwise.
+template <int MODE, int BR, bool PACK = false>
 __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
+  static_assert(!PACK || MODE == G1F || MODE == G2DXF, "the GEMMs that hold gate_up");
   constexpr int NW = kWaves<BR>;                          // waves, as NW/2 rows x 2 columns
   constexpr int NTHR = NW * 64;
   constexpr bool TOKEN = MODE <= G1DX || MODE == G2DXF;   // rows = routed rows of one expert
@@ -1010,7 +1016,11 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
       const int nr = min(c.row_end - c.row0, BR);  // >= 1; the tile's own rows, as in setup()
       const int c8 = (ln & 15) * 8, rq = ln >> 4;
       const bool fok = fw + c8 < I;
-      const auto rgu = make_rsrc(p.a1 + (int64_t)c.row0 * I2, (uint32_t)nr * (uint32_t)I2 * 2);
+      const auto rgu = PACK ? make_rsrc(p.q8 + (int64_t)c.row0 * I2, (uint32_t)nr * (uint32_t)I2)
+                            : make_rsrc(p.a1 + (int64_t)c.row0 * I2,
+                                        (uint32_t)nr * (uint32_t)I2 * 2);
+      const auto rsc = make_rsrc(p.q8_scale + (int64_t)c.row0 * (I / 32),
+                                 PACK ? (uint32_t)nr * (uint32_t)(I / 32) : 0u);
       const auto rdg = make_rsrc(p.out + (int64_t)c.row0 * I2, (uint32_t)nr * (uint32_t)I2 * 2);
       const auto raw = make_rsrc(p.out2 + (int64_t)c.row0 * I, (uint32_t)nr * (uint32_t)I * 2);
       const int n_part = 2 * p.n_ct;
@@ -1035,11 +1045,21 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
       // (HBM latency: one iteration's arithmetic is ~1 k cycles)
       constexpr int PD = 8;
       const int nn = (VH ? c.nj : TJ) * NIT;
-      u32x4 gl[PD], ul[PD];
+      u32x4 gl[PD], ul[PACK ? 1 : PD];
+      uint32_t sl8[PACK ? PD : 1];  // PACK: the two scale bytes of the lane's block
       auto load = [&](int n) {
+        if constexpr (PACK) {
+          const int d = (n / NIT) * JR + (n % NIT) * 4;
+          const uint32_t f = (uint32_t)(fw + c8), r = (uint32_t)(r0l + d);
+          gl[n % PD] = __builtin_amdgcn_raw_buffer_load_b128(
+              rgu, d < lim ? r * (uint32_t)I2 + f * 2 : kOOB, 0, 2);
+          sl8[n % PD] = __builtin_amdgcn_raw_buffer_load_b16(
+              rsc, d < lim ? r * (uint32_t)(I / 32) + (f >> 6) * 2 : kOOB, 0, 0);
+          return;
+        }
         const uint32_t o = og(n / NIT, n % NIT);
         gl[n % PD] = __builtin_amdgcn_raw_buffer_load_b128(rgu, o, 0, 2);
-        ul[n % PD] = __builtin_amdgcn_raw_buffer_load_b128(rgu, o + (uint32_t)I * 2, 0, 2);  // kOOB stays out
+        ul[PACK ? 0 : n % PD] = __builtin_amdgcn_raw_buffer_load_b128(rgu, o + (uint32_t)I * 2, 0, 2);  // kOOB stays out
       };
 #pragma unroll
       for (int n = 0; n < PD; ++n) load(n);
@@ -1077,11 +1097,18 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
               reg + r * 512 + (((lc + 1) ^ r) << 4));
           const float wgt = __uint_as_float(p.rw_bf16 ? wq[it] << 16 : wq[it]);
           float gq[8], g[8], u[8], sg[8], t[8], sl[8], a[8], da[8], ds[8];
+          const float sg8 = PACK ? unpack8_scale(sl8[PACK ? b : 0] & 0xffu) : 0.f;
+          const float su8 = PACK ? unpack8_scale(sl8[PACK ? b : 0] >> 8 & 0xffu) : 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             gq[e] = e < 4 ? g0[e] : g1[e - 4];
-            g[e] = (e & 1) ? bf_hi(gl[b][e >> 1]) : bf_lo(gl[b][e >> 1]);
-            u[e] = (e & 1) ? bf_hi(ul[b][e >> 1]) : bf_lo(ul[b][e >> 1]);
+            if constexpr (PACK) {
+              g[e] = unpack8(gl[b][e >> 2], e & 3, sg8);
+              u[e] = unpack8(gl[b][2 + (e >> 2)], e & 3, su8);
+            } else {
+              g[e] = (e & 1) ? bf_hi(gl[b][e >> 1]) : bf_lo(gl[b][e >> 1]);
+              u[e] = (e & 1) ? bf_hi(ul[b][e >> 1]) : bf_lo(ul[b][e >> 1]);
+            }
             sg[e] = fast_sigmoid(g[e]);
             t[e] = g[e] * sg[e];
           }
@@ -1131,6 +1158,9 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
       const auto ra = make_rsrc(p.out + (int64_t)r0 * I, rows * (uint32_t)I * 2);
       const auto rg = make_rsrc(p.out2 ? p.out2 + (int64_t)r0 * I2 : p.out,
                                 p.out2 ? rows * (uint32_t)I2 * 2 : 0u);
+      const auto rq = make_rsrc(p.q8 + (int64_t)r0 * I2, PACK ? rows * (uint32_t)I2 : 0u);
+      const auto rs8 = make_rsrc(p.q8_scale + (int64_t)r0 * (I / 32),
+                                 PACK ? rows * (uint32_t)(I / 32) : 0u);
 #pragma unroll
       for (int j0 = 0; j0 < TJ; j0 += 2) {
         if (VH && j0 >= c.nj) return NST / 2;
@@ -1153,8 +1183,22 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
           const int feat = fb + f8 * 8, gr = erow(j0, rr);
           const bool ok = feat < I;
           st16(ra, ok ? (uint32_t)gr * I * 2 + (uint32_t)feat * 2 : kOOB, av);
-          st16(rg, ok ? (uint32_t)gr * I2 * 2 + (uint32_t)feat * 2 : kOOB, gv);
-          st16(rg, ok ? (uint32_t)gr * I2 * 2 + (uint32_t)(I + feat) * 2 : kOOB, uv);
+          if constexpr (PACK) {
+            // eight lanes hold the row's 64 features, one block of each half:
+            // 128 bytes of q a row, the pair of scale bytes from one lane
+            const uint32_t eg = pack8_scale(group_absmax_bf16<8>(gv));
+            const uint32_t eu = pack8_scale(group_absmax_bf16<8>(uv));
+            const u32x2 qg = pack8_bf16x8(gv, pack8_inverse(eg));
+            const u32x2 qu = pack8_bf16x8(uv, pack8_inverse(eu));
+            st16(rq, ok ? (uint32_t)gr * I2 + (uint32_t)feat * 2 : kOOB,
+                 u32x4{qg[0], qg[1], qu[0], qu[1]});
+            __builtin_amdgcn_raw_buffer_store_b16(
+                (uint16_t)(eg | eu << 8), rs8,
+                ok && f8 == 0 ? (uint32_t)gr * (I / 32) + (uint32_t)feat / 32 : kOOB, 0, 2);
+          } else {
+            st16(rg, ok ? (uint32_t)gr * I2 * 2 + (uint32_t)feat * 2 : kOOB, gv);
+            st16(rg, ok ? (uint32_t)gr * I2 * 2 + (uint32_t)(I + feat) * 2 : kOOB, uv);
+          }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -1774,9 +1818,9 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
   }
 }
 
-template <int MODE, int BR>
+template <int MODE, int BR, bool PACK = false>
 __global__ __launch_bounds__(kWaves<BR> * 64, 1) void grouped_gemm_kernel(GemmArgs p) {
-  grouped_gemm<MODE, BR>(p);
+  grouped_gemm<MODE, BR, PACK>(p);
 }
 
 // A token-grouped GEMM whose row-tile height the permutation chose: one
@@ -1786,21 +1830,21 @@ __global__ __launch_bounds__(kWaves<BR> * 64, 1) void grouped_gemm_kernel(GemmAr
 // register plan: 511 rows in each of 128 experts here and 512 there, H = 2048,
 // G1F 407 / 400, G2F 213 / 218, G1DX 371 / 374, G2DXF 276 / 270 us; reading the
 // arguments anew in each branch (fewer spills) measured the same.
-template <int MODE>
+template <int MODE, bool PACK = false>
 __global__ __launch_bounds__(kWaves<256> * 64, 1) void token_gemm_kernel(GemmArgs p) {
   const int b = __builtin_amdgcn_readfirstlane(*p.row_tile);
   if (b == 0) {
     p.tile_count = p.tile_counts[0];
     p.tile_info = p.tile_infos[0];
-    grouped_gemm<MODE, 64>(p);
+    grouped_gemm<MODE, 64, PACK>(p);
   } else if (b == 1) {
     p.tile_count = p.tile_counts[1];
     p.tile_info = p.tile_infos[1];
-    grouped_gemm<MODE, 128>(p);
+    grouped_gemm<MODE, 128, PACK>(p);
   } else {
     p.tile_count = p.tile_counts[2];
     p.tile_info = p.tile_infos[2];
-    grouped_gemm<MODE, 256>(p);
+    grouped_gemm<MODE, 256, PACK>(p);
   }
 }
 
@@ -1847,7 +1891,7 @@ int launch_persistent(void (*kernel)(GemmArgs), std::atomic<int> (&lds_done)[64]
   return check_launch("grouped_gemm");
 }
 
-template <int MODE, int BR>
+template <int MODE, int BR, bool PACK = false>
 int launch(const GemmArgs& a, int max_tiles, hipStream_t st) {
   static_assert(kWaves<BR> == 4, "256 threads");
   constexpr size_t stages = (size_t)NSLOT * SLOT;
@@ -1857,7 +1901,7 @@ int launch(const GemmArgs& a, int max_tiles, hipStream_t st) {
                    : (size_t)((MODE == G2DWG || MODE == RLT || MODE == RLTK) ? BC : BR) * SROW *
                          sizeof(bf16);
   static std::atomic<int> lds_done[64];
-  return launch_persistent(grouped_gemm_kernel<MODE, BR>, lds_done,
+  return launch_persistent(grouped_gemm_kernel<MODE, BR, PACK>, lds_done,
                            stages > staging ? stages : staging, a, max_tiles, st);
 }
 
@@ -1870,7 +1914,7 @@ bool host_picks_256(int64_t S, int E) { return S / (E > 0 ? E : 1) >= 512; }
 // only the device knows: the permutation wrote the height of least streamed
 // bytes into the plan and token_gemm_kernel takes it.  Results do not depend
 // on the height: every output element is one k-ordered MFMA chain either way.
-template <int MODE>
+template <int MODE, bool PACK = false>
 int launch_token(GemmArgs a, int64_t S, int E, int ncols_per_tile_out, int ncols_total,
                  const void* tile_plan, hipStream_t st) {
   const char* pb = (const char*)tile_plan;
@@ -1886,13 +1930,13 @@ int launch_token(GemmArgs a, int64_t S, int E, int ncols_per_tile_out, int ncols
   if (host_picks_256(S, E)) {
     a.tile_count = a.tile_counts[2];
     a.tile_info = a.tile_infos[2];
-    return launch<MODE, 256>(a, (int)(plan_max_tiles(S, E, 2) * a.n_ct), st);
+    return launch<MODE, 256, PACK>(a, (int)(plan_max_tiles(S, E, 2) * a.n_ct), st);
   }
   a.row_tile = (const int*)(pb + plan_row_tile_offset(E));
   constexpr size_t staging = (size_t)256 * SROW * sizeof(bf16);
   constexpr size_t stages = (size_t)NSLOT * SLOT;
   static std::atomic<int> lds_done[64];
-  return launch_persistent(token_gemm_kernel<MODE>, lds_done, stages > staging ? stages : staging,
+  return launch_persistent(token_gemm_kernel<MODE, PACK>, lds_done, stages > staging ? stages : staging,
                            a, (int)(plan_max_tiles(S, E, 0) * a.n_ct), st);
 }
 int check_common(int64_t S, int E, int H, int I, int dtype, const char* who) {
@@ -1924,6 +1968,43 @@ using namespace moe;
 #define MOE_ALIGNED(ptr, who) \
   MOE_REQUIRE(aligned16(ptr), MOE_ERR_ALIGN, "%s: pointer %s not 16-byte aligned", who, #ptr)
 
+namespace {
+// GEMM-1 + SwiGLU, gate_up saved in bf16 (or not), or packed to 8 bits (q8).
+int gate_up_swiglu(const void* hidden_states, const int32_t* row_src, int top_k,
+                   const int32_t* offsets, const void* tile_plan, const void* gate_up_proj,
+                   int64_t T, int64_t S, int E, int H, int I, int dtype, void* gate_up_out,
+                   bool pack, void* q8, void* q8_scale, void* act_out, void* stream,
+                   const char* who) {
+  int rc = check_common(S, E, H, I, dtype, who);
+  if (rc) return rc;
+  MOE_REQUIRE(top_k >= 1 && S == T * top_k, MOE_ERR_ARG, "%s: S != T*top_k", who);
+  MOE_REQUIRE(T * (int64_t)H * 2 < ((int64_t)1 << 31), MOE_ERR_UNSUPPORTED, "%s: T*H too large",
+              who);
+  MOE_REQUIRE(offsets && tile_plan && gate_up_proj &&
+                  (S == 0 || (hidden_states && row_src && act_out && (!pack || (q8 && q8_scale)))),
+              MOE_ERR_ARG, "%s: null pointer", who);
+  MOE_ALIGNED(hidden_states, who);
+  MOE_ALIGNED(gate_up_proj, who);
+  MOE_ALIGNED(act_out, who);
+  MOE_ALIGNED(gate_up_out, who);
+  MOE_ALIGNED(q8, who);
+  MOE_ALIGNED(q8_scale, who);
+  if (S == 0) return MOE_OK;
+  GemmArgs a{};
+  a.x = (const bf16*)hidden_states;
+  a.w = (const bf16*)gate_up_proj;
+  a.row_src = row_src;
+  a.offsets = offsets;
+  a.out = (bf16*)act_out;
+  a.out2 = (bf16*)gate_up_out;
+  a.q8 = (uint8_t*)q8;
+  a.q8_scale = (uint8_t*)q8_scale;
+  a.T = T; a.S = S; a.E = E; a.H = H; a.I = I; set_topk(a, top_k);
+  if (pack) return launch_token<G1F, true>(a, S, E, 128, I, tile_plan, (hipStream_t)stream);
+  return launch_token<G1F>(a, S, E, 128, I, tile_plan, (hipStream_t)stream);
+}
+}  // namespace
+
 extern "C" int moe_amd_gemm_gate_up_swiglu(const void* hidden_states, const int32_t* row_src,
                                            int top_k, const int32_t* offsets,
                                            const void* tile_plan, const void* gate_up_proj,
@@ -1934,27 +2015,19 @@ extern "C" int moe_amd_gemm_gate_up_swiglu(const void* hidden_states, const int3
     return f32_gate_up_swiglu((const float*)hidden_states, row_src, top_k, offsets, tile_plan,
                               (const float*)gate_up_proj, T, S, E, H, I, (float*)gate_up_out,
                               (float*)act_out, (hipStream_t)stream);
-  int rc = check_common(S, E, H, I, dtype, who);
-  if (rc) return rc;
-  MOE_REQUIRE(top_k >= 1 && S == T * top_k, MOE_ERR_ARG, "%s: S != T*top_k", who);
-  MOE_REQUIRE(T * (int64_t)H * 2 < ((int64_t)1 << 31), MOE_ERR_UNSUPPORTED, "%s: T*H too large",
-              who);
-  MOE_REQUIRE(offsets && tile_plan && gate_up_proj && (S == 0 || (hidden_states && row_src && act_out)),
-              MOE_ERR_ARG, "%s: null pointer", who);
-  MOE_ALIGNED(hidden_states, who);
-  MOE_ALIGNED(gate_up_proj, who);
-  MOE_ALIGNED(act_out, who);
-  if (gate_up_out) MOE_ALIGNED(gate_up_out, who);
-  if (S == 0) return MOE_OK;
-  GemmArgs a{};
-  a.x = (const bf16*)hidden_states;
-  a.w = (const bf16*)gate_up_proj;
-  a.row_src = row_src;
-  a.offsets = offsets;
-  a.out = (bf16*)act_out;
-  a.out2 = (bf16*)gate_up_out;
-  a.T = T; a.S = S; a.E = E; a.H = H; a.I = I; set_topk(a, top_k);
-  return launch_token<G1F>(a, S, E, 128, I, tile_plan, (hipStream_t)stream);
+  return gate_up_swiglu(hidden_states, row_src, top_k, offsets, tile_plan, gate_up_proj, T, S, E,
+                        H, I, dtype, gate_up_out, false, nullptr, nullptr, act_out, stream, who);
+}
+
+extern "C" int moe_amd_gemm_gate_up_swiglu_pack8(const void* hidden_states, const int32_t* row_src,
+                                                 int top_k, const int32_t* offsets,
+                                                 const void* tile_plan, const void* gate_up_proj,
+                                                 int64_t T, int64_t S, int E, int H, int I,
+                                                 int dtype, void* gate_up_q, void* gate_up_scale,
+                                                 void* act_out, void* stream) {
+  return gate_up_swiglu(hidden_states, row_src, top_k, offsets, tile_plan, gate_up_proj, T, S, E,
+                        H, I, dtype, nullptr, true, gate_up_q, gate_up_scale, act_out, stream,
+                        "gemm_gate_up_swiglu_pack8");
 }
 
 extern "C" int moe_amd_gemm_down(const void* act, const int32_t* offsets,
@@ -2392,12 +2465,14 @@ extern "C" int moe_amd_gemm_down_backward_dx_dswiglu(const void* dy, const int32
 // (one per wave column of 128 features).
 extern "C" int moe_amd_gemm_down_backward_dx_fused_parts(int I) { return 2 * ((I + BC - 1) / BC); }
 
-extern "C" int moe_amd_gemm_down_backward_dx_fused(
-    const void* d_out, const int32_t* row_src, int top_k, const int32_t* offsets,
-    const void* tile_plan, const void* down_proj, const void* gate_up, const void* topk_weights,
-    int weights_dtype, int64_t T, int64_t S, int E, int H, int I, int dtype, void* d_gate_up,
-    void* act_w, float* dw_partials, void* stream) {
-  const char* who = "gemm_down_backward_dx_fused";
+namespace {
+// gate_up in bf16, or packed to 8 bits (q8).
+int down_dx_fused(const void* d_out, const int32_t* row_src, int top_k, const int32_t* offsets,
+                  const void* tile_plan, const void* down_proj, const void* gate_up, bool pack,
+                  const void* q8, const void* q8_scale, const void* topk_weights,
+                  int weights_dtype, int64_t T, int64_t S, int E, int H, int I, int dtype,
+                  void* d_gate_up, void* act_w, float* dw_partials, void* stream,
+                  const char* who) {
   int rc = check_common(S, E, H, I, dtype, who);
   if (rc) return rc;
   MOE_REQUIRE(top_k >= 1 && S == T * top_k, MOE_ERR_ARG, "%s: S != T*top_k", who);
@@ -2406,12 +2481,14 @@ extern "C" int moe_amd_gemm_down_backward_dx_fused(
   MOE_REQUIRE(weights_dtype == MOE_DTYPE_F32 || weights_dtype == MOE_DTYPE_BF16, MOE_ERR_ARG,
               "%s: weights_dtype must be fp32 or bf16", who);
   MOE_REQUIRE(offsets && tile_plan && down_proj &&
-                  (S == 0 || (d_out && row_src && gate_up && topk_weights && d_gate_up && act_w &&
-                              dw_partials)),
+                  (S == 0 || (d_out && row_src && (pack ? q8 && q8_scale : gate_up != nullptr) &&
+                              topk_weights && d_gate_up && act_w && dw_partials)),
               MOE_ERR_ARG, "%s: null pointer", who);
   MOE_ALIGNED(d_out, who);
   MOE_ALIGNED(down_proj, who);
   MOE_ALIGNED(gate_up, who);
+  MOE_ALIGNED(q8, who);
+  MOE_ALIGNED(q8_scale, who);
   MOE_ALIGNED(d_gate_up, who);
   MOE_ALIGNED(act_w, who);
   if (S == 0) return MOE_OK;
@@ -2419,6 +2496,8 @@ extern "C" int moe_amd_gemm_down_backward_dx_fused(
   a.x = (const bf16*)d_out;
   a.w = (const bf16*)down_proj;
   a.a1 = (const bf16*)gate_up;
+  a.q8 = (uint8_t*)q8;
+  a.q8_scale = (uint8_t*)q8_scale;
   a.row_src = row_src;
   a.offsets = offsets;
   a.out = (bf16*)d_gate_up;
@@ -2427,7 +2506,31 @@ extern "C" int moe_amd_gemm_down_backward_dx_fused(
   a.rw_bf16 = weights_dtype == MOE_DTYPE_BF16;
   a.dw_part = dw_partials;
   a.T = T; a.S = S; a.E = E; a.H = H; a.I = I; set_topk(a, top_k);
+  if (pack) return launch_token<G2DXF, true>(a, S, E, BC, I, tile_plan, (hipStream_t)stream);
   return launch_token<G2DXF>(a, S, E, BC, I, tile_plan, (hipStream_t)stream);
+}
+}  // namespace
+
+extern "C" int moe_amd_gemm_down_backward_dx_fused(
+    const void* d_out, const int32_t* row_src, int top_k, const int32_t* offsets,
+    const void* tile_plan, const void* down_proj, const void* gate_up, const void* topk_weights,
+    int weights_dtype, int64_t T, int64_t S, int E, int H, int I, int dtype, void* d_gate_up,
+    void* act_w, float* dw_partials, void* stream) {
+  return down_dx_fused(d_out, row_src, top_k, offsets, tile_plan, down_proj, gate_up, false,
+                       nullptr, nullptr, topk_weights, weights_dtype, T, S, E, H, I, dtype,
+                       d_gate_up, act_w, dw_partials, stream, "gemm_down_backward_dx_fused");
+}
+
+extern "C" int moe_amd_gemm_down_backward_dx_fused_pack8(
+    const void* d_out, const int32_t* row_src, int top_k, const int32_t* offsets,
+    const void* tile_plan, const void* down_proj, const void* gate_up_q,
+    const void* gate_up_scale, const void* topk_weights, int weights_dtype, int64_t T, int64_t S,
+    int E, int H, int I, int dtype, void* d_gate_up, void* act_w, float* dw_partials,
+    void* stream) {
+  return down_dx_fused(d_out, row_src, top_k, offsets, tile_plan, down_proj, nullptr, true,
+                       gate_up_q, gate_up_scale, topk_weights, weights_dtype, T, S, E, H, I,
+                       dtype, d_gate_up, act_w, dw_partials, stream,
+                       "gemm_down_backward_dx_fused_pack8");
 }
 
 extern "C" int moe_amd_gemm_gate_up_backward_dx(const void* d_gate_up, const int32_t* offsets,

@@ -1,0 +1,68 @@
+// Activations in 8 bits: for 64 consecutive values v of a row a power of two s
+// and the integers q = rint(v / s), halves to even.  s is the smallest power of
+// two that is at least 2^-126 and has max|v| <= 127 s, so q * s is exact in bf16
+// (7 bits) and in fp32, whoever restores it (past 127/128 2^128 it is 2^128,
+// infinity in both).  (An s of max|v| / 127 would halve
+// the step at best, sqrt(2) on average, and make the restored value a rounding
+// of its own.)  The scale byte is s's biased exponent, 1 .. 249; 255 marks a
+// block with a value that is not finite, whose q are 0: it is restored as
+// 0 * inf, NaN in every place, rather than hidden.
+#pragma once
+#include "wave_topk.h"
+
+namespace moe {
+
+constexpr int kPack8Block = 64;
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// The scale byte from the bits of the block's largest |v| as fp32 (NaN above
+// all).  2^k >= a / 127 for a = 1.m 2^e: k = e - 6, or e - 5 where 1.m > 127/64
+// (m > 0x7e0000, which the addition carries into the exponent).
+__device__ __forceinline__ uint32_t pack8_scale(uint32_t absmax_bits) {
+  const int e = (int)((absmax_bits + 0x1ffffu) >> 23) - 6;
+  return absmax_bits >= 0x7f800000u ? 255u : (uint32_t)(e < 1 ? 1 : e);
+}
+// 1 / s, or 0 for a block that is not finite.
+__device__ __forceinline__ float pack8_inverse(uint32_t scale) {
+  return scale == 255u ? 0.f : __uint_as_float((254u - scale) << 23);
+}
+// q in the low byte: v / s is exact, and adding 1.5 2^23 rounds it to an
+// integer, halves to even, whose two's complement ends the sum's bits (v NaN
+// or 0 * inf: a NaN that ends in a zero byte).
+__device__ __forceinline__ uint32_t pack8_one(float v, float inv) {
+  return __float_as_uint(__builtin_fmaf(v, inv, 12582912.f));
+}
+__device__ __forceinline__ uint32_t pack8_four(float a, float b, float c, float d, float inv) {
+  const uint32_t lo = __builtin_amdgcn_perm(pack8_one(b, inv), pack8_one(a, inv), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(pack8_one(d, inv), pack8_one(c, inv), 0x0c0c0400u);
+  return hi << 16 | lo;
+}
+// Eight bf16 values (four pairs) -> eight bytes.
+__device__ __forceinline__ u32x2 pack8_bf16x8(const u32x4& v, float inv) {
+  return u32x2{pack8_four(bf_lo(v[0]), bf_hi(v[0]), bf_lo(v[1]), bf_hi(v[1]), inv),
+               pack8_four(bf_lo(v[2]), bf_hi(v[2]), bf_lo(v[3]), bf_hi(v[3]), inv)};
+}
+
+// The bits, as fp32, of the largest |v| of the eight bf16 values that each of G
+// consecutive lanes holds: pairs of 16-bit integers compare as their magnitudes.
+template <int G>
+__device__ __forceinline__ uint32_t group_absmax_bf16(const u32x4& v) {
+  u16x2 m = __builtin_bit_cast(u16x2, v[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int w = 1; w < 4; ++w)
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[w] & 0x7fff7fffu));
+  group_steps<G>([&](auto c) {
+    const uint32_t o = dpp_u32<decltype(c)::value>(__builtin_bit_cast(uint32_t, m));
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, o));
+  });
+  return (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16;
+}
+
+__device__ __forceinline__ float unpack8_scale(uint32_t scale) { return __uint_as_float(scale << 23); }
+// Value `byte` (0 .. 3) of four packed ones.
+__device__ __forceinline__ float unpack8(uint32_t q, int byte, float scale) {
+  return (float)(int8_t)(q >> (8 * byte)) * scale;
+}
+
+}  // namespace moe

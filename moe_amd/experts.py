@@ -21,8 +21,15 @@ from . import few, library  # noqa: F401  (library registers the moe_amd:: ops)
 
 def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                     top_k_weights: torch.Tensor, gate_up_proj: torch.Tensor,
-                    down_proj: torch.Tensor) -> torch.Tensor:
+                    down_proj: torch.Tensor, saved_activations: str = "exact") -> torch.Tensor:
     """out[t] = sum_k w[t,k] * down_e(silu(gate_e(x_t)) * up_e(x_t)), e = idx[t,k].
+
+    ``saved_activations`` (bf16 layers): what the backward finds of the
+    activations.  "exact": gate_up [S,2I] and the hidden states as they are.
+    "int8": gate_up in 8 bits (half the memory; ``ops.pack8``'s values), packed
+    where GEMM-1 leaves it and read so by the backward: the gradients are those
+    of the restored gate_up, the output is the same.  "int8_all": the hidden
+    states too, for d_gate_up_proj; worth it where nothing else keeps them.
 
     hidden_states is cast to the weights' dtype (as transformers' _grouped_mm
     does, integrations/moe.py:330-335) and the result is returned in
@@ -38,13 +45,14 @@ def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
             f"{tuple(gate_up_proj.shape)}, down_proj {tuple(down_proj.shape)}")
     if top_k_index.shape != top_k_weights.shape or top_k_index.shape[0] != hidden_states.shape[0]:
         raise ValueError("top_k_index / top_k_weights must both be [T, K]")
+    library.check_keep(saved_activations, gate_up_proj.dtype)
     out_dtype = hidden_states.dtype
     x = hidden_states.to(gate_up_proj.dtype).contiguous()
     w = top_k_weights.contiguous()
     save = torch.is_grad_enabled() and any(t.requires_grad
                                            for t in (x, w, gate_up_proj, down_proj))
     out = torch.ops.moe_amd.experts_fwd(x, top_k_index, w, gate_up_proj.contiguous(),
-                                        down_proj.contiguous(), save)[0]
+                                        down_proj.contiguous(), save, saved_activations)[0]
     return out.to(out_dtype)
 
 
@@ -68,11 +76,12 @@ def mi355x_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch
     """ExpertsInterface entry ("mi355x"), drop-in for grouped_mm_experts_forward
     (transformers/integrations/moe.py:377-478).  A bank with a ``few_tokens``
     attribute runs the few-token experts up to that many tokens where no
-    gradient is wanted (``hf.install(model, few_tokens=...)`` sets it)."""
+    gradient is wanted, and a ``saved_activations`` attribute is
+    experts_forward's (``hf.install`` sets both)."""
     _check_module(self)
     if few.wanted(getattr(self, "few_tokens", 0), hidden_states, top_k_weights,
                   self.gate_up_proj, self.down_proj):
         return few.experts_forward_few(hidden_states, top_k_index, top_k_weights,
                                        self.gate_up_proj, self.down_proj)
     return experts_forward(hidden_states, top_k_index, top_k_weights, self.gate_up_proj,
-                           self.down_proj)
+                           self.down_proj, getattr(self, "saved_activations", "exact"))

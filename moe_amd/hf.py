@@ -15,6 +15,7 @@ from __future__ import annotations
 from torch import nn
 
 from .experts import mi355x_experts_forward
+from .library import KEEPS
 from .router import MI355XDeepSeekRouter, MI355XTopKRouter, _RouterBase
 
 EXPERTS_KEY = "mi355x"
@@ -53,11 +54,15 @@ def expert_banks(model: nn.Module) -> list[nn.Module]:
 
 
 def install(model: nn.Module, routers: bool = True, experts: bool = True,
-            few_tokens: int = 0) -> nn.Module:
+            few_tokens: int = 0, saved_activations: str = "exact") -> nn.Module:
     """Swaps the routers and selects the "mi355x" experts.  ``few_tokens``
     (with ``experts``): calls of at most that many tokens (up to
     ``moe_amd.few.MAX_TOKENS``) that want no gradient run the few-token
-    experts."""
+    experts.  ``saved_activations`` (with ``experts``): what the experts keep
+    for their backward, as ``experts_forward`` takes it."""
+    if saved_activations not in KEEPS:
+        raise ValueError(f"unknown saved_activations {saved_activations!r} (expected one of "
+                         f"{KEEPS})")
     register()
     if routers:
         swap_routers(model)
@@ -65,4 +70,5 @@ def install(model: nn.Module, routers: bool = True, experts: bool = True,
         model.set_experts_implementation(EXPERTS_KEY)
         for bank in expert_banks(model):
             bank.few_tokens = int(few_tokens)
+            bank.saved_activations = saved_activations
     return model

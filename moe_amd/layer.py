@@ -38,10 +38,16 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tenso
               renormalize: bool = True, logit_offset: torch.Tensor | None = None,
               expert_bias: torch.Tensor | None = None, scaling_factor: float | None = None,
               num_groups: int | None = None, group_topk: int | None = None,
-              tokens_per_expert: torch.Tensor | None = None, gating: str = "torch"):
-    """Returns (out [T,H], router_logits [T,E] fp32, weights [T,K], index [T,K])."""
+              tokens_per_expert: torch.Tensor | None = None, gating: str = "torch",
+              saved_activations: str = "exact"):
+    """Returns (out [T,H], router_logits [T,E] fp32, weights [T,K], index [T,K]).
+    ``saved_activations`` as for experts_forward; with "int8_all" the router
+    weight's gradient comes from the restored hidden states too where router
+    and experts are one node (bf16 softmax layers), and elsewhere the router
+    keeps its own."""
     if gating not in library.GATINGS:
         raise ValueError(f"unknown gating {gating!r} (expected one of {library.GATINGS})")
+    library.check_keep(saved_activations, gate_up_proj.dtype)
     hip = gating in ("hip", "hip_fused")
     if router == "softmax" and _fused_softmax_ok(x, w_router, gate_up_proj, down_proj):
         # Gating linear + softmax router + experts as ONE autograd node (op
@@ -55,7 +61,8 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tenso
             t.requires_grad for t in (x, w_router, gate_up_proj, down_proj))
         res = torch.ops.moe_amd.moe_layer_fwd(x.contiguous(), w_router, gate_up_proj.contiguous(),
                                               down_proj.contiguous(), int(top_k),
-                                              bool(renormalize), logit_offset, save, gating)
+                                              bool(renormalize), logit_offset, save, gating,
+                                              saved_activations)
         return res[0], res[1], res[2], res[3]
     if router == "softmax":
         logits = gating_linear(x, w_router, fp32=False, hip=hip)
@@ -70,7 +77,7 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tenso
                                      num_groups, group_topk, x.dtype, tokens_per_expert)
     else:
         raise ValueError(f"unknown router {router!r}")
-    out = experts_forward(x, idx, w, gate_up_proj, down_proj)
+    out = experts_forward(x, idx, w, gate_up_proj, down_proj, saved_activations)
     return out, probs, w, idx
 
 
@@ -93,9 +100,10 @@ class SparseMoeBlock(nn.Module):
 
     Up to ``few_tokens`` tokens without a gradient run the few-token layer
     (``moe_amd.few``; 0, the default: never), which computes no router_logits:
-    they are None then."""
+    they are None then.  ``saved_activations`` is moe_layer's."""
 
     few_tokens = 0
+    saved_activations = "exact"
 
     def __init__(self, hidden_size: int, num_experts: int, top_k: int, intermediate_size: int,
                  router: str = "softmax", norm_topk_prob: bool = True):
@@ -125,6 +133,7 @@ class SparseMoeBlock(nn.Module):
         out, probs, _, idx = moe_layer(
             flat, self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj, self.top_k,
             router=self.router, renormalize=self.norm_topk_prob, logit_offset=self.logit_offset,
-            expert_bias=self.expert_bias if self.router == "sigmoid" else None)
+            expert_bias=self.expert_bias if self.router == "sigmoid" else None,
+            saved_activations=self.saved_activations)
         self.router_logits, self.topk_index = probs, idx
         return out.reshape(shape)

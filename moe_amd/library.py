@@ -18,6 +18,7 @@ differentiable piece of the MI355X path, each a functional op in namespace
   linear_sigmoid_topk            its fp32 gating linear and the router in one
                                  kernel (backward: sigmoid_topk_backward, then
                                  router_linear_backward)
+  pack8 / unpack8                a tensor to 8 bits and back
   experts_few / moe_layer_few    the experts, and the layer, for a few tokens
                                  (forward only)
 
@@ -58,6 +59,63 @@ def _plan(counts, offsets, row_src, slot, tile_plan, E, K, T) -> ops.RoutingPlan
     return ops.RoutingPlan(counts, offsets, row_src, slot, tile_plan, E, K, T)
 
 
+# What an expert layer keeps of its activations for the backward: "exact", as
+# they are; "int8", gate_up in 8 bits (packed in GEMM-1's epilogue, read so by
+# the fused down backward); "int8_all", the hidden states too.
+KEEPS = ("exact", "int8", "int8_all")
+
+
+def check_keep(keep: str, dtype: torch.dtype) -> str:
+    if keep not in KEEPS:
+        raise ValueError(f"unknown saved_activations {keep!r} (expected one of {KEEPS})")
+    if keep != "exact" and dtype != torch.bfloat16:
+        raise NotImplementedError(f"saved_activations={keep!r} takes bf16 layers, not {dtype}")
+    return keep
+
+
+@torch.library.custom_op(f"{_LIB}::pack8", mutates_args=())
+def pack8(x: Tensor) -> tuple[Tensor, Tensor]:
+    """(q int8, scale uint8) of ops.pack8."""
+    p = ops.pack8(x)
+    return p.q, p.scale
+
+
+@pack8.register_fake
+def _(x):
+    blocks = (x.shape[-1] + ops.PACK8_BLOCK - 1) // ops.PACK8_BLOCK
+    return (x.new_empty(x.shape, dtype=torch.int8),
+            x.new_empty((*x.shape[:-1], blocks), dtype=torch.uint8))
+
+
+@torch.library.custom_op(f"{_LIB}::unpack8", mutates_args=())
+def unpack8(q: Tensor, scale: Tensor, dtype: torch.dtype) -> Tensor:
+    """The tensor that (q, scale) hold, in dtype (the one it came from)."""
+    return ops.unpack8(ops.Packed8(q, scale, dtype))
+
+
+@unpack8.register_fake
+def _(q, scale, dtype):
+    return q.new_empty(q.shape, dtype=dtype)
+
+
+def _kept(x: Tensor, keep: str) -> tuple[Tensor, ...]:
+    """What a node saves of its hidden states: themselves, or packed."""
+    return torch.ops.moe_amd.pack8(x) if keep == "int8_all" else (x,)
+
+
+def _restored(saved, keep: str) -> tuple[Tensor, tuple]:
+    """(hidden states, the other saved tensors)."""
+    if keep != "int8_all":
+        return saved[0], saved[1:]
+    return torch.ops.moe_amd.unpack8(saved[0], saved[1], torch.bfloat16), saved[2:]
+
+
+def _gate_up_fake(x: Tensor, S, I2, save: bool, keep: str) -> Tensor:
+    if save and keep != "exact":
+        return x.new_empty(ops.packed_gate_up_bytes(S, I2 // 2), dtype=torch.uint8)
+    return x.new_empty(S if save else 0, I2)
+
+
 def _empty_like_none(t: Tensor) -> Tensor:
     return t.new_empty(0)
 
@@ -91,15 +149,18 @@ def _saves_act_y(dtype: torch.dtype, save_for_backward: bool) -> bool:
 
 @torch.library.custom_op(f"{_LIB}::experts_fwd", mutates_args=())
 def experts_fwd(hidden_states: Tensor, top_k_index: Tensor, top_k_weights: Tensor,
-                gate_up_proj: Tensor, down_proj: Tensor, save_for_backward: bool
+                gate_up_proj: Tensor, down_proj: Tensor, save_for_backward: bool,
+                keep: str = "exact"
                 ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor,
                            Tensor]:
-    """(out [T,H], gate_up [S,2I] or [0,2I], act [S,I] and y [S,H] (fp32
+    """(out [T,H], gate_up [S,2I] or [0,2I] (packed to 8 bits, uint8, unless
+    keep is "exact"), act [S,I] and y [S,H] (fp32
     with save_for_backward; else [0,I], [0,H]), counts, offsets, row_src,
     slot, tile_plan).  transformers/integrations/moe.py:377-478."""
+    check_keep(keep, hidden_states.dtype)
     plan = ops.permute(top_k_index, gate_up_proj.shape[0])
     gu, act = ops.gemm_gate_up_swiglu(hidden_states, plan, gate_up_proj,
-                                      save_gate_up=save_for_backward)
+                                      save_gate_up=save_for_backward, pack8=keep != "exact")
     y = ops.gemm_down(act, plan, down_proj)
     out = ops.combine(y, plan, top_k_weights)
     if not _saves_act_y(hidden_states.dtype, save_for_backward):
@@ -110,12 +171,13 @@ def experts_fwd(hidden_states: Tensor, top_k_index: Tensor, top_k_weights: Tenso
 
 
 @experts_fwd.register_fake
-def _(hidden_states, top_k_index, top_k_weights, gate_up_proj, down_proj, save_for_backward):
+def _(hidden_states, top_k_index, top_k_weights, gate_up_proj, down_proj, save_for_backward,
+      keep="exact"):
     T, H = hidden_states.shape
     S = T * top_k_index.shape[1]
     E, I2 = gate_up_proj.shape[0], gate_up_proj.shape[1]
     out = hidden_states.new_empty(T, H)
-    gu = hidden_states.new_empty(S if save_for_backward else 0, I2)
+    gu = _gate_up_fake(hidden_states, S, I2, save_for_backward, keep)
     sa = S if _saves_act_y(hidden_states.dtype, save_for_backward) else 0
     act, y = hidden_states.new_empty(sa, I2 // 2), hidden_states.new_empty(sa, H)
     return (out, gu, act, y) + _plan_fake(S, E, hidden_states.device)
@@ -244,26 +306,29 @@ def _(d_out, hidden_states, top_k_weights, gate_up_proj, down_proj, gate_up, act
 
 
 def _experts_setup(ctx, inputs, output):
-    x, _, w, w1, w2, _ = inputs
+    x, _, w, w1, w2, _, keep = inputs
     _, gu, act, y, counts, offsets, row_src, slot, tile_plan = output
     # The saved activations are outputs only for saving: no zero [S, 2I]
     # gradient is materialised for them.
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(x, w, w1, w2, gu, act, y, counts, offsets, row_src, slot, tile_plan)
+    ctx.keep = keep
+    ctx.save_for_backward(*_kept(x, keep), w, w1, w2, gu, act, y, counts, offsets, row_src, slot,
+                          tile_plan)
     ctx.main_grads = (_main_grad(w1), _main_grad(w2))
 
 
 def _experts_backward(ctx, d_out, *unused):
     need_x, _, need_w, need_w1, need_w2 = ctx.needs_input_grad[:5]
     if d_out is None:
-        return (None,) * 6
+        return (None,) * 7
     acc1, acc2 = ctx.main_grads
+    x, saved = _restored(ctx.saved_tensors, ctx.keep)
     d_x, d_w, d_w1, d_w2 = torch.ops.moe_amd.experts_bwd(
-        d_out, *ctx.saved_tensors, bool(need_x), bool(need_w1), bool(need_w2),
+        d_out, x, *saved, bool(need_x), bool(need_w1), bool(need_w2),
         acc1 if need_w1 else None, acc2 if need_w2 else None)
     return (d_x if need_x else None, None, d_w if need_w else None,
             d_w1 if need_w1 and acc1 is None else None,
-            d_w2 if need_w2 and acc2 is None else None, None)
+            d_w2 if need_w2 and acc2 is None else None, None, None)
 
 
 torch.library.register_autograd(f"{_LIB}::experts_fwd", _experts_backward,
@@ -583,10 +648,10 @@ def gating_logits(x: Tensor, w_router: Tensor, gating: str, fp32: bool) -> Tenso
 @torch.library.custom_op(f"{_LIB}::moe_layer_fwd", mutates_args=())
 def moe_layer_fwd(x: Tensor, w_router: Tensor, gate_up_proj: Tensor, down_proj: Tensor,
                   top_k: int, renormalize: bool, logit_offset: Optional[Tensor],
-                  save_for_backward: bool, gating: str
+                  save_for_backward: bool, gating: str, keep: str = "exact"
                   ) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor,
                              Tensor, Tensor]:
-    """(out, probs fp32, weights fp32, index, gate_up, counts, offsets, row_src,
+    """(out, probs fp32, weights fp32, index, gate_up (as experts_fwd's), counts, offsets, row_src,
     slot, tile_plan): bf16 gating linear (source ``gating``), softmax router,
     experts (Qwen3MoeSparseMoeBlock.forward, src/models/modeling_qwen3_moe.py:
     284-289).  The backward runs the gating linear's gradients on the MFMA
@@ -600,7 +665,8 @@ def moe_layer_fwd(x: Tensor, w_router: Tensor, gate_up_proj: Tensor, down_proj: 
         probs, w, idx = ops.router_softmax_topk(logits, top_k, renormalize, logit_offset)
         del logits
     plan = ops.permute(idx, gate_up_proj.shape[0])
-    gu, act = ops.gemm_gate_up_swiglu(x, plan, gate_up_proj, save_gate_up=save_for_backward)
+    gu, act = ops.gemm_gate_up_swiglu(x, plan, gate_up_proj, save_gate_up=save_for_backward,
+                                      pack8=keep != "exact")
     y = ops.gemm_down(act, plan, down_proj)
     del act
     out = ops.combine(y, plan, w)
@@ -612,7 +678,7 @@ def moe_layer_fwd(x: Tensor, w_router: Tensor, gate_up_proj: Tensor, down_proj: 
 
 @moe_layer_fwd.register_fake
 def _(x, w_router, gate_up_proj, down_proj, top_k, renormalize, logit_offset, save_for_backward,
-      gating):
+      gating, keep="exact"):
     T, H = x.shape
     E, I2 = gate_up_proj.shape[0], gate_up_proj.shape[1]
     S = T * top_k
@@ -620,7 +686,7 @@ def _(x, w_router, gate_up_proj, down_proj, top_k, renormalize, logit_offset, sa
     f32 = dict(device=dev, dtype=torch.float32)
     return (x.new_empty(T, H), torch.empty(T, E, **f32), torch.empty(T, top_k, **f32),
             torch.empty(T, top_k, device=dev, dtype=torch.int64),
-            x.new_empty(S if save_for_backward else 0, I2)) + _plan_fake(S, E, dev)
+            _gate_up_fake(x, S, I2, save_for_backward, keep)) + _plan_fake(S, E, dev)
 
 
 @torch.library.custom_op(f"{_LIB}::moe_layer_bwd", mutates_args=("acc_w1", "acc_w2"))
@@ -675,12 +741,13 @@ def _(d_out, d_probs, d_w, x, w_router, gate_up_proj, down_proj, gate_up, probs,
 
 
 def _layer_setup(ctx, inputs, output):
-    x, w_router, gate_up_proj, down_proj, _, renormalize, _, _, _ = inputs
+    x, w_router, gate_up_proj, down_proj, _, renormalize, _, _, _, keep = inputs
     _, probs, w, idx, gu, counts, offsets, row_src, slot, tile_plan = output
     ctx.set_materialize_grads(False)
     ctx.mark_non_differentiable(idx)
-    ctx.save_for_backward(x, w_router, gate_up_proj, down_proj, gu, probs, w, idx, counts,
-                          offsets, row_src, slot, tile_plan)
+    ctx.keep = keep
+    ctx.save_for_backward(*_kept(x, keep), w_router, gate_up_proj, down_proj, gu, probs, w, idx,
+                          counts, offsets, row_src, slot, tile_plan)
     ctx.renormalize = renormalize
     ctx.main_grads = (_main_grad(gate_up_proj), _main_grad(down_proj))
 
@@ -688,14 +755,15 @@ def _layer_setup(ctx, inputs, output):
 def _layer_backward(ctx, d_out, d_probs, d_w, *unused):
     need_x, need_wr, need_w1, need_w2 = (bool(n) for n in ctx.needs_input_grad[:4])
     if d_out is None and d_probs is None and d_w is None:
-        return (None,) * 9
+        return (None,) * 10
     acc1, acc2 = ctx.main_grads
+    x, saved = _restored(ctx.saved_tensors, ctx.keep)
     d_x, d_wr, d_w1, d_w2 = torch.ops.moe_amd.moe_layer_bwd(
-        d_out, d_probs, d_w, *ctx.saved_tensors, ctx.renormalize, need_x, need_wr, need_w1,
+        d_out, d_probs, d_w, x, *saved, ctx.renormalize, need_x, need_wr, need_w1,
         need_w2, acc1 if need_w1 else None, acc2 if need_w2 else None)
     return (d_x if need_x else None, d_wr if need_wr else None,
             d_w1 if need_w1 and acc1 is None else None,
-            d_w2 if need_w2 and acc2 is None else None, None, None, None, None, None)
+            d_w2 if need_w2 and acc2 is None else None) + (None,) * 6
 
 
 torch.library.register_autograd(f"{_LIB}::moe_layer_fwd", _layer_backward,

@@ -52,6 +52,8 @@ def _device_of(args, kwargs):
     for a in (*args, *kwargs.values()) if kwargs else args:
         if isinstance(a, RoutingPlan):
             return a.counts.device.index
+        if isinstance(a, Packed8):
+            return a.q.device.index
         if getattr(a, "is_cuda", False):
             return a.device.index
     return None
@@ -487,15 +489,29 @@ def permute(topk_index: torch.Tensor, num_experts: int) -> RoutingPlan:
 
 # --------------------------------------------------------- grouped GEMMs
 
+def packed_gate_up_bytes(S: int, I: int) -> int:
+    """Bytes of S rows of gate_up in 8 bits: the values, then their scales."""
+    return S * 2 * I + S * (I // 32)
+
+
 @on_tensor_device
 def gemm_gate_up_swiglu(x: torch.Tensor, plan: RoutingPlan, gate_up_proj: torch.Tensor,
-                        save_gate_up: bool = True):
-    """Returns (gate_up [S,2I] or None, act [S,I])."""
+                        save_gate_up: bool = True, pack8: bool = False):
+    """Returns (gate_up [S,2I] or None, act [S,I]).  With ``pack8`` (bf16)
+    gate_up comes packed to 8 bits, as gemm_down_backward_fused takes it: one
+    uint8 tensor of packed_gate_up_bytes(S, I)."""
     _need_cuda(x, gate_up_proj)
     E, I2, H = gate_up_proj.shape
     I = I2 // 2
     S = plan.num_rows
     act = torch.empty(S, I, device=x.device, dtype=x.dtype)
+    if save_gate_up and pack8:
+        q = torch.empty(packed_gate_up_bytes(S, I), device=x.device, dtype=torch.uint8)
+        _call("moe_amd_gemm_gate_up_swiglu_pack8", x.data_ptr(), plan.row_src.data_ptr(),
+              plan.top_k, plan.offsets.data_ptr(), plan.tile_plan.data_ptr(),
+              gate_up_proj.data_ptr(), plan.num_tokens, S, E, H, I, _dtype_code(x.dtype),
+              q.data_ptr(), q.data_ptr() + S * I2, act.data_ptr(), _stream(x))
+        return q, act
     gu = torch.empty(S, I2, device=x.device, dtype=x.dtype) if save_gate_up else None
     _call("moe_amd_gemm_gate_up_swiglu", x.data_ptr(), plan.row_src.data_ptr(), plan.top_k,
           plan.offsets.data_ptr(), plan.tile_plan.data_ptr(), gate_up_proj.data_ptr(),
@@ -533,7 +549,8 @@ def gemm_down_backward_fused(d_out, plan: RoutingPlan, down_proj, gate_up, topk_
     """Backward of the combine and of GEMM-2 + SwiGLU in one GEMM, without
     materialising d_y = w * d_out[token] ([S,H]): per routed row, g = d_out[t]
     . down_proj[e]; d_gate_up from d_act = w * g; the routing-weight gradient
-    <d_out[t], y[r]> = <g, act[r]> (act recomputed from gate_up).  Returns
+    <d_out[t], y[r]> = <g, act[r]> (act recomputed from gate_up, which may be
+    gemm_gate_up_swiglu's packed one).  Returns
     (d_gate_up [S,2I], act_w [S,I] = w * act for gemm_down_backward_dw_gathered,
     d_topk_weights [T,K] in topk_weights' dtype)."""
     _need_cuda(d_out, down_proj, gate_up, topk_weights)
@@ -548,10 +565,16 @@ def gemm_down_backward_fused(d_out, plan: RoutingPlan, down_proj, gate_up, topk_
     part = torch.empty(S, n_part, device=dev, dtype=torch.float32)
     dw = torch.empty(T, K, device=dev, dtype=topk_weights.dtype)
     st = _stream(d_out)
-    _call("moe_amd_gemm_down_backward_dx_fused", d_out.data_ptr(), plan.row_src.data_ptr(), K,
-          plan.offsets.data_ptr(), plan.tile_plan.data_ptr(), down_proj.data_ptr(),
-          gate_up.data_ptr(), topk_weights.data_ptr(), _dtype_code(topk_weights.dtype), T, S, E,
-          H, I, _dtype_code(dt), dgu.data_ptr(), act_w.data_ptr(), part.data_ptr(), st)
+    name, saved = "moe_amd_gemm_down_backward_dx_fused", (gate_up.data_ptr(),)
+    if gate_up.dtype == torch.uint8:
+        if gate_up.numel() != packed_gate_up_bytes(S, I) or not gate_up.is_contiguous():
+            raise ValueError(f"gemm_down_backward_fused: packed gate_up of {gate_up.numel()} "
+                             f"bytes, expected {packed_gate_up_bytes(S, I)}")
+        name, saved = name + "_pack8", (gate_up.data_ptr(), gate_up.data_ptr() + S * 2 * I)
+    _call(name, d_out.data_ptr(), plan.row_src.data_ptr(), K, plan.offsets.data_ptr(),
+          plan.tile_plan.data_ptr(), down_proj.data_ptr(), *saved, topk_weights.data_ptr(),
+          _dtype_code(topk_weights.dtype), T, S, E, H, I, _dtype_code(dt), dgu.data_ptr(),
+          act_w.data_ptr(), part.data_ptr(), st)
     _call("moe_amd_weight_grad_reduce", part.data_ptr(), n_part, plan.slot.data_ptr(),
           plan.offsets.data_ptr(), T, K, E, dw.data_ptr(), _dtype_code(dw.dtype), st)
     return dgu, act_w, dw
@@ -753,6 +776,61 @@ def gather_backward(dxs, plan: RoutingPlan, addend: torch.Tensor | None = None) 
               plan.offsets.data_ptr(), addend.data_ptr(), T, K, E, H, _dtype_code(dxs.dtype),
               dx.data_ptr(), _stream(dxs))
     return dx
+
+
+# ------------------------------------------------------ activations in 8 bits
+
+PACK8_BLOCK = 64
+
+
+@dataclass
+class Packed8:
+    """A tensor in 8 bits (:func:`pack8`): q int8 of its shape, scale uint8 with
+    one byte (a power of two's biased exponent) per 64 values of the last
+    dimension, and the dtype it came from."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    dtype: torch.dtype
+
+
+@on_tensor_device
+def pack8(x: torch.Tensor) -> Packed8:
+    """x (bf16 or fp32, at least one dimension) in 8 bits: per 64 values v of
+    its last dimension s, the smallest power of two >= 2^-126 with max|v| <=
+    127 s, and rint(v / s).  The error is at most s / 2, max|v| / 127 in the
+    worst case; what unpack8 gives is exact in x's dtype.  A block with a value
+    that is not finite comes back as NaN whole."""
+    _need_cuda(x)
+    if x.dim() == 0:
+        raise ValueError("pack8 takes tensors of at least one dimension")
+    code = _dtype_code(x.dtype)
+    x = _contig(x)
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
+    scale = torch.empty(*x.shape[:-1], -(-cols // PACK8_BLOCK), device=x.device,
+                        dtype=torch.uint8)
+    _call("moe_amd_pack8", x.data_ptr(), code, rows, cols, q.data_ptr(), scale.data_ptr(),
+          _stream(x), capturable=True)
+    return Packed8(q, scale, x.dtype)
+
+
+@on_tensor_device
+def unpack8(packed: Packed8) -> torch.Tensor:
+    """The tensor that ``packed`` holds, in the dtype it came from."""
+    q, scale = packed.q, packed.scale
+    _need_cuda(q, scale)
+    cols = q.shape[-1] if q.dim() else 0
+    if q.dtype != torch.int8 or scale.dtype != torch.uint8 or q.dim() == 0 \
+            or tuple(scale.shape) != (*q.shape[:-1], -(-cols // PACK8_BLOCK)) \
+            or q.device != scale.device:
+        raise ValueError(f"unpack8: q {q.dtype} {tuple(q.shape)} and scale {scale.dtype} "
+                         f"{tuple(scale.shape)} are not a packed tensor")
+    q, scale = _contig(q), _contig(scale)
+    x = torch.empty(q.shape, device=q.device, dtype=packed.dtype)
+    _call("moe_amd_unpack8", q.data_ptr(), scale.data_ptr(), q.numel() // cols if cols else 0,
+          cols, x.data_ptr(), _dtype_code(packed.dtype), _stream(q), capturable=True)
+    return x
 
 
 # -------------------------------------------------- the layer for few tokens
