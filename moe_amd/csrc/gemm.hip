@@ -1186,14 +1186,11 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
           if constexpr (PACK) {
             // eight lanes hold the row's 64 features, one block of each half:
             // 128 bytes of q a row, the pair of scale bytes from one lane
-            const uint32_t eg = pack8_scale(group_absmax_bf16<8>(gv));
-            const uint32_t eu = pack8_scale(group_absmax_bf16<8>(uv));
-            const u32x2 qg = pack8_bf16x8(gv, pack8_inverse(eg));
-            const u32x2 qu = pack8_bf16x8(uv, pack8_inverse(eu));
-            st16(rq, ok ? (uint32_t)gr * I2 + (uint32_t)feat * 2 : kOOB,
-                 u32x4{qg[0], qg[1], qu[0], qu[1]});
+            uint32_t scales;
+            const u32x4 q = pack8_two_blocks(gv, uv, scales);
+            st16(rq, ok ? (uint32_t)gr * I2 + (uint32_t)feat * 2 : kOOB, q);
             __builtin_amdgcn_raw_buffer_store_b16(
-                (uint16_t)(eg | eu << 8), rs8,
+                (uint16_t)scales, rs8,
                 ok && f8 == 0 ? (uint32_t)gr * (I / 32) + (uint32_t)feat / 32 : kOOB, 0, 2);
           } else {
             st16(rg, ok ? (uint32_t)gr * I2 * 2 + (uint32_t)feat * 2 : kOOB, gv);

@@ -44,19 +44,28 @@ __device__ __forceinline__ u32x2 pack8_bf16x8(const u32x4& v, float inv) {
                pack8_four(bf_lo(v[2]), bf_hi(v[2]), bf_lo(v[3]), bf_hi(v[3]), inv)};
 }
 
-// The bits, as fp32, of the largest |v| of the eight bf16 values that each of G
-// consecutive lanes holds: pairs of 16-bit integers compare as their magnitudes.
-template <int G>
-__device__ __forceinline__ uint32_t group_absmax_bf16(const u32x4& v) {
-  u16x2 m = __builtin_bit_cast(u16x2, v[0] & 0x7fff7fffu);
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
+}
+// Two blocks of 64 bf16 values, eight of each (a, b) in each of eight consecutive
+// lanes -> their bytes {a, b} and their scale bytes (a's low).  Magnitudes
+// compare as 16-bit integers, the two blocks' in one register.
+__device__ __forceinline__ u32x4 pack8_two_blocks(const u32x4& a, const u32x4& b,
+                                                  uint32_t& scales) {
+  uint32_t ma = a[0] & 0x7fff7fffu, mb = b[0] & 0x7fff7fffu;
 #pragma unroll
-  for (int w = 1; w < 4; ++w)
-    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[w] & 0x7fff7fffu));
-  group_steps<G>([&](auto c) {
-    const uint32_t o = dpp_u32<decltype(c)::value>(__builtin_bit_cast(uint32_t, m));
-    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, o));
-  });
-  return (uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16;
+  for (int w = 1; w < 4; ++w) {
+    ma = max_u16x2(ma, a[w] & 0x7fff7fffu);
+    mb = max_u16x2(mb, b[w] & 0x7fff7fffu);
+  }
+  uint32_t m = max_u16x2(__builtin_amdgcn_perm(mb, ma, 0x05040100u),
+                         __builtin_amdgcn_perm(mb, ma, 0x07060302u));
+  group_steps<8>([&](auto c) { m = max_u16x2(m, dpp_u32<decltype(c)::value>(m)); });
+  const uint32_t ea = pack8_scale(m << 16), eb = pack8_scale(m & 0xffff0000u);
+  scales = ea | eb << 8;
+  const u32x2 qa = pack8_bf16x8(a, pack8_inverse(ea)), qb = pack8_bf16x8(b, pack8_inverse(eb));
+  return u32x4{qa[0], qa[1], qb[0], qb[1]};
 }
 
 __device__ __forceinline__ float unpack8_scale(uint32_t scale) { return __uint_as_float(scale << 23); }
