@@ -414,8 +414,10 @@ int moe_amd_unpack8(const void* q, const void* scale, int64_t rows, int64_t cols
  * of eight gate features beside those of the same up features: gate_up_q
  * [S][I/8][gate 8, up 8], gate_up_scale [S][I/64][gate, up], both 16-byte
  * aligned.  Rows of sentinels are not written.  act_out is
- * moe_amd_gemm_gate_up_swiglu's, and the backward's results are
- * moe_amd_gemm_down_backward_dx_fused's on the restored gate_up, bit for bit. */
+ * moe_amd_gemm_gate_up_swiglu's bit for bit; the backward's results are
+ * moe_amd_gemm_down_backward_dx_fused's on the restored gate_up, with silu,
+ * act and d_act * up kept in fp32 where that rounds them to the bf16 of the
+ * forward. */
 int moe_amd_gemm_gate_up_swiglu_pack8(const void* hidden_states, const int32_t* row_src, int top_k,
                                       const int32_t* offsets, const void* tile_plan,
                                       const void* gate_up_proj, int64_t T, int64_t S, int E, int H,

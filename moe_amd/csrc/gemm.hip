@@ -216,8 +216,10 @@ __device__ __forceinline__ float fast_sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
 }
 
-// PACK: G1F saves gate_up packed to 8 bits (pack8.h), G2DXF reads it so; the
-// same tile, main loop and number of stores otherwise.
+// PACK: G1F saves gate_up packed to 8 bits (pack8.h), G2DXF reads it so, and
+// rounds each of its results once; the same tile, main loop and number of
+// stores otherwise.  L (T = 65536): G1F's epilogue takes 4% more of its time for
+// the packing, G2DXF as long as before; half of gate_up's memory and traffic.
 template <int MODE, int BR, bool PACK = false>
 __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
   static_assert(!PACK || MODE == G1F || MODE == G2DXF, "the GEMMs that hold gate_up");
@@ -1118,17 +1120,26 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const int e0 = 2 * w, e1 = 2 * w + 1;
-            const uint32_t slp = pack_bf2(t[e0], t[e1]);
-            sl[e0] = bf_lo(slp);
-            sl[e1] = bf_hi(slp);
-            const uint32_t ap = pack_bf2(sl[e0] * u[e0], sl[e1] * u[e1]);
-            a[e0] = bf_lo(ap);
-            a[e1] = bf_hi(ap);
             da[e0] = wgt * gq[e0];
             da[e1] = wgt * gq[e1];
-            const uint32_t dsp = pack_bf2(da[e0] * u[e0], da[e1] * u[e1]);
-            ds[e0] = bf_lo(dsp);
-            ds[e1] = bf_hi(dsp);
+            if constexpr (PACK) {  // no stored bits to agree with: each result is rounded once
+#pragma unroll
+              for (int e = e0; e <= e1; ++e) {
+                sl[e] = t[e];
+                a[e] = t[e] * u[e];
+                ds[e] = da[e] * u[e];
+              }
+            } else {
+              const uint32_t slp = pack_bf2(t[e0], t[e1]);
+              sl[e0] = bf_lo(slp);
+              sl[e1] = bf_hi(slp);
+              const uint32_t ap = pack_bf2(sl[e0] * u[e0], sl[e1] * u[e1]);
+              a[e0] = bf_lo(ap);
+              a[e1] = bf_hi(ap);
+              const uint32_t dsp = pack_bf2(da[e0] * u[e0], da[e1] * u[e1]);
+              ds[e0] = bf_lo(dsp);
+              ds[e1] = bf_hi(dsp);
+            }
             // sigmoid'(g) (1 + g) form: sg (1 + g (1 - sg)) = sg + t (1 - sg)
             dgv[w] = pack_bf2(ds[e0] * fmaf(t[e0], 1.f - sg[e0], sg[e0]),
                               ds[e1] * fmaf(t[e1], 1.f - sg[e1], sg[e1]));

@@ -1,6 +1,6 @@
 """8-bit activations: pack8 / unpack8 against their definition (exact
 arithmetic in fp64, so equality), the two GEMMs that keep gate_up in 8 bits
-against the ones that keep it in bf16 (bit for bit), and the layers' gradients
+against the ones that keep it in bf16, and the layers' gradients
 against the formulas in 64 bits and against differences."""
 from __future__ import annotations
 
@@ -219,8 +219,15 @@ def test_gemms_keep_gate_up_in_8_bits(T, H, E, K, I, skew):
     for wd in (w, w.to(BF)):
         want = ops.gemm_down_backward_fused(dout, plan, w2, restored, wd)
         have = ops.gemm_down_backward_fused(dout, plan, w2, q, wd)
-        for a, b, rows in zip(have, want, (n, n, T)):
-            assert torch.equal(a[:rows], b[:rows])
+        # the same products: d_gate_up and w * act with one rounding here, three
+        # there; the weight's gradient, a sum of g * act, with act's two there
+        for a, b, rows in zip(have[:2], want[:2], (n, n)):
+            a, b = a[:rows].double(), b[:rows].double()
+            assert ((a - b).abs() <= 4.05 * U * b.abs()).all()
+        y = ops.gemm_down_backward_fused(dout.abs(), plan, w2.abs(), restored.abs(), wd)[2]
+        uw = torch.finfo(wd.dtype).eps / 2
+        assert ((have[2] - want[2]).double().abs()
+                <= (2.05 * U * y.double() + 2 * uw * want[2].double().abs())).all()
 
 
 def test_sentinel_rows_are_left_alone():
@@ -264,8 +271,8 @@ def _grads(fn, tensors, dout):
 
 def _formula(x, idx, w, w1, w2, dout, keep):
     """{name: (value, bound)} in 64 bits.  Roundings to bf16 on the way, each
-    U relative: d_gate and d_up two, act two, w act three, d_x's rows one and
-    itself one, every gradient its own; sums of n products n V relative to the
+    U relative: d_gate, d_up and w act one, d_x's rows one and itself one, every
+    gradient its own; sums of n products n V relative to the
     sum of their magnitudes; the sigmoid's hardware exp and reciprocal 8 V."""
     T, H = x.shape
     E, I, K = w1.shape[0], w2.shape[2], idx.shape[1]
@@ -289,19 +296,19 @@ def _formula(x, idx, w, w1, w2, dout, keep):
         dgu = torch.cat([g * wk * up * dsig, g * wk * gate * sig], 1)
         # relative to (1 + |gate|) sig: dsig itself may cancel
         mag = torch.cat([g.abs() * wk * up.abs() * sig * (1 + gate.abs()), dgu[:, I:].abs()], 1)
-        tgu = 2.02 * U * dgu.abs() + 16 * V * mag + torch.cat(
+        tgu = 1.01 * U * dgu.abs() + 16 * V * mag + torch.cat(
             [tg * wk * (up * dsig).abs(), tg * wk * (gate * sig).abs()], 1)
         rows = dgu @ m1
         trows = tgu @ m1.abs() + 2 * I * V * (dgu.abs() @ m1.abs())
         dx.index_add_(0, t, rows)
         tx.index_add_(0, t, trows + U * (rows.abs() + trows))
         dw[t, k] = (g * act).sum(1)
-        tw[t, k] = ((2.02 * U + (I + 16) * V) * (g * act).abs() + tg * act.abs()).sum(1)
+        tw[t, k] = (((I + 16) * V) * (g * act).abs() + tg * act.abs()).sum(1)
         d1[e] = dgu.t() @ xk[t]
         t1[e] = tgu.t() @ xk[t].abs() + n * V * (dgu.abs().t() @ xk[t].abs())
         aw = act * wk
         d2[e] = do.t() @ aw
-        t2[e] = (3.04 * U + (n + 16) * V) * (do.abs().t() @ aw.abs())
+        t2[e] = (1.01 * U + (n + 16) * V) * (do.abs().t() @ aw.abs())
     tx = tx + K * V * dx.abs()
     res = {"dx": (dx, tx + U * (dx.abs() + tx)), "dw1": (d1, t1 + U * (d1.abs() + t1)),
            "dw2": (d2, t2 + U * (d2.abs() + t2))}
@@ -376,10 +383,9 @@ def test_one_node_layer_and_its_parts(keep):
     logits = ops.router_linear(x, wr)
     probs, w, idx = ops.router_softmax_topk(logits, K)
     plan = ops.permute(idx, E)
-    gu, act = ops.gemm_gate_up_swiglu(x, plan, w1)
-    gu = ops.unpack8(ops.pack8(gu))
+    gu8, _ = ops.gemm_gate_up_swiglu(x, plan, w1, pack8=True)
     xk = ops.unpack8(ops.pack8(x)) if keep == "int8_all" else x
-    dgu, aw, dw = ops.gemm_down_backward_fused(dout, plan, w2, gu, w)
+    dgu, aw, dw = ops.gemm_down_backward_fused(dout, plan, w2, gu8, w)
     dl = ops.router_softmax_topk_backward(probs, idx, dw, None, True, BF)
     rows = ops.gemm_gate_up_backward_dx(dgu, plan, w1)
     assert torch.equal(dx, ops.gather_backward(rows, plan, ops.router_linear_backward_dx(dl, wr)))
