@@ -361,6 +361,13 @@ __device__ __forceinline__ void store_route(const FewArgs& p, int t, int lane, f
   if (p.out_idx) p.out_idx[s] = ek;
 }
 
+// Entry s of a given routing: its expert, negative for padding, and weight.
+__device__ __forceinline__ int given_route(const FewArgs& p, int s, float& w) {
+  const int64_t id = p.ids[s];
+  w = p.weights_bf16 ? bf2f(((const bf16*)p.weights)[s]) : ((const float*)p.weights)[s];
+  return id >= 0 && id < p.E ? (int)id : -1;
+}
+
 // The tokens' top-K, one token a wave or (BLOCK) a workgroup; the last
 // workgroup to finish lists the active experts and their rows.  With the
 // routing given there is one workgroup, which lists.  Places in the list and
@@ -396,11 +403,10 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
     if (tid < S) e = one ? ids[tid] : get_shared(&p.real[tid]);
   } else {
     if (tid < S) {
-      const int64_t id = p.ids[tid];
-      if (id >= 0 && id < p.E) e = (int)id;
+      float w;
+      e = given_route(p, tid, w);
       p.real[tid] = e;
-      p.w[tid] = p.weights_bf16 ? bf2f(((const bf16*)p.weights)[tid])
-                                : ((const float*)p.weights)[tid];
+      p.w[tid] = w;
     }
     __syncthreads();
   }
@@ -426,8 +432,10 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 // L2.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
 // dealt to all of them in small pieces: with 16 features a workgroup one token
 // (K = 8, I = 768) has 384 for 256 CUs.
-// NV > 0: one token, routed by every workgroup for itself; slot k is its k-th
-// expert, and the first workgroup leaves the plan for the down kernel.
+// One token (NV != 0): slot k is its k-th entry, and the first workgroup leaves
+// the plan for the down kernel.  NV > 0: every workgroup routes the token for
+// itself, up to 64 NV experts; kGiven: the routing is given.
+constexpr int kGiven = -1;
 template <typename T, int CH, int NV>
 __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   __shared__ f32x4 red[kWaves][64];
@@ -437,23 +445,27 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int4 info;
-  if constexpr (NV > 0) {
+  if constexpr (NV != 0) {
     if (wid == 0) {
-      float wk;
-      int ek;
-      route_token<NV, false>(p, p.logits, nullptr, 0, lane, wk, ek);
+      float wk = 0.f;
+      int ek = -1;
+      if constexpr (NV > 0) route_token<NV, false>(p, p.logits, nullptr, 0, lane, wk, ek);
+      else if (lane < p.K) ek = given_route(p, lane, wk);
       if (lane == slot) s_e = ek;
       if (blockIdx.x == 0) {
-        store_route(p, 0, lane, wk, ek);
+        const uint64_t real = __ballot(lane < p.K && ek >= 0);
         if (lane < p.K) {
-          p.list[lane] = make_int4(ek, lane, 1, 0);
+          if (ek >= 0)
+            p.list[__popcll(real & ((1ull << lane) - 1))] = make_int4(ek, lane, 1, 0);
           p.rows[lane] = lane;
         }
-        if (lane == 0) p.hdr[0] = p.K;
+        if (lane == 0) p.hdr[0] = __popcll(real);
+        store_route(p, 0, lane, wk, ek);
       }
     }
     __syncthreads();
     info = make_int4(__builtin_amdgcn_readfirstlane(s_e), 0, 1, 0);
+    if (info.x < 0) return;
   } else {
     const int nact = p.hdr[0];
     info = p.list[slot];  // a slot past the active experts holds anything
@@ -466,7 +478,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
                   ((int64_t)info.x * 2 * p.I + f0 + (n & 7) + (n >> 3) * p.I) * ld + g * 16;
   for (int rg = 0; rg < info.z; rg += 16) {
     const int left = info.z - rg;
-    const int token = NV > 0 ? 0 : p.rows[info.y + rg + min(n, left - 1)] / p.K;
+    const int token = NV != 0 ? 0 : p.rows[info.y + rg + min(n, left - 1)] / p.K;
     const uint32_t xo = (uint32_t)token * (uint32_t)ld + g * 16;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     chunks<CH>(s0, s1, [&](auto ch, int s) {
@@ -492,7 +504,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
           gs += red[q][l][f & 3];
           us += red[q][l + 32][f & 3];
         }
-        const int s = NV > 0 ? slot : p.rows[info.y + rg + r];
+        const int s = NV != 0 ? slot : p.rows[info.y + rg + r];
         ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
       }
     }
@@ -693,8 +705,9 @@ hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   const int threads = 64 * kWaves, gu_grid = slots * (p.I / 8);
   const auto plan = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
-    if (p.wr && p.T == 1 && !wide) {
-      few_gate_up_kernel<T, 8, NV><<<gu_grid, threads, 0, st>>>(p);
+    if (p.T == 1 && !wide) {
+      if (p.wr) few_gate_up_kernel<T, 8, NV><<<gu_grid, threads, 0, st>>>(p);
+      else few_gate_up_kernel<T, 8, kGiven><<<S * (p.I / 8), threads, 0, st>>>(p);
       return;
     }
     if (wide) {

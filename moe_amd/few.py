@@ -44,9 +44,11 @@ def experts_forward_few(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
     [0, E) contribute nothing."""
     _refuse_grad("experts_forward_few", hidden_states, top_k_weights, gate_up_proj, down_proj)
     op = (torch.ops.moe_amd.experts_few if torch.compiler.is_compiling() else ops.experts_few)
-    out = op(hidden_states.to(gate_up_proj.dtype), top_k_index, top_k_weights, gate_up_proj,
-             down_proj)
-    return out.to(hidden_states.dtype)
+    dtype = hidden_states.dtype
+    if dtype == gate_up_proj.dtype:
+        return op(hidden_states, top_k_index, top_k_weights, gate_up_proj, down_proj)
+    return op(hidden_states.to(gate_up_proj.dtype), top_k_index, top_k_weights, gate_up_proj,
+              down_proj).to(dtype)
 
 
 def moe_layer_few(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tensor,

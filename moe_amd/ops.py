@@ -858,9 +858,14 @@ def _few_inputs(name: str, x, gate_up_proj, down_proj, K: int):
     return E, H, I2 // 2
 
 
+@functools.lru_cache(maxsize=256)
+def _few_workspace_size(*shape: int) -> int:
+    return max(int(_lib.load().moe_amd_few_workspace_size(*shape)), 16)
+
+
 def _few_workspace(x, E, K, H, I) -> torch.Tensor:
-    n = _lib.load().moe_amd_few_workspace_size(x.shape[0], E, K, H, I, _dtype_code(x.dtype))
-    return torch.empty(max(int(n), 16), device=x.device, dtype=torch.uint8)
+    n = _few_workspace_size(x.shape[0], E, K, H, I, _dtype_code(x.dtype))
+    return torch.empty(n, device=x.device, dtype=torch.uint8)
 
 
 @on_tensor_device
@@ -876,8 +881,9 @@ def experts_few(x: torch.Tensor, topk_index: torch.Tensor, topk_weights: torch.T
     T, K = topk_index.shape
     E, H, I = _few_inputs("experts_few", x, gate_up_proj, down_proj, K)
     x, gate_up_proj, down_proj = _contig(x), _contig(gate_up_proj), _contig(down_proj)
-    topk_index = _contig(topk_index.to(torch.int64))
-    topk_weights = _contig(topk_weights)
+    if topk_index.dtype != torch.int64:
+        topk_index = topk_index.to(torch.int64)
+    topk_index, topk_weights = _contig(topk_index), _contig(topk_weights)
     ws = _few_workspace(x, E, K, H, I)
     out = torch.empty(T, H, device=x.device, dtype=x.dtype)
     _call("moe_amd_experts_few", x.data_ptr(), topk_index.data_ptr(), topk_weights.data_ptr(),

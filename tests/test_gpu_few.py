@@ -134,6 +134,25 @@ def test_padding_contributes_nothing(dt):
     assert (few.experts_forward_few(x, torch.full_like(idx, E), w, w1, w2) == 0).all()
 
 
+@pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("ids", [[5, -1, 7, 0], [-1, 5, 9, 7], [9, -1, 1 << 33, -3], [2, 2, 7, 2],
+                                 [0, 1, 2, 3], [8, 8, 8, 7]])
+def test_one_token_with_padding_and_repeats(ids, dt):
+    print(f"experts_few one token {ids}", flush=True)
+    H, E, I = 320, 8, 192
+    g = _gen(15)
+    x = torch.randn(1, H, generator=g, device=DEV).to(dt)
+    w1, w2 = _weights(g, E, H, I, dt)
+    idx = torch.tensor([ids], device=DEV)
+    w = torch.rand(1, 4, generator=g, device=DEV)
+    w[idx.lt(0) | idx.ge(E)] = float("nan")
+    got = few.experts_forward_few(x, idx, w, w1, w2)
+    _close(got, *_oracle(x, idx, torch.nan_to_num(w), w1, w2))
+    # as one of several tokens: the same sums
+    many = few.experts_forward_few(x.repeat(3, 1), idx.repeat(3, 1), w.repeat(3, 1), w1, w2)
+    assert torch.equal(many, got.expand(3, H))
+
+
 def test_a_value_that_is_not_finite_stays_with_its_token():
     print("experts_few not finite", flush=True)
     T, H, E, K, I = 19, 256, 2, 2, 64
