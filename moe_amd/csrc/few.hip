@@ -47,8 +47,8 @@ struct FewArgs {
   int T, E, K, H, I;
   float* logits;           // workspace from here on
   float* w;                // [S]
-  int* hdr;                // [0] active experts, [1] finished routing workgroups
-  int4* list;              // {expert, first row, rows, 0} of the active experts
+  int* hdr;                // [0] entries of the list, [1] finished routing workgroups
+  int4* list;              // {expert, first row, rows <= 16, 0} of the active experts
   int* rows;               // flat entries s = t*K + k by active expert, ascending
   void* act;               // [S,I] by flat entry
   int* real;               // [S] the entry's expert, negative for padding
@@ -369,8 +369,11 @@ __device__ __forceinline__ int given_route(const FewArgs& p, int s, float& w) {
 }
 
 // The tokens' top-K, one token a wave or (BLOCK) a workgroup; the last
-// workgroup to finish lists the active experts and their rows.  With the
-// routing given there is one workgroup, which lists.  Places in the list and
+// workgroup to finish lists the active experts and their rows, at most 16 (an
+// MFMA's columns) an entry: an expert with more has several entries, which run
+// side by side and find its weights in L2.  (One after the other in a workgroup:
+// 61 us for 64 rows in each of 4 experts, H = 2048, I = 768.)  With the routing
+// given there is one workgroup, which lists.  Places in the list and
 // among an expert's rows are taken with LDS atomics: their order may differ
 // from call to call, which no result depends on (rows are computed apart, and
 // combined by their number).
@@ -416,9 +419,12 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
   const int cnt = lead ? count[e] : 0;
   __syncthreads();
   if (lead) {
-    const int at = atomicAdd(&total, 1 << 16 | cnt);  // experts and rows before it
-    p.list[at >> 16] = make_int4(e, at & 0xffff, cnt, 0);
-    count[e] = at & 0xffff;
+    const int n = (cnt + 15) / 16;
+    const int at = atomicAdd(&total, n << 16 | cnt);  // entries and rows before it
+    const int r0 = at & 0xffff;
+    for (int i = 0; i < n; ++i)
+      p.list[(at >> 16) + i] = make_int4(e, r0 + 16 * i, min(16, cnt - 16 * i), 0);
+    count[e] = r0;
   }
   __syncthreads();
   if (e >= 0) p.rows[count[e] + rank] = tid;
@@ -426,10 +432,8 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 }
 
 // ------------------------------------------------------- gate/up + SwiGLU
-// Workgroup: 8 features of one active expert, their gate and up rows being the
-// 16 rows of the A operand; the waves split H, CH steps in flight each.  An
-// expert with more than 16 rows reads its weights again for the next 16, from
-// L2.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
+// Workgroup: 8 features of one entry of the list, their gate and up rows being
+// the 16 rows of the A operand; the waves split H, CH steps in flight each.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
 // dealt to all of them in small pieces: with 16 features a workgroup one token
 // (K = 8, I = 768) has 384 for 256 CUs.
 // One token (NV != 0): slot k is its k-th entry, and the first workgroup leaves
@@ -476,43 +480,37 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   const int64_t ld = (int64_t)p.H * sizeof(T);
   const char* w = (const char*)p.w1 +
                   ((int64_t)info.x * 2 * p.I + f0 + (n & 7) + (n >> 3) * p.I) * ld + g * 16;
-  for (int rg = 0; rg < info.z; rg += 16) {
-    const int left = info.z - rg;
-    const int token = NV != 0 ? 0 : p.rows[info.y + rg + min(n, left - 1)] / p.K;
-    const uint32_t xo = (uint32_t)token * (uint32_t)ld + g * 16;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    chunks<CH>(s0, s1, [&](auto ch, int s) {
-      constexpr int C = decltype(ch)::value;
-      const char *ws = w + s * 64, *xs = (const char*)p.x + s * 64;
-      u32x4 a[C], c[C];
+  const int token = NV != 0 ? 0 : p.rows[info.y + min(n, info.z - 1)] / p.K;
+  const uint32_t xo = (uint32_t)token * (uint32_t)ld + g * 16;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  chunks<CH>(s0, s1, [&](auto ch, int s) {
+    constexpr int C = decltype(ch)::value;
+    const char *ws = w + s * 64, *xs = (const char*)p.x + s * 64;
+    u32x4 a[C], c[C];
 #pragma unroll
-      for (int i = 0; i < C; ++i) a[i] = ld16(ws, 0, i * 64);
+    for (int i = 0; i < C; ++i) a[i] = ld16(ws, 0, i * 64);
 #pragma unroll
-      for (int i = 0; i < C; ++i) c[i] = ld16(xs, xo, i * 64);
+    for (int i = 0; i < C; ++i) c[i] = ld16(xs, xo, i * 64);
 #pragma unroll
-      for (int i = 0; i < C; ++i) acc = Mma<T>::step(a[i], c[i], acc);
-    });
-    if (rg) __syncthreads();
-    red[wid][lane] = acc;
-    __syncthreads();
-    if (threadIdx.x < 128) {
-      const int f = threadIdx.x & 7, r = threadIdx.x >> 3, l = (f >> 2) * 16 + r;
-      if (r < left) {
-        float gs = 0.f, us = 0.f;
+    for (int i = 0; i < C; ++i) acc = Mma<T>::step(a[i], c[i], acc);
+  });
+  red[wid][lane] = acc;
+  __syncthreads();
+  if (threadIdx.x >= 128) return;
+  const int f = threadIdx.x & 7, r = threadIdx.x >> 3, l = (f >> 2) * 16 + r;
+  if (r >= info.z) return;
+  float gs = 0.f, us = 0.f;
 #pragma unroll
-        for (int q = 0; q < kWaves; ++q) {
-          gs += red[q][l][f & 3];
-          us += red[q][l + 32][f & 3];
-        }
-        const int s = NV != 0 ? slot : p.rows[info.y + rg + r];
-        ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
-      }
-    }
+  for (int q = 0; q < kWaves; ++q) {
+    gs += red[q][l][f & 3];
+    us += red[q][l + 32][f & 3];
   }
+  const int s = NV != 0 ? slot : p.rows[info.y + r];
+  ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
 }
 
 // --------------------------------------------------------- down + combine
-// Workgroup: C = 16 / parts columns of the output and every active expert; a
+// Workgroup: C = 16 / parts columns of the output and every entry of the list; a
 // wave takes the next one when it is done with its own (the oldest waves get
 // their loads first: with a fixed share each, they end after half of the time
 // and the rest finishes with too few loads in flight).  `parts` makes the column slices about as many
@@ -621,7 +619,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
     u32x4 a0[CH], b0[CH], a1[CH], b1[CH];
     rows(c);
     load(c, a0, b0);
-    // Past the wave's last expert the last addresses are loaded again, unused:
+    // Past the wave's last entry the last addresses are loaded again, unused:
     // with a branch around the loads the compiler waits for all of them.
     while (true) {
       const Pos d = next(c);
@@ -697,7 +695,8 @@ int few_check(int64_t T, int K, int E, int H, int I, int dtype, const char* who)
 
 template <typename T>
 hipError_t few_launch(const FewArgs& p, hipStream_t st) {
-  const int S = p.T * p.K, slots = S < p.E ? S : p.E;
+  // entries of the list: an expert's last one may be short, the others are full
+  const int S = p.T * p.K, slots = S < p.E + S / 16 ? S : p.E + S / 16;
   if (p.wr) few_logits_kernel<T><<<dim3((p.E + 15) / 16, (p.T + 15) / 16), 64 * kWaves, 0, st>>>(p);
   // One wave routes a token of up to 256 experts, a workgroup one of more (with
   // 28 entries a lane, one wave took 46 us for each of 64 tokens, E = 1792).
