@@ -32,7 +32,7 @@ constexpr int kFewExperts = 4096;
 constexpr int kFewRows = kFewTokens * kFewTopK;
 constexpr int kWaves = 8;        // waves per workgroup of the GEMV kernels
 constexpr int kPlanWaves = 16;
-constexpr int kMaxLds = kFewRows * (16 + 64 + 12);  // of the down kernel
+constexpr int kGateUpChunk = 4;  // blocks in flight of a gate/up wave
 
 struct FewArgs {
   const void* x;           // [T,H]
@@ -57,37 +57,61 @@ struct FewArgs {
   void* out;
 };
 
-template <typename T> struct Mma;
 // One step of a contraction: 64 bytes of each of 16 rows, lane l holding 16
 // bytes of row l % 16 at chunk l / 16; A and B alike, so which k a lane's
 // elements are does not matter.
-template <> struct Mma<bf16> {
-  static constexpr int kStep = 32;
-  static __device__ __forceinline__ f32x4 step(const u32x4& a, const u32x4& b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-  }
-};
-template <> struct Mma<float> {
-  static constexpr int kStep = 16;
-  static __device__ __forceinline__ f32x4 step(const u32x4& a, const u32x4& b, f32x4 c) {
-    const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
+__device__ __forceinline__ f32x4 mma_step(bf16, const u32x4& a, const u32x4& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma_step(float, const u32x4& a, const u32x4& b, f32x4 c) {
+  const f32x4 fa = __builtin_bit_cast(f32x4, a), fb = __builtin_bit_cast(f32x4, b);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[i], c, 0, 0, 0);
-    return c;
-  }
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[i], c, 0, 0, 0);
+  return c;
+}
+
+// A block of a contraction: 128 bytes, a whole line, of each operand's 16 rows.
+// Lane l loads 16 bytes of rows l / 8 and 8 + l / 8, so that 16 lanes of a load
+// cover two lines, and the wave turns the block to the MFMA's layout in 4 KB of
+// LDS of its own (16-byte chunks XOR-swizzled by row: no bank conflicts).  Loaded
+// straight into that layout, 16 lanes touch 16 lines and a CU takes in 38 KB/us
+// of both operands together, 1 KB in 64 cycles.
+constexpr int kBlock = 128;
+constexpr int kBlockLds = 4 * 1024;  // of a wave
+constexpr int kMaxLds = kWaves * kBlockLds + kFewRows * (16 + 64 + 12);  // of the down kernel
+struct Block {
+  u32x4 a0, a1, b0, b1;
 };
+template <typename T>
+__device__ __forceinline__ f32x4 mma_block(const Block& v, char* lds, int lane, f32x4 acc) {
+  const int r = lane >> 3, n = lane & 15, g = lane >> 4;
+  char* w = lds + r * kBlock + ((lane & 7) ^ r) * 16;
+  *(u32x4*)w = v.a0;
+  *(u32x4*)(w + 1024) = v.a1;
+  *(u32x4*)(w + 2048) = v.b0;
+  *(u32x4*)(w + 3072) = v.b1;
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const char* q = lds + n * kBlock + ((t * 4 + g) ^ (n & 7)) * 16;
+    acc = mma_step(T{}, *(const u32x4*)q, *(const u32x4*)(q + 2048), acc);
+  }
+  __builtin_amdgcn_wave_barrier();  // the next block's writes stay behind these reads
+  return acc;
+}
 
 // 16 bytes of a row of a wave-uniform base: the lane's part of the address has
-// 32 bits and a step's is an immediate, which keeps a chunk of loads short (a
+// 32 bits and a block's is an immediate, which keeps a chunk of loads short (a
 // workgroup of these kernels runs each instruction once or twice, so fetching
 // them is part of its time).
 __device__ __forceinline__ u32x4 ld16(const char* base, uint32_t lane_off, int imm = 0) {
   return *(const u32x4*)(base + lane_off + imm);
 }
 
-// f(chunk length, first step) over the steps [s, end): chunks of CH, then the
+// f(chunk length, first block) over the blocks [s, end): chunks of CH, then the
 // rest in halves.
 template <int CH, typename F>
 __device__ __forceinline__ void chunks(int s, int end, F&& f) {
@@ -124,30 +148,31 @@ __device__ __forceinline__ bool last_to_arrive(int* counter, int of, int* box) {
 // clears the counter that the routing workgroups finish by.
 template <typename T>
 __global__ __launch_bounds__(64 * kWaves) void few_logits_kernel(FewArgs p) {
+  __shared__ __attribute__((aligned(16))) char turn[kWaves][kBlockLds];
   __shared__ f32x4 red[kWaves][64];
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, r = lane >> 3;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int e0 = blockIdx.x * 16;
-  const int ns = p.H / Mma<T>::kStep;
-  const int s0 = wid * ns / kWaves, s1 = (wid + 1) * ns / kWaves;
-  const int64_t ld = (int64_t)p.H * sizeof(T);
-  const uint32_t ao = (uint32_t)(min(e0 + n, p.E - 1) - e0) * (uint32_t)ld + g * 16;
-  const int t0 = blockIdx.y * 16;
-  const uint32_t bo = (uint32_t)min(t0 + n, p.T - 1) * (uint32_t)ld + g * 16;
-  const char* a = (const char*)p.wr + e0 * ld;
+  const int e0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
+  const int nb = p.H * (int)sizeof(T) / kBlock;
+  const uint32_t ld = (uint32_t)p.H * sizeof(T), j = (lane & 7) * 16;
+  const uint32_t a0 = min(r, p.E - 1 - e0) * ld + j, a1 = min(r + 8, p.E - 1 - e0) * ld + j;
+  const uint32_t b0 = min(t0 + r, p.T - 1) * ld + j, b1 = min(t0 + r + 8, p.T - 1) * ld + j;
+  const char* a = (const char*)p.wr + (int64_t)e0 * ld;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  auto chunk = [&](auto ch, int s) {
-    constexpr int CH = decltype(ch)::value;
-    const char *as = a + s * 64, *bs = (const char*)p.x + s * 64;
-    u32x4 va[CH], vb[CH];
+  chunks<4>(wid * nb / kWaves, (wid + 1) * nb / kWaves, [&](auto ch, int s) {
+    constexpr int C = decltype(ch)::value;
+    const char *as = a + s * kBlock, *bs = (const char*)p.x + s * kBlock;
+    Block v[C];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) va[i] = ld16(as, ao, i * 64);
+    for (int i = 0; i < C; ++i) {
+      v[i].a0 = ld16(as, a0, i * kBlock);
+      v[i].a1 = ld16(as, a1, i * kBlock);
+      v[i].b0 = ld16(bs, b0, i * kBlock);
+      v[i].b1 = ld16(bs, b1, i * kBlock);
+    }
 #pragma unroll
-    for (int i = 0; i < CH; ++i) vb[i] = ld16(bs, bo, i * 64);
-#pragma unroll
-    for (int i = 0; i < CH; ++i) acc = Mma<T>::step(va[i], vb[i], acc);
-  };
-  chunks<8>(s0, s1, chunk);
+    for (int i = 0; i < C; ++i) acc = mma_block<T>(v[i], turn[wid], lane, acc);
+  });
   red[wid][lane] = acc;
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.hdr[1] = 0;
   __syncthreads();
@@ -433,7 +458,7 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 
 // ------------------------------------------------------- gate/up + SwiGLU
 // Workgroup: 8 features of one entry of the list, their gate and up rows being
-// the 16 rows of the A operand; the waves split H, CH steps in flight each.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
+// the 16 rows of the A operand; the waves split H, CH blocks in flight each.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
 // dealt to all of them in small pieces: with 16 features a workgroup one token
 // (K = 8, I = 768) has 384 for 256 CUs.
 // One token (NV != 0): slot k is its k-th entry, and the first workgroup leaves
@@ -442,11 +467,11 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 constexpr int kGiven = -1;
 template <typename T, int CH, int NV>
 __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
-  __shared__ f32x4 red[kWaves][64];
+  __shared__ __attribute__((aligned(16))) char turn[kWaves][kBlockLds];
   __shared__ int s_e;
   const int nsl = p.I / 8;
   const int slot = blockIdx.x / nsl, f0 = (blockIdx.x % nsl) * 8;
-  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int4 info;
   if constexpr (NV != 0) {
@@ -475,25 +500,34 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
     info = p.list[slot];  // a slot past the active experts holds anything
     if (slot >= nact) return;
   }
-  const int ns = p.H / Mma<T>::kStep;
-  const int s0 = wid * ns / kWaves, s1 = (wid + 1) * ns / kWaves;
-  const int64_t ld = (int64_t)p.H * sizeof(T);
-  const char* w = (const char*)p.w1 +
-                  ((int64_t)info.x * 2 * p.I + f0 + (n & 7) + (n >> 3) * p.I) * ld + g * 16;
-  const int token = NV != 0 ? 0 : p.rows[info.y + min(n, info.z - 1)] / p.K;
-  const uint32_t xo = (uint32_t)token * (uint32_t)ld + g * 16;
+  const int nb = p.H * (int)sizeof(T) / kBlock, row = lane >> 3;
+  const uint32_t ld = (uint32_t)p.H * sizeof(T), j = (lane & 7) * 16;
+  const char* wg = (const char*)p.w1 + ((int64_t)info.x * 2 * p.I + f0) * ld;
+  const char* wu = wg + (int64_t)p.I * ld;
+  const uint32_t wo = row * ld + j;
+  const auto token = [&](int i) -> uint32_t {  // of the entry's row i, or its last
+    return NV != 0 ? 0 : p.rows[info.y + min(i, info.z - 1)] / p.K;
+  };
+  const uint32_t x0 = token(row) * ld + j, x1 = token(row + 8) * ld + j;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  chunks<CH>(s0, s1, [&](auto ch, int s) {
+  chunks<CH>(wid * nb / kWaves, (wid + 1) * nb / kWaves, [&](auto ch, int s) {
     constexpr int C = decltype(ch)::value;
-    const char *ws = w + s * 64, *xs = (const char*)p.x + s * 64;
-    u32x4 a[C], c[C];
+    const char *gs = wg + s * kBlock, *us = wu + s * kBlock, *xs = (const char*)p.x + s * kBlock;
+    Block v[C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) a[i] = ld16(ws, 0, i * 64);
+    for (int i = 0; i < C; ++i) {
+      v[i].a0 = ld16(gs, wo, i * kBlock);
+      v[i].a1 = ld16(us, wo, i * kBlock);
+    }
 #pragma unroll
-    for (int i = 0; i < C; ++i) c[i] = ld16(xs, xo, i * 64);
+    for (int i = 0; i < C; ++i) {
+      v[i].b0 = ld16(xs, x0, i * kBlock);
+      v[i].b1 = ld16(xs, x1, i * kBlock);
+    }
 #pragma unroll
-    for (int i = 0; i < C; ++i) acc = Mma<T>::step(a[i], c[i], acc);
+    for (int i = 0; i < C; ++i) acc = mma_block<T>(v[i], turn[wid], lane, acc);
   });
+  f32x4(*red)[kBlockLds / 16] = (f32x4(*)[kBlockLds / 16])turn;  // in each wave's own part
   red[wid][lane] = acc;
   __syncthreads();
   if (threadIdx.x >= 128) return;
@@ -517,14 +551,14 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
 // as CUs: the A operand's 16 rows are C columns' weights for each of `parts`
 // pieces of the contraction, B's 16 columns C of the expert's rows for each of
 // them, and the blocks of the product where the pieces match are added.
-// A wave needs no other one: it reads CH steps and the next CH before it
+// A wave needs no other one: it reads CH blocks and the next CH before it
 // multiplies these, and leaves y in LDS, where the workgroup then sums it with
 // the routing weights, in k order.
 template <typename T, int CH>
 __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int parts) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int S = p.T * p.K, C = 16 / parts;
-  int4* s_list = (int4*)lds;
+  int4* s_list = (int4*)(lds + kWaves * kBlockLds);
   float* s_y = (float*)(s_list + S);   // [S][C]
   int* s_rows = (int*)(s_y + S * C);
   float* s_w = (float*)(s_rows + S);
@@ -542,29 +576,33 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
   }
   if (tid == 0) s_next = kWaves;
   __syncthreads();
-  const int ns = p.I / Mma<T>::kStep / parts;
-  const int64_t ld = (int64_t)p.I * sizeof(T);
+  const int nb = p.I * (int)sizeof(T) / kBlock / parts;  // of a piece
+  const uint32_t ld = (uint32_t)p.I * sizeof(T);
   struct Pos {
     int q, rg, sb;
     bool more;
     int4 info;
     const char* w;
-    uint32_t a;
+    uint32_t b0, b1;
   };
-  const int nc = n % C;
-  const uint32_t piece = n / C * ns * 64 + g * 16;
-  const uint32_t wo = (uint32_t)nc * (uint32_t)ld + piece;
+  // the lane's two rows of a tile: a column or an entry's row, and a piece
+  const int c0 = (lane >> 3) % C, c1 = ((lane >> 3) + 8) % C;
+  const uint32_t j = (lane & 7) * 16;
+  const uint32_t p0 = (lane >> 3) / C * nb * kBlock + j, p1 = ((lane >> 3) + 8) / C * nb * kBlock + j;
+  const uint32_t a0 = c0 * ld + p0, a1 = c1 * ld + p1;
   auto start = [&](Pos& c) {
     c.more = c.q < nact;
     if (!c.more) return;
     c.info = s_list[c.q];
-    c.w = (const char*)p.w2 + ((int64_t)c.info.x * p.H + h0) * ld;
+    c.w = (const char*)p.w2 + ((int64_t)c.info.x * p.H + h0) * (int64_t)ld;
   };
   auto rows = [&](Pos& c) {
-    c.a = (uint32_t)s_rows[c.info.y + c.rg + min(nc, c.info.z - c.rg - 1)] * (uint32_t)ld + piece;
+    const int left = c.info.z - c.rg - 1, at = c.info.y + c.rg;
+    c.b0 = (uint32_t)s_rows[at + min(c0, left)] * ld + p0;
+    c.b1 = (uint32_t)s_rows[at + min(c1, left)] * ld + p1;
   };
   auto next = [&](Pos c) {  // without one: more false, the addresses as they were
-    if (c.sb + CH < ns) {
+    if (c.sb + CH < nb) {
       c.sb += CH;
       return c;
     }
@@ -581,27 +619,28 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
     return c;
   };
   // The last chunk of a contraction that CH does not divide starts earlier: its
-  // first steps are the previous chunk's and are passed over.
-  auto load = [&](const Pos& c, u32x4 (&a)[CH], u32x4 (&b)[CH]) {
-    const int sb = min(c.sb, ns - CH);
-    const char *ws = c.w + sb * 64, *as = (const char*)p.act + sb * 64;
+  // first blocks are the previous chunk's and are passed over.
+  auto load = [&](const Pos& c, Block (&v)[CH]) {
+    const int sb = min(c.sb, nb - CH);
+    const char *ws = c.w + sb * kBlock, *as = (const char*)p.act + sb * kBlock;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) a[i] = ld16(ws, wo, i * 64);
+    for (int i = 0; i < CH; ++i) {
+      v[i].a0 = ld16(ws, a0, i * kBlock);
+      v[i].a1 = ld16(ws, a1, i * kBlock);
+    }
 #pragma unroll
-    for (int i = 0; i < CH; ++i) b[i] = ld16(as, c.a, i * 64);
+    for (int i = 0; i < CH; ++i) {
+      v[i].b0 = ld16(as, c.b0, i * kBlock);
+      v[i].b1 = ld16(as, c.b1, i * kBlock);
+    }
   };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  auto step = [&](const Pos& c, const u32x4 (&a)[CH], const u32x4 (&b)[CH]) {
-    const int skip = c.sb - min(c.sb, ns - CH);
-    if (skip == 0) {
+  auto step = [&](const Pos& c, const Block (&v)[CH]) {
+    const int skip = c.sb - min(c.sb, nb - CH);
 #pragma unroll
-      for (int i = 0; i < CH; ++i) acc = Mma<T>::step(a[i], b[i], acc);
-    } else {
-#pragma unroll
-      for (int i = 1; i < CH; ++i)
-        if (i >= skip) acc = Mma<T>::step(a[i], b[i], acc);
-    }
-    if (c.sb + CH < ns) return;
+    for (int i = 0; i < CH; ++i)
+      if (i >= skip) acc = mma_block<T>(v[i], lds + wid * kBlockLds, lane, acc);
+    if (c.sb + CH < nb) return;
     // lane (n, g) holds rows 4g .. 4g+3 of column n: the block of piece f starts
     // 16 (C/4) + C = 5C lanes after that of piece f - 1
     f32x4 y = acc;
@@ -616,19 +655,19 @@ __global__ __launch_bounds__(64 * kWaves) void few_down_kernel(FewArgs p, int pa
   c.q = wid;
   start(c);
   if (c.more) {
-    u32x4 a0[CH], b0[CH], a1[CH], b1[CH];
+    Block u[CH], v[CH];
     rows(c);
-    load(c, a0, b0);
+    load(c, u);
     // Past the wave's last entry the last addresses are loaded again, unused:
     // with a branch around the loads the compiler waits for all of them.
     while (true) {
       const Pos d = next(c);
-      load(d, a1, b1);
-      step(c, a0, b0);
+      load(d, v);
+      step(c, u);
       if (!d.more) break;
       c = next(d);
-      load(c, a0, b0);
-      step(d, a1, b1);
+      load(c, u);
+      step(d, v);
       if (!c.more) break;
     }
   }
@@ -705,8 +744,8 @@ hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   const auto plan = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
     if (p.T == 1 && !wide) {
-      if (p.wr) few_gate_up_kernel<T, 8, NV><<<gu_grid, threads, 0, st>>>(p);
-      else few_gate_up_kernel<T, 8, kGiven><<<S * (p.I / 8), threads, 0, st>>>(p);
+      if (p.wr) few_gate_up_kernel<T, kGateUpChunk, NV><<<gu_grid, threads, 0, st>>>(p);
+      else few_gate_up_kernel<T, kGateUpChunk, kGiven><<<S * (p.I / 8), threads, 0, st>>>(p);
       return;
     }
     if (wide) {
@@ -718,7 +757,7 @@ hipError_t few_launch(const FewArgs& p, hipStream_t st) {
       const int entries = (S + 63) / 64;
       few_plan_kernel<NV, false><<<nr, 64 * (tokens > entries ? tokens : entries), 0, st>>>(p);
     }
-    few_gate_up_kernel<T, 8, 0><<<gu_grid, threads, 0, st>>>(p);
+    few_gate_up_kernel<T, kGateUpChunk, 0><<<gu_grid, threads, 0, st>>>(p);
   };
   const int part = wide ? (p.E + kPlanWaves - 1) / kPlanWaves : p.wr ? p.E : 1;
   if (part <= 64) plan(std::integral_constant<int, 1>{});
@@ -726,16 +765,16 @@ hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   else plan(std::integral_constant<int, 4>{});
   // column slices of 16 / parts: about one for every CU
   int parts = p.H / 16 >= 256 ? 1 : p.H / 8 >= 256 ? 2 : 4;
-  const int steps = p.I / Mma<T>::kStep;
-  while (steps % parts) parts /= 2;
-  const int ns = steps / parts;
-  const int lds = S * (16 + 64 / parts + 12);
-  // the chunk of the fewest rounds and steps read twice; never more steps than
-  // there are, as a step past the end is another row's or nobody's
+  const int blocks = p.I * (int)sizeof(T) / kBlock;
+  while (blocks % parts) parts /= 2;
+  const int nb = blocks / parts;
+  const int lds = kWaves * kBlockLds + S * (16 + 64 / parts + 12);
+  // the chunk of the fewest rounds and blocks read twice; never more than there
+  // are, as a block past the end is another row's or nobody's
   int ch = 1;
-  const auto cost = [&](int c) { return (ns + c - 1) / c * (c + 2); };
-  for (int c : {2, 4, 6, 8})
-    if (c <= ns && cost(c) <= cost(ch)) ch = c;
+  const auto cost = [&](int c) { return (nb + c - 1) / c * (c + 1); };
+  for (int c : {2, 3, 4})
+    if (c <= nb && cost(c) <= cost(ch)) ch = c;
   auto down = [&](auto c) -> hipError_t {
     static std::atomic<int> done[64];
     constexpr int CH = decltype(c)::value;
@@ -747,9 +786,8 @@ hipError_t few_launch(const FewArgs& p, hipStream_t st) {
     few_down_kernel<T, CH><<<p.H * parts / 16, 64 * kWaves, lds, st>>>(p, parts);
     return hipSuccess;
   };
-  if (ch == 8) return down(std::integral_constant<int, 8>{});
-  if (ch == 6) return down(std::integral_constant<int, 6>{});
   if (ch == 4) return down(std::integral_constant<int, 4>{});
+  if (ch == 3) return down(std::integral_constant<int, 3>{});
   if (ch == 2) return down(std::integral_constant<int, 2>{});
   return down(std::integral_constant<int, 1>{});
 }
