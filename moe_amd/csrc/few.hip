@@ -32,7 +32,9 @@ constexpr int kFewExperts = 4096;
 constexpr int kFewRows = kFewTokens * kFewTopK;
 constexpr int kWaves = 8;        // waves per workgroup of the GEMV kernels
 constexpr int kPlanWaves = 16;
-constexpr int kGateUpChunk = 4;  // blocks in flight of a gate/up wave
+// Blocks in flight of a gate/up wave: two leave room for four workgroups a CU (T = 64,
+// E = 128: 218 us; four and two workgroups 228, one 219).
+constexpr int kGateUpChunk = 2;
 
 struct FewArgs {
   const void* x;           // [T,H]
