@@ -98,7 +98,7 @@ class SparseMoeBlock(nn.Module):
     """Stand-alone MoE block: [B,S,H] (or [T,H]) -> same shape.  The last
     router outputs are kept in ``router_logits`` / ``topk_index``.
 
-    Up to ``few_tokens`` tokens without a gradient run the few-token layer
+    Up to ``few_tokens`` tokens without a gradient, outside autocast, run the few-token layer
     (``moe_amd.few``; 0, the default: never), which computes no router_logits:
     they are None then.  ``saved_activations`` is moe_layer's."""
 
@@ -121,7 +121,9 @@ class SparseMoeBlock(nn.Module):
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         shape = hidden_states.shape
         flat = hidden_states.reshape(-1, shape[-1])
-        if few.wanted(self.few_tokens, flat, *self.parameters()):
+        # (autocast's logits are bf16 whatever the weights are: the other form's)
+        if few.wanted(self.few_tokens, flat, *self.parameters()) \
+                and not torch.is_autocast_enabled():
             sig = self.router == "sigmoid"
             out, _, self.topk_index = few.moe_layer_few(
                 flat, self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj,

@@ -89,6 +89,9 @@ SHAPES = [  # T, H, E, K, I
     (64, 128, 1792, 8, 64),
     (64, 576, 4, 4, 64),        # 64 rows in every expert
     (64, 128, 40, 16, 1088),
+    (64, 4096, 20, 16, 64),     # 1024 rows: the down kernel's largest LDS
+    (3, 8192, 4, 2, 192),
+    (2, 64, 3, 2, 4160),
 ]
 
 
@@ -278,7 +281,9 @@ def _w_tol(w, E, spread):
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("T,H,E,K,I,renorm", [
     (1, 128, 128, 8, 64, True), (7, 64, 16, 16, 64, False), (64, 256, 64, 6, 64, True),
-    (5, 64, 1792, 8, 64, True), (3, 64, 4096, 4, 64, False), (33, 128, 200, 1, 64, True)])
+    (5, 64, 1792, 8, 64, True), (3, 64, 4096, 4, 64, False), (33, 128, 200, 1, 64, True),
+    (1, 64, 1, 1, 64, True), (1, 64, 300, 16, 64, True), (1, 128, 256, 16, 64, False),
+    (2, 64, 257, 5, 64, True), (19, 192, 16, 16, 128, True)])
 def test_layer_softmax_on_exact_logits(T, H, E, K, I, renorm, dt):
     print(f"moe_layer_few softmax {T} {H} {E} {K} {dt}", flush=True)
     x, wr, w1, w2 = _layer(_gen(E + K), T, H, E, I, dt, whole=True)
@@ -294,7 +299,8 @@ def test_layer_softmax_on_exact_logits(T, H, E, K, I, renorm, dt):
 
 @pytest.mark.parametrize("T,H,E,K,groups,gtopk,scale", [
     (1, 128, 64, 8, None, None, 2.5), (17, 128, 64, 8, 8, 4, None), (64, 64, 1792, 8, None, None, None),
-    (9, 64, 96, 6, 3, 2, 1.5), (4, 64, 128, 16, 64, 16, None), (5, 64, 256, 4, 1, 1, None)])
+    (9, 64, 96, 6, 3, 2, 1.5), (4, 64, 128, 16, 64, 16, None), (5, 64, 256, 4, 1, 1, None),
+    (3, 64, 1024, 8, 8, 4, None), (1, 64, 512, 8, 64, 8, 2.0), (17, 64, 320, 6, 5, 3, None)])
 def test_layer_sigmoid_on_exact_logits(T, H, E, K, groups, gtopk, scale):
     print(f"moe_layer_few sigmoid {T} {H} {E} {K} {groups}", flush=True)
     g = _gen(E * K)
@@ -407,6 +413,9 @@ def test_block_and_bank_choose_by_tokens():
     out = blk(h)                       # a gradient is wanted: the other form
     out.sum().backward()
     assert blk.experts.down_proj.grad is not None and torch.equal(out.detach(), ref)
+    with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
+        blk(h)
+        assert blk.router_logits is not None
     blk.router = "sigmoid"
     with torch.no_grad():
         got = blk(h)
