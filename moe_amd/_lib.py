@@ -143,9 +143,14 @@ def last_error() -> str:
     return msg.decode() if msg else ""
 
 
+_fns: dict[str, ctypes._CFuncPtr] = {}
+
+
 def call(name: str, *args) -> None:
     """Invokes a status-returning entry point; raises RuntimeError on failure."""
-    fn = getattr(load(), name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load(), name)
     rc = fn(*args)
     if rc != MOE_OK:
         raise RuntimeError(f"{name} failed with {STATUS_NAMES.get(rc, rc)}: {last_error()}")

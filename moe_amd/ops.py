@@ -805,11 +805,10 @@ def pack8(x: torch.Tensor) -> Packed8:
         raise ValueError("pack8 takes tensors of at least one dimension")
     code = _dtype_code(x.dtype)
     x = _contig(x)
-    cols = x.shape[-1]
+    *lead, cols = x.shape
     rows = x.numel() // cols if cols else 0
-    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-    scale = torch.empty(*x.shape[:-1], -(-cols // PACK8_BLOCK), device=x.device,
-                        dtype=torch.uint8)
+    q = torch.empty_like(x, dtype=torch.int8)
+    scale = x.new_empty((*lead, -(-cols // PACK8_BLOCK)), dtype=torch.uint8)
     _call("moe_amd_pack8", x.data_ptr(), code, rows, cols, q.data_ptr(), scale.data_ptr(),
           _stream(x), capturable=True)
     return Packed8(q, scale, x.dtype)
@@ -827,7 +826,7 @@ def unpack8(packed: Packed8) -> torch.Tensor:
         raise ValueError(f"unpack8: q {q.dtype} {tuple(q.shape)} and scale {scale.dtype} "
                          f"{tuple(scale.shape)} are not a packed tensor")
     q, scale = _contig(q), _contig(scale)
-    x = torch.empty(q.shape, device=q.device, dtype=packed.dtype)
+    x = torch.empty_like(q, dtype=packed.dtype)
     _call("moe_amd_unpack8", q.data_ptr(), scale.data_ptr(), q.numel() // cols if cols else 0,
           cols, x.data_ptr(), _dtype_code(packed.dtype), _stream(q), capturable=True)
     return x
