@@ -463,40 +463,117 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 // the 16 rows of the A operand; the waves split H, CH blocks in flight each.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
 // dealt to all of them in small pieces: with 16 features a workgroup one token
 // (K = 8, I = 768) has 384 for 256 CUs.
-// One token (NV != 0): slot k is its k-th entry, and the first workgroup leaves
-// the plan for the down kernel.  NV > 0: every workgroup routes the token for
-// itself, up to 64 NV experts; kGiven: the routing is given.
+// NV != 0: at most 64 entries, which every workgroup lists for itself; the first
+// one leaves the plan for the down kernel.  NV > 0: it routes the tokens too, a
+// wave each, up to 64 NV experts; kGiven: the routing is given.
 constexpr int kGiven = -1;
+
+// The list and rows of few_plan_kernel from up to 64 entries on one wave, lane s
+// holding entry s's expert (negative: padding): `slot`'s expert and rows (n = 0:
+// no such entry), and the whole plan where `leave`.
+struct SmallPlan {
+  int e, n;
+  int row[16];
+};
+__device__ __forceinline__ void small_plan(const FewArgs& p, int e, int lane, int slot, bool leave,
+                                           SmallPlan* out) {
+  const uint64_t before = (1ull << lane) - 1;
+  if (p.T == 1) {
+    // slot k is entry k, padding included; an expert named twice is read twice
+    // (the general form costs one token 0.7 of 24 us)
+    const int expert = __builtin_amdgcn_readlane(e, slot);
+    if (lane == 0) {
+      out->e = expert;
+      out->n = expert >= 0;
+      out->row[0] = slot;
+    }
+    if (!leave) return;
+    const uint64_t real = __ballot(e >= 0);
+    if (e >= 0) p.list[__popcll(real & before)] = make_int4(e, lane, 1, 0);
+    if (lane < p.K) p.rows[lane] = lane;
+    if (lane == 0) p.hdr[0] = __popcll(real);
+    return;
+  }
+  uint64_t peers = __ballot(e >= 0);  // entries of the same expert
+#pragma unroll
+  for (int b = 0; b < 12; ++b) {
+    const uint64_t one = __ballot(e >> b & 1);
+    peers &= e >> b & 1 ? one : ~one;
+  }
+  static_assert(kFewExperts <= 1 << 12, "a ballot for each bit of an id");
+  const int rank = __popcll(peers & before);
+  const bool lead = e >= 0 && (rank & 15) == 0;  // begins a list entry
+  const uint64_t leads = __ballot(lead);
+  const int at = __popcll(leads & before);
+  const uint64_t mine = __ballot(lead && at == slot);
+  if (mine) {
+    const int l = __builtin_ctzll(mine);
+    const bool member = e >= 0 && peers == readlane_u64(peers, l) &&
+                        rank >> 4 == __builtin_amdgcn_readlane(rank, l) >> 4;
+    if (member) out->row[rank & 15] = lane;
+    const int n = __popcll(__ballot(member)), expert = __builtin_amdgcn_readlane(e, l);
+    if (lane == 0) {
+      out->e = expert;
+      out->n = n;
+    }
+  } else if (lane == 0) {
+    out->n = 0;
+  }
+  if (!leave) return;
+  const int count = e >= 0 && rank == 0 ? __popcll(peers) : 0;
+  int upto = count;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += v;
+  }
+  const int row0 = __shfl(upto - count, e >= 0 ? __builtin_ctzll(peers) : 0, 64);
+  if (e >= 0) p.rows[row0 + rank] = lane;
+  if (lead) p.list[at] = make_int4(e, row0 + rank, min(16, __popcll(peers) - rank), 0);
+  if (lane == 0) p.hdr[0] = __popcll(leads);
+}
+
 template <typename T, int CH, int NV>
 __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   __shared__ __attribute__((aligned(16))) char turn[kWaves][kBlockLds];
-  __shared__ int s_e;
+  __shared__ SmallPlan small;
+  __shared__ int s_ids[64];
   const int nsl = p.I / 8;
   const int slot = blockIdx.x / nsl, f0 = (blockIdx.x % nsl) * 8;
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int4 info;
   if constexpr (NV != 0) {
-    if (wid == 0) {
-      float wk = 0.f;
-      int ek = -1;
-      if constexpr (NV > 0) route_token<NV, false>(p, p.logits, nullptr, 0, lane, wk, ek);
-      else if (lane < p.K) ek = given_route(p, lane, wk);
-      if (lane == slot) s_e = ek;
-      if (blockIdx.x == 0) {
-        const uint64_t real = __ballot(lane < p.K && ek >= 0);
-        if (lane < p.K) {
-          if (ek >= 0)
-            p.list[__popcll(real & ((1ull << lane) - 1))] = make_int4(ek, lane, 1, 0);
-          p.rows[lane] = lane;
-        }
-        if (lane == 0) p.hdr[0] = __popcll(real);
-        store_route(p, 0, lane, wk, ek);
+    const bool first = blockIdx.x == 0;
+    if constexpr (NV > 0) {
+      if (wid < p.T) {
+        float wk;
+        int ek;
+        route_token<NV, false>(p, p.logits + (int64_t)wid * p.E, nullptr, 0, lane, wk, ek);
+        if (lane < p.K) s_ids[wid * p.K + lane] = ek;
+        if (first) store_route(p, wid, lane, wk, ek);
       }
+      if (p.T > 1) __syncthreads();
+    }
+    if (wid == 0) {
+      const int S = p.T * p.K;
+      int e = -1;
+      if constexpr (NV > 0) {
+        if (lane < S) e = s_ids[lane];
+      } else if (lane < S) {
+        float wk;
+        e = given_route(p, lane, wk);
+        if (first) {
+          p.real[lane] = e;
+          p.w[lane] = wk;
+        }
+      }
+      small_plan(p, e, lane, slot, first, &small);
     }
     __syncthreads();
-    info = make_int4(__builtin_amdgcn_readfirstlane(s_e), 0, 1, 0);
-    if (info.x < 0) return;
+    info = make_int4(__builtin_amdgcn_readfirstlane(small.e), 0,
+                     __builtin_amdgcn_readfirstlane(small.n), 0);
+    if (info.z == 0) return;
   } else {
     const int nact = p.hdr[0];
     info = p.list[slot];  // a slot past the active experts holds anything
@@ -507,10 +584,12 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
   const char* wg = (const char*)p.w1 + ((int64_t)info.x * 2 * p.I + f0) * ld;
   const char* wu = wg + (int64_t)p.I * ld;
   const uint32_t wo = row * ld + j;
-  const auto token = [&](int i) -> uint32_t {  // of the entry's row i, or its last
-    return NV != 0 ? 0 : p.rows[info.y + min(i, info.z - 1)] / p.K;
+  const auto entry = [&](int i) {  // of row i, or the last
+    i = min(i, info.z - 1);
+    return NV != 0 ? small.row[i] : p.rows[info.y + i];
   };
-  const uint32_t x0 = token(row) * ld + j, x1 = token(row + 8) * ld + j;
+  const uint32_t x0 = (uint32_t)(entry(row) / p.K) * ld + j;
+  const uint32_t x1 = (uint32_t)(entry(row + 8) / p.K) * ld + j;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   chunks<CH>(wid * nb / kWaves, (wid + 1) * nb / kWaves, [&](auto ch, int s) {
     constexpr int C = decltype(ch)::value;
@@ -541,8 +620,7 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
     gs += red[q][l][f & 3];
     us += red[q][l + 32][f & 3];
   }
-  const int s = NV != 0 ? slot : p.rows[info.y + r];
-  ((T*)p.act)[(int64_t)s * p.I + f0 + f] = (T)(siluf_(gs) * us);
+  ((T*)p.act)[(int64_t)entry(r) * p.I + f0 + f] = (T)(siluf_(gs) * us);
 }
 
 // --------------------------------------------------------- down + combine
@@ -737,7 +815,8 @@ int few_check(int64_t T, int K, int E, int H, int I, int dtype, const char* who)
 template <typename T>
 hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   // entries of the list: an expert's last one may be short, the others are full
-  const int S = p.T * p.K, slots = S < p.E + S / 16 ? S : p.E + S / 16;
+  // (one token's are its own)
+  const int S = p.T * p.K, slots = p.T == 1 || S < p.E + S / 16 ? S : p.E + S / 16;
   if (p.wr) few_logits_kernel<T><<<dim3((p.E + 15) / 16, (p.T + 15) / 16), 64 * kWaves, 0, st>>>(p);
   // One wave routes a token of up to 256 experts, a workgroup one of more (with
   // 28 entries a lane, one wave took 46 us for each of 64 tokens, E = 1792).
@@ -745,9 +824,15 @@ hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   const int threads = 64 * kWaves, gu_grid = slots * (p.I / 8);
   const auto plan = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
-    if (p.T == 1 && !wide) {
-      if (p.wr) few_gate_up_kernel<T, kGateUpChunk, NV><<<gu_grid, threads, 0, st>>>(p);
-      else few_gate_up_kernel<T, kGateUpChunk, kGiven><<<S * (p.I / 8), threads, 0, st>>>(p);
+    // Few entries are listed by the gate/up workgroups themselves, which saves a
+    // launch of 4 us; so is the routing of one or two tokens (two: 4 of 38 us),
+    // whose instructions every workgroup repeats.
+    if (S <= 64 && !p.wr) {
+      few_gate_up_kernel<T, kGateUpChunk, kGiven><<<gu_grid, threads, 0, st>>>(p);
+      return;
+    }
+    if (S <= 64 && p.T <= 2 && !wide) {
+      few_gate_up_kernel<T, kGateUpChunk, NV><<<gu_grid, threads, 0, st>>>(p);
       return;
     }
     if (wide) {

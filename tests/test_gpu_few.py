@@ -113,10 +113,26 @@ def test_experts(T, H, E, K, I, dt):
     _close(few.experts_forward_few(x, idx, wb, w1, w2), ref, tol)
 
 
+@pytest.mark.parametrize("seed", range(6))
+def test_few_entries_in_any_arrangement(seed):
+    """Up to 64 entries, whose list every workgroup makes for itself: random ids
+    over few or many experts, padded and repeated."""
+    print(f"experts_few arrangement {seed}", flush=True)
+    g = _gen(100 + seed)
+    T, K = ((2, 3), (8, 8), (7, 9), (16, 4), (64, 1), (3, 16))[seed]
+    E, H, I = (2, 3, 200, 5, 4, 9)[seed], 128, 128
+    x = torch.randn(T, H, generator=g, device=DEV).to(BF)
+    w1, w2 = _weights(g, E, H, I, BF)
+    idx = torch.randint(-1, E + 1, (T, K), generator=g, device=DEV)
+    w = torch.rand(T, K, generator=g, device=DEV)
+    _close(few.experts_forward_few(x, idx, w, w1, w2), *_oracle(x, idx, w, w1, w2))
+
+
+@pytest.mark.parametrize("T", [21, 9])
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
-def test_padding_contributes_nothing(dt):
+def test_padding_contributes_nothing(dt, T):
     print("experts_few padding", flush=True)
-    T, H, E, K, I = 21, 256, 12, 4, 128
+    H, E, K, I = 256, 12, 4, 128
     g = _gen(5)
     x = torch.randn(T, H, generator=g, device=DEV).to(dt)
     w1, w2 = _weights(g, E, H, I, dt)
@@ -124,15 +140,16 @@ def test_padding_contributes_nothing(dt):
     idx[3] = -1
     idx[4] = E
     idx[7, 1:] = (1 << 40) + 1     # beyond 32 bits; its low half is a real id
-    idx[9, 2] = -(1 << 40) + 2
-    idx[20] = E + 5
+    idx[6, 2] = -(1 << 40) + 2
+    last = T - 1
+    idx[last] = E + 5
     # what padding names may hold anything
     w[idx.lt(0) | idx.ge(E)] = float("nan")
-    x[3], x[4], x[20] = float("nan"), float("inf"), float("-inf")
+    x[3], x[4], x[last] = float("nan"), float("inf"), float("-inf")
     ref, tol = _oracle(torch.nan_to_num(x, 0.0, 0.0, 0.0), idx, torch.nan_to_num(w), w1, w2)
     got = few.experts_forward_few(x, idx, w, w1, w2)
     _close(got, ref, tol)
-    assert (got[[3, 4, 20]] == 0).all()
+    assert (got[[3, 4, last]] == 0).all()
     # nothing but padding
     assert (few.experts_forward_few(x, torch.full_like(idx, E), w, w1, w2) == 0).all()
 
@@ -170,7 +187,7 @@ def test_a_value_that_is_not_finite_stays_with_its_token():
     assert got[0].isnan().all() and not got[18].isfinite().any()
 
 
-@pytest.mark.parametrize("T,K", [(3, 2), (64, 16)])
+@pytest.mark.parametrize("T,K", [(3, 2), (64, 16), (4, 16), (8, 8), (5, 13), (2, 16), (9, 7)])
 def test_one_expert_named_many_times(T, K):
     print(f"experts_few same expert {T} {K}", flush=True)
     H, E, I = 128, 3, 64
@@ -283,7 +300,7 @@ def _w_tol(w, E, spread):
     (1, 128, 128, 8, 64, True), (7, 64, 16, 16, 64, False), (64, 256, 64, 6, 64, True),
     (5, 64, 1792, 8, 64, True), (3, 64, 4096, 4, 64, False), (33, 128, 200, 1, 64, True),
     (1, 64, 1, 1, 64, True), (1, 64, 300, 16, 64, True), (1, 128, 256, 16, 64, False),
-    (2, 64, 257, 5, 64, True), (19, 192, 16, 16, 128, True)])
+    (2, 64, 257, 5, 64, True), (2, 256, 128, 8, 128, True), (2, 64, 20, 16, 64, False), (19, 192, 16, 16, 128, True)])
 def test_layer_softmax_on_exact_logits(T, H, E, K, I, renorm, dt):
     print(f"moe_layer_few softmax {T} {H} {E} {K} {dt}", flush=True)
     x, wr, w1, w2 = _layer(_gen(E + K), T, H, E, I, dt, whole=True)
@@ -300,7 +317,7 @@ def test_layer_softmax_on_exact_logits(T, H, E, K, I, renorm, dt):
 @pytest.mark.parametrize("T,H,E,K,groups,gtopk,scale", [
     (1, 128, 64, 8, None, None, 2.5), (17, 128, 64, 8, 8, 4, None), (64, 64, 1792, 8, None, None, None),
     (9, 64, 96, 6, 3, 2, 1.5), (4, 64, 128, 16, 64, 16, None), (5, 64, 256, 4, 1, 1, None),
-    (3, 64, 1024, 8, 8, 4, None), (1, 64, 512, 8, 64, 8, 2.0), (17, 64, 320, 6, 5, 3, None)])
+    (2, 64, 64, 8, 4, 2, None), (2, 64, 200, 16, None, None, None), (3, 64, 1024, 8, 8, 4, None), (1, 64, 512, 8, 64, 8, 2.0), (17, 64, 320, 6, 5, 3, None)])
 def test_layer_sigmoid_on_exact_logits(T, H, E, K, groups, gtopk, scale):
     print(f"moe_layer_few sigmoid {T} {H} {E} {K} {groups}", flush=True)
     g = _gen(E * K)
