@@ -6,12 +6,15 @@
 //   out_t = sum_k w[t,k] down_proj[e] act             (few_down_kernel)
 //
 // What bounds it is reading each routed expert's three matrices once: a few
-// rows per expert leave the matrix units idle.  The weights therefore stream
-// straight from memory into MFMA operands, as the 16 rows of the A operand
-// (output features), with the expert's tokens as the 16 columns of B; no
-// staging in LDS, every wave's loads in flight together.  A workgroup's eight
-// waves split the contraction and add their partial sums in LDS in a fixed
-// order, so results do not depend on timing.
+// rows per expert leave the matrix units idle.  The weights therefore go from
+// memory to the MFMA as the 16 rows of its A operand (output features), with
+// the expert's tokens as the 16 columns of B, every wave's loads in flight
+// together and the bytes dealt evenly to the CUs.  Partial sums are added in a
+// fixed order, so results do not depend on timing.
+//
+// H = 2048, E = 128, K = 8, I = 768, bf16, fresh weights: 23 us for one token
+// (75 MB), 215 us for 64 (1.18 GB: gate/up 5.9 TB/s, down 5.7); E = 1792, 64
+// tokens 620 us (3.8 GB).  The layer by grouped GEMMs takes 95, 292 and 750.
 //
 // Sums are fp32 (the logits' across waves fp64); act is rounded to x's type,
 // the next product's operand type, once; everything else is rounded once at
