@@ -1120,13 +1120,12 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const int e0 = 2 * w, e1 = 2 * w + 1;
-            da[e0] = wgt * gq[e0];
-            da[e1] = wgt * gq[e1];
             if constexpr (PACK) {  // no stored bits to agree with: each result is rounded once
 #pragma unroll
               for (int e = e0; e <= e1; ++e) {
                 sl[e] = t[e];
                 a[e] = t[e] * u[e];
+                da[e] = wgt * gq[e];
                 ds[e] = da[e] * u[e];
               }
             } else {
@@ -1136,6 +1135,8 @@ __device__ __forceinline__ void grouped_gemm(const GemmArgs& p) {
               const uint32_t ap = pack_bf2(sl[e0] * u[e0], sl[e1] * u[e1]);
               a[e0] = bf_lo(ap);
               a[e1] = bf_hi(ap);
+              da[e0] = wgt * gq[e0];
+              da[e1] = wgt * gq[e1];
               const uint32_t dsp = pack_bf2(da[e0] * u[e0], da[e1] * u[e1]);
               ds[e0] = bf_lo(dsp);
               ds[e1] = bf_hi(dsp);

@@ -79,8 +79,9 @@ def mi355x_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch
     gradient is wanted, and a ``saved_activations`` attribute is
     experts_forward's (``hf.install`` sets both)."""
     _check_module(self)
-    if few.wanted(getattr(self, "few_tokens", 0), hidden_states, top_k_weights,
-                  self.gate_up_proj, self.down_proj):
+    if few.wanted(getattr(self, "few_tokens", 0), top_k_index.shape[-1],
+                  self.gate_up_proj.shape[0], hidden_states, top_k_weights, self.gate_up_proj,
+                  self.down_proj):
         return few.experts_forward_few(hidden_states, top_k_index, top_k_weights,
                                        self.gate_up_proj, self.down_proj)
     return experts_forward(hidden_states, top_k_index, top_k_weights, self.gate_up_proj,

@@ -19,11 +19,12 @@ from . import library, ops  # noqa: F401  (library registers the moe_amd:: ops)
 MAX_TOKENS = ops.FEW_MAX_TOKENS
 
 
-def wanted(few_tokens: int, *tensors: torch.Tensor) -> bool:
+def wanted(few_tokens: int, top_k: int, num_experts: int, *tensors: torch.Tensor) -> bool:
     """Whether a layer that takes the few-token form up to ``few_tokens``
-    tokens takes it for hidden states ``tensors[0]``: no gradient is wanted of
-    any of the tensors."""
-    return 0 < tensors[0].shape[0] <= min(few_tokens, MAX_TOKENS) and not _grad(*tensors)
+    tokens takes it for hidden states ``tensors[0]``: it has the shape, and no
+    gradient is wanted of any of the tensors."""
+    return (0 < tensors[0].shape[0] <= min(few_tokens, MAX_TOKENS) and top_k <= ops.FEW_MAX_TOP_K
+            and num_experts <= ops.FEW_MAX_EXPERTS and not _grad(*tensors))
 
 
 def _grad(*tensors) -> bool:

@@ -122,7 +122,8 @@ class SparseMoeBlock(nn.Module):
         shape = hidden_states.shape
         flat = hidden_states.reshape(-1, shape[-1])
         # (autocast's logits are bf16 whatever the weights are: the other form's)
-        if few.wanted(self.few_tokens, flat, *self.parameters()) \
+        if few.wanted(self.few_tokens, self.top_k, self.gate.weight.shape[0], flat,
+                      *self.parameters()) \
                 and not torch.is_autocast_enabled():
             sig = self.router == "sigmoid"
             out, _, self.topk_index = few.moe_layer_few(

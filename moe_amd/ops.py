@@ -836,6 +836,7 @@ def unpack8(packed: Packed8) -> torch.Tensor:
 
 FEW_MAX_TOKENS = 64
 FEW_MAX_TOP_K = 16
+FEW_MAX_EXPERTS = 4096
 _ROUTERS = {"softmax": 0, "sigmoid": 1}
 
 

@@ -85,13 +85,17 @@ def test_cpu_tensors_and_gradients_are_refused():
 def test_a_block_takes_the_few_token_form_only_without_gradients():
     x = torch.zeros(4, 8)
     p = torch.nn.Parameter(torch.zeros(3))
+
+    def wanted(n, t=x, k=2, e=8):
+        return few.wanted(n, k, e, t, p)
+
     with torch.no_grad():
-        assert few.wanted(4, x, p) and few.wanted(1000, x, p)
-        assert not few.wanted(0, x, p) and not few.wanted(3, x, p)
-        assert not few.wanted(64, torch.zeros(0, 8), p)
-        assert not few.wanted(1000, torch.zeros(65, 8), p)
-    assert not few.wanted(4, x, p)
-    assert few.wanted(4, x, p.detach())
+        assert wanted(4) and wanted(1000) and wanted(4, k=16, e=4096)
+        assert not wanted(0) and not wanted(3)
+        assert not wanted(64, torch.zeros(0, 8)) and not wanted(1000, torch.zeros(65, 8))
+        assert not wanted(4, k=17) and not wanted(4, e=4097)   # the other form's
+    assert not wanted(4)
+    assert few.wanted(4, 2, 8, x, p.detach())
 
 
 def test_install_sets_the_banks(monkeypatch):

@@ -236,6 +236,23 @@ def test_strided_and_other_dtypes():
     assert torch.equal(part, few.experts_forward_few(xx[:, :H], idx % 3 + 2, w, w1, w2))
 
 
+def test_subnormal_fp32():
+    """fp32 operands and sums below 2^-126 are kept, to the last of their bits:
+    half a step of 2^-149 for each of the I products' sums and the K y's."""
+    print("experts_few subnormal", flush=True)
+    T, H, E, K, I = 3, 128, 4, 2, 64
+    g = _gen(16)
+    x = torch.randn(T, H, generator=g, device=DEV)
+    w1, w2 = _weights(g, E, H, I, F32)
+    w1 = w1 * 20
+    w2 = (w2.double() * 2.0 ** -130).float()
+    idx, w = _routing(g, T, E, K)
+    ref, tol = _oracle(x, idx, w, w1, w2)
+    got = few.experts_forward_few(x, idx, w, w1, w2)
+    assert (ref.abs().max() < 2.0 ** -126) and (got != 0).any()
+    assert ((got.double() - ref).abs() <= tol + (I + K + 1) * K * 2.0 ** -149).all()
+
+
 def test_no_tokens():
     w1, w2 = _weights(_gen(1), 4, 128, 64, BF)
     x = torch.empty(0, 128, device=DEV, dtype=BF)
@@ -525,6 +542,14 @@ def test_compiled_and_custom_ops():
     args = (x, wr, w1, w2, K, "softmax", True, None, None, None, None, None)
     torch.library.opcheck(torch.ops.moe_amd.moe_layer_few.default, args, test_utils=utils)
     assert torch.equal(torch.ops.moe_amd.moe_layer_few(*args)[0], out)
+
+    @torch.no_grad()
+    def fn(x):
+        a, w, idx = few.moe_layer_few(x, wr, w1, w2, K, return_routing=True)
+        return few.moe_layer_few(a, wr, w1, w2, K), few.experts_forward_few(a, idx, w, w1, w2)
+
+    for a, b in zip(torch.compile(fn, fullgraph=True, backend="aot_eager")(x), fn(x)):
+        assert torch.equal(a, b)
 
 
 def test_refusals_on_the_gpu():
