@@ -446,11 +446,21 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
   const int rank = e >= 0 ? atomicAdd(&count[e], 1) : 0;
   __syncthreads();
   const bool lead = e >= 0 && rank == 0;
-  const int cnt = lead ? count[e] : 0;
-  __syncthreads();
-  if (lead) {
-    const int n = (cnt + 15) / 16;
-    const int at = atomicAdd(&total, n << 16 | cnt);  // entries and rows before it
+  const int cnt = lead ? count[e] : 0, n = (cnt + 15) / 16;
+  // entries (high half) and rows before it: the wave's by a scan, one atomic a
+  // wave for the others' (with one a leader, all of the same word, this kernel took
+  // 9.8 us for 64 tokens and 128 experts and 13.7 for 1792, with the scan 8.5 and 11.4)
+  const int own = n << 16 | cnt;
+  int upto = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += v;
+  }
+  int at = 0;
+  if (lane == 63) at = atomicAdd(&total, upto);
+  at = __builtin_amdgcn_readlane(at, 63) + upto - own;
+  if (lead) {  // the one that reads or writes count[e] until the next barrier
     const int r0 = at & 0xffff;
     for (int i = 0; i < n; ++i)
       p.list[(at >> 16) + i] = make_int4(e, r0 + 16 * i, min(16, cnt - 16 * i), 0);
@@ -463,9 +473,10 @@ __global__ __launch_bounds__(64 * kPlanWaves) void few_plan_kernel(FewArgs p) {
 
 // ------------------------------------------------------- gate/up + SwiGLU
 // Workgroup: 8 features of one entry of the list, their gate and up rows being
-// the 16 rows of the A operand; the waves split H, CH blocks in flight each.  A CU takes in about 24 KB/us whatever else is idle, so the weights are
-// dealt to all of them in small pieces: with 16 features a workgroup one token
-// (K = 8, I = 768) has 384 for 256 CUs.
+// the 16 rows of the A operand; the waves split H, CH blocks in flight each.  A
+// CU takes in about 24 KB/us whatever else is idle, so the weights are dealt to
+// all of them in small pieces: with 16 features a workgroup one token (K = 8,
+// I = 768) has 384 for 256 CUs.
 // NV != 0: at most 64 entries, which every workgroup lists for itself; the first
 // one leaves the plan for the down kernel.  NV > 0: it routes the tokens too, a
 // wave each, up to 64 NV experts; kGiven: the routing is given.
