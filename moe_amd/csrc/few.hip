@@ -83,7 +83,7 @@ __device__ __forceinline__ f32x4 mma_step(float, const u32x4& a, const u32x4& b,
 // straight into that layout, 16 lanes touch 16 lines and a CU takes in 38 KB/us
 // of both operands together, 1 KB in 64 cycles.
 constexpr int kBlock = 128;
-constexpr int kBlockLds = 4 * 1024;  // of a wave
+constexpr int kBlockLds = 32 * kBlock;  // of a wave
 constexpr int kMaxLds = kWaves * kBlockLds + kFewRows * (16 + 64 + 12);  // of the down kernel
 struct Block {
   u32x4 a0, a1, b0, b1;
@@ -93,16 +93,16 @@ __device__ __forceinline__ f32x4 mma_block(const Block& v, char* lds, int lane, 
   const int r = lane >> 3, n = lane & 15, g = lane >> 4;
   char* w = lds + r * kBlock + ((lane & 7) ^ r) * 16;
   *(u32x4*)w = v.a0;
-  *(u32x4*)(w + 1024) = v.a1;
-  *(u32x4*)(w + 2048) = v.b0;
-  *(u32x4*)(w + 3072) = v.b1;
+  *(u32x4*)(w + 8 * kBlock) = v.a1;
+  *(u32x4*)(w + 16 * kBlock) = v.b0;
+  *(u32x4*)(w + 24 * kBlock) = v.b1;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const char* q = lds + n * kBlock + ((t * 4 + g) ^ (n & 7)) * 16;
-    acc = mma_step(T{}, *(const u32x4*)q, *(const u32x4*)(q + 2048), acc);
+    acc = mma_step(T{}, *(const u32x4*)q, *(const u32x4*)(q + 16 * kBlock), acc);
   }
   __builtin_amdgcn_wave_barrier();  // the next block's writes stay behind these reads
   return acc;
