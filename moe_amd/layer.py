@@ -98,9 +98,10 @@ class SparseMoeBlock(nn.Module):
     """Stand-alone MoE block: [B,S,H] (or [T,H]) -> same shape.  The last
     router outputs are kept in ``router_logits`` / ``topk_index``.
 
-    Up to ``few_tokens`` tokens without a gradient, outside autocast, run the few-token layer
-    (``moe_amd.few``; 0, the default: never), which computes no router_logits:
-    they are None then.  ``saved_activations`` is moe_layer's."""
+    Up to ``few_tokens`` tokens without a gradient, outside autocast and of the
+    weights' dtype, run the few-token layer (``moe_amd.few``; 0, the default:
+    never), which computes no router_logits: they are None then.
+    ``saved_activations`` is moe_layer's."""
 
     few_tokens = 0
     saved_activations = "exact"
@@ -121,9 +122,11 @@ class SparseMoeBlock(nn.Module):
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         shape = hidden_states.shape
         flat = hidden_states.reshape(-1, shape[-1])
-        # (autocast's logits are bf16 whatever the weights are: the other form's)
-        if few.wanted(self.few_tokens, self.top_k, self.gate.weight.shape[0], flat,
-                      *self.parameters()) \
+        params = (self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj)
+        # (autocast's logits are bf16 whatever the weights are, and the sigmoid
+        # router takes a weight of another dtype: the other form's)
+        if few.wanted(self.few_tokens, self.top_k, self.gate.weight.shape[0], flat, *params) \
+                and all(p.dtype == flat.dtype for p in params) \
                 and not torch.is_autocast_enabled():
             sig = self.router == "sigmoid"
             out, _, self.topk_index = few.moe_layer_few(

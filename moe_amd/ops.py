@@ -840,8 +840,13 @@ FEW_MAX_EXPERTS = 4096
 _ROUTERS = {"softmax": 0, "sigmoid": 1}
 
 
-def _few_inputs(name: str, x, gate_up_proj, down_proj, K: int):
-    """(E, H, I) of a few-token call after checking its shapes and types."""
+def _few_inputs(name: str, x, gate_up_proj, down_proj, K: int, *others):
+    """(E, H, I) of a few-token call after checking its shapes and types, and
+    that all its tensors are on one device."""
+    dev = x.get_device()
+    for t in (gate_up_proj, down_proj, *others):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name}: tensors on {x.device} and {t.device}, expected one device")
     if x.dim() != 2 or gate_up_proj.dim() != 3 or down_proj.dim() != 3:
         raise ValueError(f"{name}: hidden_states must be [T, H], gate_up_proj [E, 2I, H] and "
                          "down_proj [E, H, I]")
@@ -879,7 +884,7 @@ def experts_few(x: torch.Tensor, topk_index: torch.Tensor, topk_weights: torch.T
             or topk_index.shape[0] != x.shape[0]:
         raise ValueError("experts_few: topk_index / topk_weights must both be [T, K]")
     T, K = topk_index.shape
-    E, H, I = _few_inputs("experts_few", x, gate_up_proj, down_proj, K)
+    E, H, I = _few_inputs("experts_few", x, gate_up_proj, down_proj, K, topk_index, topk_weights)
     x, gate_up_proj, down_proj = _contig(x), _contig(gate_up_proj), _contig(down_proj)
     if topk_index.dtype != torch.int64:
         topk_index = topk_index.to(torch.int64)
@@ -913,7 +918,7 @@ def moe_layer_few(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.T
     extra = logit_offset if router == "softmax" else expert_bias
     _need_cuda(x, w_router, gate_up_proj, down_proj, extra)
     K = int(top_k)
-    E, H, I = _few_inputs(name, x, gate_up_proj, down_proj, K)
+    E, H, I = _few_inputs(name, x, gate_up_proj, down_proj, K, w_router, extra)
     if tuple(w_router.shape) != (E, H) or w_router.dtype != x.dtype:
         raise ValueError(f"{name}: router weight {tuple(w_router.shape)} {w_router.dtype}, "
                          f"expected {(E, H)} {x.dtype}")

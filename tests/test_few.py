@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 from moe_amd import _lib, few, hf, ops
 from moe_amd.layer import SparseMoeBlock
@@ -102,3 +103,46 @@ def test_install_sets_the_banks(monkeypatch):
     block = SparseMoeBlock(64, 4, 2, 64)
     assert hf.expert_banks(block) == [block.experts]
     assert few.MAX_TOKENS == ops.FEW_MAX_TOKENS == 64
+
+
+def test_a_block_of_mixed_dtypes_keeps_the_other_form(monkeypatch):
+    """The sigmoid router takes a router weight of another dtype than the
+    experts', the few-token layer does not."""
+    from moe_amd import layer
+
+    took = []
+    monkeypatch.setattr(few, "moe_layer_few",
+                        lambda x, *a, **k: took.append("few") or (x, None, None))
+    monkeypatch.setattr(layer, "moe_layer",
+                        lambda x, *a, **k: took.append("layer") or (x, None, None, None))
+    block = SparseMoeBlock(64, 4, 2, 64, router="sigmoid").to(torch.bfloat16)
+    block.few_tokens = 4
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    with torch.no_grad():
+        block(x)
+        block(x.float())
+        block.gate.float()
+        block(x)
+        block(x.float())
+    assert took == ["few", "layer", "layer", "layer"]
+
+
+def test_tensors_of_two_devices_are_refused():
+    bf = torch.bfloat16
+    with FakeTensorMode():
+        def make(shape, dtype=bf, dev="cuda:0"):
+            return torch.empty(shape, dtype=dtype, device=dev)
+
+        good = dict(x=((4, 128), bf), idx=((4, 2), torch.int64), w=((4, 2), torch.float32),
+                    w1=((8, 128, 128), bf), w2=((8, 128, 64), bf))
+        for other in good:
+            t = {n: make(*s, dev="cuda:1" if n == other else "cuda:0") for n, s in good.items()}
+            with pytest.raises(ValueError, match="one device"):
+                ops.experts_few.__wrapped__(t["x"], t["idx"], t["w"], t["w1"], t["w2"])
+        good = dict(x=((4, 128), bf), wr=((8, 128), bf), w1=((8, 128, 128), bf),
+                    w2=((8, 128, 64), bf), off=((8,), torch.float32))
+        for other in good:
+            t = {n: make(*s, dev="cuda:1" if n == other else "cuda:0") for n, s in good.items()}
+            with pytest.raises(ValueError, match="one device"):
+                ops.moe_layer_few.__wrapped__(t["x"], t["wr"], t["w1"], t["w2"], 2,
+                                              logit_offset=t["off"])

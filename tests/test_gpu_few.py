@@ -581,3 +581,21 @@ def test_refusals_on_the_gpu():
     flat = torch.empty(4 * 128 + 4, device=DEV, dtype=BF)
     with pytest.raises(RuntimeError, match="MOE_ERR_ALIGN"):
         few.experts_forward_few(flat[4:].view(4, 128), idx, w, w1, w2)
+
+
+def test_block_of_mixed_dtypes():
+    """fp32 router weights over bf16 experts: the same with few_tokens as without."""
+    print("SparseMoeBlock fp32 gate", flush=True)
+    torch.manual_seed(1)
+    blk = SparseMoeBlock(128, 8, 2, 64, router="sigmoid").to(DEV, BF)
+    with torch.no_grad():
+        for p in blk.parameters():
+            p.normal_(0, 0.1)
+        blk.gate.float()
+        for dt in (BF, torch.float32):
+            h = torch.randn(5, 128, device=DEV).to(dt)
+            blk.few_tokens = 0
+            ref = blk(h)
+            blk.few_tokens = 8
+            got = blk(h)
+            assert got.dtype == dt and torch.equal(got, ref)
