@@ -28,8 +28,10 @@ __device__ __forceinline__ float pack8_inverse(uint32_t scale) {
   return scale == 255u ? 0.f : __uint_as_float((254u - scale) << 23);
 }
 // q in the low byte: v / s is exact, and adding 1.5 2^23 rounds it to an
-// integer, halves to even, whose two's complement ends the sum's bits (v NaN
-// or 0 * inf: a NaN that ends in a zero byte).
+// integer, halves to even, whose two's complement ends the sum's bits.  In a
+// block that is not finite: 0 for finite v and for 0 * inf, whose NaN ends in a
+// zero byte, and for a NaN of bf16, the low half of whose bits is 0; a NaN of
+// fp32 keeps its payload, so packing from fp32 sets that block's q to 0 itself.
 __device__ __forceinline__ uint32_t pack8_one(float v, float inv) {
   return __float_as_uint(__builtin_fmaf(v, inv, 12582912.f));
 }

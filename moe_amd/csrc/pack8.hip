@@ -48,10 +48,9 @@ __global__ __launch_bounds__(kThreads) void pack8_kernel(const T* __restrict__ x
       if constexpr (V == 8) {
         __builtin_nontemporal_store(pack8_bf16x8(w[k], inv), (u32x2*)q + i);
       } else {
-        __builtin_nontemporal_store(
-            pack8_four(__uint_as_float(w[k][0]), __uint_as_float(w[k][1]),
-                       __uint_as_float(w[k][2]), __uint_as_float(w[k][3]), inv),
-            (uint32_t*)q + i);
+        const uint32_t v = pack8_four(__uint_as_float(w[k][0]), __uint_as_float(w[k][1]),
+                                      __uint_as_float(w[k][2]), __uint_as_float(w[k][3]), inv);
+        __builtin_nontemporal_store(e == 255u ? 0u : v, (uint32_t*)q + i);  // no NaN's payload
       }
       if (i % L == 0) scale[i / L] = (uint8_t)e;
     }
@@ -122,7 +121,7 @@ __global__ __launch_bounds__(kThreads) void pack8_any_kernel(const T* __restrict
     const float inv = pack8_inverse(e);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (col + 8 * i < cols) q[at + 8 * i] = (uint8_t)pack8_one(v[i], inv);
+      if (col + 8 * i < cols) q[at + 8 * i] = e == 255u ? 0 : (uint8_t)pack8_one(v[i], inv);
     if (g == 0) scale[b] = (uint8_t)e;
   }
 }

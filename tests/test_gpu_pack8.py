@@ -109,6 +109,25 @@ def test_blocks_that_are_not_finite(dt):
     assert torch.equal(got[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("shape", [(4, 128), (3, 100)], ids=["whole", "ragged"])
+@pytest.mark.parametrize("bits", [0x7fc00001, 0x7fc000ff, 0xffffffff, 0x7f800001, 0xff80007f,
+                                  0x7f800000])
+def test_any_nan_makes_the_block_nan(bits, shape):
+    """A NaN's payload stays out of q: every q of its block is 0, every value NaN."""
+    print(f"pack8 NaN {bits:#x} {shape}", flush=True)
+    x = torch.randn(shape, generator=_gen(7), device=DEV)
+    clean = ops.pack8(x)
+    raw = x.view(torch.int32)
+    raw[0, 5] = raw[2, 64] = raw[2, 99] = bits - (1 << 32 if bits >> 31 else 0)
+    p = ops.pack8(x)
+    bad = torch.zeros(shape, dtype=torch.bool, device=DEV)
+    bad[0, :64] = bad[2, 64:128] = True
+    assert p.scale[0, 0] == p.scale[2, 1] == 255
+    assert (p.q[bad] == 0).all() and torch.equal(p.q[~bad], clean.q[~bad])
+    back = ops.unpack8(p)
+    assert back[bad].isnan().all() and back[~bad].isfinite().all()
+
+
 @pytest.mark.parametrize("dt", [BF, F32], ids=["bf16", "f32"])
 def test_strides_and_alignment(dt):
     print(f"pack8 strides {dt}", flush=True)
