@@ -14,11 +14,28 @@ ExpertsInterface signature
 """
 from __future__ import annotations
 
+import functools
+import inspect
+
 import torch
 
 from . import few, library  # noqa: F401  (library registers the moe_amd:: ops)
 
 
+def traced_with_defaults(fn):
+    """torch.fx's tracers (make_fx) want a value for each parameter that a
+    function declares, those with a default too; of one that takes any arguments
+    they take as many as they are given.  So a new option with a default does not
+    refuse the traces that do without it."""
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        return fn(*args, **kwargs)
+    del call.__wrapped__  # the tracers count the innermost function's parameters
+    call.__signature__ = inspect.signature(fn)
+    return call
+
+
+@traced_with_defaults
 def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                     top_k_weights: torch.Tensor, gate_up_proj: torch.Tensor,
                     down_proj: torch.Tensor, saved_activations: str = "exact") -> torch.Tensor:

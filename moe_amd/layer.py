@@ -21,7 +21,7 @@ import torch
 from torch import nn
 
 from . import few, library  # library registers the moe_amd:: ops
-from .experts import experts_forward
+from .experts import experts_forward, traced_with_defaults
 from .router import gating_linear, linear_sigmoid_topk, sigmoid_topk, softmax_topk
 
 
@@ -33,6 +33,7 @@ def _fused_softmax_ok(x, w_router, gate_up_proj, down_proj) -> bool:
             and gate_up_proj.shape[0] == E)
 
 
+@traced_with_defaults
 def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tensor,
               down_proj: torch.Tensor, top_k: int, router: str = "softmax",
               renormalize: bool = True, logit_offset: torch.Tensor | None = None,

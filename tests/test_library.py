@@ -99,6 +99,37 @@ def test_experts_and_gradient_trace_into_one_graph():
     assert "moe_amd.experts_bwd.default" in targets
 
 
+@pytest.mark.parametrize("mode", ["fake", "symbolic"])
+def test_layers_trace_with_and_without_their_options(mode):
+    """make_fx on the functions themselves: a parameter with a default may be
+    left out of the trace's arguments, or given."""
+    from moe_amd.layer import moe_layer
+
+    x, idx, w, w1, w2 = _inputs()
+    wr = torch.empty(w1.shape[0], x.shape[1], dtype=torch.bfloat16)
+    layer = (x, wr, w1, w2, 2, "softmax", True, None, None, None, None, None, None, "torch")
+    cases = ((experts_forward, (x, idx, w, w1, w2), ()),
+             (experts_forward, (x, idx, w, w1, w2), ("int8",)),
+             (moe_layer, layer[:5], ()), (moe_layer, layer, ()), (moe_layer, layer, ("int8",)))
+    for fn, args, option in cases:
+        gm = make_fx(fn, tracing_mode=mode)(*args, *option)
+        # (router and experts are one op on GPU tensors alone)
+        call, = (n for n in gm.graph.nodes if str(n.target) == "moe_amd.experts_fwd.default")
+        assert ("int8" in call.args) == bool(option)
+
+
+def test_layers_keep_their_signatures():
+    import inspect
+    import pickle
+
+    from moe_amd.layer import moe_layer
+
+    for fn in (experts_forward, moe_layer):
+        names = list(inspect.signature(fn).parameters)
+        assert names[-1] == "saved_activations" and "gate_up_proj" in names
+        assert pickle.loads(pickle.dumps(fn)) is fn
+
+
 def test_ops_refuse_stream_capture(monkeypatch):
     """Under stream capture every C-ABI call raises before reaching the
     library (HIP graph capture is not supported)."""
