@@ -23,8 +23,10 @@ def wanted(few_tokens: int, top_k: int, num_experts: int, *tensors: torch.Tensor
     """Whether a layer that takes the few-token form up to ``few_tokens``
     tokens takes it for hidden states ``tensors[0]``: it has the shape, and no
     gradient is wanted of any of the tensors."""
-    return (0 < tensors[0].shape[0] <= min(few_tokens, MAX_TOKENS) and top_k <= ops.FEW_MAX_TOP_K
-            and num_experts <= ops.FEW_MAX_EXPERTS and not _grad(*tensors))
+    # (the number of tokens last, so that a trace in which it is data-dependent
+    # is asked for it only where the answer depends on it)
+    return (few_tokens > 0 and top_k <= ops.FEW_MAX_TOP_K and num_experts <= ops.FEW_MAX_EXPERTS
+            and not _grad(*tensors) and 0 < tensors[0].shape[0] <= min(few_tokens, MAX_TOKENS))
 
 
 def _grad(*tensors) -> bool:

@@ -146,3 +146,23 @@ def test_tensors_of_two_devices_are_refused():
             with pytest.raises(ValueError, match="one device"):
                 ops.moe_layer_few.__wrapped__(t["x"], t["wr"], t["w1"], t["w2"], 2,
                                               logit_offset=t["off"])
+
+
+@pytest.mark.parametrize("few_tokens,grad", [(0, False), (0, True), (8, True)])
+def test_a_number_of_tokens_that_depends_on_data(few_tokens, grad):
+    """Without the few-token form, and where a gradient is wanted, the layers
+    trace whatever the number of tokens turns out to be."""
+    from torch.fx.experimental.symbolic_shapes import ShapeEnv
+
+    from moe_amd.experts import mi355x_experts_forward
+
+    env = ShapeEnv()
+    with FakeTensorMode(shape_env=env):
+        block = SparseMoeBlock(128, 8, 2, 64).requires_grad_(grad)
+        block.few_tokens = block.experts.few_tokens = few_tokens
+        n = env.create_unbacked_symint()
+        x = torch.empty(n, 128)
+        assert block(x).shape == (n, 128)
+        out = mi355x_experts_forward(block.experts, x, torch.empty(n, 2, dtype=torch.int64),
+                                     torch.empty(n, 2))
+        assert out.shape == (n, 128)
