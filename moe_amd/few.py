@@ -21,11 +21,13 @@ MAX_TOKENS = ops.FEW_MAX_TOKENS
 
 def wanted(few_tokens: int, top_k: int, num_experts: int, *tensors: torch.Tensor) -> bool:
     """Whether a layer that takes the few-token form up to ``few_tokens``
-    tokens takes it for hidden states ``tensors[0]``: it has the shape, and no
-    gradient is wanted of any of the tensors."""
+    tokens takes it for ``tensors``, its hidden states [T, H] and what else goes
+    into it, the weights' last dimensions being H or I: it has the shape, and no
+    gradient is wanted of any of them."""
     # (the number of tokens last, so that a trace in which it is data-dependent
     # is asked for it only where the answer depends on it)
     return (few_tokens > 0 and top_k <= ops.FEW_MAX_TOP_K and num_experts <= ops.FEW_MAX_EXPERTS
+            and all(t.shape[-1] <= ops.FEW_MAX_FEATURES for t in tensors)
             and not _grad(*tensors) and 0 < tensors[0].shape[0] <= min(few_tokens, MAX_TOKENS))
 
 

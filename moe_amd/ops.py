@@ -837,6 +837,7 @@ def unpack8(packed: Packed8) -> torch.Tensor:
 FEW_MAX_TOKENS = 64
 FEW_MAX_TOP_K = 16
 FEW_MAX_EXPERTS = 4096
+FEW_MAX_FEATURES = 1 << 16   # of H and of I
 _ROUTERS = {"softmax": 0, "sigmoid": 1}
 
 

@@ -166,3 +166,18 @@ def test_a_number_of_tokens_that_depends_on_data(few_tokens, grad):
         out = mi355x_experts_forward(block.experts, x, torch.empty(n, 2, dtype=torch.int64),
                                      torch.empty(n, 2))
         assert out.shape == (n, 128)
+
+
+@pytest.mark.parametrize("H,I", [(1 << 17, 64), (64, 1 << 17), ((1 << 16) + 64, 64)])
+def test_a_layer_of_more_features_keeps_the_other_form(H, I):
+    # the few-token entry points refuse its shape
+    assert _ws(H=H, I=I) == 0 and _ws(H=1 << 16, I=1 << 16) > 0
+    with FakeTensorMode(), torch.no_grad():
+        block = SparseMoeBlock(H, 4, 2, I)
+        p = (block.gate.weight, block.experts.gate_up_proj, block.experts.down_proj)
+        x = torch.empty(2, H)
+        assert not few.wanted(8, 2, 4, x, *p)
+        assert not few.wanted(8, 2, 4, x, torch.empty(2, 2), *p[1:])
+        small = SparseMoeBlock(1 << 16, 4, 2, 1 << 16)
+        p = (small.gate.weight, small.experts.gate_up_proj, small.experts.down_proj)
+        assert few.wanted(8, 2, 4, torch.empty(2, 1 << 16), *p)
