@@ -181,3 +181,80 @@ def test_a_layer_of_more_features_keeps_the_other_form(H, I):
         small = SparseMoeBlock(1 << 16, 4, 2, 1 << 16)
         p = (small.gate.weight, small.experts.gate_up_proj, small.experts.down_proj)
         assert few.wanted(8, 2, 4, torch.empty(2, 1 << 16), *p)
+
+
+def _blocks():
+    return [SparseMoeBlock(128, 8, 2, 64, router=r).requires_grad_(False)
+            for r in ("softmax", "sigmoid")]
+
+
+@pytest.mark.parametrize("few_tokens", [0, 8])
+def test_fake_tensors_pass_through_either_form(few_tokens):
+    from moe_amd.experts import mi355x_experts_forward
+
+    with FakeTensorMode():
+        for block in _blocks():
+            block.few_tokens = block.experts.few_tokens = few_tokens
+            x = torch.empty(4, 128)
+            assert block(x).shape == (4, 128) and block.topk_index.shape == (4, 2)
+            assert (block.router_logits is None) == bool(few_tokens)
+            idx, w = torch.empty(4, 2, dtype=torch.int64), torch.empty(4, 2)
+            assert mi355x_experts_forward(block.experts, x, idx, w).shape == (4, 128)
+    # fake tensors outside their mode
+    assert few.experts_forward_few(x, idx, w, block.experts.gate_up_proj,
+                                   block.experts.down_proj).shape == (4, 128)
+
+
+def _traced(pre_dispatch, mode):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def fn(x, idx, w, wr, w1, w2):
+        return few.experts_forward_few(few.moe_layer_few(x, wr, w1, w2, 2), idx, w, w1, w2)
+
+    x, idx, w, w1, w2 = _inputs()
+    gm = make_fx(fn, tracing_mode=mode, pre_dispatch=pre_dispatch)(
+        x, idx, w, torch.zeros(8, 128), w1, w2)
+    return {str(n.target).removesuffix(".default") for n in gm.graph.nodes
+            if n.op == "call_function"}
+
+
+@pytest.mark.parametrize("pre_dispatch", [False, True])
+def test_a_trace_holds_the_ops(pre_dispatch):
+    with torch.no_grad():
+        assert {"moe_amd.experts_few", "moe_amd.moe_layer_few"} <= _traced(pre_dispatch, "fake")
+
+
+def test_modes_tracers_and_transforms_see_the_ops():
+    """Under each of them the call is the moe_amd:: op's, not the kernels' own."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, fn, types, args=(), kwargs=None):
+            seen.append(str(fn))
+            return torch.empty(4, 128) if "moe_amd" in str(fn) else fn(*args, **(kwargs or {}))
+
+    x, idx, w, w1, w2 = _inputs()
+    seen = []
+    with torch.no_grad(), Mode():
+        few.experts_forward_few(x, idx, w, w1, w2)
+    assert seen == ["moe_amd.experts_few.default"]
+
+    unseen = []
+
+    def probe(t):
+        unseen.append(few._unseen(t))
+        return t + 1
+
+    probe(x)
+    with torch.inference_mode():
+        probe(x)
+    with torch.no_grad():
+        probe(torch.nn.Parameter(x))
+    assert unseen == [True, True, True] and few._unseen(x, None)
+    unseen.clear()
+    torch.func.vmap(probe)(x)
+    torch.func.functionalize(probe)(x)
+    torch.jit.trace(probe, x, check_trace=False)
+    assert unseen == [False, False, False]
+    # a tensor whose values the dispatcher would negate first
+    assert not few._unseen(x._neg_view())

@@ -599,3 +599,39 @@ def test_block_of_mixed_dtypes():
             blk.few_tokens = 8
             got = blk(h)
             assert got.dtype == dt and torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("how", ["make_fx", "make_fx_pre_dispatch", "jit_trace"])
+def test_traces_repeat_on_other_inputs(how):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    print(f"few: {how}", flush=True)
+    T, H, E, K, I = 5, 128, 8, 2, 64
+    x, wr, w1, w2 = _layer(_gen(70), T, H, E, I, BF)
+    idx, w = _routing(_gen(71), T, E, K)
+
+    def fn(x, idx, w):
+        return few.experts_forward_few(few.moe_layer_few(x, wr, w1, w2, K), idx, w, w1, w2)
+
+    with torch.no_grad():
+        if how == "jit_trace":
+            traced = torch.jit.trace(fn, (x, idx, w))
+        else:
+            traced = make_fx(fn, pre_dispatch=how != "make_fx")(x, idx, w)
+        for seed in (72, 73):
+            x = _layer(_gen(seed), T, H, E, I, BF)[0]
+            idx, w = _routing(_gen(seed), T, E, K)
+            assert torch.equal(traced(x, idx, w), fn(x, idx, w))
+
+
+def test_a_negated_view():
+    """Hidden states that torch holds as the negative of their memory."""
+    print("few: negated view", flush=True)
+    T, H, E, K, I = 5, 128, 8, 2, 64
+    x, wr, w1, w2 = _layer(_gen(74), T, H, E, I, F32)
+    idx, w = _routing(_gen(75), T, E, K)
+    assert x._neg_view().is_neg() and x._neg_view().is_contiguous()
+    assert torch.equal(few.experts_forward_few(x._neg_view(), idx, w, w1, w2),
+                       few.experts_forward_few(-x, idx, w, w1, w2))
+    assert torch.equal(few.moe_layer_few(x._neg_view(), wr, w1, w2, K),
+                       few.moe_layer_few(-x, wr, w1, w2, K))
