@@ -928,6 +928,8 @@ def moe_layer_few(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.T
             raise ValueError(f"{name}: offset or bias {tuple(extra.shape)}, expected {(E,)}")
         extra = _contig(extra.to(torch.float32))
     x, w_router = _contig(x), _contig(w_router)
+    if w_router.data_ptr() % 16:  # moe_layer's gating product takes any alignment
+        w_router = w_router.clone()
     gate_up_proj, down_proj = _contig(gate_up_proj), _contig(down_proj)
     T = x.shape[0]
     grouped = num_groups is not None and group_topk is not None

@@ -635,3 +635,18 @@ def test_a_negated_view():
                        few.experts_forward_few(-x, idx, w, w1, w2))
     assert torch.equal(few.moe_layer_few(x._neg_view(), wr, w1, w2, K),
                        few.moe_layer_few(-x, wr, w1, w2, K))
+
+
+@pytest.mark.parametrize("router", ["softmax", "sigmoid"])
+def test_a_router_weight_of_any_alignment(router):
+    """As moe_layer's gating product takes it, a slice of a flat buffer say."""
+    print(f"few: unaligned router weight {router}", flush=True)
+    T, H, E, K, I = 5, 128, 8, 2, 64
+    x, wr, w1, w2 = _layer(_gen(76), T, H, E, I, BF)
+    flat = torch.empty(E * H + 3, device=DEV, dtype=BF)
+    odd = flat[3:].view(E, H).copy_(wr)
+    assert odd.is_contiguous() and odd.data_ptr() % 16
+    for a, b in zip(few.moe_layer_few(x, odd, w1, w2, K, router=router, return_routing=True),
+                    few.moe_layer_few(x, wr, w1, w2, K, router=router, return_routing=True)):
+        assert torch.equal(a, b)
+    assert moe_layer(x, odd, w1, w2, K, router=router)[0].shape == x.shape
