@@ -101,5 +101,7 @@ def mi355x_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch
                   self.down_proj):
         return few.experts_forward_few(hidden_states, top_k_index, top_k_weights,
                                        self.gate_up_proj, self.down_proj)
+    keep = library.keep_of_call(getattr(self, "saved_activations", "exact"), hidden_states,
+                                top_k_weights, self.gate_up_proj, self.down_proj)
     return experts_forward(hidden_states, top_k_index, top_k_weights, self.gate_up_proj,
-                           self.down_proj, getattr(self, "saved_activations", "exact"))
+                           self.down_proj, keep)

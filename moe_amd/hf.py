@@ -59,7 +59,8 @@ def install(model: nn.Module, routers: bool = True, experts: bool = True,
     (with ``experts``): calls of at most that many tokens (up to
     ``moe_amd.few.MAX_TOKENS``) that want no gradient run the few-token
     experts.  ``saved_activations`` (with ``experts``): what the experts keep
-    for their backward, as ``experts_forward`` takes it."""
+    for their backward, as ``experts_forward`` takes it: other than "exact", calls
+    that want a gradient take bf16 experts only."""
     if saved_activations not in KEEPS:
         raise ValueError(f"unknown saved_activations {saved_activations!r} (expected one of "
                          f"{KEEPS})")

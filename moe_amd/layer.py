@@ -102,7 +102,7 @@ class SparseMoeBlock(nn.Module):
     Up to ``few_tokens`` tokens without a gradient, outside autocast and of the
     weights' dtype, run the few-token layer (``moe_amd.few``; 0, the default:
     never), which computes no router_logits: they are None then.
-    ``saved_activations`` is moe_layer's."""
+    ``saved_activations`` is moe_layer's where a gradient is wanted."""
 
     few_tokens = 0
     saved_activations = "exact"
@@ -141,6 +141,6 @@ class SparseMoeBlock(nn.Module):
             flat, self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj, self.top_k,
             router=self.router, renormalize=self.norm_topk_prob, logit_offset=self.logit_offset,
             expert_bias=self.expert_bias if self.router == "sigmoid" else None,
-            saved_activations=self.saved_activations)
+            saved_activations=library.keep_of_call(self.saved_activations, flat, *params))
         self.router_logits, self.topk_index = probs, idx
         return out.reshape(shape)

@@ -73,6 +73,14 @@ def check_keep(keep: str, dtype: torch.dtype) -> str:
     return keep
 
 
+def keep_of_call(keep: str, *tensors: Tensor) -> str:
+    """A module's ``saved_activations`` for a call on ``tensors``: "exact", which
+    every dtype takes, where no gradient is wanted and so nothing is kept."""
+    if keep in KEEPS and not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
+        return "exact"
+    return keep
+
+
 @torch.library.custom_op(f"{_LIB}::pack8", mutates_args=())
 def pack8(x: Tensor) -> tuple[Tensor, Tensor]:
     """(q int8, scale uint8) of ops.pack8."""

@@ -89,3 +89,39 @@ def test_the_choice_reaches_the_experts(monkeypatch):
     experts.mi355x_experts_forward(bank, *args)
     assert seen == ["exact", "int8"] and library.KEEPS == ("exact", "int8", "int8_all")
     assert block.saved_activations == "exact"
+
+
+@pytest.mark.parametrize("keep", ["int8", "int8_all"])
+def test_fp32_modules_that_keep_nothing_run(keep):
+    """Only what a backward will read is packed, so a call that wants no gradient
+    takes any dtype; one that wants one refuses fp32."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from moe_amd.experts import mi355x_experts_forward
+
+    with FakeTensorMode():
+        block = SparseMoeBlock(128, 8, 2, 64)
+        block.saved_activations = block.experts.saved_activations = keep
+        x = torch.empty(100, 128)
+        routing = torch.empty(100, 2, dtype=torch.int64), torch.empty(100, 2)
+
+        def run():
+            assert block(x).shape == x.shape
+            assert mi355x_experts_forward(block.experts, x, *routing).shape == x.shape
+
+        with torch.no_grad():
+            run()
+        block.requires_grad_(False)
+        run()
+        for part in (block.gate, block.experts):     # the routing weights' gradient too
+            part.requires_grad_(True)
+            with pytest.raises(NotImplementedError, match="bf16 layers"):
+                block(x)
+            part.requires_grad_(False)
+        with pytest.raises(NotImplementedError, match="bf16 layers"):
+            mi355x_experts_forward(block.experts, x.requires_grad_(True), *routing)
+        block.saved_activations = block.experts.saved_activations = "int4"
+        with torch.no_grad(), pytest.raises(ValueError, match="int4"):
+            block(x)
+        with torch.no_grad(), pytest.raises(ValueError, match="int4"):
+            mi355x_experts_forward(block.experts, x, *routing)
