@@ -258,3 +258,31 @@ def test_modes_tracers_and_transforms_see_the_ops():
     assert unseen == [False, False, False]
     # a tensor whose values the dispatcher would negate first
     assert not few._unseen(x._neg_view())
+
+
+def test_install_sets_and_resets_the_banks():
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.blocks = torch.nn.ModuleList(SparseMoeBlock(64, 4, 2, 64) for _ in range(2))
+            self.other = torch.nn.Linear(4, 4)
+            self.chosen = []
+
+        def set_experts_implementation(self, name):
+            self.chosen.append(name)
+
+    def options():
+        return {(b.few_tokens, b.saved_activations) for b in hf.expert_banks(model)}
+
+    model = Model()
+    banks = hf.expert_banks(model)
+    assert banks == [b.experts for b in model.blocks]
+    assert hf.install(model, few_tokens=16, saved_activations="int8") is model
+    assert options() == {(16, "int8")} and not hasattr(model.other, "few_tokens")
+    hf.install(model, few_tokens=8, saved_activations="int8_all", experts=False)   # experts' options
+    assert options() == {(16, "int8")} and model.chosen == [hf.EXPERTS_KEY]
+    hf.install(model)
+    assert options() == {(0, "exact")} and model.chosen == [hf.EXPERTS_KEY] * 2
+    with pytest.raises(ValueError, match="saved_activations"):
+        hf.install(model, few_tokens=4, saved_activations="int4")
+    assert options() == {(0, "exact")}
