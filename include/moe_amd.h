@@ -400,9 +400,11 @@ int moe_amd_gather_backward_add(const void* d_xs, const int32_t* slot, const int
 /* For 64 consecutive values v of a row (its last block may be shorter) a power
  * of two s and the integers q = rint(v / s), halves to even: s is the smallest
  * power of two >= 2^-126 with max|v| <= 127 s.  What is restored, q * s, is
- * exact in bf16 and fp32.  q int8 [rows, cols], scale [rows, ceil(cols / 64)]
+ * exact in bf16 and fp32, but for finite |v| above 127/128 2^128 (q s = 2^128),
+ * restored as infinity.  q int8 [rows, cols], scale [rows, ceil(cols / 64)]
  * bytes: s's biased exponent, or 255 for a block with a value that is not
- * finite, which is restored as NaN whole.  No counterpart in the reference. */
+ * finite, whose q are 0 and which is restored as NaN whole.  No counterpart in
+ * the reference. */
 int moe_amd_pack8(const void* x, int dtype, int64_t rows, int64_t cols, void* q, void* scale,
                   void* stream);
 int moe_amd_unpack8(const void* q, const void* scale, int64_t rows, int64_t cols, void* x,

@@ -642,9 +642,10 @@ __global__ __launch_bounds__(64 * kWaves) void few_gate_up_kernel(FewArgs p) {
 // wave takes the next one when it is done with its own (the oldest waves get
 // their loads first: with a fixed share each, they end after half of the time
 // and the rest finishes with too few loads in flight).  `parts` makes the column slices about as many
-// as CUs: the A operand's 16 rows are C columns' weights for each of `parts`
-// pieces of the contraction, B's 16 columns C of the expert's rows for each of
-// them, and the blocks of the product where the pieces match are added.
+// as CUs where it divides the contraction's blocks: the A operand's 16 rows are
+// C columns' weights for each of `parts` pieces of the contraction, B's 16
+// columns C of the expert's rows for each of them, and the blocks of the product
+// where the pieces match are added.
 // A wave needs no other one: it reads CH blocks and the next CH before it
 // multiplies these, and leaves y in LDS, where the workgroup then sums it with
 // the routing weights, in k order.
@@ -864,7 +865,10 @@ hipError_t few_launch(const FewArgs& p, hipStream_t st) {
   if (part <= 64) plan(std::integral_constant<int, 1>{});
   else if (part <= 128) plan(std::integral_constant<int, 2>{});
   else plan(std::integral_constant<int, 4>{});
-  // column slices of 16 / parts: about one for every CU
+  // Column slices of 16 / parts: about one for every CU, where the contraction has
+  // a multiple of parts blocks.  With an odd number there are H / 16, too few below
+  // H = 4096: bf16, E = 128, T = 64, I = 704 (11 blocks) and 768 (12), H = 1024:
+  // 83 and 54 us (2.2 and 3.8 TB/s), H = 2048: 89 and 68 (4.1 and 5.9).
   int parts = p.H / 16 >= 256 ? 1 : p.H / 8 >= 256 ? 2 : 4;
   const int blocks = p.I * (int)sizeof(T) / kBlock;
   while (blocks % parts) parts /= 2;

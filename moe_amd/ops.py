@@ -797,9 +797,12 @@ class Packed8:
 def pack8(x: torch.Tensor) -> Packed8:
     """x (bf16 or fp32, at least one dimension) in 8 bits: per 64 values v of
     its last dimension s, the smallest power of two >= 2^-126 with max|v| <=
-    127 s, and rint(v / s).  The error is at most s / 2, max|v| / 127 in the
-    worst case; what unpack8 gives is exact in x's dtype.  A block with a value
-    that is not finite comes back as NaN whole."""
+    127 s, and rint(v / s).  The error is at most s / 2, which is at most max|v|
+    / 127 where max|v| >= 2^-120 (below, s may be the 2^-126 that it never falls
+    under, and a value up to 2^-127 becomes 0).  What unpack8 gives is exact in
+    x's dtype, but for values above 127/128 2^128, bf16's largest for one, which
+    come back as infinity.  A block with a value that is not finite comes back
+    as NaN whole."""
     _need_cuda(x)
     if x.dim() == 0:
         raise ValueError("pack8 takes tensors of at least one dimension")
