@@ -432,6 +432,53 @@ int moe_amd_gemm_down_backward_dx_fused_pack8(
     int E, int H, int I, int dtype, void* d_gate_up, void* act_w, float* dw_partials,
     void* stream);
 
+/* ---------------------------------------------------- weights in 4 bits */
+
+/* For 32 consecutive values v of a row (zeros follow its last ones) a power of
+ * two s and a code a value: bit 3 its sign, bits 0 to 2 the magnitude of v / s
+ * rounded to 0, 1/2, 1, 3/2, 2, 3, 4 or 6, halves to the even code.  s is the
+ * smallest power of two >= 2^-125 with max|v| <= 7 s; its byte is the biased
+ * exponent, 2 to 253, or 255 for a block with a value that is not finite, whose
+ * codes are 0 and which is restored as NaN whole.  What is restored is exact in
+ * bf16 and fp32, but for finite |v| above 7/8 2^128, restored as infinity.  The
+ * error is at most s (half the step between 4 s and 6 s).  (E2M1 codes, E8M0
+ * scales: any byte but 255 stands for 2^(byte - 127).)
+ *
+ * Tiles of 16 rows by 128 columns, each of the `batch` matrices [n,k] beginning
+ * with one of its own, zeros where it ends inside a tile: with nt = ceil(n / 16),
+ * kt = ceil(k / 128),
+ *   q      [batch][nt][kt][block of 32 columns 4][row 16][16 bytes], a byte two
+ *          values, the first one in its low half;
+ *   scale  [batch][nt][kt][row 16][block of 32 columns 4] bytes.
+ * pack4 writes all of a tile.  x is aligned to its values, q and scale to 4 bytes.
+ * No counterpart in the reference. */
+enum { MOE_PACK4_Q_BYTES = 1024, MOE_PACK4_SCALE_BYTES = 64 }; /* of a tile */
+int moe_amd_pack4(const void* x, int dtype, int64_t batch, int64_t n, int64_t k, void* q,
+                  void* scale, void* stream);
+int moe_amd_unpack4(const void* q, const void* scale, int64_t batch, int64_t n, int64_t k, void* x,
+                    int dtype, void* stream);
+
+/* The expert layer's products on a bank in 4 bits, forward only, bf16 rows:
+ * moe_amd_gemm_gate_up_swiglu and moe_amd_gemm_down with gate_up_proj
+ * [E,2I,H] and down_proj [E,H,I] as moe_amd_pack4 leaves them (batch = E), and the
+ * combine of what they give.  act_out [S,I] = bf16(silu(gate) * up), gate and up in
+ * fp32; y_out int16 [S,H] with a byte for 64 columns of a row in y_scale_out
+ * [S,H/64]: y = y_out * 2^(byte - 127), within half of that power, which is at
+ * most 2^-14 of the block's largest value (255: a value is not finite, NaN whole);
+ * out [T,H] bf16, sums in fp32.  Sentinel rows are not written and contribute
+ * nothing.  H and I multiples of 64, S < 2^29, T H 2 < 2^31, an expert's codes
+ * below 2 GB; codes and scales 16-byte aligned. */
+int moe_amd_gemm_gate_up_swiglu4(const void* hidden_states, const int32_t* row_src, int top_k,
+                                 const int32_t* offsets, const void* tile_plan,
+                                 const void* gate_up_q, const void* gate_up_scale, int64_t T,
+                                 int64_t S, int E, int H, int I, void* act_out, void* stream);
+int moe_amd_gemm_down4(const void* act, const int32_t* offsets, const void* tile_plan,
+                       const void* down_q, const void* down_scale, int64_t S, int E, int H, int I,
+                       void* y_out, void* y_scale_out, void* stream);
+int moe_amd_combine16(const void* y, const void* y_scale, const int32_t* slot,
+                      const int32_t* offsets, const void* topk_weights, int weights_dtype,
+                      int64_t T, int K, int E, int H, void* out, void* stream);
+
 /* --------------------------------------------- the layer for a few tokens */
 
 /* The expert layer for up to MOE_FEW_MAX_TOKENS tokens, forward only: the
@@ -470,6 +517,23 @@ int moe_amd_moe_layer_few(const void* hidden_states, const void* router_weight,
                           int renormalize, float scaling_factor, int num_groups, int group_topk,
                           void* workspace, size_t workspace_bytes, float* topk_weights,
                           int64_t* topk_index, void* out, void* stream);
+
+/* The same two on a bank in 4 bits (gate_up_proj and down_proj as moe_amd_pack4
+ * leaves them, 16-byte aligned): hidden_states, router_weight and out bf16, the
+ * other arguments, limits and workspace rules as above. */
+size_t moe_amd_few4_workspace_size(int64_t T, int E, int K, int H, int I);
+int moe_amd_experts_few4(const void* hidden_states, const int64_t* topk_index,
+                         const void* topk_weights, int weights_dtype, const void* gate_up_q,
+                         const void* gate_up_scale, const void* down_q, const void* down_scale,
+                         int64_t T, int K, int E, int H, int I, void* workspace,
+                         size_t workspace_bytes, void* out, void* stream);
+int moe_amd_moe_layer_few4(const void* hidden_states, const void* router_weight,
+                           const void* gate_up_q, const void* gate_up_scale, const void* down_q,
+                           const void* down_scale, int64_t T, int K, int E, int H, int I,
+                           int router, const float* offset_or_bias, int renormalize,
+                           float scaling_factor, int num_groups, int group_topk, void* workspace,
+                           size_t workspace_bytes, float* topk_weights, int64_t* topk_index,
+                           void* out, void* stream);
 
 /* ---------------------------------------------------- routing consumers */
 

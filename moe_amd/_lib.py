@@ -85,6 +85,8 @@ SIGNATURES: dict[str, tuple] = {
     "moe_amd_gather_backward_add": (_i, [_p, _p, _p, _p, _i64, _i, _i, _i, _i, _p, _p]),
     "moe_amd_pack8": (_i, [_p, _i, _i64, _i64, _p, _p, _p]),
     "moe_amd_unpack8": (_i, [_p, _p, _i64, _i64, _p, _i, _p]),
+    "moe_amd_pack4": (_i, [_p, _i, _i64, _i64, _i64, _p, _p, _p]),
+    "moe_amd_unpack4": (_i, [_p, _p, _i64, _i64, _i64, _p, _i, _p]),
     "moe_amd_gemm_gate_up_swiglu_pack8": (
         _i, [_p, _p, _i, _p, _p, _p, _i64, _i64, _i, _i, _i, _i, _p, _p, _p, _p]),
     "moe_amd_gemm_down_backward_dx_fused_pack8": (
@@ -96,6 +98,16 @@ SIGNATURES: dict[str, tuple] = {
     "moe_amd_moe_layer_few": (
         _i, [_p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _i, _p, _i, _f, _i, _i, _p, _sz, _p, _p,
              _p, _p]),
+    "moe_amd_few4_workspace_size": (_sz, [_i64, _i, _i, _i, _i]),
+    "moe_amd_experts_few4": (
+        _i, [_p, _p, _p, _i, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _p, _sz, _p, _p]),
+    "moe_amd_moe_layer_few4": (
+        _i, [_p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _p, _i, _f, _i, _i, _p, _sz, _p,
+             _p, _p, _p]),
+    "moe_amd_gemm_gate_up_swiglu4": (
+        _i, [_p, _p, _i, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _p, _p]),
+    "moe_amd_gemm_down4": (_i, [_p, _p, _p, _p, _p, _i64, _i, _i, _i, _p, _p, _p]),
+    "moe_amd_combine16": (_i, [_p, _p, _p, _p, _p, _i, _i64, _i, _i, _i, _p, _p]),
     "moe_amd_topk_stats_workspace_size": (_sz, [_i64, _i]),
     "moe_amd_topk_stats": (_i, [_p, _i, _p, _i64, _i, _i, _p, _sz, _p, _p, _p, _p]),
     "moe_amd_seq_stats_workspace_size": (_sz, [_i64, _i, _i]),

@@ -19,7 +19,9 @@ import inspect
 
 import torch
 
-from . import few, library  # noqa: F401  (library registers the moe_amd:: ops)
+from torch import nn
+
+from . import few, library, ops  # library registers the moe_amd:: ops
 
 
 def traced_with_defaults(fn):
@@ -37,8 +39,9 @@ def traced_with_defaults(fn):
 
 @traced_with_defaults
 def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
-                    top_k_weights: torch.Tensor, gate_up_proj: torch.Tensor,
-                    down_proj: torch.Tensor, saved_activations: str = "exact") -> torch.Tensor:
+                    top_k_weights: torch.Tensor, gate_up_proj: torch.Tensor | ops.Packed4,
+                    down_proj: torch.Tensor | ops.Packed4,
+                    saved_activations: str = "exact") -> torch.Tensor:
     """out[t] = sum_k w[t,k] * down_e(silu(gate_e(x_t)) * up_e(x_t)), e = idx[t,k].
 
     ``saved_activations`` (bf16 layers): what the backward finds of the
@@ -48,11 +51,17 @@ def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
     of the restored gate_up, the output is the same.  "int8_all": the hidden
     states too, for d_gate_up_proj; worth it where nothing else keeps them.
 
+    A bank in 4 bits (``ops.Packed4`` for both weights; bf16 layers) is forward
+    only: calls that want a gradient are refused.
+
     hidden_states is cast to the weights' dtype (as transformers' _grouped_mm
     does, integrations/moe.py:330-335) and the result is returned in
     hidden_states' dtype (:478)."""
     if hidden_states.dim() != 2:
         raise ValueError("hidden_states must be [T, H]")
+    if isinstance(gate_up_proj, ops.Packed4) or isinstance(down_proj, ops.Packed4):
+        return _experts_forward4(hidden_states, top_k_index, top_k_weights, gate_up_proj,
+                                 down_proj, saved_activations)
     if gate_up_proj.dim() != 3 or down_proj.dim() != 3:
         raise ValueError("gate_up_proj must be [E, 2I, H] and down_proj [E, H, I]")
     E, I2, H = gate_up_proj.shape
@@ -73,6 +82,26 @@ def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
     return out.to(out_dtype)
 
 
+def _experts_forward4(hidden_states, top_k_index, top_k_weights, gate_up_proj, down_proj,
+                      saved_activations):
+    bank = library.check_bank4("experts_forward", hidden_states, gate_up_proj, down_proj)
+    if top_k_index.dim() != 2 or top_k_index.shape != top_k_weights.shape \
+            or top_k_index.shape[0] != hidden_states.shape[0]:
+        raise ValueError("top_k_index / top_k_weights must both be [T, K]")
+    library.check_keep(saved_activations, gate_up_proj.dtype)
+    refuse_grad4("experts_forward", hidden_states, top_k_weights)
+    out = torch.ops.moe_amd.experts_fwd4(hidden_states.to(torch.bfloat16).contiguous(), top_k_index,
+                                         top_k_weights.contiguous(), *bank)
+    return out.to(hidden_states.dtype)
+
+
+def refuse_grad4(name: str, *tensors: torch.Tensor) -> None:
+    """A bank in 4 bits has no backward."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name}: a bank in 4 bits is forward only: call it under "
+                           "torch.no_grad()")
+
+
 def _check_module(self) -> None:
     if not getattr(self, "has_gate", True):
         raise NotImplementedError("mi355x experts: only gated (gate_up_proj) experts are supported")
@@ -88,20 +117,58 @@ def _check_module(self) -> None:
         raise NotImplementedError(f"mi355x experts: activation {type(act).__name__} is not SiLU")
 
 
+_BANK = ("gate_up_proj", "down_proj")
+
+
+def is_packed_bank(bank: nn.Module) -> bool:
+    return hasattr(bank, "packed_shapes")
+
+
+def pack_bank(bank: nn.Module) -> nn.Module:
+    """Replaces a bank's parameters gate_up_proj and down_proj (bf16, on the GPU) by
+    their 4 bits, in place: buffers gate_up_proj_q, gate_up_proj_scale and down_proj's,
+    which state_dict holds and ``to`` moves.  The bank is forward only from then on."""
+    if is_packed_bank(bank):
+        return bank
+    weights = [getattr(bank, name) for name in _BANK]
+    for name, w in zip(_BANK, weights):
+        if w.dtype != torch.bfloat16:
+            raise NotImplementedError(f"pack_bank: {name} of {w.dtype}; banks in 4 bits take bf16 "
+                                      "layers")
+        if w.dim() != 3 or w.shape[1] % 64 or w.shape[2] % 64:
+            raise ValueError(f"pack_bank: {name} {tuple(w.shape)}: both of its dimensions must be "
+                             "multiples of 64")
+    packed = [ops.pack4(w.detach()) for w in weights]
+    for name, p in zip(_BANK, packed):
+        delattr(bank, name)
+        bank.register_buffer(f"{name}_q", p.q)
+        bank.register_buffer(f"{name}_scale", p.scale)
+    bank.packed_shapes = tuple(p.shape for p in packed)
+    return bank
+
+
+def bank_weights(bank: nn.Module):
+    """(gate_up_proj, down_proj) of a bank: its parameters, or its weights in 4
+    bits."""
+    if not is_packed_bank(bank):
+        return bank.gate_up_proj, bank.down_proj
+    return tuple(ops.Packed4(getattr(bank, f"{name}_q"), getattr(bank, f"{name}_scale"), shape,
+                             torch.bfloat16) for name, shape in zip(_BANK, bank.packed_shapes))
+
+
 def mi355x_experts_forward(self, hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                            top_k_weights: torch.Tensor) -> torch.Tensor:
     """ExpertsInterface entry ("mi355x"), drop-in for grouped_mm_experts_forward
     (transformers/integrations/moe.py:377-478).  A bank with a ``few_tokens``
     attribute runs the few-token experts up to that many tokens where no
     gradient is wanted, and a ``saved_activations`` attribute is
-    experts_forward's (``hf.install`` sets both)."""
+    experts_forward's (``hf.install`` sets both).  A bank that ``pack_bank`` packed
+    runs on its weights in 4 bits."""
     _check_module(self)
-    if few.wanted(getattr(self, "few_tokens", 0), top_k_index.shape[-1],
-                  self.gate_up_proj.shape[0], hidden_states, top_k_weights, self.gate_up_proj,
-                  self.down_proj):
-        return few.experts_forward_few(hidden_states, top_k_index, top_k_weights,
-                                       self.gate_up_proj, self.down_proj)
+    w1, w2 = bank_weights(self)
+    if few.wanted(getattr(self, "few_tokens", 0), top_k_index.shape[-1], w1.shape[0],
+                  hidden_states, top_k_weights, w1, w2):
+        return few.experts_forward_few(hidden_states, top_k_index, top_k_weights, w1, w2)
     keep = library.keep_of_call(getattr(self, "saved_activations", "exact"), hidden_states,
-                                top_k_weights, self.gate_up_proj, self.down_proj)
-    return experts_forward(hidden_states, top_k_index, top_k_weights, self.gate_up_proj,
-                           self.down_proj, keep)
+                                top_k_weights, w1, w2)
+    return experts_forward(hidden_states, top_k_index, top_k_weights, w1, w2, keep)

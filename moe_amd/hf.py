@@ -14,7 +14,7 @@ from __future__ import annotations
 
 from torch import nn
 
-from .experts import mi355x_experts_forward
+from .experts import is_packed_bank, mi355x_experts_forward, pack_bank
 from .library import KEEPS
 from .router import MI355XDeepSeekRouter, MI355XTopKRouter, _RouterBase
 
@@ -47,10 +47,21 @@ def swap_routers(model: nn.Module) -> int:
 
 
 def expert_banks(model: nn.Module) -> list[nn.Module]:
-    """The modules that hold an expert bank (gate_up_proj and down_proj)."""
+    """The modules that hold an expert bank (gate_up_proj and down_proj, or their
+    4 bits)."""
     return [m for m in model.modules()
-            if hasattr(m, "gate_up_proj") and hasattr(m, "down_proj")
-            and getattr(m.gate_up_proj, "ndim", 0) == 3]
+            if is_packed_bank(m) or (hasattr(m, "gate_up_proj") and hasattr(m, "down_proj")
+                                     and getattr(m.gate_up_proj, "ndim", 0) == 3)]
+
+
+def pack_experts(model: nn.Module) -> int:
+    """Puts every expert bank (bf16, on the GPU) in 4 bits, in place and for good: a
+    served model's form, forward only, whose "mi355x" experts (``install``) read
+    the banks as they are.  Returns the number of banks packed."""
+    banks = [m for m in expert_banks(model) if not is_packed_bank(m)]
+    for bank in banks:
+        pack_bank(bank)
+    return len(banks)
 
 
 def install(model: nn.Module, routers: bool = True, experts: bool = True,

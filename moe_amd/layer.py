@@ -20,22 +20,23 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import few, library  # library registers the moe_amd:: ops
-from .experts import experts_forward, traced_with_defaults
+from . import few, library, ops  # library registers the moe_amd:: ops
+from .experts import (bank_weights, experts_forward, pack_bank, refuse_grad4,
+                      traced_with_defaults)
 from .router import gating_linear, linear_sigmoid_topk, sigmoid_topk, softmax_topk
 
 
 def _fused_softmax_ok(x, w_router, gate_up_proj, down_proj) -> bool:
     E, H = w_router.shape
-    return (x.is_cuda and x.dim() == 2 and x.dtype == torch.bfloat16
+    return (not isinstance(gate_up_proj, ops.Packed4) and x.is_cuda and x.dim() == 2 and x.dtype == torch.bfloat16
             and w_router.dtype == torch.bfloat16 and gate_up_proj.dtype == torch.bfloat16
             and down_proj.dtype == torch.bfloat16 and H % 256 == 0 and E % 8 == 0
             and gate_up_proj.shape[0] == E)
 
 
 @traced_with_defaults
-def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tensor,
-              down_proj: torch.Tensor, top_k: int, router: str = "softmax",
+def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tensor | ops.Packed4,
+              down_proj: torch.Tensor | ops.Packed4, top_k: int, router: str = "softmax",
               renormalize: bool = True, logit_offset: torch.Tensor | None = None,
               expert_bias: torch.Tensor | None = None, scaling_factor: float | None = None,
               num_groups: int | None = None, group_topk: int | None = None,
@@ -45,10 +46,13 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tenso
     ``saved_activations`` as for experts_forward; with "int8_all" the router
     weight's gradient comes from the restored hidden states too where router
     and experts are one node (bf16 softmax layers), and elsewhere the router
-    keeps its own."""
+    keeps its own.  A bank in 4 bits (``ops.Packed4``) is forward only."""
     if gating not in library.GATINGS:
         raise ValueError(f"unknown gating {gating!r} (expected one of {library.GATINGS})")
     library.check_keep(saved_activations, gate_up_proj.dtype)
+    if isinstance(gate_up_proj, ops.Packed4):
+        library.check_bank4("moe_layer", x, gate_up_proj, down_proj)
+        refuse_grad4("moe_layer", x, w_router)
     hip = gating in ("hip", "hip_fused")
     if router == "softmax" and _fused_softmax_ok(x, w_router, gate_up_proj, down_proj):
         # Gating linear + softmax router + experts as ONE autograd node (op
@@ -102,7 +106,8 @@ class SparseMoeBlock(nn.Module):
     Up to ``few_tokens`` tokens without a gradient, outside autocast and of the
     weights' dtype, run the few-token layer (``moe_amd.few``; 0, the default:
     never), which computes no router_logits: they are None then.
-    ``saved_activations`` is moe_layer's where a gradient is wanted."""
+    ``saved_activations`` is moe_layer's where a gradient is wanted.
+    ``pack_experts`` puts the bank in 4 bits."""
 
     few_tokens = 0
     saved_activations = "exact"
@@ -120,10 +125,15 @@ class SparseMoeBlock(nn.Module):
         self.router_logits = None
         self.topk_index = None
 
+    def pack_experts(self) -> "SparseMoeBlock":
+        """Holds the bank (bf16, on the GPU) in 4 bits from now on, forward only."""
+        pack_bank(self.experts)
+        return self
+
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         shape = hidden_states.shape
         flat = hidden_states.reshape(-1, shape[-1])
-        params = (self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj)
+        params = (self.gate.weight, *bank_weights(self.experts))
         # (autocast's logits are bf16 whatever the weights are, and the sigmoid
         # router takes a weight of another dtype: the other form's)
         if few.wanted(self.few_tokens, self.top_k, self.gate.weight.shape[0], flat, *params) \
@@ -131,15 +141,13 @@ class SparseMoeBlock(nn.Module):
                 and not torch.is_autocast_enabled():
             sig = self.router == "sigmoid"
             out, _, self.topk_index = few.moe_layer_few(
-                flat, self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj,
-                self.top_k, router=self.router, renormalize=self.norm_topk_prob,
+                flat, *params, self.top_k, router=self.router, renormalize=self.norm_topk_prob,
                 logit_offset=None if sig else self.logit_offset,
                 expert_bias=self.expert_bias if sig else None, return_routing=True)
             self.router_logits = None
             return out.reshape(shape)
         out, probs, _, idx = moe_layer(
-            flat, self.gate.weight, self.experts.gate_up_proj, self.experts.down_proj, self.top_k,
-            router=self.router, renormalize=self.norm_topk_prob, logit_offset=self.logit_offset,
+            flat, *params, self.top_k, router=self.router, renormalize=self.norm_topk_prob, logit_offset=self.logit_offset,
             expert_bias=self.expert_bias if self.router == "sigmoid" else None,
             saved_activations=library.keep_of_call(self.saved_activations, flat, *params))
         self.router_logits, self.topk_index = probs, idx

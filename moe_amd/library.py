@@ -21,6 +21,9 @@ differentiable piece of the MI355X path, each a functional op in namespace
   pack8 / unpack8                a tensor to 8 bits and back
   experts_few / moe_layer_few    the experts, and the layer, for a few tokens
                                  (forward only)
+  pack4 / unpack4                a weight to 4 bits and back
+  experts_fwd4 / experts_few4 /  the experts, and those and the layer for a few
+  moe_layer_few4                 tokens, on a bank in 4 bits (forward only)
 
 A forward op returns, besides its results, the tensors its backward needs
 (the routing plan, gate_up), so that setup_context saves only op outputs; the
@@ -806,6 +809,114 @@ def moe_layer_few(x: Tensor, w_router: Tensor, gate_up_proj: Tensor, down_proj: 
 @moe_layer_few.register_fake
 def _(x, w_router, gate_up_proj, down_proj, top_k, router, renormalize, logit_offset, expert_bias,
       scaling_factor, num_groups, group_topk):
+    T = x.shape[0]
+    return (x.new_empty(x.shape), x.new_empty(T, top_k, dtype=torch.float32),
+            x.new_empty(T, top_k, dtype=torch.int64))
+
+
+# ------------------------------------------------- banks in 4 bits (forward)
+
+@torch.library.custom_op(f"{_LIB}::pack4", mutates_args=())
+def pack4(w: Tensor) -> tuple[Tensor, Tensor]:
+    """(q, scale) of ops.pack4."""
+    p = ops.pack4(w)
+    return p.q, p.scale
+
+
+@pack4.register_fake
+def _(w):
+    *lead, n, k = w.shape
+    rows, cols = ops.PACK4_TILE
+    tiles = (*lead, (n + rows - 1) // rows, (k + cols - 1) // cols)
+    return (w.new_empty((*tiles, 1024), dtype=torch.uint8),
+            w.new_empty((*tiles, 64), dtype=torch.uint8))
+
+
+@torch.library.custom_op(f"{_LIB}::unpack4", mutates_args=())
+def unpack4(q: Tensor, scale: Tensor, n: int, k: int, dtype: torch.dtype) -> Tensor:
+    """The weight [..., n, k] that (q, scale) hold, in dtype."""
+    return ops.unpack4(ops.Packed4(q, scale, (*q.shape[:-3], n, k), dtype))
+
+
+@unpack4.register_fake
+def _(q, scale, n, k, dtype):
+    return q.new_empty((*q.shape[:-3], n, k), dtype=dtype)
+
+
+def check_bank4(name: str, x: Tensor, gate_up_proj, down_proj) -> tuple[Tensor, ...]:
+    """(gate_up's q and scale, down's) of a call on a bank in 4 bits, its shapes
+    and types checked."""
+    if not (isinstance(gate_up_proj, ops.Packed4) and isinstance(down_proj, ops.Packed4)):
+        raise TypeError(f"{name}: gate_up_proj and down_proj must both be in 4 bits, or neither")
+    for p in (gate_up_proj, down_proj):
+        ops.check_packed4(name, p)
+        if p.dtype != torch.bfloat16:
+            raise NotImplementedError(f"{name}: banks in 4 bits take bf16 layers, not {p.dtype}")
+    s1, s2 = gate_up_proj.shape, down_proj.shape
+    if len(s1) != 3 or s1[1] % 2 or tuple(s2) != (s1[0], s1[2], s1[1] // 2) or x.dim() != 2 \
+            or x.shape[1] != s1[2]:
+        raise ValueError(f"{name}: shape mismatch: hidden {tuple(x.shape)}, gate_up_proj "
+                         f"{tuple(s1)}, down_proj {tuple(s2)}")
+    if s1[2] % 64 or s2[2] % 64:
+        raise ValueError(f"{name}: H={s1[2]} and I={s2[2]} must be multiples of 64")
+    return gate_up_proj.q, gate_up_proj.scale, down_proj.q, down_proj.scale
+
+
+def _bank4(x: Tensor, q1: Tensor, s1: Tensor, q2: Tensor, s2: Tensor):
+    """(gate_up_proj, down_proj) of bf16 hidden states x [T,H]: I is a multiple of
+    64, so that gate_up_proj's tiles have no padded rows."""
+    E, H, I = q1.shape[0], x.shape[1], q1.shape[1] * 8
+    return (ops.Packed4(q1, s1, (E, 2 * I, H), torch.bfloat16),
+            ops.Packed4(q2, s2, (E, H, I), torch.bfloat16))
+
+
+@torch.library.custom_op(f"{_LIB}::experts_fwd4", mutates_args=())
+def experts_fwd4(x: Tensor, topk_index: Tensor, topk_weights: Tensor, gate_up_q: Tensor,
+                 gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor) -> Tensor:
+    """The experts on a bank in 4 bits; no autograd formula."""
+    w1, w2 = _bank4(x, gate_up_q, gate_up_scale, down_q, down_scale)
+    plan = ops.permute(topk_index, w1.shape[0])
+    act = ops.gemm_gate_up_swiglu4(x, plan, w1)
+    y, ys = ops.gemm_down4(act, plan, w2)
+    del act
+    return ops.combine16(y, ys, plan, topk_weights)
+
+
+@experts_fwd4.register_fake
+def _(x, topk_index, topk_weights, gate_up_q, gate_up_scale, down_q, down_scale):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{_LIB}::experts_few4", mutates_args=())
+def experts_few4(x: Tensor, topk_index: Tensor, topk_weights: Tensor, gate_up_q: Tensor,
+                 gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor) -> Tensor:
+    """The experts for a few tokens on a bank in 4 bits; no autograd formula."""
+    return ops.experts_few4(x, topk_index, topk_weights,
+                            *_bank4(x, gate_up_q, gate_up_scale, down_q, down_scale))
+
+
+@experts_few4.register_fake
+def _(x, topk_index, topk_weights, gate_up_q, gate_up_scale, down_q, down_scale):
+    return x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{_LIB}::moe_layer_few4", mutates_args=())
+def moe_layer_few4(x: Tensor, w_router: Tensor, gate_up_q: Tensor, gate_up_scale: Tensor,
+                   down_q: Tensor, down_scale: Tensor, top_k: int, router: str, renormalize: bool,
+                   logit_offset: Optional[Tensor], expert_bias: Optional[Tensor],
+                   scaling_factor: Optional[float], num_groups: Optional[int],
+                   group_topk: Optional[int]) -> tuple[Tensor, Tensor, Tensor]:
+    """(out, weights fp32, index) of the layer for a few tokens on a bank in 4
+    bits; no autograd formula."""
+    return ops.moe_layer_few4(x, w_router,
+                              *_bank4(x, gate_up_q, gate_up_scale, down_q, down_scale), top_k,
+                              router, renormalize, logit_offset, expert_bias, scaling_factor,
+                              num_groups, group_topk)
+
+
+@moe_layer_few4.register_fake
+def _(x, w_router, gate_up_q, gate_up_scale, down_q, down_scale, top_k, router, renormalize,
+      logit_offset, expert_bias, scaling_factor, num_groups, group_topk):
     T = x.shape[0]
     return (x.new_empty(x.shape), x.new_empty(T, top_k, dtype=torch.float32),
             x.new_empty(T, top_k, dtype=torch.int64))

@@ -8,6 +8,7 @@ path: non-CUDA tensors or a missing library raise.
 from __future__ import annotations
 
 import functools
+import math
 from dataclasses import dataclass
 
 import torch
@@ -52,7 +53,7 @@ def _device_of(args, kwargs):
     for a in (*args, *kwargs.values()) if kwargs else args:
         if isinstance(a, RoutingPlan):
             return a.counts.device.index
-        if isinstance(a, Packed8):
+        if isinstance(a, (Packed8, Packed4)):
             return a.q.device.index
         if getattr(a, "is_cuda", False):
             return a.device.index
@@ -835,6 +836,169 @@ def unpack8(packed: Packed8) -> torch.Tensor:
     return x
 
 
+# ---------------------------------------------------------- weights in 4 bits
+
+PACK4_BLOCK = 32          # values that share a scale
+PACK4_TILE = (16, 128)    # rows and columns of a tile
+
+
+@dataclass
+class Packed4:
+    """A weight in 4 bits (:func:`pack4`), or a bank of them, [..., N, K]: its
+    codes and scales in tiles of 16 rows by 128 columns (zeros where the matrix
+    ends inside one), q uint8 [..., ceil(N/16), ceil(K/128), 1024], by block of 32
+    columns, row, two values a byte with the first one in its low half; scale uint8
+    [..., ceil(N/16), ceil(K/128), 64], by row, block of 32 columns; the shape, and
+    the dtype that it is restored in."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    shape: tuple[int, ...]
+    dtype: torch.dtype
+
+    requires_grad = False   # held for its values alone
+
+    @property
+    def device(self) -> torch.device:
+        return self.q.device
+
+
+def _pack4_shapes(shape) -> tuple[tuple[int, ...], tuple[int, ...]]:
+    """The shapes of q and scale."""
+    *lead, n, k = shape
+    tiles = (*lead, -(-n // PACK4_TILE[0]), -(-k // PACK4_TILE[1]))
+    return (*tiles, 1024), (*tiles, 64)
+
+
+def check_packed4(name: str, p: Packed4) -> None:
+    """Raises unless p's tensors are those of a packed weight of its shape."""
+    if len(p.shape) < 2 or p.q.dtype != torch.uint8 or p.scale.dtype != torch.uint8 \
+            or p.q.device != p.scale.device \
+            or (tuple(p.q.shape), tuple(p.scale.shape)) != _pack4_shapes(p.shape):
+        raise ValueError(f"{name}: q {p.q.dtype} {tuple(p.q.shape)} and scale {p.scale.dtype} "
+                         f"{tuple(p.scale.shape)} are not a packed {tuple(p.shape)} weight")
+
+
+def _matrices(shape) -> tuple[int, int, int]:
+    """(number of matrices, rows, columns)."""
+    *lead, n, k = shape
+    return math.prod(lead), n, k
+
+
+@on_tensor_device
+def pack4(w: torch.Tensor, dtype: torch.dtype | None = None) -> Packed4:
+    """w [..., N, K] (bf16 or fp32) in 4 bits: per 32 values v of a row s, the
+    smallest power of two >= 2^-125 with max|v| <= 7 s, and v / s rounded to
+    0, 1/2, 1, 3/2, 2, 3, 4 or 6 and a sign, halves to the even code: 17 bytes
+    for 32 values.  The error is at most s, of normal values a ninth of theirs in the
+    root mean square.  What unpack4 gives is exact in bf16 and fp32, but for values
+    above 7/8 2^128, which come back as infinity; a block with a value that is not
+    finite comes back as NaN whole.  ``dtype``: what the weight is restored in, and
+    what an expert layer on it computes in; w's own by default."""
+    _need_cuda(w)
+    if w.dim() < 2:
+        raise ValueError("pack4 takes matrices, of at least two dimensions")
+    code = _dtype_code(w.dtype)
+    _dtype_code(dtype := dtype or w.dtype)
+    w = _contig(w)
+    shape = tuple(w.shape)
+    qs, ss = _pack4_shapes(shape)
+    q, scale = w.new_empty(qs, dtype=torch.uint8), w.new_empty(ss, dtype=torch.uint8)
+    batch, n, k = _matrices(shape)
+    _call("moe_amd_pack4", w.data_ptr(), code, batch, n, k, q.data_ptr(), scale.data_ptr(),
+          _stream(w), capturable=True)
+    return Packed4(q, scale, shape, dtype)
+
+
+@on_tensor_device
+def unpack4(packed: Packed4) -> torch.Tensor:
+    """The weight that ``packed`` holds, in its dtype."""
+    _need_cuda(packed.q, packed.scale)
+    check_packed4("unpack4", packed)
+    code = _dtype_code(packed.dtype)
+    q, scale = _contig(packed.q), _contig(packed.scale)
+    w = q.new_empty(packed.shape, dtype=packed.dtype)
+    batch, n, k = _matrices(packed.shape)
+    _call("moe_amd_unpack4", q.data_ptr(), scale.data_ptr(), batch, n, k, w.data_ptr(), code,
+          _stream(q), capturable=True)
+    return w
+
+
+def _packed_operand(name: str, p: Packed4, like: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of a packed bank that a kernel takes beside ``like``."""
+    _need_cuda(p.q, p.scale)
+    check_packed4(name, p)
+    if len(p.shape) != 3:
+        raise ValueError(f"{name}: packed weight {tuple(p.shape)}, expected a bank [E, N, K]")
+    if like.dtype != torch.bfloat16 or p.dtype != torch.bfloat16:
+        raise NotImplementedError(f"{name}: banks in 4 bits take bf16 layers, not {like.dtype} "
+                                  f"hidden states on {p.dtype} weights")
+    if p.device != like.device:
+        raise ValueError(f"{name}: tensors on {like.device} and {p.device}, expected one device")
+    return _contig(p.q), _contig(p.scale)
+
+
+@on_tensor_device
+def gemm_gate_up_swiglu4(x: torch.Tensor, plan: RoutingPlan, gate_up_proj: Packed4) -> torch.Tensor:
+    """act [S,I] = bf16(silu(gate) * up) of gemm_gate_up_swiglu on a bank in 4
+    bits; gate and up stay fp32."""
+    name = "gemm_gate_up_swiglu4"
+    _need_cuda(x)
+    q, scale = _packed_operand(name, gate_up_proj, x)
+    E, I2, H = gate_up_proj.shape
+    if tuple(x.shape) != (plan.num_tokens, H) or I2 % 2 or E != plan.num_experts:
+        raise ValueError(f"{name}: hidden {tuple(x.shape)}, gate_up_proj "
+                         f"{tuple(gate_up_proj.shape)}, a plan of {plan.num_tokens} tokens and "
+                         f"{plan.num_experts} experts")
+    x = _contig(x)
+    act = torch.empty(plan.num_rows, I2 // 2, device=x.device, dtype=x.dtype)
+    _call("moe_amd_gemm_gate_up_swiglu4", x.data_ptr(), plan.row_src.data_ptr(), plan.top_k,
+          plan.offsets.data_ptr(), plan.tile_plan.data_ptr(), q.data_ptr(), scale.data_ptr(),
+          plan.num_tokens, plan.num_rows, E, H, I2 // 2, act.data_ptr(), _stream(x))
+    return act
+
+
+@on_tensor_device
+def gemm_down4(act: torch.Tensor, plan: RoutingPlan, down_proj: Packed4
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """y [S,H] of gemm_down on a bank in 4 bits, in 16-bit blocks: (int16 [S,H],
+    uint8 [S,H/64]), y = int16 * 2^(byte - 127), for combine16."""
+    name = "gemm_down4"
+    _need_cuda(act)
+    q, scale = _packed_operand(name, down_proj, act)
+    E, H, I = down_proj.shape
+    if tuple(act.shape) != (plan.num_rows, I) or E != plan.num_experts:
+        raise ValueError(f"{name}: act {tuple(act.shape)}, down_proj {tuple(down_proj.shape)}, a "
+                         f"plan of {plan.num_rows} rows and {plan.num_experts} experts")
+    act = _contig(act)
+    y = torch.empty(plan.num_rows, H, device=act.device, dtype=torch.int16)
+    ys = torch.empty(plan.num_rows, H // 64, device=act.device, dtype=torch.uint8)
+    _call("moe_amd_gemm_down4", act.data_ptr(), plan.offsets.data_ptr(), plan.tile_plan.data_ptr(),
+          q.data_ptr(), scale.data_ptr(), plan.num_rows, E, H, I, y.data_ptr(), ys.data_ptr(),
+          _stream(act))
+    return y, ys
+
+
+@on_tensor_device
+def combine16(y: torch.Tensor, y_scale: torch.Tensor, plan: RoutingPlan,
+              topk_weights: torch.Tensor) -> torch.Tensor:
+    """out [T,H] bf16 = sum_k w[t,k] y[row of (t,k)] of gemm_down4's y."""
+    _need_cuda(y, y_scale, topk_weights)
+    T, K, H = plan.num_tokens, plan.top_k, y.shape[1]
+    if y.dtype != torch.int16 or y_scale.dtype != torch.uint8 or H % 64 \
+            or tuple(y.shape) != (plan.num_rows, H) \
+            or tuple(y_scale.shape) != (plan.num_rows, H // 64) \
+            or tuple(topk_weights.shape) != (T, K):
+        raise ValueError(f"combine16: y {y.dtype} {tuple(y.shape)}, scale {y_scale.dtype} "
+                         f"{tuple(y_scale.shape)}, weights {tuple(topk_weights.shape)}, a plan of "
+                         f"{T} tokens and {plan.num_rows} rows")
+    y, y_scale, topk_weights = _contig(y), _contig(y_scale), _contig(topk_weights)
+    out = torch.empty(T, H, device=y.device, dtype=torch.bfloat16)
+    _call("moe_amd_combine16", y.data_ptr(), y_scale.data_ptr(), plan.slot.data_ptr(),
+          plan.offsets.data_ptr(), topk_weights.data_ptr(), _dtype_code(topk_weights.dtype), T, K,
+          plan.num_experts, H, out.data_ptr(), _stream(y))
+    return out
+
+
 # -------------------------------------------------- the layer for few tokens
 
 FEW_MAX_TOKENS = 64
@@ -867,6 +1031,32 @@ def _few_inputs(name: str, x, gate_up_proj, down_proj, K: int, *others):
     return E, H, I2 // 2
 
 
+def _few_router(name: str, router: str, logit_offset, expert_bias):
+    """The router's offset or bias."""
+    if router not in _ROUTERS:
+        raise ValueError(f"unknown router {router!r}")
+    if (logit_offset is not None and router != "softmax") or \
+            (expert_bias is not None and router != "sigmoid"):
+        raise ValueError(f"{name}: logit_offset is the softmax router's, expert_bias the "
+                         "sigmoid router's")
+    return logit_offset if router == "softmax" else expert_bias
+
+
+def _few_router_inputs(name: str, x, w_router, extra, E: int, H: int):
+    """(x, w_router, offset or bias) as the C entries take them."""
+    if tuple(w_router.shape) != (E, H) or w_router.dtype != x.dtype:
+        raise ValueError(f"{name}: router weight {tuple(w_router.shape)} {w_router.dtype}, "
+                         f"expected {(E, H)} {x.dtype}")
+    if extra is not None:
+        if tuple(extra.shape) != (E,):
+            raise ValueError(f"{name}: offset or bias {tuple(extra.shape)}, expected {(E,)}")
+        extra = _contig(extra.to(torch.float32))
+    x, w_router = _contig(x), _contig(w_router)
+    if w_router.data_ptr() % 16:  # moe_layer's gating product takes any alignment
+        w_router = w_router.clone()
+    return x, w_router, extra
+
+
 @functools.lru_cache(maxsize=256)
 def _few_workspace_size(*shape: int) -> int:
     return max(int(_lib.load().moe_amd_few_workspace_size(*shape)), 16)
@@ -875,6 +1065,30 @@ def _few_workspace_size(*shape: int) -> int:
 def _few_workspace(x, E, K, H, I) -> torch.Tensor:
     n = _few_workspace_size(x.shape[0], E, K, H, I, _dtype_code(x.dtype))
     return torch.empty(n, device=x.device, dtype=torch.uint8)
+
+
+def _packed_bank(name: str, x, gate_up_proj: Packed4, down_proj: Packed4, K: int, *others):
+    """((gate_up's q and scale, down's), E, H, I) of a few-token call on a bank in
+    4 bits, checked as _few_inputs does."""
+    if not (isinstance(gate_up_proj, Packed4) and isinstance(down_proj, Packed4)):
+        raise TypeError(f"{name}: one of gate_up_proj and down_proj is in 4 bits, the other is not")
+    operands = (*_packed_operand(name, gate_up_proj, x), *_packed_operand(name, down_proj, x))
+    for t in others:
+        if t is not None and t.get_device() != x.get_device():
+            raise ValueError(f"{name}: tensors on {x.device} and {t.device}, expected one device")
+    E, I2, H = gate_up_proj.shape
+    if x.dim() != 2 or tuple(down_proj.shape) != (E, H, I2 // 2) or I2 % 2 or x.shape[1] != H:
+        raise ValueError(f"{name}: shape mismatch: hidden {tuple(x.shape)}, gate_up_proj "
+                         f"{tuple(gate_up_proj.shape)}, down_proj {tuple(down_proj.shape)}")
+    if x.shape[0] > FEW_MAX_TOKENS or K > FEW_MAX_TOP_K:
+        raise RuntimeError(f"{name}: {x.shape[0]} tokens with top-{K}; it takes at most "
+                           f"{FEW_MAX_TOKENS} and {FEW_MAX_TOP_K}")
+    return operands, E, H, I2 // 2
+
+
+@functools.lru_cache(maxsize=256)
+def _few4_workspace_size(*shape: int) -> int:
+    return max(int(_lib.load().moe_amd_few4_workspace_size(*shape)), 16)
 
 
 @on_tensor_device
@@ -913,26 +1127,11 @@ def moe_layer_few(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.T
     (out [T,H], weights fp32 [T,K], index int64 [T,K]), or out alone without
     return_routing.  May be captured in a HIP graph."""
     name = "moe_layer_few"
-    if router not in _ROUTERS:
-        raise ValueError(f"unknown router {router!r}")
-    if (logit_offset is not None and router != "softmax") or \
-            (expert_bias is not None and router != "sigmoid"):
-        raise ValueError(f"{name}: logit_offset is the softmax router's, expert_bias the "
-                         "sigmoid router's")
-    extra = logit_offset if router == "softmax" else expert_bias
+    extra = _few_router(name, router, logit_offset, expert_bias)
     _need_cuda(x, w_router, gate_up_proj, down_proj, extra)
     K = int(top_k)
     E, H, I = _few_inputs(name, x, gate_up_proj, down_proj, K, w_router, extra)
-    if tuple(w_router.shape) != (E, H) or w_router.dtype != x.dtype:
-        raise ValueError(f"{name}: router weight {tuple(w_router.shape)} {w_router.dtype}, "
-                         f"expected {(E, H)} {x.dtype}")
-    if extra is not None:
-        if tuple(extra.shape) != (E,):
-            raise ValueError(f"{name}: offset or bias {tuple(extra.shape)}, expected {(E,)}")
-        extra = _contig(extra.to(torch.float32))
-    x, w_router = _contig(x), _contig(w_router)
-    if w_router.data_ptr() % 16:  # moe_layer's gating product takes any alignment
-        w_router = w_router.clone()
+    x, w_router, extra = _few_router_inputs(name, x, w_router, extra, E, H)
     gate_up_proj, down_proj = _contig(gate_up_proj), _contig(down_proj)
     T = x.shape[0]
     grouped = num_groups is not None and group_topk is not None
@@ -947,4 +1146,57 @@ def moe_layer_few(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.T
           _ptr(extra), int(renormalize), float(scaling_factor or 0.0),
           int(num_groups) if grouped else 0, int(group_topk) if grouped else 0, ws.data_ptr(),
           ws.numel(), _ptr(w), _ptr(idx), out.data_ptr(), _stream(x), capturable=True)
+    return (out, w, idx) if return_routing else out
+
+
+@on_tensor_device
+def experts_few4(x: torch.Tensor, topk_index: torch.Tensor, topk_weights: torch.Tensor,
+                 gate_up_proj: Packed4, down_proj: Packed4) -> torch.Tensor:
+    """experts_few on a bank in 4 bits (bf16 hidden states)."""
+    name = "experts_few4"
+    _need_cuda(x, topk_index, topk_weights)
+    if topk_index.dim() != 2 or topk_index.shape != topk_weights.shape \
+            or topk_index.shape[0] != x.shape[0]:
+        raise ValueError(f"{name}: topk_index / topk_weights must both be [T, K]")
+    T, K = topk_index.shape
+    bank, E, H, I = _packed_bank(name, x, gate_up_proj, down_proj, K, topk_index, topk_weights)
+    x = _contig(x)
+    if topk_index.dtype != torch.int64:
+        topk_index = topk_index.to(torch.int64)
+    topk_index, topk_weights = _contig(topk_index), _contig(topk_weights)
+    ws = torch.empty(_few4_workspace_size(T, E, K, H, I), device=x.device, dtype=torch.uint8)
+    out = torch.empty(T, H, device=x.device, dtype=x.dtype)
+    _call("moe_amd_experts_few4", x.data_ptr(), topk_index.data_ptr(), topk_weights.data_ptr(),
+          _dtype_code(topk_weights.dtype), *(t.data_ptr() for t in bank), T, K, E, H, I,
+          ws.data_ptr(), ws.numel(), out.data_ptr(), _stream(x), capturable=True)
+    return out
+
+
+@on_tensor_device
+def moe_layer_few4(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: Packed4,
+                   down_proj: Packed4, top_k: int, router: str = "softmax",
+                   renormalize: bool = True, logit_offset: torch.Tensor | None = None,
+                   expert_bias: torch.Tensor | None = None, scaling_factor: float | None = None,
+                   num_groups: int | None = None, group_topk: int | None = None,
+                   return_routing: bool = True):
+    """moe_layer_few on a bank in 4 bits (bf16 hidden states and router weight)."""
+    name = "moe_layer_few4"
+    extra = _few_router(name, router, logit_offset, expert_bias)
+    _need_cuda(x, w_router, extra)
+    K = int(top_k)
+    bank, E, H, I = _packed_bank(name, x, gate_up_proj, down_proj, K, w_router, extra)
+    x, w_router, extra = _few_router_inputs(name, x, w_router, extra, E, H)
+    T = x.shape[0]
+    grouped = num_groups is not None and group_topk is not None
+    ws = torch.empty(_few4_workspace_size(T, E, K, H, I), device=x.device, dtype=torch.uint8)
+    out = torch.empty(T, H, device=x.device, dtype=x.dtype)
+    w = idx = None
+    if return_routing:
+        w = torch.empty(T, K, device=x.device, dtype=torch.float32)
+        idx = torch.empty(T, K, device=x.device, dtype=torch.int64)
+    _call("moe_amd_moe_layer_few4", x.data_ptr(), w_router.data_ptr(),
+          *(t.data_ptr() for t in bank), T, K, E, H, I, _ROUTERS[router], _ptr(extra),
+          int(renormalize), float(scaling_factor or 0.0), int(num_groups) if grouped else 0,
+          int(group_topk) if grouped else 0, ws.data_ptr(), ws.numel(), _ptr(w), _ptr(idx),
+          out.data_ptr(), _stream(x), capturable=True)
     return (out, w, idx) if return_routing else out

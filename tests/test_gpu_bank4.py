@@ -1,0 +1,376 @@
+"""The expert layer on banks in 4 bits against the formulas in 64 bits.
+
+Tolerances.  The weights that a bank holds are exact bf16 values, so only the
+layer rounds.  Let u = 2^-8, half a step of bf16 relative to a value, and v =
+2^-24.  A sum of n fp32 products is off by at most n v sum|a b|, so gate and up are
+off by dg = H v |W1| |x|; with |silu'| < 1.1 and |silu(g)| <= |g|, act before its
+rounding by da = 1.1 dg |up| + |gate| du + dg du + 16 v |act| (the last term: the
+hardware's exp2 and reciprocal, 1 ulp each, exp2's argument rounded once, which
+its size |g| log2 e multiplies, where sigmoid's own slope is below 1/|g|; and the
+products), and by u (|act| + da) more after it.  y is off by dy = |W2| da' + I v
+|W2| (|act| + da'); grouped products hold it in 16-bit blocks of 64 columns, off by
+2^-15 (max|y| + dy) of the block at most.  out is off by the weighted sum of that,
+(K + 1) v |w y| more and its own rounding.  The bounds below are these sums,
+evaluated in 64 bits.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from moe_amd import experts_forward, few, hf, library, ops  # noqa: F401
+from moe_amd.layer import SparseMoeBlock, moe_layer
+from pack4_oracle import tiles
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+U, V = 2.0 ** -8, 2.0 ** -24
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _bank(g, E, H, I):
+    w1 = torch.randn(E, 2 * I, H, generator=g, device=DEV) * 0.02
+    w2 = torch.randn(E, H, I, generator=g, device=DEV) * 0.02
+    return ops.pack4(w1, dtype=BF), ops.pack4(w2, dtype=BF)
+
+
+def _routing(g, T, E, K, skew=0.0):
+    logits = torch.rand(T, E, generator=g, device=DEV)
+    logits += skew * torch.linspace(1, 0, E, device=DEV) ** 4
+    idx = logits.argsort(1, descending=True)[:, :K].contiguous()
+    return idx, torch.rand(T, K, generator=g, device=DEV) + 0.1
+
+
+def _oracle(x, idx, w, b1, b2, blocks=False):
+    """(out, bound) in 64 bits, expert by expert; blocks: y in 16-bit blocks."""
+    T, H = x.shape
+    E, I, K = b1.shape[0], b2.shape[2], idx.shape[1]
+    out = torch.zeros(T, H, device=DEV, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    for e in torch.unique(idx).tolist():
+        if not 0 <= e < E:
+            continue
+        t, k = torch.nonzero(idx == e, as_tuple=True)
+        m1 = tiles(b1.q[e], b1.scale[e], b1.shape[1:]).to(DEV)
+        m2 = tiles(b2.q[e], b2.scale[e], b2.shape[1:]).to(DEV)
+        xt, wk = x[t].double(), w[t, k].double()[:, None]
+        gu, dgu = xt @ m1.t(), H * V * (xt.abs() @ m1.abs().t())
+        gt, up, dg, du = gu[:, :I], gu[:, I:], dgu[:, :I], dgu[:, I:]
+        act = gt * torch.sigmoid(gt) * up
+        da = 1.1 * dg * up.abs() + gt.abs() * du + dg * du + 16 * V * act.abs()
+        da = da + U * (act.abs() + da)
+        y = act @ m2.t()
+        dy = da @ m2.abs().t() + I * V * ((act.abs() + da) @ m2.abs().t())
+        if blocks:
+            most = (y.abs() + dy).unflatten(1, (-1, 64)).amax(-1, keepdim=True)
+            dy = dy + (most * 2.0 ** -15).expand(-1, -1, 64).flatten(1)
+        out.index_add_(0, t, y * wk)
+        tol.index_add_(0, t, wk.abs() * (dy + (K + 1) * V * y.abs()))
+    return out, tol + U * (out.abs() + tol)
+
+
+def _close(got, ref, tol):
+    assert torch.isfinite(got).all()
+    bad = (got.double() - ref).abs() > tol
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} values off, worst by " \
+        f"{float(((got.double() - ref).abs() / tol.clamp(min=1e-300)).max()):.2f} bounds"
+
+
+def _x(g, T, H):
+    return torch.randn(T, H, generator=g, device=DEV, dtype=BF)
+
+
+FEW = [  # T, H, E, K, I
+    (1, 64, 4, 2, 64), (1, 2048, 128, 8, 768), (2, 192, 16, 4, 192), (3, 128, 1, 1, 64),
+    (5, 320, 7, 3, 448), (13, 1024, 128, 4, 768), (17, 64, 300, 16, 128), (37, 704, 40, 8, 576),
+    (64, 256, 8, 8, 64), (64, 1088, 512, 6, 320), (64, 2048, 128, 8, 768), (33, 128, 3, 2, 832),
+]
+
+
+@pytest.mark.parametrize("T,H,E,K,I", FEW)
+def test_experts_few(T, H, E, K, I):
+    g = _gen(T + H)
+    b1, b2 = _bank(g, E, H, I)
+    x, (idx, w) = _x(g, T, H), _routing(g, T, E, K)
+    out = few.experts_forward_few(x, idx, w, b1, b2)
+    _close(out, *_oracle(x, idx, w, b1, b2))
+    assert torch.equal(out, few.experts_forward_few(x, idx, w, b1, b2))
+
+
+@pytest.mark.parametrize("T,K", [(1, 4), (16, 4), (40, 8)])
+def test_experts_few_padding_and_repeats(T, K):
+    """Ids outside [0, E), tokens without any expert, one expert named twice and by
+    everybody, bf16 weights."""
+    g = _gen(7)
+    E, H, I = 6, 192, 128
+    b1, b2 = _bank(g, E, H, I)
+    x = _x(g, T, H)
+    idx = torch.randint(-1, E + 2, (T, K), generator=g, device=DEV)
+    idx[-1] = E
+    idx[0, :2] = 3
+    w = (torch.rand(T, K, generator=g, device=DEV) - 0.5).to(BF)
+    _close(few.experts_forward_few(x, idx, w, b1, b2), *_oracle(x, idx, w, b1, b2))
+    _close(experts_forward(x, idx, w, b1, b2), *_oracle(x, idx, w, b1, b2, blocks=True))
+    none = torch.full_like(idx, E)
+    assert (few.experts_forward_few(x, none, w, b1, b2) == 0).all()
+    assert (experts_forward(x, none, w, b1, b2) == 0).all()
+    same = torch.full_like(idx, 5)
+    _close(few.experts_forward_few(x, same, w, b1, b2), *_oracle(x, same, w, b1, b2))
+
+
+@pytest.mark.parametrize("router", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("T,H,E,K,I", [(1, 256, 128, 8, 128), (2, 128, 64, 4, 192),
+                                       (9, 192, 300, 6, 64), (64, 512, 32, 8, 320)])
+def test_moe_layer_few(router, T, H, E, K, I):
+    """The routing is that of the layer on an exact bank, bit for bit."""
+    g = _gen(E)
+    b1, b2 = _bank(g, E, H, I)
+    x, wr = _x(g, T, H), torch.randn(E, H, generator=g, device=DEV, dtype=BF) * 0.05
+    bias = torch.rand(E, generator=g, device=DEV) * 0.1 if router == "sigmoid" else None
+    kw = dict(router=router, expert_bias=bias, return_routing=True)
+    out, w, idx = few.moe_layer_few(x, wr, b1, b2, K, **kw)
+    _, w0, idx0 = few.moe_layer_few(x, wr, ops.unpack4(b1), ops.unpack4(b2), K, **kw)
+    assert torch.equal(idx, idx0) and torch.equal(w, w0)
+    _close(out, *_oracle(x, idx, w, b1, b2))
+    kw["return_routing"] = False
+    assert torch.equal(out, few.moe_layer_few(x, wr, b1, b2, K, **kw))
+
+
+PROMPT = [  # T, H, E, K, I, skew
+    (1, 64, 4, 2, 64, 0.0), (3, 192, 128, 8, 192, 0.0), (65, 320, 16, 4, 448, 0.0),
+    (200, 64, 3, 1, 832, 0.0), (509, 1024, 128, 4, 768, 0.0), (300, 128, 2, 2, 128, 0.0),
+    (1021, 256, 16, 8, 320, 2.0), (777, 704, 8, 3, 576, 0.0), (1500, 192, 4, 4, 128, 0.0),
+    (4096, 512, 24, 8, 256, 3.0), (2050, 2048, 128, 8, 768, 1.0), (127, 64, 1, 1, 64, 0.0),
+    (64, 64, 1, 1, 64, 0.0),
+]
+
+
+@pytest.mark.parametrize("T,H,E,K,I,skew", PROMPT)
+def test_experts_forward(T, H, E, K, I, skew):
+    g = _gen(T + I)
+    b1, b2 = _bank(g, E, H, I)
+    x, (idx, w) = _x(g, T, H), _routing(g, T, E, K, skew)
+    out = experts_forward(x, idx, w, b1, b2)
+    _close(out, *_oracle(x, idx, w, b1, b2, blocks=True))
+    assert torch.equal(out, experts_forward(x, idx, w, b1, b2))
+
+
+@pytest.mark.parametrize("rows", [1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300])
+def test_rows_of_an_expert(rows):
+    """Row counts around the tiles' heights; one expert without a row, one with all."""
+    g = _gen(rows)
+    E, H, I = 3, 192, 192
+    b1, b2 = _bank(g, E, H, I)
+    for e in (0, 2):
+        x, idx = _x(g, rows, H), torch.full((rows, 1), e, device=DEV)
+        w = torch.ones(rows, 1, device=DEV)
+        _close(experts_forward(x, idx, w, b1, b2), *_oracle(x, idx, w, b1, b2, blocks=True))
+
+
+def test_row_heights_give_the_same_bits():
+    """A row's results do not depend on how many others there are."""
+    g = _gen(5)
+    E, H, I = 2, 256, 192
+    b1, b2 = _bank(g, E, H, I)
+    x = _x(g, 1500, H)
+    idx = torch.arange(1500, device=DEV)[:, None] % 2
+    w = torch.rand(1500, 1, generator=g, device=DEV)
+    all_ = experts_forward(x, idx, w, b1, b2)
+    for n in (10, 140, 300):
+        assert torch.equal(all_[:n], experts_forward(x[:n], idx[:n], w[:n], b1, b2)), n
+
+
+def test_not_finite_values_stay_in_their_rows():
+    g = _gen(6)
+    E, H, I = 4, 128, 128
+    b1, b2 = _bank(g, E, H, I)
+    x, (idx, w) = _x(g, 200, H), _routing(g, 200, E, 2)
+    ref = experts_forward(x, idx, w, b1, b2)
+    bad = x.clone()
+    bad[17, 5], bad[60, 9] = torch.nan, torch.inf
+    got = experts_forward(bad, idx, w, b1, b2)
+    rows = torch.ones(200, dtype=torch.bool, device=DEV)
+    rows[[17, 60]] = False
+    assert torch.equal(got[rows], ref[rows]) and torch.isnan(got[17]).all()
+    assert not torch.isfinite(got[60]).any()
+    few_ref = few.experts_forward_few(x[:40], idx[:40], w[:40], b1, b2)
+    few_got = few.experts_forward_few(bad[:40], idx[:40], w[:40], b1, b2)
+    assert torch.equal(few_got[rows[:40]], few_ref[rows[:40]]) and torch.isnan(few_got[17]).all()
+    # a weight that is not finite: the tokens of its expert alone
+    w1 = ops.unpack4(b1)
+    w1[2, 3, 40] = torch.inf
+    bank = ops.pack4(w1)
+    hit = (idx == 2).any(1)
+    got = experts_forward(x, idx, w, bank, b2)
+    assert torch.isnan(got[hit]).all() and torch.equal(got[~hit], ref[~hit])
+    got = few.experts_forward_few(x[:40], idx[:40], w[:40], bank, b2)
+    assert torch.isnan(got[hit[:40]]).all() and torch.equal(got[~hit[:40]], few_ref[~hit[:40]])
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** 40])
+def test_magnitudes_of_y(scale):
+    """The 16-bit blocks have y's range: weights of down_proj far from 1."""
+    g = _gen(8)
+    E, H, I, T = 2, 128, 64, 150
+    b1, _ = _bank(g, E, H, I)
+    b2 = ops.pack4(torch.randn(E, H, I, generator=g, device=DEV) * scale, dtype=BF)
+    x, (idx, w) = _x(g, T, H), _routing(g, T, E, 1)
+    _close(experts_forward(x, idx, w, b1, b2), *_oracle(x, idx, w, b1, b2, blocks=True))
+
+
+def test_inputs_of_any_stride_and_type():
+    g = _gen(9)
+    E, H, I, T, K = 5, 128, 64, 70, 3
+    b1, b2 = _bank(g, E, H, I)
+    wide = _x(g, T, 2 * H)
+    x, (idx, w) = wide[:, ::2], _routing(g, T, E, K)
+    for fn, n in ((experts_forward, T), (few.experts_forward_few, 40)):
+        ref = fn(x[:n].contiguous(), idx[:n], w[:n], b1, b2)
+        assert torch.equal(ref, fn(x[:n], idx[:n].int(), w.t().contiguous().t()[:n], b1, b2))
+        f32 = fn(x[:n].float(), idx[:n], w[:n], b1, b2)
+        assert f32.dtype == F32 and torch.equal(f32, ref.float())
+        moved = ops.Packed4(b1.q.transpose(1, 2).contiguous().transpose(1, 2), b1.scale, b1.shape, BF)
+        assert torch.equal(ref, fn(x[:n], idx[:n], w[:n], moved, b2))
+    assert experts_forward(x[:0], idx[:0], w[:0], b1, b2).shape == (0, H)
+    assert few.experts_forward_few(x[:0], idx[:0], w[:0], b1, b2).shape == (0, H)
+
+
+@pytest.mark.parametrize("router", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("gating", ["torch", "hip", "hip_fused"])
+def test_moe_layer(router, gating):
+    g = _gen(10)
+    T, H, E, K, I = 150, 256, 128, 8, 64
+    b1, b2 = _bank(g, E, H, I)
+    x, wr = _x(g, T, H), torch.randn(E, H, generator=g, device=DEV, dtype=BF) * 0.05
+    with torch.no_grad():
+        out, probs, w, idx = moe_layer(x, wr, b1, b2, K, router=router, gating=gating)
+        _, probs0, w0, idx0 = moe_layer(x, wr, ops.unpack4(b1), ops.unpack4(b2), K, router=router,
+                                        gating=gating)
+    assert torch.equal(idx, idx0) and torch.equal(w, w0) and torch.equal(probs, probs0)
+    _close(out, *_oracle(x, idx, w, b1, b2, blocks=True))
+
+
+def test_block_serves_prompt_and_tokens():
+    """A block put in 4 bits: a prompt, then single tokens, as it is served; its
+    state goes through state_dict."""
+    H, E, K, I = 256, 32, 4, 128
+    block = SparseMoeBlock(H, E, K, I).to(DEV, BF)
+    g = _gen(11)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.copy_(torch.randn(p.shape, generator=g, device=DEV) * 0.02)
+    exact1, exact2 = block.experts.gate_up_proj.detach(), block.experts.down_proj.detach()
+    b1, b2 = ops.pack4(exact1), ops.pack4(exact2)
+    assert block.pack_experts() is block
+    block.few_tokens = 64
+    assert [n for n, _ in block.experts.named_parameters()] == []
+    x = _x(g, 3 * 50, H).view(3, 50, H)
+    with torch.no_grad():
+        out = block(x)
+        w, idx = block.router_logits.gather(1, block.topk_index), block.topk_index
+        w = w / w.sum(-1, keepdim=True)
+        _close(out.view(-1, H), *_oracle(x.view(-1, H), idx, w, b1, b2, blocks=True))
+        for t in range(3):
+            y = _x(g, 3, H).view(3, 1, H)
+            got = block(y)
+            assert block.router_logits is None and got.shape == y.shape
+            ref, w, idx = few.moe_layer_few(y.view(-1, H), block.gate.weight, b1, b2, K,
+                                            return_routing=True)
+            assert torch.equal(got.view(-1, H), ref)
+            _close(ref, *_oracle(y.view(-1, H), idx, w, b1, b2))
+        other = SparseMoeBlock(H, E, K, I).to(DEV, BF).pack_experts()
+        other.load_state_dict(block.state_dict())
+        assert torch.equal(other(x), out)
+    with pytest.raises(RuntimeError, match="forward only"):
+        block(x)
+
+
+def test_transformers_bank():
+    from transformers import Qwen3MoeConfig
+    from transformers.models.qwen3_moe.modeling_qwen3_moe import Qwen3MoeForCausalLM
+    cfg = Qwen3MoeConfig(vocab_size=64, hidden_size=128, intermediate_size=128,
+                         moe_intermediate_size=64, num_hidden_layers=2, num_attention_heads=2,
+                         num_key_value_heads=1, head_dim=64, num_experts=16, num_experts_per_tok=4,
+                         norm_topk_prob=True, max_position_embeddings=64)
+    torch.manual_seed(0)
+    model = Qwen3MoeForCausalLM(cfg).to(DEV, BF).eval()
+    twin = Qwen3MoeForCausalLM(cfg).to(DEV, BF).eval()
+    twin.load_state_dict(model.state_dict())
+    with torch.no_grad():   # the twin holds what the packed banks hold
+        for bank in hf.expert_banks(twin):
+            for p in (bank.gate_up_proj, bank.down_proj):
+                p.copy_(ops.unpack4(ops.pack4(p)))
+    hf.install(twin)
+    assert hf.pack_experts(model) == 2 and hf.pack_experts(model) == 0
+    hf.install(model, few_tokens=64)
+    assert all(bank.few_tokens == 64 for bank in hf.expert_banks(model))
+    for shape in ((2, 40), (2, 3)):
+        ids = torch.randint(0, 64, shape, device=DEV)
+        with torch.no_grad():
+            a, b = model(ids).logits.float(), twin(ids).logits.float()
+        # the twin rounds gate, up, silu and y to bf16 besides act; a layer's output is
+        # within 4 roundings of 2^-8 of its sums' magnitudes, two layers and a head follow
+        assert float((a - b).norm() / b.norm()) < 2 * 4 * U
+    with pytest.raises(RuntimeError, match="forward only"):
+        model(ids.repeat(1, 30))
+
+
+def test_graphs_streams_and_workspaces():
+    """Two captured graphs, each with its workspace, replayed by turns and beside
+    eager calls; another stream."""
+    g = _gen(12)
+    H, E, K, I = 256, 16, 4, 128
+    b1, b2 = _bank(g, E, H, I)
+    wr = torch.randn(E, H, generator=g, device=DEV, dtype=BF) * 0.05
+    xs = [_x(g, 3, H), _x(g, 20, H)]
+
+    def call(x):
+        return few.moe_layer_few(x, wr, b1, b2, K)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    with torch.cuda.stream(s):
+        for x in xs:
+            call(x)
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=s):
+                outs.append(call(x))
+    torch.cuda.synchronize()
+    for k in range(4):
+        for x in xs:
+            x.copy_(torch.randn(x.shape, generator=g, device=DEV))
+        for i in (0, 1) if k % 2 else (1, 0):
+            graphs[i].replay()
+        eager = [call(x) for x in xs]
+        torch.cuda.synchronize()
+        for o, e in zip(outs, eager):
+            assert torch.equal(o, e), k
+    with torch.cuda.stream(s):
+        side = experts_forward(xs[1], *_routing(_gen(1), 20, E, K), b1, b2)
+    torch.cuda.synchronize()
+    assert torch.equal(side, experts_forward(xs[1], *_routing(_gen(1), 20, E, K), b1, b2))
+
+
+def test_custom_ops():
+    g = _gen(13)
+    T, H, E, K, I = 12, 128, 8, 2, 64
+    b1, b2 = _bank(g, E, H, I)
+    x, (idx, w) = _x(g, T, H), _routing(g, T, E, K)
+    bank = (b1.q, b1.scale, b2.q, b2.scale)
+    wr = torch.randn(E, H, generator=g, device=DEV, dtype=BF)
+    torch.library.opcheck(torch.ops.moe_amd.experts_fwd4.default, (x, idx, w, *bank))
+    torch.library.opcheck(torch.ops.moe_amd.experts_few4.default, (x, idx, w, *bank))
+    torch.library.opcheck(torch.ops.moe_amd.moe_layer_few4.default,
+                          (x, wr, *bank, K, "softmax", True, None, None, None, None, None))
+    ref = experts_forward(x, idx, w, b1, b2), few.experts_forward_few(x, idx, w, b1, b2)
+
+    def both(x, idx, w):
+        return experts_forward(x, idx, w, b1, b2), few.experts_forward_few(x, idx, w, b1, b2)
+
+    got = torch.compile(both, fullgraph=True)(x, idx, w)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))
