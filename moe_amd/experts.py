@@ -84,7 +84,7 @@ def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
 
 def _experts_forward4(hidden_states, top_k_index, top_k_weights, gate_up_proj, down_proj,
                       saved_activations):
-    bank = library.check_bank4("experts_forward", hidden_states, gate_up_proj, down_proj)
+    bank, *_ = ops.packed_bank("experts_forward", hidden_states, gate_up_proj, down_proj)
     if top_k_index.dim() != 2 or top_k_index.shape != top_k_weights.shape \
             or top_k_index.shape[0] != hidden_states.shape[0]:
         raise ValueError("top_k_index / top_k_weights must both be [T, K]")

@@ -77,6 +77,12 @@ def _unseen(*tensors) -> bool:
     return True
 
 
+def _tensors4(*weights):
+    """The tensors of weights of which one at least is in 4 bits (both, else the
+    call is refused)."""
+    return [t for w in weights for t in ((w.q, w.scale) if type(w) is ops.Packed4 else (w,))]
+
+
 def experts_forward_few(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
                         top_k_weights: torch.Tensor, gate_up_proj: torch.Tensor | ops.Packed4,
                         down_proj: torch.Tensor | ops.Packed4) -> torch.Tensor:
@@ -85,13 +91,14 @@ def experts_forward_few(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
     [0, E) contribute nothing."""
     _refuse_grad("experts_forward_few", hidden_states, top_k_weights, gate_up_proj, down_proj)
     if isinstance(gate_up_proj, ops.Packed4) or isinstance(down_proj, ops.Packed4):
-        bank = library.check_bank4("experts_forward_few", hidden_states, gate_up_proj, down_proj)
-        x = hidden_states.to(torch.bfloat16)
-        if _unseen(x, top_k_index, top_k_weights, *bank):
+        dtype = hidden_states.dtype
+        x = hidden_states if dtype == torch.bfloat16 else hidden_states.to(torch.bfloat16)
+        if _unseen(x, top_k_index, top_k_weights, *_tensors4(gate_up_proj, down_proj)):
             out = ops.experts_few4(x, top_k_index, top_k_weights, gate_up_proj, down_proj)
         else:
+            bank, *_ = ops.packed_bank("experts_forward_few", x, gate_up_proj, down_proj)
             out = torch.ops.moe_amd.experts_few4(x, top_k_index, top_k_weights, *bank)
-        return out.to(hidden_states.dtype)
+        return out if dtype == torch.bfloat16 else out.to(dtype)
     op = (ops.experts_few if _unseen(hidden_states, top_k_index, top_k_weights, gate_up_proj,
                                      down_proj) else torch.ops.moe_amd.experts_few)
     dtype = hidden_states.dtype
@@ -117,10 +124,10 @@ def moe_layer_few(x: torch.Tensor, w_router: torch.Tensor,
     rest = (int(top_k), router, bool(renormalize), logit_offset, expert_bias, scaling_factor,
             num_groups, group_topk)
     if isinstance(gate_up_proj, ops.Packed4) or isinstance(down_proj, ops.Packed4):
-        bank = library.check_bank4("moe_layer_few", x, gate_up_proj, down_proj)
-        if _unseen(x, w_router, logit_offset, expert_bias, *bank):
+        if _unseen(x, w_router, logit_offset, expert_bias, *_tensors4(gate_up_proj, down_proj)):
             return ops.moe_layer_few4(x, w_router, gate_up_proj, down_proj, *rest,
                                       return_routing=return_routing)
+        bank, *_ = ops.packed_bank("moe_layer_few", x, gate_up_proj, down_proj)
         res = torch.ops.moe_amd.moe_layer_few4(x, w_router, *bank, *rest)
         return res if return_routing else res[0]
     args = (x, w_router, gate_up_proj, down_proj, *rest)

@@ -51,7 +51,7 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tenso
         raise ValueError(f"unknown gating {gating!r} (expected one of {library.GATINGS})")
     library.check_keep(saved_activations, gate_up_proj.dtype)
     if isinstance(gate_up_proj, ops.Packed4):
-        library.check_bank4("moe_layer", x, gate_up_proj, down_proj)
+        ops.packed_bank("moe_layer", x, gate_up_proj, down_proj)
         refuse_grad4("moe_layer", x, w_router)
     hip = gating in ("hip", "hip_fused")
     if router == "softmax" and _fused_softmax_ok(x, w_router, gate_up_proj, down_proj):

@@ -843,25 +843,6 @@ def _(q, scale, n, k, dtype):
     return q.new_empty((*q.shape[:-3], n, k), dtype=dtype)
 
 
-def check_bank4(name: str, x: Tensor, gate_up_proj, down_proj) -> tuple[Tensor, ...]:
-    """(gate_up's q and scale, down's) of a call on a bank in 4 bits, its shapes
-    and types checked."""
-    if not (isinstance(gate_up_proj, ops.Packed4) and isinstance(down_proj, ops.Packed4)):
-        raise TypeError(f"{name}: gate_up_proj and down_proj must both be in 4 bits, or neither")
-    for p in (gate_up_proj, down_proj):
-        ops.check_packed4(name, p)
-        if p.dtype != torch.bfloat16:
-            raise NotImplementedError(f"{name}: banks in 4 bits take bf16 layers, not {p.dtype}")
-    s1, s2 = gate_up_proj.shape, down_proj.shape
-    if len(s1) != 3 or s1[1] % 2 or tuple(s2) != (s1[0], s1[2], s1[1] // 2) or x.dim() != 2 \
-            or x.shape[1] != s1[2]:
-        raise ValueError(f"{name}: shape mismatch: hidden {tuple(x.shape)}, gate_up_proj "
-                         f"{tuple(s1)}, down_proj {tuple(s2)}")
-    if s1[2] % 64 or s2[2] % 64:
-        raise ValueError(f"{name}: H={s1[2]} and I={s2[2]} must be multiples of 64")
-    return gate_up_proj.q, gate_up_proj.scale, down_proj.q, down_proj.scale
-
-
 def _bank4(x: Tensor, q1: Tensor, s1: Tensor, q2: Tensor, s2: Tensor):
     """(gate_up_proj, down_proj) of bf16 hidden states x [T,H]: I is a multiple of
     64, so that gate_up_proj's tiles have no padded rows."""

@@ -1067,23 +1067,56 @@ def _few_workspace(x, E, K, H, I) -> torch.Tensor:
     return torch.empty(n, device=x.device, dtype=torch.uint8)
 
 
-def _packed_bank(name: str, x, gate_up_proj: Packed4, down_proj: Packed4, K: int, *others):
-    """((gate_up's q and scale, down's), E, H, I) of a few-token call on a bank in
-    4 bits, checked as _few_inputs does."""
-    if not (isinstance(gate_up_proj, Packed4) and isinstance(down_proj, Packed4)):
-        raise TypeError(f"{name}: one of gate_up_proj and down_proj is in 4 bits, the other is not")
-    operands = (*_packed_operand(name, gate_up_proj, x), *_packed_operand(name, down_proj, x))
+@functools.lru_cache(maxsize=256)
+def _bank4_shapes(shape1: tuple[int, ...], shape2: tuple[int, ...]):
+    """The shapes of the four tensors of a bank [E, 2I, H], [E, H, I]; None if it
+    is none."""
+    if len(shape1) != 3 or shape1[1] % 2 or shape2 != (shape1[0], shape1[2], shape1[1] // 2):
+        return None
+    return (*_pack4_shapes(shape1), *_pack4_shapes(shape2))
+
+
+def packed_bank(name: str, x: torch.Tensor, gate_up_proj: Packed4, down_proj: Packed4):
+    """((gate_up's q and scale, down's), E, H, I) of a call of hidden states x [T, H]
+    on a bank in 4 bits, its shapes, types and device checked (a single token's
+    call takes the host about as long as the GPU)."""
+    if type(gate_up_proj) is not Packed4 or type(down_proj) is not Packed4:
+        raise TypeError(f"{name}: gate_up_proj and down_proj must both be in 4 bits, or neither")
+    shape1, shape2 = gate_up_proj.shape, down_proj.shape
+    bank = gate_up_proj.q, gate_up_proj.scale, down_proj.q, down_proj.scale
+    expect = _bank4_shapes(tuple(shape1), tuple(shape2))
+    if expect is None or x.dim() != 2 or x.shape[1] != shape1[2]:
+        raise ValueError(f"{name}: shape mismatch: hidden {tuple(x.shape)}, gate_up_proj "
+                         f"{tuple(shape1)}, down_proj {tuple(shape2)}")
+    dev = x.get_device()
+    for t, shape in zip(bank, expect):
+        if t.shape != shape or t.dtype != torch.uint8:
+            check_packed4(name, gate_up_proj)
+            check_packed4(name, down_proj)
+        if t.get_device() != dev:
+            raise ValueError(f"{name}: tensors on {x.device} and {t.device}, expected one device")
+    E, I2, H = shape1
+    if H % 64 or I2 % 128:
+        raise ValueError(f"{name}: H={H} and I={I2 // 2} must be multiples of 64")
+    if gate_up_proj.dtype != torch.bfloat16 or down_proj.dtype != torch.bfloat16:
+        raise NotImplementedError(f"{name}: banks in 4 bits take bf16 layers, not "
+                                  f"{gate_up_proj.dtype} and {down_proj.dtype}")
+    return bank, E, H, I2 // 2
+
+
+def _few4_inputs(name: str, x, gate_up_proj, down_proj, K: int, *others):
+    """packed_bank of a few-token call, contiguous, and the rest of its checks."""
+    bank, E, H, I = packed_bank(name, x, gate_up_proj, down_proj)
+    _need_cuda(x)
+    if x.dtype != torch.bfloat16:
+        raise NotImplementedError(f"{name}: banks in 4 bits take bf16 hidden states, not {x.dtype}")
     for t in others:
         if t is not None and t.get_device() != x.get_device():
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}, expected one device")
-    E, I2, H = gate_up_proj.shape
-    if x.dim() != 2 or tuple(down_proj.shape) != (E, H, I2 // 2) or I2 % 2 or x.shape[1] != H:
-        raise ValueError(f"{name}: shape mismatch: hidden {tuple(x.shape)}, gate_up_proj "
-                         f"{tuple(gate_up_proj.shape)}, down_proj {tuple(down_proj.shape)}")
     if x.shape[0] > FEW_MAX_TOKENS or K > FEW_MAX_TOP_K:
         raise RuntimeError(f"{name}: {x.shape[0]} tokens with top-{K}; it takes at most "
                            f"{FEW_MAX_TOKENS} and {FEW_MAX_TOP_K}")
-    return operands, E, H, I2 // 2
+    return [_contig(t) for t in bank], E, H, I
 
 
 @functools.lru_cache(maxsize=256)
@@ -1154,12 +1187,11 @@ def experts_few4(x: torch.Tensor, topk_index: torch.Tensor, topk_weights: torch.
                  gate_up_proj: Packed4, down_proj: Packed4) -> torch.Tensor:
     """experts_few on a bank in 4 bits (bf16 hidden states)."""
     name = "experts_few4"
-    _need_cuda(x, topk_index, topk_weights)
     if topk_index.dim() != 2 or topk_index.shape != topk_weights.shape \
             or topk_index.shape[0] != x.shape[0]:
         raise ValueError(f"{name}: topk_index / topk_weights must both be [T, K]")
     T, K = topk_index.shape
-    bank, E, H, I = _packed_bank(name, x, gate_up_proj, down_proj, K, topk_index, topk_weights)
+    bank, E, H, I = _few4_inputs(name, x, gate_up_proj, down_proj, K, topk_index, topk_weights)
     x = _contig(x)
     if topk_index.dtype != torch.int64:
         topk_index = topk_index.to(torch.int64)
@@ -1182,9 +1214,8 @@ def moe_layer_few4(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: Packed
     """moe_layer_few on a bank in 4 bits (bf16 hidden states and router weight)."""
     name = "moe_layer_few4"
     extra = _few_router(name, router, logit_offset, expert_bias)
-    _need_cuda(x, w_router, extra)
     K = int(top_k)
-    bank, E, H, I = _packed_bank(name, x, gate_up_proj, down_proj, K, w_router, extra)
+    bank, E, H, I = _few4_inputs(name, x, gate_up_proj, down_proj, K, w_router, extra)
     x, w_router, extra = _few_router_inputs(name, x, w_router, extra, E, H)
     T = x.shape[0]
     grouped = num_groups is not None and group_topk is not None

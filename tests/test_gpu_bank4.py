@@ -87,6 +87,7 @@ def _x(g, T, H):
 FEW = [  # T, H, E, K, I
     (1, 64, 4, 2, 64), (1, 2048, 128, 8, 768), (2, 192, 16, 4, 192), (3, 128, 1, 1, 64),
     (5, 320, 7, 3, 448), (13, 1024, 128, 4, 768), (17, 64, 300, 16, 128), (37, 704, 40, 8, 576),
+    (20, 4160, 6, 2, 1600), (1, 2112, 4, 2, 6208), (2, 64, 8, 8, 768), (1, 8256, 3, 3, 64),
     (64, 256, 8, 8, 64), (64, 1088, 512, 6, 320), (64, 2048, 128, 8, 768), (33, 128, 3, 2, 832),
 ]
 
