@@ -2,13 +2,13 @@
 // only, bf16 rows: the routed rows of each expert, as the permutation sorted
 // them, times its packed weights (pack4.h).
 //
-//   gemm4_kernel<BR, true>   act [S,I] = silu(x Wg^T) * (x Wu^T), x gathered by token
-//   gemm4_kernel<BR, false>  y [S,H] = act W2^T, in 16-bit blocks
-//   combine16_kernel         out [T,H] = sum_k w[t,k] y[row of (t,k)]
+//   gemm4_kernel<BR, true, NW>   act [S,I] = silu(x Wg^T) * (x Wu^T), x gathered by token
+//   gemm4_kernel<BR, false, NW>  y [S,H] = act W2^T, in 16-bit blocks
+//   combine16_kernel             out [T,H] = sum_k w[t,k] y[row of (t,k)]
 //
-// A workgroup owns BR rows by 256 weight rows (gate and up: 128 features of
-// each), a wave all its rows by 64 weight rows of its own.  So no weight is
-// wanted by two waves: each goes from memory to its lane's registers, 16 bytes of
+// A workgroup of NW waves owns BR rows by 64 NW weight rows (gate and up: 32 NW
+// features of each), a wave all its rows by 64 weight rows of its own.  So no weight
+// is wanted by two waves: each goes from memory to its lane's registers, 16 bytes of
 // codes a load and whole lines a wave, and becomes an MFMA operand there by four
 // conversions for eight values; converted or not, weights never pass
 // through LDS, which holds rows only.  MFMA v_mfma_f32_32x32x16_bf16: weights as
@@ -17,16 +17,28 @@
 // takes columns 32 h + 8 j of a stage's 64, of both operands alike.
 //
 // Rows come by LDS DMA, 64 columns a stage (128-byte lines, 16-byte chunks
-// XOR-swizzled by row: no bank conflicts), into a ring of four slots, three stages
-// in flight; weights D stage pairs ahead, in registers.  Loads past the end of the
-// contraction are issued all the same, from empty descriptors (zeros, no memory
-// access), so that the wait counts hold in every stage.
+// XOR-swizzled by row: no bank conflicts), into a ring of four slots; weights into
+// registers, four stages ahead too.  The stages of a workgroup's tiles are one
+// stream: a tile's last stages ask for the next tile's first ones, which arrive
+// under its epilogue.  Loads past the end of the contraction are issued all the same,
+// from empty descriptors (zeros, no memory access), so that the wait counts hold in
+// every stage.
 //
 // act is rounded to bf16 once.  y is held in 16 bits a value with a power of two for
 // 64 columns of a row: as small as bf16, but within 2^-15 of the block's largest
 // value instead of 2^-9 of each (three roundings of bf16 size in a row would
 // show: 1.7 times the error of one); a block with a value that is not finite is
 // NaN whole.  Each output is rounded once.
+//
+// Measured (gate/up, down, combine; H 2048, I 768, top 8 of 128 experts):
+//   16384 tokens  648 us (1.27 PF), 374 us (1.10 PF), 116 us (5.2 TB/s); a plain bf16
+//                 product reaches 1.4 to 1.6 PF on this card: bound by the matrix
+//                 units, the rest is the short contraction's epilogues and
+//                 the conversions' issue slots
+//    1021 tokens  63 us, 41 us, 9 us: 320 MB of weights, an expert's 64 rows mean
+//                 both bounds are near (3.4 TB/s, 0.8 PF)
+// and 2048 tokens on 1792 experts (9 rows each): 514 us, 314 us, 17 us, bound by the
+// 4.5 GB of weights (5.8 and 4.9 TB/s).
 //
 // Reference: transformers/integrations/moe.py:377-478.
 #include "common.h"
@@ -36,7 +48,6 @@ namespace moe {
 namespace {
 
 constexpr int BK = 64;     // columns of the contraction a stage
-constexpr int BC = 256;    // weight rows of a workgroup's tile
 constexpr int NSLOT = 4;   // stages of rows in LDS
 constexpr int kBlock16 = 64;  // columns of a block of y
 
@@ -76,20 +87,32 @@ __device__ __forceinline__ float fast_sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
 }
 
-// The biased exponent of a block's power of two from the bits of its largest |v|:
-// |v| < 2^15 of it.  255: a value is not finite.
-__device__ __forceinline__ uint32_t block16_scale(uint32_t absmax_bits) {
-  const int e = (int)(absmax_bits >> 23) - 14;
-  return absmax_bits >= 0x7f800000u ? 255u : (uint32_t)(e < 1 ? 1 : e);
+// The biased exponent of a block's power of two from its largest |v|: rint(v / 2^k) is
+// within 32767 (a mantissa from 0x7fff00 on would round to 2^15: the addition carries).
+// 255: a value is not finite.
+__device__ __forceinline__ uint32_t block16_scale(float most) {
+  const uint32_t bits = __float_as_uint(most) & 0x7fffffffu;
+  const int e = (int)((bits + 0x100u) >> 23) - 14;
+  return bits >= 0x7f800000u ? 255u : (uint32_t)(e < 1 ? 1 : e);
 }
 
-template <int BR, bool GATE, int D>
-__global__ __launch_bounds__(256, BR == 256 ? 1 : 2) void gemm4_kernel(Gemm4Args p) {
-  constexpr int TJ = BR / 32;   // row sub-tiles, all of them every wave's
-  constexpr int RPW = BR / 32;  // 1 KB DMA blocks of a stage's rows per wave
-  constexpr int W = 6;          // loads of a pair of stages' weights
-  constexpr int NB = D + 1;     // weight buffers
-  static_assert(2 * RPW + D * W <= 63, "vmcnt");
+// f(integral_constant<int, nj>, g): a main loop for each number of row sub-tiles.
+template <int TJ, typename F, typename G>
+__device__ __forceinline__ void with_sub_tiles(int nj, F&& f, G&& g) {
+  if constexpr (TJ > 1) {
+    if (nj < TJ) return with_sub_tiles<TJ - 1>(nj, f, g);
+  }
+  f(std::integral_constant<int, TJ>{}, g);
+}
+
+// NW waves, each with 64 weight rows of its own.
+template <int BR, bool GATE, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
+  constexpr int TJ = BR / 32;              // row sub-tiles, all of them every wave's
+  constexpr int RPW = BR / 8 / NW;         // 1 KB DMA blocks of a stage's rows per wave
+  constexpr int BC = 64 * NW;              // weight rows of a tile
+  constexpr int OUT = GATE ? BC / 2 : BC;  // output columns of a tile
+  static_assert(RPW >= 1, "DMA blocks per wave");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -100,156 +123,254 @@ __global__ __launch_bounds__(256, BR == 256 ? 1 : 2) void gemm4_kernel(Gemm4Args
   const int n_tiles = *p.tile_count * p.n_ct;
   const int xcd = blockIdx.x & 7, stride = gridDim.x >> 3, chunk = (n_tiles + 7) >> 3;
   const int t_end = min(n_tiles, (xcd + 1) * chunk);
-  const int nk = (p.K + BK - 1) / BK, np = p.kt;
+  int t = xcd * chunk + (int)(blockIdx.x >> 3);
+  if (t >= t_end) return;
+  const int nk = (p.K + BK - 1) / BK;
   const uint32_t ebytes = (uint32_t)p.nt * p.kt * kPack4Q, sbytes = (uint32_t)p.nt * p.kt * kPack4S;
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)(const lds_char_t*)smem;
-  auto lds_at = [](uint32_t a) { return (const lds_char_t*)(uintptr_t)a; };
-  uint32_t b_off[4];  // of sub-step j: row l32, chunk 4 hl + j
+  auto lds_at = [](uint32_t a) { return (lds_char_t*)(uintptr_t)a; };
+  uint32_t b_off[4];  // of step j: row l32, chunk 4 hl + j
 #pragma unroll
   for (int j = 0; j < 4; ++j)
     b_off[j] = lds0 + l32 * 128 + (((4 * hl + j) ^ ((l32 >> 1) & 7)) << 4);
 
-  struct Pair {  // a pair of stages' weights: [column sub-tile][stage]
-    u32x4 q[2][2];
-    uint32_t s[2];
+  // ------------------------------------------------------------- operands
+  struct Tile {
+    int e, row0, row_end, ct;
   };
-
-  for (int t = xcd * chunk + (int)(blockIdx.x >> 3); t < t_end; t += stride) {
-    const int ct = __builtin_amdgcn_readfirstlane(t % p.n_ct);
-    const int4 ti = p.tile_info[t / p.n_ct];
-    const int e = __builtin_amdgcn_readfirstlane(ti.x);
-    const int row0 = __builtin_amdgcn_readfirstlane(ti.y);
-    const int row_end = __builtin_amdgcn_readfirstlane(ti.z);
-
-    // ------------------------------------------------------------ operands
-    const char* rptr = (const char*)(GATE ? p.x : p.x + (int64_t)row0 * p.K);
-    const uint32_t rbytes =
-        GATE ? (uint32_t)(p.T * p.K * 2) : (uint32_t)((int64_t)min(row_end - row0, BR) * p.K * 2);
-    uint32_t roff[RPW];
-#pragma unroll
-    for (int i = 0; i < RPW; ++i) {
-      const int f = (wid + 4 * i) * 8 + (lane >> 3);
-      const uint32_t c = ((lane & 7) ^ ((f >> 1) & 7)) * 16;
-      const bool there = row0 + f < row_end;
-      int r = f;
-      if constexpr (GATE) {
-        const int src = p.row_src[there ? row0 + f : row0];
-        r = (int)(((uint64_t)(uint32_t)src * p.tok_mul) >> p.tok_shift);
-      }
-      roff[i] = there ? (uint32_t)r * (uint32_t)(p.K * 2) + c : kOOB;
-    }
-    // weight rows of the wave's two sub-tiles: gate and up of 32 features, or 64 columns
-    const char* qptr = p.q + (int64_t)e * ebytes;
-    const char* sptr = p.s + (int64_t)e * sbytes;
-    uint32_t qoff[2], soff[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int f0 = GATE ? ct * 128 + wid * 32 : ct * BC + wid * 64 + c * 32;
-      const uint32_t tile = (uint32_t)(((GATE && c ? p.N : 0) + f0) / 16 + (l32 >> 4)) * p.kt;
-      qoff[c] = f0 < p.N ? tile * kPack4Q + hl * 256 + (l32 & 15) * 16 : kOOB;
-      soff[c] = f0 < p.N ? tile * kPack4S + (l32 & 15) * 4 : kOOB;
-    }
-    auto issue_rows = [&](int s) {
-      const uint32_t adv = (uint32_t)s * (BK * 2);
-      const auto rs = make_rsrc(
-          rptr + adv, __builtin_amdgcn_readfirstlane(s < nk && adv < rbytes ? rbytes - adv : 0u));
-      char* slot = smem + (s & 3) * kSlot<BR>;
-#pragma unroll
-      for (int i = 0; i < RPW; ++i) dma16(rs, roff[i], slot + (wid + 4 * i) * 1024);
-    };
-    auto issue_weights = [&](int pr, Pair& w) {
-      const bool in = pr < np;
-      const uint32_t aq = (uint32_t)pr * kPack4Q, as = (uint32_t)pr * kPack4S;
-      const auto rq = make_rsrc(qptr + aq, __builtin_amdgcn_readfirstlane(in ? ebytes - aq : 0u));
-      const auto rs = make_rsrc(sptr + as, __builtin_amdgcn_readfirstlane(in ? sbytes - as : 0u));
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-          w.q[c][st] = __builtin_bit_cast(
-              u32x4, __builtin_amdgcn_raw_buffer_load_b128(rq, qoff[c] + st * 512, 0, 0));
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        w.s[c] = __builtin_amdgcn_raw_buffer_load_b32(rs, soff[c], 0, 0);
-    };
-
-    f32x16 acc[2][TJ];
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int r = 0; r < TJ; ++r)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[c][r][i] = 0.f;
-
-    Pair w[NB];
-    issue_rows(0);
-    __builtin_amdgcn_sched_barrier(0);
-    issue_weights(0, w[0]);
-    __builtin_amdgcn_sched_barrier(0);
-    issue_rows(1);
-    __builtin_amdgcn_sched_barrier(0);
-    issue_rows(2);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int d = 1; d < D; ++d) {
-      issue_weights(d, w[d]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-
-    // One stage: its rows are waited for, those three stages on (and, in an even
-    // stage, the weights D pairs on) asked for, then four steps of 16 columns.
-    auto stage = [&](int s, int pr, const Pair& cur, Pair* next, auto st_t) {
-      constexpr int st = decltype(st_t)::value;
-      // issued after these rows: two stages of rows, and weights: D pairs' in the first
-      // three stages, one pair's later (two in odd stages, of which one is in use)
-      if (pr == 0 || (D > 1 && s < 3)) __builtin_amdgcn_s_waitcnt(wait_imm(2 * RPW + D * W));
-      else __builtin_amdgcn_s_waitcnt(wait_imm(2 * RPW + W));
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-      issue_rows(s + 3);
-      __builtin_amdgcn_sched_barrier(0);
-      if (next) issue_weights(pr + D, *next);
-      __builtin_amdgcn_sched_barrier(0);
-      const uint32_t base = (uint32_t)(s & 3) * kSlot<BR>;
-      float sc[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) sc[c] = unpack4_scale(cur.s[c] >> (16 * st + 8 * hl) & 0xffu);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bf16x8 fa[2], fb[TJ];
-#pragma unroll
-        for (int r = 0; r < TJ; ++r)
-          fb[r] = *(const __attribute__((address_space(3))) bf16x8*)lds_at(base + b_off[j] + r * 4096);
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          fa[c] = __builtin_bit_cast(bf16x8, unpack4_eight(cur.q[c][st][j], sc[c]));
-#pragma unroll
-        for (int r = 0; r < TJ; ++r)
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            acc[c][r] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[c], fb[r], acc[c][r], 0, 0, 0);
-      }
-    };
-    for (int p0 = 0; p0 < np; p0 += NB) {
-#pragma unroll
-      for (int u = 0; u < NB; ++u) {
-        if (p0 + u >= np) break;
-        stage(2 * (p0 + u), p0 + u, w[u], &w[(u + D) % NB], std::integral_constant<int, 0>{});
-        stage(2 * (p0 + u) + 1, p0 + u, w[u], nullptr, std::integral_constant<int, 1>{});
-      }
-    }
-    // what is still in flight are loads from empty descriptors, into the ring
-    __builtin_amdgcn_s_waitcnt(wait_imm(0));
-    __syncthreads();
-
-    // ------------------------------------------------------------ epilogue
-    // The tile to LDS in row order (16-byte chunks swizzled by row), then out in
-    // whole lines.
-    const int rows = min(row_end - row0, BR);
+  auto tile_at = [&](int tt, const int4& ti) {
+    return Tile{ti.x, ti.y, ti.z, tt % p.n_ct};
+  };
+  auto dma_row = [&](int i) { return (wid + NW * i) * 8 + (lane >> 3); };  // the lane's, of block i
+  auto rows_load = [&](const int4& ti, int (&src)[RPW]) {  // their flat entries
     if constexpr (GATE) {
 #pragma unroll
-      for (int r = 0; r < TJ; ++r)
+      for (int i = 0; i < RPW; ++i) src[i] = p.row_src[min(ti.y + dma_row(i), ti.z - 1)];
+    }
+  };
+  const char *rptr = nullptr, *qptr = nullptr, *sptr = nullptr;
+  uint32_t rbytes = 0, roff[RPW], qoff[2], soff[2];
+  auto setup = [&](const Tile& d, const int (&src)[RPW]) {
+    int ln = lane, wd = wid;
+    asm volatile("" : "+v"(ln), "+s"(wd));  // as in the epilogue
+    rptr = (const char*)(GATE ? p.x : p.x + (int64_t)d.row0 * p.K);
+    rbytes = GATE ? (uint32_t)(p.T * p.K * 2)
+                  : (uint32_t)((int64_t)min(d.row_end - d.row0, BR) * p.K * 2);
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+      const int f = (wd + NW * i) * 8 + (ln >> 3);
+      const uint32_t c = ((ln & 7) ^ ((f >> 1) & 7)) * 16;
+      int r = f;
+      if constexpr (GATE) r = (int)(((uint64_t)(uint32_t)src[i] * p.tok_mul) >> p.tok_shift);
+      roff[i] = d.row0 + f < d.row_end ? (uint32_t)r * (uint32_t)(p.K * 2) + c : kOOB;
+    }
+    // weight rows of the wave's two sub-tiles: gate and up of 32 features, or 64 columns
+    qptr = p.q + (int64_t)d.e * ebytes;
+    sptr = p.s + (int64_t)d.e * sbytes;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int f0 = d.ct * OUT + (GATE ? wd * 32 : wd * 64 + c * 32);
+      const uint32_t tile = (uint32_t)(((GATE && c ? p.N : 0) + f0) / 16 + (ln >> 4 & 1)) * p.kt;
+      qoff[c] = f0 < p.N ? tile * kPack4Q + (ln >> 5) * 256 + (ln & 15) * 16 : kOOB;
+      soff[c] = f0 < p.N ? tile * kPack4S + (ln & 15) * 4 : kOOB;
+    }
+  };
+  auto issue_rows = [&](int s) {
+    const uint32_t adv = (uint32_t)s * (BK * 2);
+    const auto rs = make_rsrc(
+        rptr + adv, __builtin_amdgcn_readfirstlane(s < nk && adv < rbytes ? rbytes - adv : 0u));
+    char* slot = smem + (s & 3) * kSlot<BR>;
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) dma16(rs, roff[i], slot + (wid + NW * i) * 1024);
+  };
+  // The weights of four stages, the scales of their pairs.
+  u32x4 wq[4][2];
+  uint32_t ws[2][2];
+  auto issue_codes = [&](int s, u32x4 (&w)[2]) {  // stage s: half a tile
+    const uint32_t adv = (uint32_t)(s >> 1) * kPack4Q + (uint32_t)(s & 1) * 512;
+    const auto rs = make_rsrc(qptr + adv, __builtin_amdgcn_readfirstlane(s < nk ? ebytes - adv : 0u));
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      w[c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, qoff[c], 0, 0));
+  };
+  auto issue_scales = [&](int pr, uint32_t (&w)[2]) {
+    const uint32_t adv = (uint32_t)pr * kPack4S;
+    const auto rs =
+        make_rsrc(sptr + adv, __builtin_amdgcn_readfirstlane(pr < p.kt ? sbytes - adv : 0u));
+#pragma unroll
+    for (int c = 0; c < 2; ++c) w[c] = __builtin_amdgcn_raw_buffer_load_b32(rs, soff[c], 0, 0);
+  };
+
+  // ------------------------------------------------------------- main loop
+  // Stages run in groups of four, the last one filled up with empty stages.  A stage's
+  // rows, codes and (with odd ones) scales are asked for four stages ahead, in the last
+  // group those of the next tile's first: so a tile begins with its loads under way.
+  const int groups = (nk + 3) / 4;
+  f32x16 acc[2][TJ];
+  auto fragment = [&](int s, int j, int r) {
+    return *(const __attribute__((address_space(3))) bf16x8*)lds_at(
+        (uint32_t)(s & 3) * kSlot<BR> + b_off[j] + r * 4096);
+  };
+  auto weights = [&](int u, int c, int j) {  // stage u of a group
+    const uint32_t sc = ws[u / 2][c] >> (16 * (u & 1) + 8 * hl) & 0xffu;
+    return __builtin_bit_cast(bf16x8, unpack4_eight(wq[u][c][j], unpack4_scale(sc)));
+  };
+  auto mma = [](const bf16x8& w, const bf16x8& x, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, x, c, 0, 0, 0);
+  };
+  // Until the next stage's rows are there, and every wave has read all of this one's.
+  // Asked for after them were two stages' rows, four loads of codes and two of scales
+  // at least; in a tile's first stages, the previous one's stores too (`stored`
+  // sub-tiles, kStores each), which may still be on their way (loads and stores
+  // complete in order).
+  constexpr int kStores = GATE ? 2 : 4, kAfter = 2 * RPW + 6;
+  static_assert(kAfter + 4 * kStores <= 63 && TJ <= 4, "vmcnt");
+  int stored = 0;
+  auto wait_rows = [&](bool first_stages) {
+    const int n = first_stages ? stored : 0;
+    if (n == 0) __builtin_amdgcn_s_waitcnt(wait_imm(kAfter));
+    else if (n == 1) __builtin_amdgcn_s_waitcnt(wait_imm(kAfter + kStores));
+    else if (n == 2) __builtin_amdgcn_s_waitcnt(wait_imm(kAfter + 2 * kStores));
+    else if (n == 3) __builtin_amdgcn_s_waitcnt(wait_imm(kAfter + 3 * kStores));
+    else __builtin_amdgcn_s_waitcnt(wait_imm(kAfter + 4 * kStores));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // Many rows (bound by the matrix units): a stage's four steps, each reading and
+  // converting the next one's fragments while it multiplies; before the last step the
+  // next stage's rows are waited for, and behind that barrier stage `at`, the one four
+  // on, is asked for in this one's place.
+  auto many_rows = [&](auto nj_t, auto&& next_tile) {
+    constexpr int NJ = decltype(nj_t)::value;
+    bf16x8 fa[2][2], fb[2][NJ];
+    auto read = [&](int buf, int u, int j) {
+#pragma unroll
+      for (int r = 0; r < NJ; ++r) fb[buf][r] = fragment(u, j, r);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) fa[buf][c] = weights(u, c, j);
+    };
+    auto multiply = [&](int buf) {
+#pragma unroll
+      for (int r = 0; r < NJ; ++r)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) acc[c][r] = mma(fa[buf][c], fb[buf][r], acc[c][r]);
+    };
+    // order within a step: loads, fragment reads and conversions between the MFMAs
+    auto order = [&](auto loads_t) {
+      constexpr int LOADS = decltype(loads_t)::value;
+#pragma unroll
+      for (int r = 0; r < NJ; ++r) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        if (LOADS) __builtin_amdgcn_sched_group_barrier(0x020, (LOADS + NJ - 1) / NJ, 0);  // VMEM
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // DS read
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (16 + NJ - 1) / NJ, 0);  // VALU
+      }
+    };
+    read(0, 0, 0);
+    for (int group = 0; group < groups; ++group) {
+      int at = 4 * group + 4;
+      if (group == groups - 1) {
+        next_tile();
+        at = 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          read((j + 1) & 1, u, j + 1);
+          multiply(j & 1);
+          order(std::integral_constant<int, 0>{});
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        wait_rows(u < 3 && group == 0);
+        issue_rows(at + u);
+        issue_codes(at + u, wq[u]);
+        if (u & 1) issue_scales((at + u) >> 1, ws[u / 2]);
+        if (u < 3) read(0, u + 1, 0);
+        else read(0, 0, 0);
+        multiply(1);
+        order(std::integral_constant<int, RPW + 4>{});
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // Few rows (bound by the weights): a stage's fragments are all read a stage ahead, so
+  // that a stage waits once.
+  auto few_rows = [&](auto nj_t, auto&& next_tile) {
+    constexpr int NJ = decltype(nj_t)::value;
+    bf16x8 fb[2][4][NJ];
+    auto read = [&](int buf, int u) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int r = 0; r < NJ; ++r) fb[buf][j][r] = fragment(u, j, r);
+    };
+    read(0, 0);
+    for (int group = 0; group < groups; ++group) {
+      int at = 4 * group + 4;
+      if (group == groups - 1) {
+        next_tile();
+        at = 0;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        wait_rows(u < 3 && group == 0);
+        issue_rows(at + u);
+        __builtin_amdgcn_sched_barrier(0);
+        read((u + 1) & 1, (u + 1) & 3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const bf16x8 w = weights(u, c, j);
+#pragma unroll
+            for (int r = 0; r < NJ; ++r) acc[c][r] = mma(w, fb[u & 1][j][r], acc[c][r]);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+        issue_codes(at + u, wq[u]);
+        if (u & 1) issue_scales((at + u) >> 1, ws[u / 2]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  // -------------------------------------------------------------- epilogue
+  // Row sub-tiles through LDS to memory in row order, whole lines, while the next
+  // tile's first stages are on their way.
+  const uint32_t stage = lds0 + NSLOT * kSlot<BR>;
+  typedef __attribute__((address_space(3))) u32x2 lds_u32x2_t;
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4_t;
+  auto lds_barrier = [&]() {  // (loads stay in flight)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  };
+  auto turn = [&]() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  };
+  auto epilogue = [&](const Tile& d, int nj) {
+    // lane and wave opaque to the optimizer, which would otherwise hoist the addresses
+    // out of the tile loop and spill them (a reload waits for every load before it)
+    int ln = lane, wd = wid;
+    asm volatile("" : "+v"(ln), "+s"(wd));
+    const int el32 = ln & 31, ehl = ln >> 5;
+    const uint32_t rows = (uint32_t)min(d.row_end - d.row0, BR);
+    if constexpr (GATE) {
+      // a wave has 64 bytes of a row: the workgroup's waves write a sub-tile together,
+      // in two halves of the staging by turns (and between two tiles lie the main
+      // loop's barriers)
+      constexpr int LINE = OUT * 2;            // bytes of a row
+      constexpr int PER = 1024 / LINE;         // rows a store of a wave
+      static_assert(kStores * NW * PER == 32, "a sub-tile's rows");
+      const auto rs = make_rsrc(p.act + (int64_t)d.row0 * p.N, rows * (uint32_t)p.N * 2);
+#pragma unroll
+      for (int r = 0; r < TJ; ++r) {
+        if (r >= nj) break;
+        const uint32_t buf = stage + (r & 1) * (32 * LINE);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float v[4];
@@ -258,100 +379,211 @@ __global__ __launch_bounds__(256, BR == 256 ? 1 : 2) void gemm4_kernel(Gemm4Args
             const float g = acc[0][r][4 * q + i];
             v[i] = g * fast_sigmoid(g) * acc[1][r][4 * q + i];
           }
-          const int row = r * 32 + l32, ch = wid * 4 + q;
-          *(u32x2*)(smem + row * 256 + ((ch ^ (row & 15)) << 4) + hl * 8) =
+          *(lds_u32x2_t*)lds_at(buf + el32 * LINE + (((wd * 4 + q) ^ (el32 & 15)) << 4) + ehl * 8) =
               u32x2{pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3])};
         }
-      __syncthreads();
-      for (int i = tid; i < rows * 16; i += 256) {
-        const int row = i >> 4, ch = i & 15, col = ct * 128 + ch * 8;
-        if (col < p.N)
-          __builtin_nontemporal_store(*(const u32x4*)(smem + row * 256 + ((ch ^ (row & 15)) << 4)),
-                                      (u32x4*)(p.act + (int64_t)(row0 + row) * p.N + col));
+        lds_barrier();
+#pragma unroll
+        for (int h = 0; h < kStores; ++h) {
+          const int row = (h * NW + wd) * PER + ln / (LINE / 16), ch = ln % (LINE / 16);
+          const int col = d.ct * OUT + ch * 8;
+          const u32x4 v = *(const lds_u32x4_t*)lds_at(buf + row * LINE + ((ch ^ (row & 15)) << 4));
+          __builtin_amdgcn_raw_buffer_store_b128(
+              v, rs, col < p.N ? (uint32_t)(r * 32 + row) * (uint32_t)p.N * 2 + (uint32_t)col * 2 : kOOB,
+              0, 2);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
+      const int f0 = d.ct * OUT + wd * 64;
+      const auto rs = make_rsrc(p.y + (int64_t)d.row0 * p.N, rows * (uint32_t)p.N * 2);
+      const uint32_t mine = stage + wd * 4096, scales = stage + NW * 4096;
+      if (f0 < p.N) {
 #pragma unroll
-      for (int r = 0; r < TJ; ++r) {
-        uint32_t m = 0;
+        for (int r = 0; r < TJ; ++r) {
+          if (r >= nj) break;
+          float m = 0.f;  // (maximum: NaN if any is)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(acc[c][r][i]) & 0x7fffffffu);
-        m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
-        const uint32_t sb = block16_scale(m);
-        const float inv = sb == 255u ? 0.f : __uint_as_float((254u - sb) << 23);
-        const int row = r * 32 + l32;
+            for (int i = 0; i < 16; ++i)
+              m = __builtin_elementwise_maximum(m, __builtin_fabsf(acc[c][r][i]));
+          const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m),
+                                                             false, false);
+          m = __builtin_elementwise_maximum(__uint_as_float(both[0]), __uint_as_float(both[1]));
+          const uint32_t sb = block16_scale(m);
+          const float inv = __uint_as_float((254u - sb) << 23);  // of 255: anything
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            int v[4];
+            for (int q = 0; q < 4; ++q) {
+              // adding 1.5 2^23 rounds to an integer, halves to even, whose two's
+              // complement ends the sum's bits
+              uint32_t v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = (int)__builtin_rintf(acc[c][r][4 * q + i] * inv);
-            const int ch = wid * 8 + c * 4 + q;
-            *(u32x2*)(smem + row * 512 + ((ch ^ (row & 31)) << 4) + hl * 8) =
-                u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pk_i16(v[0], v[1])),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pk_i16(v[2], v[3]))};
+              for (int i = 0; i < 4; ++i)
+                v[i] = __float_as_uint(__builtin_fmaf(acc[c][r][4 * q + i], inv, 12582912.f));
+              *(lds_u32x2_t*)lds_at(mine + el32 * 128 + (((c * 4 + q) ^ (el32 & 7)) << 4) + ehl * 8) =
+                  u32x2{__builtin_amdgcn_perm(v[1], v[0], 0x05040100u),
+                        __builtin_amdgcn_perm(v[3], v[2], 0x05040100u)};
+            }
+          if (ehl == 0)
+            *(__attribute__((address_space(3))) uint8_t*)lds_at(scales + (r * 32 + el32) * NW + wd) =
+                (uint8_t)sb;
+          turn();
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int row = h * 8 + (ln >> 3), ch = ln & 7;
+            const u32x4 v = *(const lds_u32x4_t*)lds_at(mine + row * 128 + ((ch ^ (row & 7)) << 4));
+            __builtin_amdgcn_raw_buffer_store_b128(
+                v, rs, (uint32_t)(r * 32 + row) * (uint32_t)p.N * 2 + (uint32_t)(f0 + ch * 8) * 2, 0, 2);
           }
-        const int blk = ct * 4 + wid;
-        if (hl == 0 && row < rows && blk * kBlock16 < p.N)
-          p.ys[(int64_t)(row0 + row) * (p.N / kBlock16) + blk] = (uint8_t)sb;
+          turn();
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-      __syncthreads();
-      for (int i = tid; i < rows * 32; i += 256) {
-        const int row = i >> 5, ch = i & 31, col = ct * BC + ch * 8;
-        if (col < p.N)
-          __builtin_nontemporal_store(*(const u32x4*)(smem + row * 512 + ((ch ^ (row & 31)) << 4)),
-                                      (u32x4*)(p.y + (int64_t)(row0 + row) * p.N + col));
+      // a row's scale bytes together: one at a time they would be as many writes of memory
+      lds_barrier();
+      const int blocks = p.N / kBlock16, have = min(NW, blocks - d.ct * NW);
+      for (uint32_t row = wd * 64 + ln; row < rows; row += 64 * NW) {
+        uint8_t* at = p.ys + (int64_t)(d.row0 + row) * blocks + d.ct * NW;
+        const lds_char_t* from = lds_at(scales + row * NW);
+        if (have == NW && ((uintptr_t)at & 3) == 0) {
+#pragma unroll
+          for (int i = 0; i < NW / 4; ++i)
+            ((uint32_t*)at)[i] = ((const __attribute__((address_space(3))) uint32_t*)from)[i];
+        } else {
+          for (int i = 0; i < have; ++i) at[i] = (uint8_t)from[i];
+        }
       }
     }
-    __syncthreads();  // read out before the next tile's rows land
+  };
+
+  // ------------------------------------------------------------- the tiles
+  // (a table that no kernel writes meanwhile, read to scalar registers)
+  typedef const __attribute__((address_space(4))) int const_int_t;
+  const auto* infos = (const_int_t*)(uintptr_t)p.tile_info;
+  auto info_at = [&](int tt) {
+    const int64_t i = 4 * (int64_t)(min(tt, t_end - 1) / p.n_ct);
+    return make_int4(infos[i], infos[i + 1], infos[i + 2], 0);
+  };
+  int4 ti = info_at(t);
+  int src[RPW] = {};
+  rows_load(ti, src);
+  Tile d = tile_at(t, ti);
+  setup(d, src);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    issue_rows(u);
+    issue_codes(u, wq[u]);
+    if (u & 1) issue_scales(u >> 1, ws[u / 2]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  __builtin_amdgcn_s_waitcnt(wait_imm(3 * RPW));
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  while (true) {
+    const Tile done = d;
+    const int nj = (min(d.row_end - d.row0, BR) + 31) / 32;
+    t += stride;
+    const bool more = t < t_end;
+    ti = info_at(t);
+    rows_load(ti, src);  // lands under the main loop
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int r = 0; r < TJ; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[c][r][i] = 0.f;
+    auto next_tile = [&]() {
+      if (more) {
+        d = tile_at(t, ti);
+        setup(d, src);
+      } else {  // loads as many as ever, of nothing
+        rbytes = 0;
+        qoff[0] = qoff[1] = soff[0] = soff[1] = kOOB;
+      }
+    };
+    if constexpr (BR <= 64) with_sub_tiles<TJ>(nj, few_rows, next_tile);
+    else with_sub_tiles<TJ>(nj, many_rows, next_tile);
+    epilogue(done, nj);
+    if (!more) return;
+    // (a wave past the last column stores nothing)
+    stored = GATE || done.ct * OUT + wid * 64 < p.N ? nj : 0;
   }
 }
 
 // ---------------------------------------------------------------- combine
-// A wave a token, eight columns a lane; up to eight rows of y in flight.
+// A wave a token, eight columns a lane, two pieces of 512 columns of up to eight rows
+// of y in flight; the next token's rows and weights are read meanwhile.
 constexpr int kCombineWaves = 4;
-__global__ __launch_bounds__(64 * kCombineWaves) void combine16_kernel(
+constexpr int kPieces = 2;
+__global__ __launch_bounds__(64 * kCombineWaves, 4) void combine16_kernel(
     const int16_t* __restrict__ y, const uint8_t* __restrict__ ys, const int* __restrict__ slot,
     const int* __restrict__ offsets, const void* __restrict__ w, int wdt, int64_t T, int K, int E,
     int H, bf16* __restrict__ out) {
   const int lane = threadIdx.x & 63;
-  const int nvalid = offsets[E];
+  const int nvalid = offsets[E], blocks = H / kBlock16;
   const int64_t nw = (int64_t)gridDim.x * kCombineWaves;
-  for (int64_t t = (int64_t)blockIdx.x * kCombineWaves + (threadIdx.x >> 6); t < T; t += nw) {
-    for (int h = ((int)blockIdx.y * 64 + lane) * 8; h < H; h += (int)gridDim.y * 512) {
-      float o[8];
+  const auto entry_load = [&](int64_t t, int kb, int& row, float& wk) {  // entries kb + lane
+    const int64_t at = t * K + kb + lane;
+    const bool in = t < T && kb + lane < K;
+    row = in ? slot[at] : 0x7fffffff;
+    wk = !in ? 0.f : wdt == MOE_DTYPE_BF16 ? bf2f(((const bf16*)w)[at]) : ((const float*)w)[at];
+  };
+  int64_t t = (int64_t)blockIdx.x * kCombineWaves + (threadIdx.x >> 6);
+  int row, row_next;
+  float wk, wk_next;
+  entry_load(t, 0, row, wk);
+  for (; t < T; t += nw) {
+    entry_load(t + nw, 0, row_next, wk_next);
+    for (int h0 = (int)blockIdx.y * 512 * kPieces; h0 < H; h0 += (int)gridDim.y * 512 * kPieces) {
+      float o[kPieces][8] = {};
+      for (int kb = 0; kb < K; kb += 64) {
+        if (K > 64) entry_load(t, kb, row, wk);
+        for (int k0 = 0; k0 < min(K - kb, 64); k0 += 8) {
+          u32x4 v[kPieces][8];
+          uint32_t sb[kPieces][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = 0.f;
-      for (int k0 = 0; k0 < K; k0 += 8) {
-        u32x4 v[8];
-        float f[8];
+          for (int k = 0; k < 8; ++k) {
+            const int s = __builtin_amdgcn_readlane(row, k0 + k);
+            if (s >= nvalid) continue;  // a sentinel, or none
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          f[k] = 0.f;
-          v[k] = u32x4{0, 0, 0, 0};
-          if (k0 + k >= K) continue;  // uniform
-          const int64_t at = t * K + k0 + k;
-          const int s = __builtin_amdgcn_readfirstlane(slot[at]);
-          if (s >= nvalid) continue;  // a sentinel contributes nothing
-          v[k] = __builtin_nontemporal_load((const u32x4*)(y + (int64_t)s * H + h));
-          const uint32_t sb = ys[(int64_t)s * (H / kBlock16) + h / kBlock16];
-          // 0 * inf, NaN, for a block that is not finite
-          f[k] = __uint_as_float(sb << 23) *
-                 (wdt == MOE_DTYPE_BF16 ? bf2f(((const bf16*)w)[at]) : ((const float*)w)[at]);
+            for (int c = 0; c < kPieces; ++c) {
+              const int h = h0 + c * 512 + lane * 8;
+              if (h < H) {
+                v[c][k] = __builtin_nontemporal_load((const u32x4*)(y + (int64_t)s * H + h));
+                sb[c][k] = ys[(int64_t)s * blocks + h / kBlock16];
+              }
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            if (__builtin_amdgcn_readlane(row, k0 + k) >= nvalid) continue;
+            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wk), k0 + k));
+#pragma unroll
+            for (int c = 0; c < kPieces; ++c) {
+              // 255: the block is NaN whole
+              const float s = __uint_as_float(sb[c][k] == 255u ? 0x7fc00000u : sb[c][k] << 23) * f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                o[c][i] = fmaf((float)(int16_t)(v[c][k][i >> 1] >> (16 * (i & 1))), s, o[c][i]);
+            }
+          }
         }
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o[i] = fmaf((float)(int16_t)(v[k][i >> 1] >> (16 * (i & 1))), f[k], o[i]);
       }
-      u32x4 r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = pack_bf2(o[2 * i], o[2 * i + 1]);
-      *(u32x4*)(out + t * H + h) = r;
+      for (int c = 0; c < kPieces; ++c) {
+        const int h = h0 + c * 512 + lane * 8;
+        if (h >= H) continue;
+        u32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = pack_bf2(o[c][2 * i], o[c][2 * i + 1]);
+        __builtin_nontemporal_store(r, (u32x4*)(out + t * H + h));
+      }
     }
+    row = row_next;
+    wk = wk_next;
   }
 }
 
@@ -382,32 +614,45 @@ int check4(int64_t S, int E, int H, int I, const char* who) {
   return MOE_OK;
 }
 
-template <int BR, bool GATE, int D>
+template <int BR, bool GATE, int NW>
 int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStream_t st,
             const char* who) {
+  static_assert(kTileSizes[0] == 64 && kTileSizes[1] == 128, "the plan's row tiles");
   const char* pb = (const char*)tile_plan;
   a.tile_count = (const int*)pb + (size_t)b * (E + 1) + E;
   a.tile_info = (const int4*)(pb + plan_info_offset(S, E, b));
+  constexpr int OUT = GATE ? 32 * NW : 64 * NW;
+  a.n_ct = (a.N + OUT - 1) / OUT;
   const int64_t most = plan_max_tiles(S, E, b) * a.n_ct;
   MOE_REQUIRE(most <= (int64_t)1 << 30, MOE_ERR_UNSUPPORTED, "%s: too many tiles", who);
-  constexpr int lds = NSLOT * kSlot<BR>;
+  // the ring of rows, and two halves of 32 rows or a part for each wave and the scales
+  constexpr int lds = NSLOT * kSlot<BR> + (GATE ? 2 * 32 * OUT * 2 : NW * 4096 + BR * NW);
   static std::atomic<int> done[64];
-  const hipError_t err = set_dynamic_lds_once(done, (const void*)gemm4_kernel<BR, GATE, D>, lds);
+  const hipError_t err = set_dynamic_lds_once(done, (const void*)gemm4_kernel<BR, GATE, NW>, lds);
   MOE_REQUIRE(err == hipSuccess, MOE_ERR_HIP, "%s: HIP error %d (%s)", who, (int)err,
               hipGetErrorString(err));
-  int64_t grid = (int64_t)num_cus() / 8 * 8 * (BR == 256 ? 1 : 2);
+  int64_t grid = (int64_t)num_cus() / 8 * 8 * (8 / NW);
   if (grid > (most + 7) / 8 * 8) grid = (most + 7) / 8 * 8;
   if (grid < 8) grid = 8;
-  gemm4_kernel<BR, GATE, D><<<(int)grid, 256, lds, st>>>(a);
+  gemm4_kernel<BR, GATE, NW><<<(int)grid, 64 * NW, lds, st>>>(a);
   return check_launch(who);
 }
 
+// Row tiles by the mean rows of an expert (us at 2048 columns, I 768, top 8; few: 64
+// rows and four waves; many: 128 rows, and four waves for gate and up, eight, which
+// read a row's stage half as often, for down):
+//   mean rows, experts  8, 128  32, 128  48, 128  64, 128  187, 128  256, 128  9, 1792  36, 1792
+//   gate/up  few          41.2     45.7     62.3     66.6     152.5     226.0     519       672
+//            many         50.5     55.9     57.6     62.6     151.5     209.7     582       691
+//   down     few          23.4     27.8     33.3     40.6      93.1     125.6     314       375
+//            many         28.2     32.0     35.4     38.7      92.9     123.9     303       380
+// and at 1024 rows (16384 tokens) 692 to 648 and 404 to 374.  Few rows leave half of a
+// 128-row tile's registers idle; many read the weights half as often.
 template <bool GATE>
 int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, hipStream_t st, const char* who) {
-  const int64_t mean = S / E;
-  if (mean >= 256) return launch4<256, GATE, 1>(a, S, E, tile_plan, 2, st, who);
-  if (mean >= 96) return launch4<128, GATE, 2>(a, S, E, tile_plan, 1, st, who);
-  return launch4<64, GATE, 3>(a, S, E, tile_plan, 0, st, who);
+  if (S / E >= (GATE ? 40 : 256))
+    return launch4<128, GATE, GATE ? 4 : 8>(a, S, E, tile_plan, 1, st, who);
+  return launch4<64, GATE, 4>(a, S, E, tile_plan, 0, st, who);
 }
 
 }  // namespace
@@ -447,7 +692,6 @@ extern "C" int moe_amd_gemm_gate_up_swiglu4(const void* hidden_states, const int
   a.N = I;
   a.kt = (H + kPack4Cols - 1) / kPack4Cols;
   a.nt = 2 * I / kPack4Rows;
-  a.n_ct = (I + 127) / 128;
   // division by top_k as in gemm.hip: exact for 31 bits
   int sh = 0;
   while ((1 << sh) < top_k) ++sh;
@@ -480,7 +724,6 @@ extern "C" int moe_amd_gemm_down4(const void* act, const int32_t* offsets, const
   a.N = H;
   a.kt = (I + kPack4Cols - 1) / kPack4Cols;
   a.nt = H / kPack4Rows;
-  a.n_ct = (H + BC - 1) / BC;
   return launch4<false>(a, S, E, tile_plan, (hipStream_t)stream, who);
 }
 
@@ -498,11 +741,10 @@ extern "C" int moe_amd_combine16(const void* y, const void* y_scale, const int32
               "%s: null pointer", who);
   MOE_ALIGNED(y, who);
   MOE_ALIGNED(out, who);
-  // few tokens: a row's columns to several waves
+  // few tokens: a row's columns to several waves; many: as many waves as are resident
   int64_t gx = (T + kCombineWaves - 1) / kCombineWaves;
-  int gy = (H + 511) / 512;
-  if (gx >= 2048) gy = 1;
-  if (gx > 256 * 32) gx = 256 * 32;
+  const int gy = gx >= 1024 ? 1 : (H + 512 * kPieces - 1) / (512 * kPieces);
+  if (gx > 1024) gx = 1024;
   combine16_kernel<<<dim3((unsigned)gx, (unsigned)gy), 64 * kCombineWaves, 0, (hipStream_t)stream>>>(
       (const int16_t*)y, (const uint8_t*)y_scale, slot, offsets, topk_weights, weights_dtype, T, K, E,
       H, (bf16*)out);
