@@ -90,8 +90,11 @@ def _experts_forward4(hidden_states, top_k_index, top_k_weights, gate_up_proj, d
         raise ValueError("top_k_index / top_k_weights must both be [T, K]")
     library.check_keep(saved_activations, gate_up_proj.dtype)
     refuse_grad4("experts_forward", hidden_states, top_k_weights)
-    out = torch.ops.moe_amd.experts_fwd4(hidden_states.to(torch.bfloat16).contiguous(), top_k_index,
-                                         top_k_weights.contiguous(), *bank)
+    x = hidden_states.to(torch.bfloat16)
+    if few._unseen(x, top_k_index, top_k_weights, *bank):
+        out = ops.experts4(x, top_k_index, top_k_weights, gate_up_proj, down_proj)
+    else:
+        out = torch.ops.moe_amd.experts_fwd4(x, top_k_index, top_k_weights, *bank)
     return out.to(hidden_states.dtype)
 
 

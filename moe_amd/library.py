@@ -855,12 +855,8 @@ def _bank4(x: Tensor, q1: Tensor, s1: Tensor, q2: Tensor, s2: Tensor):
 def experts_fwd4(x: Tensor, topk_index: Tensor, topk_weights: Tensor, gate_up_q: Tensor,
                  gate_up_scale: Tensor, down_q: Tensor, down_scale: Tensor) -> Tensor:
     """The experts on a bank in 4 bits; no autograd formula."""
-    w1, w2 = _bank4(x, gate_up_q, gate_up_scale, down_q, down_scale)
-    plan = ops.permute(topk_index, w1.shape[0])
-    act = ops.gemm_gate_up_swiglu4(x, plan, w1)
-    y, ys = ops.gemm_down4(act, plan, w2)
-    del act
-    return ops.combine16(y, ys, plan, topk_weights)
+    return ops.experts4(x, topk_index, topk_weights,
+                        *_bank4(x, gate_up_q, gate_up_scale, down_q, down_scale))
 
 
 @experts_fwd4.register_fake

@@ -923,8 +923,9 @@ def unpack4(packed: Packed4) -> torch.Tensor:
     return w
 
 
-def _packed_operand(name: str, p: Packed4, like: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """(q, scale) of a packed bank that a kernel takes beside ``like``."""
+def _packed_operand(name: str, p: Packed4, like: torch.Tensor, plan: RoutingPlan
+                    ) -> tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of a packed bank that a kernel takes beside ``like`` and ``plan``."""
     _need_cuda(p.q, p.scale)
     check_packed4(name, p)
     if len(p.shape) != 3:
@@ -932,8 +933,9 @@ def _packed_operand(name: str, p: Packed4, like: torch.Tensor) -> tuple[torch.Te
     if like.dtype != torch.bfloat16 or p.dtype != torch.bfloat16:
         raise NotImplementedError(f"{name}: banks in 4 bits take bf16 layers, not {like.dtype} "
                                   f"hidden states on {p.dtype} weights")
-    if p.device != like.device:
-        raise ValueError(f"{name}: tensors on {like.device} and {p.device}, expected one device")
+    if not p.device == plan.offsets.device == like.device:
+        raise ValueError(f"{name}: tensors on {like.device}, {p.device} and {plan.offsets.device}, "
+                         "expected one device")
     return _contig(p.q), _contig(p.scale)
 
 
@@ -943,7 +945,7 @@ def gemm_gate_up_swiglu4(x: torch.Tensor, plan: RoutingPlan, gate_up_proj: Packe
     bits; gate and up stay fp32."""
     name = "gemm_gate_up_swiglu4"
     _need_cuda(x)
-    q, scale = _packed_operand(name, gate_up_proj, x)
+    q, scale = _packed_operand(name, gate_up_proj, x, plan)
     E, I2, H = gate_up_proj.shape
     if tuple(x.shape) != (plan.num_tokens, H) or I2 % 2 or E != plan.num_experts:
         raise ValueError(f"{name}: hidden {tuple(x.shape)}, gate_up_proj "
@@ -964,7 +966,7 @@ def gemm_down4(act: torch.Tensor, plan: RoutingPlan, down_proj: Packed4
     uint8 [S,H/64]), y = int16 * 2^(byte - 127), for combine16."""
     name = "gemm_down4"
     _need_cuda(act)
-    q, scale = _packed_operand(name, down_proj, act)
+    q, scale = _packed_operand(name, down_proj, act, plan)
     E, H, I = down_proj.shape
     if tuple(act.shape) != (plan.num_rows, I) or E != plan.num_experts:
         raise ValueError(f"{name}: act {tuple(act.shape)}, down_proj {tuple(down_proj.shape)}, a "
@@ -991,6 +993,9 @@ def combine16(y: torch.Tensor, y_scale: torch.Tensor, plan: RoutingPlan,
         raise ValueError(f"combine16: y {y.dtype} {tuple(y.shape)}, scale {y_scale.dtype} "
                          f"{tuple(y_scale.shape)}, weights {tuple(topk_weights.shape)}, a plan of "
                          f"{T} tokens and {plan.num_rows} rows")
+    if not y.device == y_scale.device == topk_weights.device == plan.offsets.device:
+        raise ValueError(f"combine16: tensors on {y.device}, {y_scale.device}, "
+                         f"{topk_weights.device} and {plan.offsets.device}, expected one device")
     y, y_scale, topk_weights = _contig(y), _contig(y_scale), _contig(topk_weights)
     out = torch.empty(T, H, device=y.device, dtype=torch.bfloat16)
     _call("moe_amd_combine16", y.data_ptr(), y_scale.data_ptr(), plan.slot.data_ptr(),
@@ -1122,6 +1127,21 @@ def _few4_inputs(name: str, x, gate_up_proj, down_proj, K: int, *others):
 @functools.lru_cache(maxsize=256)
 def _few4_workspace_size(*shape: int) -> int:
     return max(int(_lib.load().moe_amd_few4_workspace_size(*shape)), 16)
+
+
+@on_tensor_device
+def experts4(x: torch.Tensor, topk_index: torch.Tensor, topk_weights: torch.Tensor,
+             gate_up_proj: Packed4, down_proj: Packed4) -> torch.Tensor:
+    """out [T,H] of the experts on a bank in 4 bits with the routing given (weights
+    fp32 or bf16); forward only."""
+    if topk_index.dim() != 2 or topk_index.shape != topk_weights.shape \
+            or topk_index.shape[0] != x.shape[0]:
+        raise ValueError("experts4: topk_index / topk_weights must both be [T, K]")
+    plan = permute(topk_index, gate_up_proj.shape[0])
+    act = gemm_gate_up_swiglu4(x, plan, gate_up_proj)
+    y, ys = gemm_down4(act, plan, down_proj)
+    del act
+    return combine16(y, ys, plan, topk_weights)
 
 
 @on_tensor_device
