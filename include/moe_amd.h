@@ -479,6 +479,16 @@ int moe_amd_combine16(const void* y, const void* y_scale, const int32_t* slot,
                       const int32_t* offsets, const void* topk_weights, int weights_dtype,
                       int64_t T, int K, int E, int H, void* out, void* stream);
 
+/* All of it with a caller's routing topk_index, topk_weights [T,K]: moe_amd_permute,
+ * the two products and the combine, in a 16-byte aligned workspace of
+ * moe_amd_experts4_workspace_size bytes (0: sizes that the call refuses).  Ids outside
+ * [0, E) contribute nothing. */
+size_t moe_amd_experts4_workspace_size(int64_t T, int E, int K, int H, int I);
+int moe_amd_experts4(const void* hidden_states, const int64_t* topk_index, const void* topk_weights,
+                     int weights_dtype, const void* gate_up_q, const void* gate_up_scale,
+                     const void* down_q, const void* down_scale, int64_t T, int K, int E, int H,
+                     int I, void* workspace, size_t workspace_bytes, void* out, void* stream);
+
 /* --------------------------------------------- the layer for a few tokens */
 
 /* The expert layer for up to MOE_FEW_MAX_TOKENS tokens, forward only: the

@@ -104,6 +104,9 @@ SIGNATURES: dict[str, tuple] = {
     "moe_amd_moe_layer_few4": (
         _i, [_p, _p, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _p, _i, _f, _i, _i, _p, _sz, _p,
              _p, _p, _p]),
+    "moe_amd_experts4_workspace_size": (_sz, [_i64, _i, _i, _i, _i]),
+    "moe_amd_experts4": (
+        _i, [_p, _p, _p, _i, _p, _p, _p, _p, _i64, _i, _i, _i, _i, _p, _sz, _p, _p]),
     "moe_amd_gemm_gate_up_swiglu4": (
         _i, [_p, _p, _i, _p, _p, _p, _p, _i64, _i64, _i, _i, _i, _p, _p]),
     "moe_amd_gemm_down4": (_i, [_p, _p, _p, _p, _p, _i64, _i, _i, _i, _p, _p, _p]),

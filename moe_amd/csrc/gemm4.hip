@@ -655,6 +655,40 @@ int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, hipStream_t s
   return launch4<64, GATE, 4>(a, S, E, tile_plan, 0, st, who);
 }
 
+// moe_amd_experts4's workspace: each array 256-byte aligned.
+struct Layout4 {
+  size_t counts, offsets, row_src, slot, plan, sort, act, y, ys, bytes;
+  size_t plan_bytes, sort_bytes;
+};
+Layout4 layout4(int64_t S, int E, int H, int I) {
+  Layout4 l{};
+  const auto take = [&](size_t n) {
+    const size_t at = l.bytes;
+    l.bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  l.counts = take((size_t)E * 4);
+  l.offsets = take((size_t)(E + 1) * 4);
+  l.row_src = take((size_t)S * 4);
+  l.slot = take((size_t)S * 4);
+  l.plan = take(l.plan_bytes = moe_amd_tile_plan_size(S, E));
+  l.sort = take(l.sort_bytes = moe_amd_permute_workspace_size(S, E));
+  l.act = take((size_t)S * I * 2);
+  l.y = take((size_t)S * H * 2);
+  l.ys = take((size_t)S * (H / kBlock16));
+  return l;
+}
+
+int check_experts4(int64_t T, int K, int E, int H, int I, const char* who) {
+  MOE_REQUIRE(T >= 0 && K >= 1 && E <= 16384, MOE_ERR_ARG, "%s: T=%lld, K=%d or E=%d out of range",
+              who, (long long)T, K, E);
+  MOE_REQUIRE(T < (int64_t)1 << 31, MOE_ERR_UNSUPPORTED, "%s: T=%lld too large", who, (long long)T);
+  const int rc = check4(T * K, E, H, I, who);
+  if (rc) return rc;
+  MOE_REQUIRE(T * (int64_t)H * 2 < ((int64_t)1 << 31), MOE_ERR_UNSUPPORTED, "%s: T*H too large", who);
+  return MOE_OK;
+}
+
 }  // namespace
 }  // namespace moe
 
@@ -749,4 +783,51 @@ extern "C" int moe_amd_combine16(const void* y, const void* y_scale, const int32
       (const int16_t*)y, (const uint8_t*)y_scale, slot, offsets, topk_weights, weights_dtype, T, K, E,
       H, (bf16*)out);
   return check_launch(who);
+}
+
+extern "C" size_t moe_amd_experts4_workspace_size(int64_t T, int E, int K, int H, int I) {
+  if (check_experts4(T, K, E, H, I, "experts4_workspace_size") != MOE_OK) return 0;
+  return layout4(T * K, E, H, I).bytes;
+}
+
+extern "C" int moe_amd_experts4(const void* hidden_states, const int64_t* topk_index,
+                                const void* topk_weights, int weights_dtype, const void* gate_up_q,
+                                const void* gate_up_scale, const void* down_q,
+                                const void* down_scale, int64_t T, int K, int E, int H, int I,
+                                void* workspace, size_t workspace_bytes, void* out, void* stream) {
+  const char* who = "experts4";
+  int rc = check_experts4(T, K, E, H, I, who);
+  if (rc) return rc;
+  if (T == 0) return MOE_OK;
+  // all of it before the first launch
+  MOE_REQUIRE(weights_dtype == MOE_DTYPE_F32 || weights_dtype == MOE_DTYPE_BF16, MOE_ERR_DTYPE,
+              "%s: weights dtype %d", who, weights_dtype);
+  MOE_REQUIRE(hidden_states && topk_index && topk_weights && gate_up_q && gate_up_scale && down_q &&
+                  down_scale && out,
+              MOE_ERR_ARG, "%s: null pointer", who);
+  MOE_ALIGNED(hidden_states, who);
+  MOE_ALIGNED(gate_up_q, who);
+  MOE_ALIGNED(gate_up_scale, who);
+  MOE_ALIGNED(down_q, who);
+  MOE_ALIGNED(down_scale, who);
+  MOE_ALIGNED(out, who);
+  const int64_t S = T * K;
+  const Layout4 l = layout4(S, E, H, I);
+  MOE_REQUIRE(workspace && workspace_bytes >= l.bytes, MOE_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes, needs %zu", who, workspace_bytes, l.bytes);
+  MOE_ALIGNED(workspace, who);
+  char* const ws = (char*)workspace;
+  int* const offsets = (int*)(ws + l.offsets);
+  int* const row_src = (int*)(ws + l.row_src);
+  int* const slot = (int*)(ws + l.slot);
+  char* const plan = ws + l.plan;
+  if ((rc = moe_amd_permute(topk_index, S, E, ws + l.sort, l.sort_bytes, (int*)(ws + l.counts),
+                            offsets, row_src, slot, plan, l.plan_bytes, stream)) ||
+      (rc = moe_amd_gemm_gate_up_swiglu4(hidden_states, row_src, K, offsets, plan, gate_up_q,
+                                         gate_up_scale, T, S, E, H, I, ws + l.act, stream)) ||
+      (rc = moe_amd_gemm_down4(ws + l.act, offsets, plan, down_q, down_scale, S, E, H, I, ws + l.y,
+                               ws + l.ys, stream)))
+    return rc;
+  return moe_amd_combine16(ws + l.y, ws + l.ys, slot, offsets, topk_weights, weights_dtype, T, K, E,
+                           H, out, stream);
 }

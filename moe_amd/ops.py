@@ -1109,8 +1109,8 @@ def packed_bank(name: str, x: torch.Tensor, gate_up_proj: Packed4, down_proj: Pa
     return bank, E, H, I2 // 2
 
 
-def _few4_inputs(name: str, x, gate_up_proj, down_proj, K: int, *others):
-    """packed_bank of a few-token call, contiguous, and the rest of its checks."""
+def _bank4_inputs(name: str, x, gate_up_proj, down_proj, *others):
+    """packed_bank, contiguous, and the rest of the checks of a C entry on it."""
     bank, E, H, I = packed_bank(name, x, gate_up_proj, down_proj)
     _need_cuda(x)
     if x.dtype != torch.bfloat16:
@@ -1118,10 +1118,21 @@ def _few4_inputs(name: str, x, gate_up_proj, down_proj, K: int, *others):
     for t in others:
         if t is not None and t.get_device() != x.get_device():
             raise ValueError(f"{name}: tensors on {x.device} and {t.device}, expected one device")
+    return [_contig(t) for t in bank], E, H, I
+
+
+def _few4_inputs(name: str, x, gate_up_proj, down_proj, K: int, *others):
+    """_bank4_inputs of a few-token call."""
+    res = _bank4_inputs(name, x, gate_up_proj, down_proj, *others)
     if x.shape[0] > FEW_MAX_TOKENS or K > FEW_MAX_TOP_K:
         raise RuntimeError(f"{name}: {x.shape[0]} tokens with top-{K}; it takes at most "
                            f"{FEW_MAX_TOKENS} and {FEW_MAX_TOP_K}")
-    return [_contig(t) for t in bank], E, H, I
+    return res
+
+
+@functools.lru_cache(maxsize=256)
+def _experts4_workspace_size(*shape: int) -> int:
+    return max(int(_lib.load().moe_amd_experts4_workspace_size(*shape)), 16)
 
 
 @functools.lru_cache(maxsize=256)
@@ -1134,14 +1145,23 @@ def experts4(x: torch.Tensor, topk_index: torch.Tensor, topk_weights: torch.Tens
              gate_up_proj: Packed4, down_proj: Packed4) -> torch.Tensor:
     """out [T,H] of the experts on a bank in 4 bits with the routing given (weights
     fp32 or bf16); forward only."""
+    name = "experts4"
     if topk_index.dim() != 2 or topk_index.shape != topk_weights.shape \
             or topk_index.shape[0] != x.shape[0]:
-        raise ValueError("experts4: topk_index / topk_weights must both be [T, K]")
-    plan = permute(topk_index, gate_up_proj.shape[0])
-    act = gemm_gate_up_swiglu4(x, plan, gate_up_proj)
-    y, ys = gemm_down4(act, plan, down_proj)
-    del act
-    return combine16(y, ys, plan, topk_weights)
+        raise ValueError(f"{name}: topk_index / topk_weights must both be [T, K]")
+    T, K = topk_index.shape
+    bank, E, H, I = _bank4_inputs(name, x, gate_up_proj, down_proj, topk_index, topk_weights)
+    x = _contig(x)
+    if topk_index.dtype != torch.int64:
+        topk_index = topk_index.to(torch.int64)
+    topk_index, topk_weights = _contig(topk_index), _contig(topk_weights)
+    n = _experts4_workspace_size(T, E, K, H, I)
+    ws = torch.empty(n, device=x.device, dtype=torch.uint8)
+    out = torch.empty(T, H, device=x.device, dtype=x.dtype)
+    _call("moe_amd_experts4", x.data_ptr(), topk_index.data_ptr(), topk_weights.data_ptr(),
+          _dtype_code(topk_weights.dtype), *[t.data_ptr() for t in bank], T, K, E, H, I,
+          ws.data_ptr(), n, out.data_ptr(), _stream(x))
+    return out
 
 
 @on_tensor_device

@@ -375,3 +375,23 @@ def test_custom_ops():
 
     got = torch.compile(both, fullgraph=True)(x, idx, w)
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_the_products_one_by_one():
+    """The entries that experts_forward consists of, and the op of its dispatcher."""
+    g = _gen(11)
+    T, H, E, K, I = 333, 192, 9, 3, 128
+    b1, b2 = _bank(g, E, H, I)
+    x = _x(g, T, H)
+    idx = torch.randint(-1, E + 1, (T, K), generator=g, device=DEV)
+    w = torch.rand(T, K, generator=g, device=DEV)
+    out = experts_forward(x, idx, w, b1, b2)
+    plan = ops.permute(idx, E)
+    y, ys = ops.gemm_down4(ops.gemm_gate_up_swiglu4(x, plan, b1), plan, b2)
+    assert torch.equal(out, ops.combine16(y, ys, plan, w))
+    assert torch.equal(out, torch.ops.moe_amd.experts_fwd4(x, idx, w, b1.q, b1.scale, b2.q, b2.scale))
+    # other strides and types of the same values
+    wide = torch.randn(T, 2 * H, generator=g, device=DEV, dtype=BF)
+    wide[:, ::2] = x
+    assert torch.equal(out, experts_forward(wide[:, ::2], idx.to(torch.int32), w.t().contiguous().t(),
+                                            b1, b2))

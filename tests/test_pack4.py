@@ -43,6 +43,8 @@ def test_nothing_to_do_is_no_call(built_lib):
     _lib.call("moe_amd_combine16", None, None, None, None, None, 0, 0, 2, 4, 64, None, None)
     _lib.call("moe_amd_experts_few4", None, None, None, 0, None, None, None, None, 0, 2, 4, 64, 64,
               None, 0, None, None)
+    _lib.call("moe_amd_experts4", None, None, None, 0, None, None, None, None, 0, 2, 4, 64, 64, None,
+              0, None, None)
 
 
 @pytest.mark.parametrize("at,value,status,text", [
@@ -94,6 +96,39 @@ def test_combine16_refuses(built_lib, at, value, status, text):
     args[at] = value
     with pytest.raises(RuntimeError, match=f"{status}.*combine16.*{text}"):
         _lib.call("moe_amd_combine16", *args)
+
+
+def _experts4_ws(T=4, E=8, K=2, H=128, I=64):
+    return _lib.load().moe_amd_experts4_workspace_size(T, E, K, H, I)
+
+
+def test_experts4_workspace(built_lib):
+    # act, y and the sorted rows' indices at least
+    assert _experts4_ws() >= 8 * (64 * 2 + 128 * 2 + 2 + 8)
+    assert 0 < _experts4_ws() < _experts4_ws(T=64) < _experts4_ws(T=64, K=16)
+    for bad in (dict(T=-1), dict(K=0), dict(E=0), dict(E=16385), dict(H=96), dict(I=32), dict(H=0),
+                dict(T=1 << 28), dict(T=1 << 20, H=1024)):
+        assert _experts4_ws(**bad) == 0, bad
+
+
+@pytest.mark.parametrize("at,value,status,text", [
+    (0, None, "MOE_ERR_ARG", "null"), (0, A + 8, "MOE_ERR_ALIGN", "not 16-byte"),
+    (1, None, "MOE_ERR_ARG", "null"), (2, None, "MOE_ERR_ARG", "null"),
+    (3, 7, "MOE_ERR_DTYPE", "weights dtype"), (4, None, "MOE_ERR_ARG", "null"),
+    (4, A + 8, "MOE_ERR_ALIGN", "not 16-byte"), (5, A + 4, "MOE_ERR_ALIGN", "not 16-byte"),
+    (6, None, "MOE_ERR_ARG", "null"), (6, A + 8, "MOE_ERR_ALIGN", "not 16-byte"),
+    (7, A + 4, "MOE_ERR_ALIGN", "not 16-byte"), (8, -1, "MOE_ERR_ARG", "T=-1"),
+    (8, 1 << 24, "MOE_ERR_UNSUPPORTED", r"T\*H"), (9, 0, "MOE_ERR_ARG", "K=0"),
+    (10, 16385, "MOE_ERR_ARG", "E=16385"), (11, 96, "MOE_ERR_ARG", "multiples of 64"),
+    (12, 32, "MOE_ERR_ARG", "multiples of 64"), (13, None, "MOE_ERR_WORKSPACE", "needs"),
+    (13, A + 8, "MOE_ERR_ALIGN", "not 16-byte"), (14, 16, "MOE_ERR_WORKSPACE", "needs"),
+    (15, None, "MOE_ERR_ARG", "null"), (15, A + 8, "MOE_ERR_ALIGN", "not 16-byte"),
+])
+def test_experts4_refuses(built_lib, at, value, status, text):
+    args = [A, A, A, 0, A, A, A, A, 4, 2, 8, 128, 64, A, 1 << 20, A, None]
+    args[at] = value
+    with pytest.raises(RuntimeError, match=f"{status}.*experts4.*{text}"):
+        _lib.call("moe_amd_experts4", *args)
 
 
 def _ws(T=4, E=8, K=2, H=128, I=64):
