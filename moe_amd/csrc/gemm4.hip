@@ -31,13 +31,13 @@
 // NaN whole.  Each output is rounded once.
 //
 // Measured (gate/up, down, combine; H 2048, I 768, top 8 of 128 experts):
-//   16384 tokens  648 us (1.27 PF), 374 us (1.10 PF), 116 us (5.2 TB/s); a plain bf16
+//   16384 tokens  645 us (1.28 PF), 350 us (1.18 PF), 107 us (5.6 TB/s); a plain bf16
 //                 product reaches 1.4 to 1.6 PF on this card: bound by the matrix
-//                 units, the rest is the short contraction's epilogues and
-//                 the conversions' issue slots
-//    1021 tokens  63 us, 41 us, 9 us: 320 MB of weights, an expert's 64 rows mean
-//                 both bounds are near (3.4 TB/s, 0.8 PF)
-// and 2048 tokens on 1792 experts (9 rows each): 514 us, 314 us, 17 us, bound by the
+//                 units.  Without epilogues 600 and 310 us; the rest are the
+//                 conversions' issue slots and each expert's last, partial tile
+//    1021 tokens  60 us, 38 us, 9 us: 320 MB of weights and 64 rows an expert, so
+//                 that both bounds are near (3.6 TB/s, 0.86 PF)
+// and 2048 tokens on 1792 experts (9 rows each): 515 us, 308 us, 15 us, bound by the
 // 4.5 GB of weights (5.8 and 4.9 TB/s).
 //
 // Reference: transformers/integrations/moe.py:377-478.
@@ -105,9 +105,12 @@ __device__ __forceinline__ void with_sub_tiles(int nj, F&& f, G&& g) {
   f(std::integral_constant<int, TJ>{}, g);
 }
 
+// Waves a SIMD: 64 rows leave the registers and the LDS for three.
+template <int BR> constexpr int kWavesSimd = BR <= 64 ? 3 : 2;
+
 // NW waves, each with 64 weight rows of its own.
 template <int BR, bool GATE, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
+__global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Args p) {
   constexpr int TJ = BR / 32;              // row sub-tiles, all of them every wave's
   constexpr int RPW = BR / 8 / NW;         // 1 KB DMA blocks of a stage's rows per wave
   constexpr int BC = 64 * NW;              // weight rows of a tile
@@ -142,18 +145,29 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
   auto tile_at = [&](int tt, const int4& ti) {
     return Tile{ti.x, ti.y, ti.z, tt % p.n_ct};
   };
-  auto dma_row = [&](int i) { return (wid + NW * i) * 8 + (lane >> 3); };  // the lane's, of block i
+  // What is computed once a tile is computed from the lane and the wave as the
+  // optimizer does not know them: else it moves the addresses out of the tile loop,
+  // or to the tile's beginning, and spills them (a reload waits for every load
+  // before it).
   auto rows_load = [&](const int4& ti, int (&src)[RPW]) {  // their flat entries
     if constexpr (GATE) {
+      int ln = lane, wd = wid;
+      asm volatile("" : "+v"(ln), "+s"(wd));
 #pragma unroll
-      for (int i = 0; i < RPW; ++i) src[i] = p.row_src[min(ti.y + dma_row(i), ti.z - 1)];
+      for (int i = 0; i < RPW; ++i)
+        src[i] = p.row_src[min(ti.y + (wd + NW * i) * 8 + (ln >> 3), ti.z - 1)];
     }
   };
   const char *rptr = nullptr, *qptr = nullptr, *sptr = nullptr;
   uint32_t rbytes = 0, roff[RPW], qoff[2], soff[2];
-  auto setup = [&](const Tile& d, const int (&src)[RPW]) {
-    int ln = lane, wd = wid;
-    asm volatile("" : "+v"(ln), "+s"(wd));  // as in the epilogue
+  auto setup = [&](const Tile& d, int (&src)[RPW]) {
+    int ln = lane, wd = wid, shift = p.tok_shift;
+    uint32_t mul = p.tok_mul;
+    asm volatile("" : "+v"(ln), "+s"(wd), "+s"(mul), "+s"(shift));
+    if constexpr (GATE) {
+#pragma unroll
+      for (int i = 0; i < RPW; ++i) asm volatile("" : "+v"(src[i]));
+    }
     rptr = (const char*)(GATE ? p.x : p.x + (int64_t)d.row0 * p.K);
     rbytes = GATE ? (uint32_t)(p.T * p.K * 2)
                   : (uint32_t)((int64_t)min(d.row_end - d.row0, BR) * p.K * 2);
@@ -162,7 +176,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
       const int f = (wd + NW * i) * 8 + (ln >> 3);
       const uint32_t c = ((ln & 7) ^ ((f >> 1) & 7)) * 16;
       int r = f;
-      if constexpr (GATE) r = (int)(((uint64_t)(uint32_t)src[i] * p.tok_mul) >> p.tok_shift);
+      if constexpr (GATE) r = (int)(((uint64_t)(uint32_t)src[i] * mul) >> shift);
       roff[i] = d.row0 + f < d.row_end ? (uint32_t)r * (uint32_t)(p.K * 2) + c : kOOB;
     }
     // weight rows of the wave's two sub-tiles: gate and up of 32 features, or 64 columns
@@ -269,7 +283,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
       }
     };
     read(0, 0, 0);
-    for (int group = 0; group < groups; ++group) {
+    int group = 0;
+    do {
       int at = 4 * group + 4;
       if (group == groups - 1) {
         next_tile();
@@ -294,7 +309,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
         order(std::integral_constant<int, RPW + 4>{});
         __builtin_amdgcn_sched_barrier(0);
       }
-    }
+    } while (++group < groups);
   };
   // Few rows (bound by the weights): a stage's fragments are all read a stage ahead, so
   // that a stage waits once.
@@ -308,7 +323,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
         for (int r = 0; r < NJ; ++r) fb[buf][j][r] = fragment(u, j, r);
     };
     read(0, 0);
-    for (int group = 0; group < groups; ++group) {
+    int group = 0;
+    do {
       int at = 4 * group + 4;
       if (group == groups - 1) {
         next_tile();
@@ -333,7 +349,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
         if (u & 1) issue_scales((at + u) >> 1, ws[u / 2]);
         __builtin_amdgcn_sched_barrier(0);
       }
-    }
+    } while (++group < groups);
   };
 
   // -------------------------------------------------------------- epilogue
@@ -353,8 +369,6 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
   };
   auto epilogue = [&](const Tile& d, int nj) {
-    // lane and wave opaque to the optimizer, which would otherwise hoist the addresses
-    // out of the tile loop and spill them (a reload waits for every load before it)
     int ln = lane, wd = wid;
     asm volatile("" : "+v"(ln), "+s"(wd));
     const int el32 = ln & 31, ehl = ln >> 5;
@@ -467,7 +481,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
     const int64_t i = 4 * (int64_t)(min(tt, t_end - 1) / p.n_ct);
     return make_int4(infos[i], infos[i + 1], infos[i + 2], 0);
   };
-  int4 ti = info_at(t);
+  int4 ti = info_at(t), ti_next = info_at(t + stride);
   int src[RPW] = {};
   rows_load(ti, src);
   Tile d = tile_at(t, ti);
@@ -487,8 +501,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gemm4_kernel(Gemm4Args p) {
     const int nj = (min(d.row_end - d.row0, BR) + 31) / 32;
     t += stride;
     const bool more = t < t_end;
-    ti = info_at(t);
-    rows_load(ti, src);  // lands under the main loop
+    ti = ti_next;
+    ti_next = info_at(t + stride);
+    rows_load(ti, src);  // (both land under the main loop)
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -631,7 +646,7 @@ int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStr
   const hipError_t err = set_dynamic_lds_once(done, (const void*)gemm4_kernel<BR, GATE, NW>, lds);
   MOE_REQUIRE(err == hipSuccess, MOE_ERR_HIP, "%s: HIP error %d (%s)", who, (int)err,
               hipGetErrorString(err));
-  int64_t grid = (int64_t)num_cus() / 8 * 8 * (8 / NW);
+  int64_t grid = (int64_t)num_cus() / 8 * 8 * (kWavesSimd<BR> * 4 / NW);
   if (grid > (most + 7) / 8 * 8) grid = (most + 7) / 8 * 8;
   if (grid < 8) grid = 8;
   gemm4_kernel<BR, GATE, NW><<<(int)grid, 64 * NW, lds, st>>>(a);
@@ -639,18 +654,18 @@ int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStr
 }
 
 // Row tiles by the mean rows of an expert (us at 2048 columns, I 768, top 8; few: 64
-// rows and four waves; many: 128 rows, and four waves for gate and up, eight, which
-// read a row's stage half as often, for down):
-//   mean rows, experts  8, 128  32, 128  48, 128  64, 128  187, 128  256, 128  9, 1792  36, 1792
-//   gate/up  few          41.2     45.7     62.3     66.6     152.5     226.0     519       672
-//            many         50.5     55.9     57.6     62.6     151.5     209.7     582       691
-//   down     few          23.4     27.8     33.3     40.6      93.1     125.6     314       375
-//            many         28.2     32.0     35.4     38.7      92.9     123.9     303       380
-// and at 1024 rows (16384 tokens) 692 to 648 and 404 to 374.  Few rows leave half of a
-// 128-row tile's registers idle; many read the weights half as often.
+// rows, four waves; many: 128 rows, four waves for gate and up, eight, which read a row
+// half as often, for down: its contraction is short):
+//   mean rows, experts  8, 128  32, 128  48, 128  64, 128  128, 128  512, 128  1024, 128  9, 1792
+//   gate/up  few            39       47       69       78       104       371        713     524
+//            many           41       46       56       60       118       388        682     557
+//   down     few            23       27       33       42        60       216        414     313
+//            many           24       28       34       38        65       204        382     309
+// Few rows take half the registers, so that three workgroups share a CU where two do
+// of many, which read the weights half as often.
 template <bool GATE>
 int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, hipStream_t st, const char* who) {
-  if (S / E >= (GATE ? 40 : 256))
+  if (S / E >= 40)
     return launch4<128, GATE, GATE ? 4 : 8>(a, S, E, tile_plan, 1, st, who);
   return launch4<64, GATE, 4>(a, S, E, tile_plan, 0, st, who);
 }
