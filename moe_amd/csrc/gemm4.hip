@@ -50,6 +50,7 @@ namespace {
 constexpr int BK = 64;     // columns of the contraction a stage
 constexpr int NSLOT = 4;   // stages of rows in LDS
 constexpr int kBlock16 = 64;  // columns of a block of y
+constexpr int kMostColumns = 1 << 22;
 
 template <int BR> constexpr int kSlot = BR * BK * 2;  // bytes
 
@@ -622,7 +623,9 @@ int check4(int64_t S, int E, int H, int I, const char* who) {
               who, H, I);
   MOE_REQUIRE(S < ((int64_t)1 << 29), MOE_ERR_UNSUPPORTED, "%s: S=%lld routed rows, limit 2^29", who,
               (long long)S);
-  // an expert's codes are read through a descriptor of 32 bits
+  // a tile's rows and an expert's codes are read through descriptors of 32 bits
+  MOE_REQUIRE(H <= kMostColumns && I <= kMostColumns, MOE_ERR_UNSUPPORTED,
+              "%s: H=%d or I=%d above 2^22", who, H, I);
   MOE_REQUIRE(pack4_tiles(2 * (int64_t)I, H) * kPack4Q < ((int64_t)1 << 31) &&
                   pack4_tiles(H, I) * kPack4Q < ((int64_t)1 << 31),
               MOE_ERR_UNSUPPORTED, "%s: H=%d, I=%d: an expert's weights exceed 2 GB", who, H, I);
@@ -785,6 +788,7 @@ extern "C" int moe_amd_combine16(const void* y, const void* y_scale, const int32
               "%s: weights dtype %d", who, weights_dtype);
   MOE_REQUIRE(T >= 0 && K >= 1 && E >= 1 && H > 0 && H % 64 == 0, MOE_ERR_ARG,
               "%s: T=%lld K=%d E=%d H=%d", who, (long long)T, K, E, H);
+  MOE_REQUIRE(H <= kMostColumns, MOE_ERR_UNSUPPORTED, "%s: H=%d above 2^22", who, H);
   if (T == 0) return MOE_OK;
   MOE_REQUIRE(y && y_scale && slot && offsets && topk_weights && out, MOE_ERR_ARG,
               "%s: null pointer", who);

@@ -133,6 +133,7 @@ def pack_bank(bank: nn.Module) -> nn.Module:
     which state_dict holds and ``to`` moves.  The bank is forward only from then on."""
     if is_packed_bank(bank):
         return bank
+    _check_module(bank)
     weights = [getattr(bank, name) for name in _BANK]
     for name, w in zip(_BANK, weights):
         if w.dtype != torch.bfloat16:

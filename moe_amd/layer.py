@@ -28,10 +28,10 @@ from .router import gating_linear, linear_sigmoid_topk, sigmoid_topk, softmax_to
 
 def _fused_softmax_ok(x, w_router, gate_up_proj, down_proj) -> bool:
     E, H = w_router.shape
-    return (not isinstance(gate_up_proj, ops.Packed4) and x.is_cuda and x.dim() == 2 and x.dtype == torch.bfloat16
-            and w_router.dtype == torch.bfloat16 and gate_up_proj.dtype == torch.bfloat16
-            and down_proj.dtype == torch.bfloat16 and H % 256 == 0 and E % 8 == 0
-            and gate_up_proj.shape[0] == E)
+    return (not isinstance(gate_up_proj, ops.Packed4) and x.is_cuda and x.dim() == 2
+            and x.dtype == torch.bfloat16 and w_router.dtype == torch.bfloat16
+            and gate_up_proj.dtype == torch.bfloat16 and down_proj.dtype == torch.bfloat16
+            and H % 256 == 0 and E % 8 == 0 and gate_up_proj.shape[0] == E)
 
 
 @traced_with_defaults
@@ -147,7 +147,8 @@ class SparseMoeBlock(nn.Module):
             self.router_logits = None
             return out.reshape(shape)
         out, probs, _, idx = moe_layer(
-            flat, *params, self.top_k, router=self.router, renormalize=self.norm_topk_prob, logit_offset=self.logit_offset,
+            flat, *params, self.top_k, router=self.router, renormalize=self.norm_topk_prob,
+            logit_offset=self.logit_offset,
             expert_bias=self.expert_bias if self.router == "sigmoid" else None,
             saved_activations=library.keep_of_call(self.saved_activations, flat, *params))
         self.router_logits, self.topk_index = probs, idx

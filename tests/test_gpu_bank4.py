@@ -146,7 +146,7 @@ PROMPT = [  # T, H, E, K, I, skew
     (200, 64, 3, 1, 832, 0.0), (509, 1024, 128, 4, 768, 0.0), (300, 128, 2, 2, 128, 0.0),
     (1021, 256, 16, 8, 320, 2.0), (777, 704, 8, 3, 576, 0.0), (1500, 192, 4, 4, 128, 0.0),
     (4096, 512, 24, 8, 256, 3.0), (2050, 2048, 128, 8, 768, 1.0), (127, 64, 1, 1, 64, 0.0),
-    (64, 64, 1, 1, 64, 0.0),
+    (64, 64, 1, 1, 64, 0.0), (20, 128, 80, 70, 64, 0.0),
 ]
 
 
@@ -395,3 +395,29 @@ def test_the_products_one_by_one():
     wide[:, ::2] = x
     assert torch.equal(out, experts_forward(wide[:, ::2], idx.to(torch.int32), w.t().contiguous().t(),
                                             b1, b2))
+
+
+def test_banks_past_four_gigabytes():
+    """The last experts of a bank whose codes take more than 2^32 bytes."""
+    g = _gen(14)
+    E, H, I, K = 2800, 2048, 768, 2
+
+    def bank(n, k):
+        q = torch.empty(E, n // 16, k // 128, 1024, device=DEV, dtype=torch.uint8)
+        for part in q.split(200):
+            part.random_(0, 256, generator=g)
+        s = torch.randint(119, 122, (E, n // 16, k // 128, 64), generator=g, device=DEV)
+        return ops.Packed4(q, s.to(torch.uint8), (E, n, k), BF)
+
+    b1, b2 = bank(2 * I, H), bank(H, I)
+    assert b1.q.numel() > 1 << 32
+    idx = torch.tensor([[E - 1, 0], [E - 2, E - 1], [2733, 1400]], device=DEV).repeat(14, 1)
+    x, w = _x(g, len(idx), H), torch.rand(len(idx), K, generator=g, device=DEV)
+    _close(few.experts_forward_few(x, idx, w, b1, b2), *_oracle(x, idx, w, b1, b2))
+    _close(few.experts_forward_few(x[:1], idx[:1], w[:1], b1, b2),
+           *_oracle(x[:1], idx[:1], w[:1], b1, b2))
+    _close(experts_forward(x, idx, w, b1, b2), *_oracle(x, idx, w, b1, b2, blocks=True))
+    # a tile row and an expert's end of the bank through the packing too
+    last = ops.Packed4(b1.q[E - 1:], b1.scale[E - 1:], (1, 2 * I, H), BF)
+    whole = ops.unpack4(ops.Packed4(b1.q, b1.scale, b1.shape, BF))
+    assert torch.equal(whole[E - 1:], ops.unpack4(last))

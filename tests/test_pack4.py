@@ -65,7 +65,8 @@ def test_gate_up4_refuses(built_lib, at, value, status, text):
 
 def test_gate_up4_limits(built_lib):
     for T, K, E, H, I, text in ((1 << 28, 2, 4, 64, 64, "2\\^29"), (1 << 20, 1, 4, 1024, 64, "T\\*H"),
-                                (4, 2, 4, 1 << 16, 1 << 16, "exceed 2 GB")):
+                                (4, 2, 4, 1 << 16, 1 << 16, "exceed 2 GB"),
+                                (4, 2, 4, 64, 1 << 23, "2\\^22"), (1, 2, 4, 1 << 23, 64, "2\\^22")):
         with pytest.raises(RuntimeError, match=f"MOE_ERR_UNSUPPORTED.*{text}"):
             _lib.call("moe_amd_gemm_gate_up_swiglu4", A, A, K, A, A, A, A, T, T * K, E, H, I, A, None)
 
@@ -88,7 +89,7 @@ def test_down4_refuses(built_lib, at, value, status, text):
     (0, None, "MOE_ERR_ARG", "null"), (1, None, "MOE_ERR_ARG", "null"),
     (0, A + 8, "MOE_ERR_ALIGN", "not 16-byte"), (4, None, "MOE_ERR_ARG", "null"),
     (5, 7, "MOE_ERR_DTYPE", "weights dtype"), (6, -1, "MOE_ERR_ARG", "T=-1"),
-    (9, 96, "MOE_ERR_ARG", "H=96"), (10, None, "MOE_ERR_ARG", "null"),
+    (9, 96, "MOE_ERR_ARG", "H=96"), (9, 1 << 23, "MOE_ERR_UNSUPPORTED", r"2\^22"), (10, None, "MOE_ERR_ARG", "null"),
     (10, A + 8, "MOE_ERR_ALIGN", "not 16-byte"),
 ])
 def test_combine16_refuses(built_lib, at, value, status, text):
@@ -221,6 +222,11 @@ def test_python_refusals():
         pack_bank(SparseMoeBlock(64, 3, 2, 64).experts)
     with pytest.raises(ValueError, match="multiples of 64"):
         pack_bank(SparseMoeBlock(96, 3, 2, 64).bfloat16().experts)
+    bank = SparseMoeBlock(64, 3, 2, 64).bfloat16().experts
+    bank.is_transposed = True   # no call would take it
+    with pytest.raises(NotImplementedError, match="transposed"):
+        pack_bank(bank)
+    assert bank.gate_up_proj.dtype == BF
 
 
 def _pack_on_cpu(monkeypatch):
