@@ -218,10 +218,13 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
   };
 
   // ------------------------------------------------------------- main loop
-  // Stages run in groups of four, the last one filled up with empty stages.  A stage's
-  // rows, codes and (with odd ones) scales are asked for four stages ahead, in the last
+  // Stages run in groups of four, the last one filled up to two or four with empty stages
+  // (to four for gate and up of few rows, whose registers do not hold the branch: 22.0 us
+  // become 24.4 for 509 tokens of 1024 columns; elsewhere 320 and 576 columns gain 5 to 10%).
+  // A stage's rows, codes and (with odd ones) scales are asked for four stages ahead, in the last
   // group those of the next tile's first: so a tile begins with its loads under way.
   const int groups = (nk + 3) / 4;
+  const bool half = (BR > 64 || !GATE) && nk - 4 * (groups - 1) <= 2;  // the last group
   f32x16 acc[2][TJ];
   auto fragment = [&](int s, int j, int r) {
     return *(const __attribute__((address_space(3))) bf16x8*)lds_at(
@@ -251,6 +254,18 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
     else __builtin_amdgcn_s_waitcnt(wait_imm(kAfter + 4 * kStores));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
+  };
+  // The second half of a group that has only one: the next tile's stages in its place, and
+  // what the last one would have waited for, the next tile's first rows.
+  auto leave_out = [&]() {
+#pragma unroll
+    for (int u = 2; u < 4; ++u) {
+      if (u == 3) wait_rows(false);
+      issue_rows(u);
+      issue_codes(u, wq[u]);
+      if (u & 1) issue_scales(u >> 1, ws[u / 2]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   // Many rows (bound by the matrix units): a stage's four steps, each reading and
   // converting the next one's fragments while it multiplies; before the last step the
@@ -287,12 +302,18 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
     int group = 0;
     do {
       int at = 4 * group + 4;
+      bool leave = false;
       if (group == groups - 1) {
         next_tile();
         at = 0;
+        leave = half;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
+        if (u == 2 && leave) {
+          leave_out();
+          break;
+        }
 #pragma unroll
         for (int j = 0; j < 3; ++j) {
           read((j + 1) & 1, u, j + 1);
@@ -327,12 +348,18 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
     int group = 0;
     do {
       int at = 4 * group + 4;
+      bool leave = false;
       if (group == groups - 1) {
         next_tile();
         at = 0;
+        leave = half;
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
+        if (u == 2 && leave) {
+          leave_out();
+          break;
+        }
         wait_rows(u < 3 && group == 0);
         issue_rows(at + u);
         __builtin_amdgcn_sched_barrier(0);
@@ -664,11 +691,15 @@ int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStr
 //            many           41       46       56       60       118       388        682     557
 //   down     few            23       27       33       42        60       216        414     313
 //            many           24       28       34       38        65       204        382     309
+// and many down's columns want to be a whole number of 512: where 256 do as well and the
+// rest is more than a ninth, few (3000 tokens on 32 experts, top 6, I 320, 576 columns:
+// 26.2 and 15.6; 8192 on 64, top 4, I 512, 1280 columns: 58.9 and 49.3).
 // Few rows take half the registers, so that three workgroups share a CU where two do
 // of many, which read the weights half as often.
 template <bool GATE>
 int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, hipStream_t st, const char* who) {
-  if (S / E >= 40)
+  const int quarters = (a.N + 255) / 256;
+  if (S / E >= 40 && (GATE || quarters % 2 == 0 || quarters >= 9))
     return launch4<128, GATE, GATE ? 4 : 8>(a, S, E, tile_plan, 1, st, who);
   return launch4<64, GATE, 4>(a, S, E, tile_plan, 0, st, who);
 }

@@ -147,6 +147,7 @@ PROMPT = [  # T, H, E, K, I, skew
     (1021, 256, 16, 8, 320, 2.0), (777, 704, 8, 3, 576, 0.0), (1500, 192, 4, 4, 128, 0.0),
     (4096, 512, 24, 8, 256, 3.0), (2050, 2048, 128, 8, 768, 1.0), (127, 64, 1, 1, 64, 0.0),
     (64, 64, 1, 1, 64, 0.0), (20, 128, 80, 70, 64, 0.0),
+    (900, 448, 4, 3, 320, 0.0), (700, 960, 6, 2, 192, 1.0), (333, 512, 2, 1, 576, 0.0),
 ]
 
 
@@ -160,11 +161,12 @@ def test_experts_forward(T, H, E, K, I, skew):
     assert torch.equal(out, experts_forward(x, idx, w, b1, b2))
 
 
+@pytest.mark.parametrize("H", [192, 448])
 @pytest.mark.parametrize("rows", [1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300])
-def test_rows_of_an_expert(rows):
+def test_rows_of_an_expert(rows, H):
     """Row counts around the tiles' heights; one expert without a row, one with all."""
     g = _gen(rows)
-    E, H, I = 3, 192, 192
+    E, I = 3, 192
     b1, b2 = _bank(g, E, H, I)
     for e in (0, 2):
         x, idx = _x(g, rows, H), torch.full((rows, 1), e, device=DEV)
@@ -175,7 +177,7 @@ def test_rows_of_an_expert(rows):
 def test_row_heights_give_the_same_bits():
     """A row's results do not depend on how many others there are."""
     g = _gen(5)
-    E, H, I = 2, 256, 192
+    E, H, I = 2, 512, 192
     b1, b2 = _bank(g, E, H, I)
     x = _x(g, 1500, H)
     idx = torch.arange(1500, device=DEV)[:, None] % 2
