@@ -84,16 +84,16 @@ def experts_forward(hidden_states: torch.Tensor, top_k_index: torch.Tensor,
 
 def _experts_forward4(hidden_states, top_k_index, top_k_weights, gate_up_proj, down_proj,
                       saved_activations):
-    bank, *_ = ops.packed_bank("experts_forward", hidden_states, gate_up_proj, down_proj)
-    if top_k_index.dim() != 2 or top_k_index.shape != top_k_weights.shape \
-            or top_k_index.shape[0] != hidden_states.shape[0]:
-        raise ValueError("top_k_index / top_k_weights must both be [T, K]")
     library.check_keep(saved_activations, gate_up_proj.dtype)
-    refuse_grad4("experts_forward", hidden_states, top_k_weights)
+    refuse_grad4("experts_forward", hidden_states, top_k_weights, gate_up_proj, down_proj)
     x = hidden_states.to(torch.bfloat16)
-    if few._unseen(x, top_k_index, top_k_weights, *bank):
+    if few._unseen(x, top_k_index, top_k_weights, *few._tensors4(gate_up_proj, down_proj)):
         out = ops.experts4(x, top_k_index, top_k_weights, gate_up_proj, down_proj)
     else:
+        bank, *_ = ops.packed_bank("experts_forward", x, gate_up_proj, down_proj)
+        if top_k_index.dim() != 2 or top_k_index.shape != top_k_weights.shape \
+                or top_k_index.shape[0] != x.shape[0]:
+            raise ValueError("top_k_index / top_k_weights must both be [T, K]")
         out = torch.ops.moe_amd.experts_fwd4(x, top_k_index, top_k_weights, *bank)
     return out.to(hidden_states.dtype)
 
