@@ -2,9 +2,9 @@
 // only, bf16 rows: the routed rows of each expert, as the permutation sorted
 // them, times its packed weights (pack4.h).
 //
-//   gemm4_kernel<BR, true, NW>   act [S,I] = silu(x Wg^T) * (x Wu^T), x gathered by token
-//   gemm4_kernel<BR, false, NW>  y [S,H] = act W2^T, in 16-bit blocks
-//   combine16_kernel             out [T,H] = sum_k w[t,k] y[row of (t,k)]
+//   gemm4_kernel<.., GATE = true>   act [S,I] = silu(x Wg^T) * (x Wu^T), x gathered by token
+//   gemm4_kernel<.., GATE = false>  y [S,H] = act W2^T, in 16-bit blocks
+//   combine16_kernel                out [T,H] = sum_k w[t,k] y[row of (t,k)]
 //
 // A workgroup of NW waves owns BR rows by 64 NW weight rows (gate and up: 32 NW
 // features of each), a wave all its rows by 64 weight rows of its own.  So no weight
@@ -109,8 +109,8 @@ __device__ __forceinline__ void with_sub_tiles(int nj, F&& f, G&& g) {
 // Waves a SIMD: 64 rows leave the registers and the LDS for three.
 template <int BR> constexpr int kWavesSimd = BR <= 64 ? 3 : 2;
 
-// NW waves, each with 64 weight rows of its own.
-template <int BR, bool GATE, int NW>
+// NW waves, each with 64 weight rows of its own; STREAM: weights by non-temporal loads.
+template <int BR, bool GATE, int NW, bool STREAM>
 __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Args p) {
   constexpr int TJ = BR / 32;              // row sub-tiles, all of them every wave's
   constexpr int RPW = BR / 8 / NW;         // 1 KB DMA blocks of a stage's rows per wave
@@ -207,7 +207,8 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
     const auto rs = make_rsrc(qptr + adv, __builtin_amdgcn_readfirstlane(s < nk ? ebytes - adv : 0u));
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      w[c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, qoff[c], 0, 0));
+      w[c] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, qoff[c], 0,
+                                                                          STREAM ? 2 : 0));
   };
   auto issue_scales = [&](int pr, uint32_t (&w)[2]) {
     const uint32_t adv = (uint32_t)pr * kPack4S;
@@ -659,7 +660,7 @@ int check4(int64_t S, int E, int H, int I, const char* who) {
   return MOE_OK;
 }
 
-template <int BR, bool GATE, int NW>
+template <int BR, bool GATE, int NW, bool STREAM>
 int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStream_t st,
             const char* who) {
   static_assert(kTileSizes[0] == 64 && kTileSizes[1] == 128, "the plan's row tiles");
@@ -673,13 +674,13 @@ int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStr
   // the ring of rows, and two halves of 32 rows or a part for each wave and the scales
   constexpr int lds = NSLOT * kSlot<BR> + (GATE ? 2 * 32 * OUT * 2 : NW * 4096 + BR * NW);
   static std::atomic<int> done[64];
-  const hipError_t err = set_dynamic_lds_once(done, (const void*)gemm4_kernel<BR, GATE, NW>, lds);
+  const hipError_t err = set_dynamic_lds_once(done, (const void*)gemm4_kernel<BR, GATE, NW, STREAM>, lds);
   MOE_REQUIRE(err == hipSuccess, MOE_ERR_HIP, "%s: HIP error %d (%s)", who, (int)err,
               hipGetErrorString(err));
   int64_t grid = (int64_t)num_cus() / 8 * 8 * (kWavesSimd<BR> * 4 / NW);
   if (grid > (most + 7) / 8 * 8) grid = (most + 7) / 8 * 8;
   if (grid < 8) grid = 8;
-  gemm4_kernel<BR, GATE, NW><<<(int)grid, 64 * NW, lds, st>>>(a);
+  gemm4_kernel<BR, GATE, NW, STREAM><<<(int)grid, 64 * NW, lds, st>>>(a);
   return check_launch(who);
 }
 
@@ -696,12 +697,18 @@ int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStr
 // 26.2 and 15.6; 8192 on 64, top 4, I 512, 1280 columns: 58.9 and 49.3).
 // Few rows take half the registers, so that three workgroups share a CU where two do
 // of many, which read the weights half as often.
+// Few rows stream the codes of a bank that the memory-side cache cannot hold: 2048
+// tokens on 1792 experts 517 and 309 us become 480 and 297, while with 300 on 128 the
+// same bank's next call takes 45 and 26 us where it finds a part of it there in 41 and 23.
+constexpr int64_t kMemoryCache = 256ll << 20;
 template <bool GATE>
 int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, hipStream_t st, const char* who) {
   const int quarters = (a.N + 255) / 256;
   if (S / E >= 40 && (GATE || quarters % 2 == 0 || quarters >= 9))
-    return launch4<128, GATE, GATE ? 4 : 8>(a, S, E, tile_plan, 1, st, who);
-  return launch4<64, GATE, 4>(a, S, E, tile_plan, 0, st, who);
+    return launch4<128, GATE, GATE ? 4 : 8, false>(a, S, E, tile_plan, 1, st, who);
+  if (S / E < 40 && (int64_t)E * a.nt * a.kt * kPack4Q > kMemoryCache)
+    return launch4<64, GATE, 4, true>(a, S, E, tile_plan, 0, st, who);
+  return launch4<64, GATE, 4, false>(a, S, E, tile_plan, 0, st, who);
 }
 
 // moe_amd_experts4's workspace: each array 256-byte aligned.
