@@ -4,6 +4,7 @@ Public API:
   experts_forward(hidden_states, top_k_index, top_k_weights, gate_up_proj, down_proj)
   mi355x_experts_forward(self, hidden_states, top_k_index, top_k_weights)   # ExpertsInterface
   few.moe_layer_few / few.experts_forward_few                                 # a few tokens, forward
+  ops.pack4 / hf.pack_experts: expert banks in 4 bits, which the three above take, forward
   MI355XTopKRouter / MI355XDeepSeekRouter                                     # router modules
   hf.register() / hf.install(model)                                           # transformers hook
   ops.*                                                                       # one wrapper per C entry

@@ -19,8 +19,8 @@
 // item ahead; nothing that a step waits for is asked for behind them, since loads
 // complete in order.
 //
-// H = 2048, E = 128, K = 8, I = 768: 22 us for one token, 76 for 64 (gate/up 5.9 TB/s,
-// down 4.6); E = 1792: 184 us (7.1 and 6.1 TB/s).  few.hip: 23, 215 and 620.
+// H = 2048, E = 128, K = 8, I = 768: 22 us for one token, 75 for 64 (gate/up 5.8 TB/s,
+// down 4.4); E = 1792: 183 us (6.5 and 5.6 TB/s).  few.hip: 23, 215 and 620.
 //
 // Sums are fp32; act is rounded to bf16, the next product's operand type, once
 // (not at all for a token or two); y and the routing weights stay fp32 and each

@@ -33,12 +33,12 @@
 // Measured (gate/up, down, combine; H 2048, I 768, top 8 of 128 experts):
 //   16384 tokens  645 us (1.28 PF), 350 us (1.18 PF), 107 us (5.6 TB/s); a plain bf16
 //                 product reaches 1.4 to 1.6 PF on this card: bound by the matrix
-//                 units.  Without epilogues 600 and 310 us; the rest are the
+//                 units.  The epilogues are 8% and 19% of that; the rest are the
 //                 conversions' issue slots and each expert's last, partial tile
 //    1021 tokens  60 us, 38 us, 9 us: 320 MB of weights and 64 rows an expert, so
 //                 that both bounds are near (3.6 TB/s, 0.86 PF)
-// and 2048 tokens on 1792 experts (9 rows each): 515 us, 308 us, 15 us, bound by the
-// 4.5 GB of weights (5.8 and 4.9 TB/s).
+// and 2048 tokens on 1792 experts (9 rows each): 480 us, 298 us, 15 us, bound by the
+// 4.5 GB of weights (6.2 and 5.0 TB/s).
 //
 // Reference: transformers/integrations/moe.py:377-478.
 #include "common.h"
