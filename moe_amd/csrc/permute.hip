@@ -5,18 +5,15 @@
 // All of it is latency: a few MB move, and every launch costs about 5 us in
 // the chain.  So there are two forms.
 //
-// Small (S <= kSmallRows, LDS for the counters and ids): one launch of three
-// workgroups that share nothing.  Each counts the ids itself (16 waves, one
-// contiguous run of entries each, LDS counters per wave and expert); then
-// block 0 scans them into offsets and scatters within LDS, block 1 writes the
-// tile tables, block 2 the dW schedule.  6 us at S = 32 and 8 us at S = 2664,
-// where seven launches (a fill, histogram, two scans, tables, schedule,
-// scatter) took 21 and 26; past kSmallRows the one workgroup's scatter is
-// slower than the general form's many (S = 32760: 50 us against 18 us with
-// scattered stores from one workgroup).
+// Small (S <= kSmallRows, LDS for the counters): one launch of workgroups that share
+// nothing.  Each counts all ids itself (LDS counters); then block 0 writes the tile
+// tables, block 1 the dW schedule, and the others scan the counts into offsets and
+// scatter 1024 entries each.  E = 128: 5 us at S = 32, 7 at 8168 (11.5 with the scatter in
+// one workgroup), 8 to 9 at 16384, where the general form's kernels take 13.5; past it
+// counting all ids in every workgroup costs more than two launches (S = 32768: 10.5 to
+// 19.5 us by E and skew).  E = 1792: 8, 10 and 11 us, the general form 26.
 //
-// General, three launches (23 us at S = 524288, E = 128, where seven took 41;
-// 18 against 35 us at S = 32760):
+// General, three launches (23 us at S = 524288, E = 128, where seven took 41):
 //   hist        one wave per 256-entry chunk, LDS atomics -> per-chunk
 //               counts, stored expert-major [E+1][nchunks]
 //   scan        per-expert exclusive scan over chunks (one block per expert)
@@ -406,10 +403,11 @@ __global__ __launch_bounds__(64 * kWaves) void tail_kernel(
   }
 }
 
-// The small form: 3 blocks of 1024 threads, see the head of the file.  LDS:
-// counters [waves][E+1] ((w, e) at w * (E + 1) + e), totals / offsets [E+1],
-// the sorted rows [S] and the entries' bins [S] (16 bits: E < 65536).
+// The small form: 2 blocks and one for each 1024 entries, of 1024 threads, see the head of
+// the file.  LDS: counters [E+1] of all entries and, for the scatter, of those before the
+// block's and of its waves' ((w, e) at w * (E + 1) + e).
 constexpr int kSmallWaves = 16;
+constexpr int kSmallChunk = 64 * kSmallWaves;
 __global__ __launch_bounds__(1024) void small_kernel(
     const int64_t* __restrict__ ids, int S, int E, int* __restrict__ counts,
     int* __restrict__ offsets, int* __restrict__ row_src, int* __restrict__ slot,
@@ -419,28 +417,27 @@ __global__ __launch_bounds__(1024) void small_kernel(
   __shared__ int tmp[17];
   __shared__ int sched_scratch[64 + 1024];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = E + 1;
-  const int rows = blockIdx.x == 0 ? kSmallWaves : 1;
+  const int chunk = (int)blockIdx.x - 2, first = chunk * kSmallChunk;
+  const int rows = chunk >= 0 ? kSmallWaves + 2 : 1;
   for (int i = tid; i < rows * n; i += 1024) lds[i] = 0;
   __syncthreads();
-  int* const tot = lds + kSmallWaves * n;
-  int* const sorted = tot + n;
-  uint16_t* const bins = (uint16_t*)(sorted + S);
-  // each wave's contiguous run of entries, a multiple of 64
-  const int per = (S + kSmallWaves * 64 - 1) / (kSmallWaves * 64) * 64;
-  const int beg = min(wid * per, S), end = min(beg + per, S);
-  int* const mine = blockIdx.x == 0 ? lds + wid * n : lds;
+  int* const pre = lds + n;
+  int* const mine = lds + (2 + wid) * n;
+  int own = -1;  // the bin of the block's entry first + tid
 #pragma unroll 4
-  for (int s = beg + lane; s < end; s += 64) {
+  for (int s = tid; s < S; s += 1024) {
     const int key = bin_of(ids[s], E);
-    atomicAdd(&mine[key], 1);
-    if (blockIdx.x == 0) bins[s] = (uint16_t)key;
+    atomicAdd(&lds[key], 1);
+    if (chunk >= 0 && s < first) atomicAdd(&pre[key], 1);
+    if (s - tid == first) own = key;
   }
+  if (chunk >= 0 && own >= 0) atomicAdd(&mine[own], 1);
   __syncthreads();
-  if (blockIdx.x == 2) {
+  if (blockIdx.x == 1) {
     dw_schedule<1024>([&](int e) { return lds[e]; }, E, sched, sched_scratch);
     return;
   }
-  if (blockIdx.x == 1) {
+  if (blockIdx.x == 0) {
     int carry[1 + MOE_NUM_TILE_SIZES] = {0, 0, 0, 0};
     for (int base = 0; base <= E; base += 1024) {
       const int e = base + tid;
@@ -469,46 +466,35 @@ __global__ __launch_bounds__(1024) void small_kernel(
     }
     return;
   }
-  // block 0: each bin's exclusive scan over the waves
-  for (int e = tid; e < n; e += 1024) {
-    int acc = 0;
-#pragma unroll
-    for (int w = 0; w < kSmallWaves; ++w) {
-      const int c = lds[w * n + e];
-      lds[w * n + e] = acc;
-      acc += c;
-    }
-    tot[e] = acc;
-  }
-  __syncthreads();
+  // each bin's first row of each wave
   int carry = 0;
   for (int base = 0; base < n; base += 1024) {
     const int e = base + tid;
-    const int c = e < n ? tot[e] : 0;
+    const int c = e < n ? lds[e] : 0;
     int t;
     const int ex = carry + block_excl_scan(c, tmp, &t);
     carry += t;
     if (e < n) {
-      offsets[e] = ex;
-      tot[e] = ex;
-      if (e < E) counts[e] = c;
+      int at = ex + pre[e];
+#pragma unroll
+      for (int w = 0; w < kSmallWaves; ++w) {
+        const int of = lds[(2 + w) * n + e];
+        lds[(2 + w) * n + e] = at;
+        at += of;
+      }
+      if (chunk == 0) {
+        offsets[e] = ex;
+        if (e < E) counts[e] = c;
+      }
     }
   }
   __syncthreads();
-  const int key_bits = bits_of(E);
-  for (int at = beg; at < end; at += 64) {
-    const int s = at + lane;
-    const bool valid = s < end;
-    const int key = valid ? bins[s] : -1;
-    const int pos = place64(key, valid, key_bits, lane, mine);
-    if (valid) {
-      const int dest = tot[key] + pos;
-      sorted[dest] = s;
-      slot[s] = dest;
-    }
+  const int s = first + tid;
+  const int dest = place64(own, own >= 0, bits_of(E), lane, mine);
+  if (own >= 0) {
+    row_src[dest] = s;
+    slot[s] = dest;
   }
-  __syncthreads();
-  for (int s = tid; s < S; s += 1024) row_src[s] = sorted[s];
 }
 
 // LDS that tail_kernel needs whatever E: the schedule's scratch, the segment
@@ -516,11 +502,9 @@ __global__ __launch_bounds__(1024) void small_kernel(
 constexpr size_t kTailScratch = 512 * sizeof(int);
 
 // Rows up to which the small form is taken, and the LDS it needs.
-constexpr int kSmallRows = 8192;
+constexpr int kSmallRows = 16384;
 constexpr int kSmallLds = 152 * 1024;
-size_t small_lds(int64_t S, int E) {
-  return (size_t)(kSmallWaves + 1) * (E + 1) * sizeof(int) + (size_t)S * 6;
-}
+size_t small_lds(int E) { return (size_t)(kSmallWaves + 2) * (E + 1) * sizeof(int); }
 
 size_t permute_ws_bytes(int64_t S, int E) {
   int64_t nch = (S + kChunk - 1) / kChunk;
@@ -572,12 +556,13 @@ int permute_run(const int64_t* topk_index, int64_t S, int E, void* workspace,
   int4* const info1 = (int4*)(pb + plan_info_offset(S, E, 1));
   int4* const info2 = (int4*)(pb + plan_info_offset(S, E, 2));
   int* sched = (int*)(pb + plan_sched_offset(S, E));
-  if (S <= kSmallRows && small_lds(S, E) <= kSmallLds) {
+  if (S <= kSmallRows && small_lds(E) <= kSmallLds) {
     static std::atomic<int> lds_done[64];
     hipError_t err = set_dynamic_lds_once(lds_done, (const void*)small_kernel, kSmallLds);
     MOE_REQUIRE(err == hipSuccess, MOE_ERR_HIP, "%s: hipFuncSetAttribute failed: %s", who,
                 hipGetErrorString(err));
-    small_kernel<<<3, 1024, small_lds(S, E), st>>>(topk_index, (int)S, E, counts, offsets, row_src,
+    const int blocks = S == 0 ? 1 : (int)((S + kSmallChunk - 1) / kSmallChunk);
+    small_kernel<<<2 + blocks, 1024, small_lds(E), st>>>(topk_index, (int)S, E, counts, offsets, row_src,
                                                    slot, tile_starts, info0, info1, info2, sched);
     return check_launch(who);
   }
