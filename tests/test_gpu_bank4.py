@@ -423,3 +423,25 @@ def test_banks_past_four_gigabytes():
     last = ops.Packed4(b1.q[E - 1:], b1.scale[E - 1:], (1, 2 * I, H), BF)
     whole = ops.unpack4(ops.Packed4(b1.q, b1.scale, b1.shape, BF))
     assert torch.equal(whole[E - 1:], ops.unpack4(last))
+
+
+@pytest.mark.parametrize("T", [1, 3, 40])
+def test_masked_places_hold_anything(T):
+    """Ids far outside [0, E), NaN and infinite weights beside them, and hidden states that
+    are not finite in a token without experts."""
+    g = _gen(15)
+    E, H, I, K = 9, 128, 192, 4
+    b1, b2 = _bank(g, E, H, I)
+    x = _x(g, T + 1, H)
+    idx = torch.randint(0, E, (T + 1, K), generator=g, device=DEV)
+    w = torch.rand(T + 1, K, generator=g, device=DEV)
+    idx[:, 1], w[:, 1] = (1 << 33) + 2, torch.nan
+    idx[0, 2], w[0, 2] = -(1 << 40), torch.inf
+    idx[T], x[T] = E, torch.nan
+    clean = torch.where((idx >= 0) & (idx < E), w, torch.zeros_like(w))
+    for fn, blocks in ((experts_forward, True), (few.experts_forward_few, False)):
+        out = fn(x, idx, w, b1, b2)
+        assert (out[T] == 0).all()
+        _close(out[:T], *_oracle(x[:T], idx[:T], clean[:T], b1, b2, blocks=blocks))
+        one = fn(x[:1], idx[:1], w[:1], b1, b2)
+        _close(one, *_oracle(x[:1], idx[:1], clean[:1], b1, b2, blocks=blocks))
