@@ -445,3 +445,44 @@ def test_masked_places_hold_anything(T):
         _close(out[:T], *_oracle(x[:T], idx[:T], clean[:T], b1, b2, blocks=blocks))
         one = fn(x[:1], idx[:1], w[:1], b1, b2)
         _close(one, *_oracle(x[:1], idx[:1], clean[:1], b1, b2, blocks=blocks))
+
+
+def test_as_many_tokens_as_are_taken():
+    """The most tokens of 2048 columns, y beyond 2^32 bytes: some of them give the bits
+    that they give alone; one token more is refused."""
+    g = _gen(16)
+    T, H, E, K, I = (1 << 19) - 1, 2048, 4, 3, 64
+    b1, b2 = _bank(g, E, H, I)
+    x = _x(g, T, H)
+    idx = torch.randint(-1, E, (T, K), generator=g, device=DEV)
+    w = torch.rand(T, K, generator=g, device=DEV)
+    out = experts_forward(x, idx, w, b1, b2)
+    some = torch.cat([torch.arange(0, T, 4099, device=DEV), torch.arange(T - 70, T, device=DEV)])
+    assert torch.equal(out[some], experts_forward(x[some], idx[some], w[some], b1, b2))
+    _close(out[some[-70:]], *_oracle(x[some[-70:]], idx[some[-70:]], w[some[-70:]], b1, b2,
+                                     blocks=True))
+    del out, x
+    with pytest.raises(RuntimeError, match="T.H too large"):
+        experts_forward(torch.zeros(T + 1, H, device=DEV, dtype=BF), idx[:1].expand(T + 1, K),
+                        w[:1].expand(T + 1, K), b1, b2)
+
+
+def test_calls_that_overlap():
+    """Prompts and tokens on the same bank from two streams at once."""
+    g = _gen(17)
+    H, E, K, I = 512, 32, 4, 256
+    b1, b2 = _bank(g, E, H, I)
+    sets = [(_x(g, T, H), *_routing(g, T, E, K)) for T in (2000, 1500)]
+    ref = [(experts_forward(*s, b1, b2), few.experts_forward_few(*(t[:50] for t in s), b1, b2))
+           for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(8):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append((experts_forward(*sets[i], b1, b2),
+                               few.experts_forward_few(*(t[:50] for t in sets[i]), b1, b2)))
+    torch.cuda.synchronize()
+    for r, outs in zip(ref, got):
+        assert all(torch.equal(a, b) for o in outs for a, b in zip(o, r))
