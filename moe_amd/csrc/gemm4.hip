@@ -31,13 +31,13 @@
 // NaN whole.  Each output is rounded once.
 //
 // Measured (gate/up, down, combine; H 2048, I 768, top 8 of 128 experts):
-//   16384 tokens  645 us (1.28 PF), 350 us (1.18 PF), 107 us (5.6 TB/s); a plain bf16
+//   16384 tokens  645 us (1.28 PF), 350 us (1.18 PF), 100 us (6.0 TB/s); a plain bf16
 //                 product reaches 1.4 to 1.6 PF on this card: bound by the matrix
 //                 units.  The epilogues are 8% and 19% of that; the rest are the
 //                 conversions' issue slots and each expert's last, partial tile
 //    1021 tokens  60 us, 38 us, 9 us: 320 MB of weights and 64 rows an expert, so
 //                 that both bounds are near (3.6 TB/s, 0.86 PF)
-// and 2048 tokens on 1792 experts (9 rows each): 480 us, 298 us, 15 us, bound by the
+// and 2048 tokens on 1792 experts (9 rows each): 480 us, 298 us, 14 us, bound by the
 // 4.5 GB of weights (6.2 and 5.0 TB/s).
 //
 // Reference: transformers/integrations/moe.py:377-478.
@@ -74,6 +74,11 @@ struct Gemm4Args {
 };
 
 constexpr uint32_t kOOB = 0x80000000u;  // offset that always reads as zero
+// act and y are written through the L2 (cache bits sc0 and sc1): their lines are not
+// evicted among the weights' later, and the next launch finds more of them in the
+// memory-side cache (combine of 16384 tokens 108 -> 99.5 us, 2048 tokens on 1792 experts
+// 808 -> 798 us in all, against non-temporal stores; plain ones 101 and 804).
+constexpr int kThrough = 17;
 typedef __attribute__((address_space(3))) void lds_void_t;
 typedef __attribute__((address_space(3))) char lds_char_t;
 
@@ -433,7 +438,7 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
           const u32x4 v = *(const lds_u32x4_t*)lds_at(buf + row * LINE + ((ch ^ (row & 15)) << 4));
           __builtin_amdgcn_raw_buffer_store_b128(
               v, rs, col < p.N ? (uint32_t)(r * 32 + row) * (uint32_t)p.N * 2 + (uint32_t)col * 2 : kOOB,
-              0, 2);
+              0, kThrough);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -479,7 +484,8 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
             const int row = h * 8 + (ln >> 3), ch = ln & 7;
             const u32x4 v = *(const lds_u32x4_t*)lds_at(mine + row * 128 + ((ch ^ (row & 7)) << 4));
             __builtin_amdgcn_raw_buffer_store_b128(
-                v, rs, (uint32_t)(r * 32 + row) * (uint32_t)p.N * 2 + (uint32_t)(f0 + ch * 8) * 2, 0, 2);
+                v, rs, (uint32_t)(r * 32 + row) * (uint32_t)p.N * 2 + (uint32_t)(f0 + ch * 8) * 2, 0,
+                kThrough);
           }
           turn();
           __builtin_amdgcn_sched_barrier(0);
