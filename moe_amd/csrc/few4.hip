@@ -23,8 +23,8 @@
 // down 4.4); E = 1792: 183 us (6.5 and 5.6 TB/s).  few.hip: 23, 215 and 620.
 //
 // Sums are fp32; act is rounded to bf16, the next product's operand type, once
-// (not at all for a token or two); y and the routing weights stay fp32 and each
-// output is rounded once.  Partial sums are added in a fixed order, so results do
+// (not at all for up to 16 rows of 12288 values together: kSmallRows, kSmallValues); y
+// and the routing weights stay fp32 and each output is rounded once.  Partial sums are added in a fixed order, so results do
 // not depend on timing.
 //
 // Reference: src/models/modeling_qwen3_moe.py:266-289, src/models/router.py:103-152,
@@ -310,6 +310,14 @@ constexpr int kSmallWaves = 16;
 constexpr int kSmallRows = 16;
 constexpr int kSmallTiles = 3;
 constexpr int kSmallValues = 12288;  // of all rows
+// v as a + r, both bf16 values once r is rounded: a the nearest one, or where that is
+// infinite and v is not, the one next to v towards 0.  Where v is not finite, a alone
+// (inf - inf would be NaN).
+__device__ __forceinline__ void two_terms(float v, float& a, float& r) {
+  a = round_bf(v);
+  if (!(__builtin_fabsf(a) < INFINITY)) a = __uint_as_float(__float_as_uint(v) & 0xffff0000u);
+  r = __builtin_fabsf(a) < INFINITY ? v - a : 0.f;
+}
 __global__ __launch_bounds__(64 * kSmallWaves) void few4_down_small_kernel(Few4Args p) {
   __shared__ __attribute__((aligned(16))) bf16 s_act[2][kSmallValues];  // the two terms
   __shared__ float s_y[2][kSmallRows][16];
@@ -336,10 +344,11 @@ __global__ __launch_bounds__(64 * kSmallWaves) void few4_down_small_kernel(Few4A
   __builtin_amdgcn_sched_barrier(0);
   for (int i = tid; i < S * f.I / 4; i += 64 * kSmallWaves) {
     const f32x4 v = ((const f32x4*)f.act)[i];
-    const uint32_t a = pack_bf2(v[0], v[1]), b = pack_bf2(v[2], v[3]);
-    *(u32x2*)&s_act[0][i * 4] = u32x2{a, b};
-    *(u32x2*)&s_act[1][i * 4] = u32x2{pack_bf2(v[0] - bf_lo(a), v[1] - bf_hi(a)),
-                                      pack_bf2(v[2] - bf_lo(b), v[3] - bf_hi(b))};
+    float a[4], r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) two_terms(v[j], a[j], r[j]);
+    *(u32x2*)&s_act[0][i * 4] = u32x2{pack_bf2(a[0], a[1]), pack_bf2(a[2], a[3])};
+    *(u32x2*)&s_act[1][i * 4] = u32x2{pack_bf2(r[0], r[1]), pack_bf2(r[2], r[3])};
   }
   if (tid < S) {
     s_w[tid] = my_w;
