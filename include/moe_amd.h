@@ -462,10 +462,10 @@ int moe_amd_unpack4(const void* q, const void* scale, int64_t batch, int64_t n, 
  * moe_amd_gemm_gate_up_swiglu and moe_amd_gemm_down with gate_up_proj
  * [E,2I,H] and down_proj [E,H,I] as moe_amd_pack4 leaves them (batch = E), and the
  * combine of what they give.  act_out [S,I] = bf16(silu(gate) * up), gate and up in
- * fp32; y_out int16 [S,H] with a byte for 64 columns of a row in y_scale_out
- * [S,H/64]: y = y_out * 2^(byte - 127), within half of that power, which is at
- * most 2^-14 of the block's largest value (255: a value is not finite, NaN whole);
- * out [T,H] bf16, sums in fp32.  Sentinel rows are not written and contribute
+ * fp32; y_out fp16 [S,H] with a byte for 64 columns of a row in y_scale_out
+ * [S,H/64]: y = y_out * 2^(byte - 127), within 2^-11 of each value down to 2^-28 of the
+ * block's largest finite one, and within 2^-39 of that below; out [T,H] bf16, sums in
+ * fp32.  Sentinel rows are not written and contribute
  * nothing.  H and I multiples of 64, S < 2^29, T H 2 < 2^31, an expert's codes
  * below 2 GB; codes and scales 16-byte aligned. */
 int moe_amd_gemm_gate_up_swiglu4(const void* hidden_states, const int32_t* row_src, int top_k,

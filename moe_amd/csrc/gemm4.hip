@@ -3,7 +3,7 @@
 // them, times its packed weights (pack4.h).
 //
 //   gemm4_kernel<.., GATE = true>   act [S,I] = silu(x Wg^T) * (x Wu^T), x gathered by token
-//   gemm4_kernel<.., GATE = false>  y [S,H] = act W2^T, in 16-bit blocks
+//   gemm4_kernel<.., GATE = false>  y [S,H] = act W2^T, fp16 in blocks of 64 columns
 //   combine16_kernel                out [T,H] = sum_k w[t,k] y[row of (t,k)]
 //
 // A workgroup of NW waves owns BR rows by 64 NW weight rows (gate and up: 32 NW
@@ -24,11 +24,13 @@
 // from empty descriptors (zeros, no memory access), so that the wait counts hold in
 // every stage.
 //
-// act is rounded to bf16 once.  y is held in 16 bits a value with a power of two for
-// 64 columns of a row: as small as bf16, but within 2^-15 of the block's largest
-// value instead of 2^-9 of each (three roundings of bf16 size in a row would
-// show: 1.7 times the error of one); a block with a value that is not finite is
-// NaN whole.  Each output is rounded once.
+// act is rounded to bf16 once.  y is held in fp16 with a power of two for 64 columns of
+// a row, which puts the largest finite one at 2^14 or above: as small as bf16, but within
+// 2^-11 of each value instead of 2^-8 (three roundings of bf16 size in a row would
+// show: 1.7 times the error of one) down to 2^-28 of the largest, and within 2^-39 of the
+// largest below that.  (As whole numbers of the power of two, within 2^-15 of the
+// largest, a column 2^12 times its neighbours leaves those 5e-2 off.)  Each output is
+// rounded once.
 //
 // Measured (gate/up, down, combine; H 2048, I 768, top 8 of 128 experts):
 //   16384 tokens  645 us (1.28 PF), 350 us (1.18 PF), 100 us (6.0 TB/s); a plain bf16
@@ -53,6 +55,8 @@ constexpr int kBlock16 = 64;  // columns of a block of y
 constexpr int kMostColumns = 1 << 22;
 
 template <int BR> constexpr int kSlot = BR * BK * 2;  // bytes
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 struct Gemm4Args {
   const bf16* x;         // hidden states [T,H] (gate/up) or act [S,I]
@@ -61,7 +65,7 @@ struct Gemm4Args {
   const int* tile_count; // row tiles
   const int4* tile_info; // {expert, first row, end row, 0} of each
   bf16* act;             // [S,I]
-  int16_t* y;            // [S,H] and its scale bytes [S,H/64]
+  _Float16* y;           // [S,H] and its scale bytes [S,H/64]
   uint8_t* ys;
   int64_t T;
   int K;                 // contraction
@@ -93,13 +97,11 @@ __device__ __forceinline__ float fast_sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896341f));
 }
 
-// The biased exponent of a block's power of two from its largest |v|: rint(v / 2^k) is
-// within 32767 (a mantissa from 0x7fff00 on would round to 2^15: the addition carries).
-// 255: a value is not finite.
+// The biased exponent of a block's power of two from its largest finite |v|, which is
+// from 2^14 to 2^15 of it, and of fp16's range once rounded.
 __device__ __forceinline__ uint32_t block16_scale(float most) {
-  const uint32_t bits = __float_as_uint(most) & 0x7fffffffu;
-  const int e = (int)((bits + 0x100u) >> 23) - 14;
-  return bits >= 0x7f800000u ? 255u : (uint32_t)(e < 1 ? 1 : e);
+  const int e = (int)(__float_as_uint(most) >> 23) - 14;
+  return (uint32_t)(e < 1 ? 1 : e);
 }
 
 // f(integral_constant<int, nj>, g): a main loop for each number of row sub-tiles.
@@ -450,30 +452,42 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
 #pragma unroll
         for (int r = 0; r < TJ; ++r) {
           if (r >= nj) break;
+          const auto row_most = [](float m) {  // of both lanes of a row
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m),
+                                                               false, false);
+            return __builtin_elementwise_maximum(__uint_as_float(both[0]), __uint_as_float(both[1]));
+          };
           float m = 0.f;  // (maximum: NaN if any is)
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               m = __builtin_elementwise_maximum(m, __builtin_fabsf(acc[c][r][i]));
-          const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m),
-                                                             false, false);
-          m = __builtin_elementwise_maximum(__uint_as_float(both[0]), __uint_as_float(both[1]));
+          m = row_most(m);
+          if (__builtin_amdgcn_ballot_w64(!(m < INFINITY))) {  // of those that are finite
+            m = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float a = __builtin_fabsf(acc[c][r][i]);
+                m = a < INFINITY && a > m ? a : m;
+              }
+            m = row_most(m);
+          }
           const uint32_t sb = block16_scale(m);
-          const float inv = __uint_as_float((254u - sb) << 23);  // of 255: anything
+          const float inv = __uint_as_float((254u - sb) << 23);
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              // adding 1.5 2^23 rounds to an integer, halves to even, whose two's
-              // complement ends the sum's bits
-              uint32_t v[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                v[i] = __float_as_uint(__builtin_fmaf(acc[c][r][4 * q + i], inv, 12582912.f));
+              const auto two = [&](int i) {
+                const f16x2 v = {(_Float16)(acc[c][r][4 * q + i] * inv),
+                                 (_Float16)(acc[c][r][4 * q + i + 1] * inv)};
+                return __builtin_bit_cast(uint32_t, v);
+              };
               *(lds_u32x2_t*)lds_at(mine + el32 * 128 + (((c * 4 + q) ^ (el32 & 7)) << 4) + ehl * 8) =
-                  u32x2{__builtin_amdgcn_perm(v[1], v[0], 0x05040100u),
-                        __builtin_amdgcn_perm(v[3], v[2], 0x05040100u)};
+                  u32x2{two(0), two(2)};
             }
           if (ehl == 0)
             *(__attribute__((address_space(3))) uint8_t*)lds_at(scales + (r * 32 + el32) * NW + wd) =
@@ -569,7 +583,7 @@ __global__ __launch_bounds__(64 * NW, kWavesSimd<BR>) void gemm4_kernel(Gemm4Arg
 constexpr int kCombineWaves = 4;
 constexpr int kPieces = 2;
 __global__ __launch_bounds__(64 * kCombineWaves, 4) void combine16_kernel(
-    const int16_t* __restrict__ y, const uint8_t* __restrict__ ys, const int* __restrict__ slot,
+    const _Float16* __restrict__ y, const uint8_t* __restrict__ ys, const int* __restrict__ slot,
     const int* __restrict__ offsets, const void* __restrict__ w, int wdt, int64_t T, int K, int E,
     int H, bf16* __restrict__ out) {
   const int lane = threadIdx.x & 63;
@@ -613,11 +627,10 @@ __global__ __launch_bounds__(64 * kCombineWaves, 4) void combine16_kernel(
             const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wk), k0 + k));
 #pragma unroll
             for (int c = 0; c < kPieces; ++c) {
-              // 255: the block is NaN whole
-              const float s = __uint_as_float(sb[c][k] == 255u ? 0x7fc00000u : sb[c][k] << 23) * f;
+              const float s = __uint_as_float(sb[c][k] << 23) * f;
+              const f16x8 h = __builtin_bit_cast(f16x8, v[c][k]);
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                o[c][i] = fmaf((float)(int16_t)(v[c][k][i >> 1] >> (16 * (i & 1))), s, o[c][i]);
+              for (int i = 0; i < 8; ++i) o[c][i] = fmaf((float)h[i], s, o[c][i]);
             }
           }
         }
@@ -814,7 +827,7 @@ extern "C" int moe_amd_gemm_down4(const void* act, const int32_t* offsets, const
   a.x = (const bf16*)act;
   a.q = (const char*)down_q;
   a.s = (const char*)down_scale;
-  a.y = (int16_t*)y_out;
+  a.y = (_Float16*)y_out;
   a.ys = (uint8_t*)y_scale_out;
   a.K = I;
   a.N = H;
@@ -843,7 +856,7 @@ extern "C" int moe_amd_combine16(const void* y, const void* y_scale, const int32
   const int gy = gx >= 1024 ? 1 : (H + 512 * kPieces - 1) / (512 * kPieces);
   if (gx > 1024) gx = 1024;
   combine16_kernel<<<dim3((unsigned)gx, (unsigned)gy), 64 * kCombineWaves, 0, (hipStream_t)stream>>>(
-      (const int16_t*)y, (const uint8_t*)y_scale, slot, offsets, topk_weights, weights_dtype, T, K, E,
+      (const _Float16*)y, (const uint8_t*)y_scale, slot, offsets, topk_weights, weights_dtype, T, K, E,
       H, (bf16*)out);
   return check_launch(who);
 }

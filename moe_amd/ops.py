@@ -962,8 +962,8 @@ def gemm_gate_up_swiglu4(x: torch.Tensor, plan: RoutingPlan, gate_up_proj: Packe
 @on_tensor_device
 def gemm_down4(act: torch.Tensor, plan: RoutingPlan, down_proj: Packed4
                ) -> tuple[torch.Tensor, torch.Tensor]:
-    """y [S,H] of gemm_down on a bank in 4 bits, in 16-bit blocks: (int16 [S,H],
-    uint8 [S,H/64]), y = int16 * 2^(byte - 127), for combine16."""
+    """y [S,H] of gemm_down on a bank in 4 bits, in blocks of 64 columns: (fp16 [S,H],
+    uint8 [S,H/64]), y = fp16 * 2^(byte - 127), for combine16."""
     name = "gemm_down4"
     _need_cuda(act)
     q, scale = _packed_operand(name, down_proj, act, plan)
@@ -972,7 +972,7 @@ def gemm_down4(act: torch.Tensor, plan: RoutingPlan, down_proj: Packed4
         raise ValueError(f"{name}: act {tuple(act.shape)}, down_proj {tuple(down_proj.shape)}, a "
                          f"plan of {plan.num_rows} rows and {plan.num_experts} experts")
     act = _contig(act)
-    y = torch.empty(plan.num_rows, H, device=act.device, dtype=torch.int16)
+    y = torch.empty(plan.num_rows, H, device=act.device, dtype=torch.float16)
     ys = torch.empty(plan.num_rows, H // 64, device=act.device, dtype=torch.uint8)
     _call("moe_amd_gemm_down4", act.data_ptr(), plan.offsets.data_ptr(), plan.tile_plan.data_ptr(),
           q.data_ptr(), scale.data_ptr(), plan.num_rows, E, H, I, y.data_ptr(), ys.data_ptr(),
@@ -986,7 +986,7 @@ def combine16(y: torch.Tensor, y_scale: torch.Tensor, plan: RoutingPlan,
     """out [T,H] bf16 = sum_k w[t,k] y[row of (t,k)] of gemm_down4's y."""
     _need_cuda(y, y_scale, topk_weights)
     T, K, H = plan.num_tokens, plan.top_k, y.shape[1]
-    if y.dtype != torch.int16 or y_scale.dtype != torch.uint8 or H % 64 \
+    if y.dtype != torch.float16 or y_scale.dtype != torch.uint8 or H % 64 \
             or tuple(y.shape) != (plan.num_rows, H) \
             or tuple(y_scale.shape) != (plan.num_rows, H // 64) \
             or tuple(topk_weights.shape) != (T, K):

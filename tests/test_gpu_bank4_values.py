@@ -1,13 +1,88 @@
-"""The values of the layer on a bank in 4 bits where they are largest."""
+"""The values of the layer on a bank in 4 bits, form by form, in the 2-norm
+(bank4_values has the tolerance and its derivation), and where they are largest."""
 from __future__ import annotations
 
 import pytest
 import torch
 
-from moe_amd import few, ops
+from bank4_values import LIMIT, distance, layer
+from moe_amd import experts_forward, few, ops
+from pack4_oracle import tiles
 
 pytestmark = pytest.mark.gpu
 DEV, BF = "cuda", torch.bfloat16
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+class Bank:
+    """A packed weight, an expert of which indexing gives in 64 bits."""
+
+    def __init__(self, w):
+        self.packed = ops.pack4(w, dtype=BF)
+
+    def __len__(self):
+        return self.packed.shape[0]
+
+    def __getitem__(self, e):
+        p = self.packed
+        return tiles(p.q[e], p.scale[e], p.shape[1:]).to(DEV)
+
+
+def _banks(g, E, H, I):
+    return (Bank(torch.randn(E, 2 * I, H, generator=g, device=DEV) * 0.02),
+            Bank(torch.randn(E, H, I, generator=g, device=DEV) * 0.02))
+
+
+def _inputs(g, T, H, E, K):
+    x = torch.randn(T, H, generator=g, device=DEV, dtype=BF)
+    idx = torch.rand(T, E, generator=g, device=DEV).argsort(1)[:, :K].contiguous()
+    return x, idx, torch.rand(T, K, generator=g, device=DEV) + 0.1
+
+
+@pytest.mark.parametrize("ratio", [2.0 ** 4, 2.0 ** 10, 2.0 ** 12, 2.0 ** 20])
+@pytest.mark.parametrize("T,E", [(40, 2), (300, 2), (300, 16)])
+def test_columns_beside_a_large_one(T, E, ratio):
+    """Output columns far larger than their neighbours: the others keep their exactness
+    (down to 2^-28 of the largest, fp16 holds 2^-11 of a value)."""
+    g = _gen(T)
+    H, I, K = 256, 128, 2
+    b1, _ = _banks(g, E, H, I)
+    w2 = torch.randn(E, H, I, generator=g, device=DEV) * 0.02
+    large = torch.tensor([5, 64, 127, 200], device=DEV)
+    w2[:, large] *= ratio
+    b2 = Bank(w2)
+    x, idx, w = _inputs(g, T, H, E, K)
+    ref = layer(x, idx, w, b1, b2, True)
+    others = torch.ones(H, dtype=torch.bool, device=DEV)
+    others[large] = False
+    fns = [experts_forward] + [few.experts_forward_few] * (T <= 64)
+    for fn in fns:
+        out = fn(x, idx, w, b1.packed, b2.packed)
+        assert distance(out[:, others], ref[:, others]) < LIMIT
+        assert distance(out[:, large], ref[:, large]) < LIMIT
+
+
+@pytest.mark.parametrize("T", [40, 300])
+def test_a_column_that_is_not_finite(T):
+    """Weights of one output column so large that its sums are infinite: its
+    neighbours are what they are without them."""
+    g = _gen(T)
+    E, H, I, K = 2, 128, 64, 1
+    b1 = Bank(torch.rand(E, 2 * I, H, generator=g, device=DEV) * 0.02)
+    w2 = torch.randn(E, H, I, generator=g, device=DEV) * 0.02
+    x, idx, w = _inputs(g, T, H, E, K)
+    clean = ops.pack4(w2, dtype=BF)
+    w2[:, 70] = 2.0 ** 127
+    bad = ops.pack4(w2, dtype=BF)
+    x = x.abs() * 8    # and all acts above 1
+    others = torch.arange(H, device=DEV) != 70
+    for fn in [experts_forward] + [few.experts_forward_few] * (T <= 64):
+        got, ref = (fn(x, idx, w, b1.packed, b) for b in (bad, clean))
+        assert torch.isfinite(ref).all() and torch.isinf(got[:, 70]).all()
+        assert torch.equal(got[:, others], ref[:, others])
 
 
 @pytest.mark.parametrize("T", [1, 2, 16])
