@@ -7,6 +7,7 @@ import torch
 
 from bank4_values import LIMIT, distance, layer
 from moe_amd import experts_forward, few, ops
+from moe_amd.layer import moe_layer
 from pack4_oracle import tiles
 
 pytestmark = pytest.mark.gpu
@@ -40,6 +41,88 @@ def _inputs(g, T, H, E, K):
     x = torch.randn(T, H, generator=g, device=DEV, dtype=BF)
     idx = torch.rand(T, E, generator=g, device=DEV).argsort(1)[:, :K].contiguous()
     return x, idx, torch.rand(T, K, generator=g, device=DEV) + 0.1
+
+
+def _small(T, K, I):
+    """Whether act of a few tokens is not rounded."""
+    return T * K <= 16 and T * K * I <= 12288
+
+
+FEW = [  # T, H, E, K, I
+    (1, 2048, 128, 8, 768), (2, 1024, 16, 8, 768), (1, 8192, 3, 3, 64), (1, 1024, 8, 8, 1600),
+    (3, 2048, 128, 8, 768), (13, 1024, 128, 4, 768), (64, 2048, 128, 8, 768),
+    (20, 4160, 6, 2, 1600), (64, 256, 8, 8, 64),
+]
+
+
+@pytest.mark.parametrize("T,H,E,K,I", FEW)
+def test_few(T, H, E, K, I):
+    g = _gen(T + I)
+    b1, b2 = _banks(g, E, H, I)
+    x, idx, w = _inputs(g, T, H, E, K)
+    out = few.experts_forward_few(x, idx, w, b1.packed, b2.packed)
+    assert distance(out, layer(x, idx, w, b1, b2, not _small(T, K, I))) < LIMIT
+
+
+ROUTERS = [
+    ("softmax", {}), ("softmax", dict(offset=True)), ("softmax", dict(renormalize=False)),
+    ("sigmoid", {}), ("sigmoid", dict(scaling_factor=2.5)),
+    ("sigmoid", dict(num_groups=8, group_topk=4, scaling_factor=1.5)),
+    ("sigmoid", dict(num_groups=16, group_topk=2, renormalize=False)),
+]
+
+
+def _layer_case(router, kw, T, E, H=512, I=128):
+    g = _gen(T + E)
+    b1, b2 = _banks(g, E, H, I)
+    x, wr = (torch.randn(n, H, generator=g, device=DEV, dtype=BF) * s for n, s in ((T, 1), (E, 0.05)))
+    kw, extra = dict(kw, router=router), torch.rand(E, generator=g, device=DEV)
+    if kw.pop("offset", False):
+        kw["logit_offset"] = extra
+    if router == "sigmoid":
+        kw["expert_bias"] = extra * 0.1
+    return x, wr, b1, b2, kw
+
+
+@pytest.mark.parametrize("router,kw", ROUTERS)
+@pytest.mark.parametrize("T", [1, 2, 7, 64])
+@pytest.mark.parametrize("E", [64, 512])
+def test_routers_few(router, kw, T, E):
+    """Offsets, biases, scaling and groups: the routing is the exact bank's, bit for
+    bit, and the experts follow it."""
+    K = 8
+    x, wr, b1, b2, kw = _layer_case(router, kw, T, E)
+    out, w, idx = few.moe_layer_few(x, wr, b1.packed, b2.packed, K, return_routing=True, **kw)
+    _, w0, idx0 = few.moe_layer_few(x, wr, ops.unpack4(b1.packed), ops.unpack4(b2.packed), K,
+                                    return_routing=True, **kw)
+    assert torch.equal(idx, idx0) and torch.equal(w, w0)
+    assert distance(out, layer(x, idx, w, b1, b2, not _small(T, K, 128))) < LIMIT
+
+
+@pytest.mark.parametrize("router,kw", ROUTERS)
+def test_routers(router, kw):
+    x, wr, b1, b2, kw = _layer_case(router, kw, 150, 64)
+    with torch.no_grad():
+        out, probs, w, idx = moe_layer(x, wr, b1.packed, b2.packed, 8, **kw)
+        _, probs0, w0, idx0 = moe_layer(x, wr, ops.unpack4(b1.packed), ops.unpack4(b2.packed), 8,
+                                        **kw)
+    assert torch.equal(idx, idx0) and torch.equal(w, w0) and torch.equal(probs, probs0)
+    assert distance(out, layer(x, idx, w, b1, b2, True)) < LIMIT
+
+
+PROMPT = [  # T, H, E, K, I
+    (509, 1024, 128, 4, 768), (200, 1024, 3, 1, 832), (1021, 2048, 128, 8, 768),
+    (1500, 512, 4, 4, 320), (2050, 576, 16, 8, 256), (70, 128, 1, 1, 64),
+]
+
+
+@pytest.mark.parametrize("T,H,E,K,I", PROMPT)
+def test_prompt(T, H, E, K, I):
+    g = _gen(T + I)
+    b1, b2 = _banks(g, E, H, I)
+    x, idx, w = _inputs(g, T, H, E, K)
+    out = experts_forward(x, idx, w, b1.packed, b2.packed)
+    assert distance(out, layer(x, idx, w, b1, b2, True)) < LIMIT
 
 
 @pytest.mark.parametrize("ratio", [2.0 ** 4, 2.0 ** 10, 2.0 ** 12, 2.0 ** 20])
