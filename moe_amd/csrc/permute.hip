@@ -404,8 +404,8 @@ __global__ __launch_bounds__(64 * kWaves) void tail_kernel(
 }
 
 // The small form: 2 blocks and one for each 1024 entries, of 1024 threads, see the head of
-// the file.  LDS: counters [E+1] of all entries and, for the scatter, of those before the
-// block's and of its waves' ((w, e) at w * (E + 1) + e).
+// the file.  LDS: counters [E+1] of all entries, in the upper halves of the scatter's blocks
+// of those before the block's (S < 2^16), and there its waves' ((w, e) at w * (E + 1) + e).
 constexpr int kSmallWaves = 16;
 constexpr int kSmallChunk = 64 * kSmallWaves;
 __global__ __launch_bounds__(1024) void small_kernel(
@@ -418,17 +418,15 @@ __global__ __launch_bounds__(1024) void small_kernel(
   __shared__ int sched_scratch[64 + 1024];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = E + 1;
   const int chunk = (int)blockIdx.x - 2, first = chunk * kSmallChunk;
-  const int rows = chunk >= 0 ? kSmallWaves + 2 : 1;
+  const int rows = chunk >= 0 ? kSmallWaves + 1 : 1;
   for (int i = tid; i < rows * n; i += 1024) lds[i] = 0;
   __syncthreads();
-  int* const pre = lds + n;
-  int* const mine = lds + (2 + wid) * n;
+  int* const mine = lds + (1 + wid) * n;
   int own = -1;  // the bin of the block's entry first + tid
 #pragma unroll 4
   for (int s = tid; s < S; s += 1024) {
     const int key = bin_of(ids[s], E);
-    atomicAdd(&lds[key], 1);
-    if (chunk >= 0 && s < first) atomicAdd(&pre[key], 1);
+    atomicAdd(&lds[key], s < first ? 0x10001 : 1);
     if (s - tid == first) own = key;
   }
   if (chunk >= 0 && own >= 0) atomicAdd(&mine[own], 1);
@@ -470,16 +468,17 @@ __global__ __launch_bounds__(1024) void small_kernel(
   int carry = 0;
   for (int base = 0; base < n; base += 1024) {
     const int e = base + tid;
-    const int c = e < n ? lds[e] : 0;
+    const uint32_t both = e < n ? (uint32_t)lds[e] : 0u;
+    const int c = (int)(both & 0xffffu);
     int t;
     const int ex = carry + block_excl_scan(c, tmp, &t);
     carry += t;
     if (e < n) {
-      int at = ex + pre[e];
+      int at = ex + (int)(both >> 16);
 #pragma unroll
       for (int w = 0; w < kSmallWaves; ++w) {
-        const int of = lds[(2 + w) * n + e];
-        lds[(2 + w) * n + e] = at;
+        const int of = lds[(1 + w) * n + e];
+        lds[(1 + w) * n + e] = at;
         at += of;
       }
       if (chunk == 0) {
@@ -504,7 +503,8 @@ constexpr size_t kTailScratch = 512 * sizeof(int);
 // Rows up to which the small form is taken, and the LDS it needs.
 constexpr int kSmallRows = 16384;
 constexpr int kSmallLds = 152 * 1024;
-size_t small_lds(int E) { return (size_t)(kSmallWaves + 2) * (E + 1) * sizeof(int); }
+static_assert(kSmallRows < 1 << 16, "counts in half a word");
+size_t small_lds(int E) { return (size_t)(kSmallWaves + 1) * (E + 1) * sizeof(int); }
 
 size_t permute_ws_bytes(int64_t S, int E) {
   int64_t nch = (S + kChunk - 1) / kChunk;
