@@ -8,10 +8,11 @@
 // Small (S <= kSmallRows, LDS for the counters): one launch of workgroups that share
 // nothing.  Each counts all ids itself (LDS counters); then block 0 writes the tile
 // tables, block 1 the dW schedule, and the others scan the counts into offsets and
-// scatter 1024 entries each.  E = 128: 5 us at S = 32, 7 at 8168 (11.5 with the scatter in
-// one workgroup), 8 to 9 at 16384, where the general form's kernels take 13.5; past it
-// counting all ids in every workgroup costs more than two launches (S = 32768: 10.5 to
-// 19.5 us by E and skew).  E = 1792: 8, 10 and 11 us, the general form 26.
+// scatter 1024 entries each.  E = 128: 5 us at S = 32, 6.4 at 8168 (11.5 with the scatter in
+// one workgroup), 8 at 16384, skewed routing up to 10, where the general form's kernels take
+// 13.5; past it counting all ids in every workgroup costs more than two launches.
+// E = 1792: 8, 10 and 11 us, the general form 26.  (Calls one after another, the ids in the
+// L2; 12 us at 8168 and 22 at E = 1792, 16384 between products that fill it.)
 //
 // General, three launches (23 us at S = 524288, E = 128, where seven took 41):
 //   hist        one wave per 256-entry chunk, LDS atomics -> per-chunk
@@ -404,10 +405,12 @@ __global__ __launch_bounds__(64 * kWaves) void tail_kernel(
 }
 
 // The small form: 2 blocks and one for each 1024 entries, of 1024 threads, see the head of
-// the file.  LDS: counters [E+1] of all entries, in the upper halves of the scatter's blocks
+// the file.  MANY: more than kManyRows entries, of which many may be one expert's.  LDS: counters [E+1] of all entries, in the upper halves of the scatter's blocks
 // of those before the block's (S < 2^16), and there its waves' ((w, e) at w * (E + 1) + e).
 constexpr int kSmallWaves = 16;
 constexpr int kSmallChunk = 64 * kSmallWaves;
+constexpr int kOwnRows = 512;  // MANY: an expert's tiles by one thread, of more rows by a wave
+template <bool MANY>
 __global__ __launch_bounds__(1024) void small_kernel(
     const int64_t* __restrict__ ids, int S, int E, int* __restrict__ counts,
     int* __restrict__ offsets, int* __restrict__ row_src, int* __restrict__ slot,
@@ -416,18 +419,54 @@ __global__ __launch_bounds__(1024) void small_kernel(
   extern __shared__ int lds[];
   __shared__ int tmp[17];
   __shared__ int sched_scratch[64 + 1024];
+  __shared__ int n_many;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, n = E + 1;
   const int chunk = (int)blockIdx.x - 2, first = chunk * kSmallChunk;
   const int rows = chunk >= 0 ? kSmallWaves + 1 : 1;
   for (int i = tid; i < rows * n; i += 1024) lds[i] = 0;
+  if (tid == 0) n_many = 0;
   __syncthreads();
   int* const mine = lds + (1 + wid) * n;
   int own = -1;  // the bin of the block's entry first + tid
+  if constexpr (MANY) {
+    // Atomics on one counter take their turns: a bin that more than 24 of a wave's first 64
+    // entries go to (of those that four of them name) is counted by ballots.
+    int hot = -1, of_hot = 0;
+    for (int at0 = wid * 64; at0 < S; at0 += 8 * kSmallChunk) {
+      int key[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int s = at0 + i * kSmallChunk + lane, k = bin_of(ids[min(s, S - 1)], E);
+        key[i] = s < S ? k : -1;
+      }
+      if (at0 == wid * 64) {
+        int votes = 24;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int k = __builtin_amdgcn_readlane(key[0], 16 * q);
+          const int n = __popcll(__ballot(key[0] == k));
+          if (n > votes) {
+            votes = n;
+            hot = k;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = at0 + i * kSmallChunk, one = at < first ? 0x10001 : 1;
+        if (hot >= 0) of_hot += __popcll(__ballot(key[i] == hot)) * one;
+        if (key[i] >= 0 && key[i] != hot) atomicAdd(&lds[key[i]], one);
+        if (at - wid * 64 == first) own = key[i];
+      }
+    }
+    if (of_hot && lane == 0) atomicAdd(&lds[hot], of_hot);
+  } else {
 #pragma unroll 4
-  for (int s = tid; s < S; s += 1024) {
-    const int key = bin_of(ids[s], E);
-    atomicAdd(&lds[key], s < first ? 0x10001 : 1);
-    if (s - tid == first) own = key;
+    for (int s = tid; s < S; s += kSmallChunk) {
+      const int key = bin_of(ids[s], E);
+      atomicAdd(&lds[key], s < first ? 0x10001 : 1);
+      if (s - tid == first) own = key;
+    }
   }
   if (chunk >= 0 && own >= 0) atomicAdd(&mine[own], 1);
   __syncthreads();
@@ -437,19 +476,38 @@ __global__ __launch_bounds__(1024) void small_kernel(
   }
   if (blockIdx.x == 0) {
     int carry[1 + MOE_NUM_TILE_SIZES] = {0, 0, 0, 0};
+    int* const many = sched_scratch;  // experts of more than kOwnRows rows, 6 words each
+    const auto info_of = [&](int b) { return b == 0 ? info0 : (b == 1 ? info1 : info2); };
     for (int base = 0; base <= E; base += 1024) {
       const int e = base + tid;
       const int c = e < E ? lds[e] : 0;
-      int t;
+      int t, t0[MOE_NUM_TILE_SIZES];
       const int r0 = carry[0] + block_excl_scan(c, tmp, &t);
       carry[0] += t;
 #pragma unroll
       for (int b = 0; b < MOE_NUM_TILE_SIZES; ++b) {
         const int nt = (c + kTileSizes[b] - 1) / kTileSizes[b];
-        const int t0 = carry[1 + b] + block_excl_scan(nt, tmp, &t);
+        t0[b] = carry[1 + b] + block_excl_scan(nt, tmp, &t);
         carry[1 + b] += t;
-        if (e <= E) tile_starts[b * n + e] = t0;
-        write_tiles(b == 0 ? info0 : (b == 1 ? info1 : info2), e, b, t0, t0 + nt, r0, r0 + c, 0, 1);
+        if (e <= E) tile_starts[b * n + e] = t0[b];
+        if (!MANY || c <= kOwnRows) write_tiles(info_of(b), e, b, t0[b], t0[b] + nt, r0, r0 + c, 0, 1);
+      }
+      if (MANY && c > kOwnRows) {
+        const int i = 6 * atomicAdd(&n_many, 1);
+        many[i] = e, many[i + 1] = r0, many[i + 2] = r0 + c;
+#pragma unroll
+        for (int b = 0; b < MOE_NUM_TILE_SIZES; ++b) many[i + 3 + b] = t0[b];
+      }
+    }
+    if constexpr (MANY) {
+      __syncthreads();
+      for (int i = 6 * wid; i < 6 * n_many; i += 6 * kSmallWaves) {
+        const int r0 = many[i + 1], r1 = many[i + 2];
+#pragma unroll
+        for (int b = 0; b < MOE_NUM_TILE_SIZES; ++b) {
+          const int t0 = many[i + 3 + b], nt = (r1 - r0 + kTileSizes[b] - 1) / kTileSizes[b];
+          write_tiles(info_of(b), many[i], b, t0, t0 + nt, r0, r1, lane, 64);
+        }
       }
     }
     if (tid == 0) {
@@ -458,9 +516,8 @@ __global__ __launch_bounds__(1024) void small_kernel(
     }
 #pragma unroll
     for (int b = 0; b < MOE_NUM_TILE_SIZES; ++b) {
-      int4* const info = b == 0 ? info0 : (b == 1 ? info1 : info2);
       const int m = (S + kTileSizes[b] - 1) / kTileSizes[b] + E;
-      for (int t = carry[1 + b] + tid; t < m; t += 1024) info[t] = make_int4(0, 0, 0, 0);
+      for (int t = carry[1 + b] + tid; t < m; t += 1024) info_of(b)[t] = make_int4(0, 0, 0, 0);
     }
     return;
   }
@@ -502,8 +559,14 @@ constexpr size_t kTailScratch = 512 * sizeof(int);
 
 // Rows up to which the small form is taken, and the LDS it needs.
 constexpr int kSmallRows = 16384;
+// The form for many of them above (us for 128 experts, even routing and all to one):
+//   rows      4104        6000        8168        16384
+//   few   5.4, 11.4   5.7, 15.4   6.4, 18.2   7.7, 31.9
+//   many  6.4,  6.9   6.4,  6.9   6.4,  6.9   7.8,  8.3
+constexpr int kManyRows = 6144;
 constexpr int kSmallLds = 152 * 1024;
-static_assert(kSmallRows < 1 << 16, "counts in half a word");
+static_assert(kSmallRows < 1 << 16 && kSmallRows / kOwnRows * 6 <= 64 + 1024,
+              "counts in half a word, experts of many rows in the scratch");
 size_t small_lds(int E) { return (size_t)(kSmallWaves + 1) * (E + 1) * sizeof(int); }
 
 size_t permute_ws_bytes(int64_t S, int E) {
@@ -557,12 +620,13 @@ int permute_run(const int64_t* topk_index, int64_t S, int E, void* workspace,
   int4* const info2 = (int4*)(pb + plan_info_offset(S, E, 2));
   int* sched = (int*)(pb + plan_sched_offset(S, E));
   if (S <= kSmallRows && small_lds(E) <= kSmallLds) {
-    static std::atomic<int> lds_done[64];
-    hipError_t err = set_dynamic_lds_once(lds_done, (const void*)small_kernel, kSmallLds);
+    static std::atomic<int> lds_done[2][64];
+    const auto kernel = S > kManyRows ? small_kernel<true> : small_kernel<false>;
+    hipError_t err = set_dynamic_lds_once(lds_done[S > kManyRows], (const void*)kernel, kSmallLds);
     MOE_REQUIRE(err == hipSuccess, MOE_ERR_HIP, "%s: hipFuncSetAttribute failed: %s", who,
                 hipGetErrorString(err));
     const int blocks = S == 0 ? 1 : (int)((S + kSmallChunk - 1) / kSmallChunk);
-    small_kernel<<<2 + blocks, 1024, small_lds(E), st>>>(topk_index, (int)S, E, counts, offsets, row_src,
+    kernel<<<2 + blocks, 1024, small_lds(E), st>>>(topk_index, (int)S, E, counts, offsets, row_src,
                                                    slot, tile_starts, info0, info1, info2, sched);
     return check_launch(who);
   }
