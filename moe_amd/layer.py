@@ -50,7 +50,7 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, gate_up_proj: torch.Tenso
     if gating not in library.GATINGS:
         raise ValueError(f"unknown gating {gating!r} (expected one of {library.GATINGS})")
     library.check_keep(saved_activations, gate_up_proj.dtype)
-    if isinstance(gate_up_proj, ops.Packed4):
+    if isinstance(gate_up_proj, ops.Packed4) or isinstance(down_proj, ops.Packed4):
         ops.packed_bank("moe_layer", x, gate_up_proj, down_proj)
         refuse_grad4("moe_layer", x, w_router)
     hip = gating in ("hip", "hip_fused")

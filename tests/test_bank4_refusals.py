@@ -5,10 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
-from moe_amd import hf, ops
-from moe_amd.experts import pack_bank
-from moe_amd.layer import SparseMoeBlock, moe_layer
-from test_pack4 import _pack_on_cpu, _packed
+from moe_amd.layer import moe_layer
+from test_pack4 import _packed
 
 BF = torch.bfloat16
 
