@@ -127,12 +127,8 @@ def is_packed_bank(bank: nn.Module) -> bool:
     return hasattr(bank, "packed_shapes")
 
 
-def pack_bank(bank: nn.Module) -> nn.Module:
-    """Replaces a bank's parameters gate_up_proj and down_proj (bf16, on the GPU) by
-    their 4 bits, in place: buffers gate_up_proj_q, gate_up_proj_scale and down_proj's,
-    which state_dict holds and ``to`` moves.  The bank is forward only from then on."""
-    if is_packed_bank(bank):
-        return bank
+def check_packable(bank: nn.Module) -> None:
+    """Raises unless the experts take the bank in 4 bits."""
     _check_module(bank)
     weights = [getattr(bank, name) for name in _BANK]
     for name, w in zip(_BANK, weights):
@@ -142,7 +138,21 @@ def pack_bank(bank: nn.Module) -> nn.Module:
         if w.dim() != 3 or w.shape[1] % 64 or w.shape[2] % 64:
             raise ValueError(f"pack_bank: {name} {tuple(w.shape)}: both of its dimensions must be "
                              "multiples of 64")
-    packed = [ops.pack4(w.detach()) for w in weights]
+    shape1, shape2 = (tuple(w.shape) for w in weights)
+    E, I2, H = shape1
+    if shape2 != (E, H, I2 // 2):
+        raise ValueError(f"pack_bank: gate_up_proj {shape1} and down_proj {shape2}, expected "
+                         "[E, 2I, H] and [E, H, I]")
+
+
+def pack_bank(bank: nn.Module) -> nn.Module:
+    """Replaces a bank's parameters gate_up_proj and down_proj (bf16, on the GPU) by
+    their 4 bits, in place: buffers gate_up_proj_q, gate_up_proj_scale and down_proj's,
+    which state_dict holds and ``to`` moves.  The bank is forward only from then on."""
+    if is_packed_bank(bank):
+        return bank
+    check_packable(bank)
+    packed = [ops.pack4(getattr(bank, name).detach()) for name in _BANK]
     for name, p in zip(_BANK, packed):
         delattr(bank, name)
         bank.register_buffer(f"{name}_q", p.q)

@@ -14,7 +14,8 @@ from __future__ import annotations
 
 from torch import nn
 
-from .experts import is_packed_bank, mi355x_experts_forward, pack_bank
+from . import ops
+from .experts import check_packable, is_packed_bank, mi355x_experts_forward, pack_bank
 from .library import KEEPS
 from .router import MI355XDeepSeekRouter, MI355XTopKRouter, _RouterBase
 
@@ -57,8 +58,12 @@ def expert_banks(model: nn.Module) -> list[nn.Module]:
 def pack_experts(model: nn.Module) -> int:
     """Puts every expert bank (bf16, on the GPU) in 4 bits, in place and for good: a
     served model's form, forward only, whose "mi355x" experts (``install``) read
-    the banks as they are.  Returns the number of banks packed."""
+    the banks as they are.  All are checked before the first one is packed.  Returns the
+    number of banks packed."""
     banks = [m for m in expert_banks(model) if not is_packed_bank(m)]
+    for bank in banks:
+        check_packable(bank)
+    ops._need_cuda(*(w for bank in banks for w in (bank.gate_up_proj, bank.down_proj)))
     for bank in banks:
         pack_bank(bank)
     return len(banks)

@@ -4,9 +4,11 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch import nn
 
-from moe_amd.layer import moe_layer
-from test_pack4 import _packed
+from moe_amd import hf, ops
+from moe_amd.layer import SparseMoeBlock, moe_layer
+from test_pack4 import _pack_on_cpu, _packed
 
 BF = torch.bfloat16
 
@@ -16,3 +18,32 @@ def test_neither_or_both_weights_are_packed():
     for router in ("softmax", "sigmoid"):
         with pytest.raises(TypeError, match="both be in 4 bits"):
             moe_layer(x, wr, torch.zeros(3, 128, 64, dtype=BF), _packed(3, 64, 64), 2, router=router)
+
+
+@pytest.mark.parametrize("spoil,error", [
+    (lambda b: b.float(), NotImplementedError),
+    (lambda b: setattr(b, "has_bias", True), NotImplementedError),
+    (lambda b: setattr(b, "down_proj", nn.Parameter(torch.zeros(3, 64, 128, dtype=BF))), ValueError),
+    (lambda b: setattr(b, "gate_up_proj", nn.Parameter(torch.zeros(3, 128, 96, dtype=BF))),
+     ValueError),
+])
+def test_a_model_is_packed_whole_or_not_at_all(monkeypatch, spoil, error):
+    _pack_on_cpu(monkeypatch)
+    monkeypatch.setattr(ops, "_need_cuda", lambda *ts: None)
+    model = nn.ModuleList(SparseMoeBlock(64, 3, 2, 64).bfloat16() for _ in range(3))
+    spoil(model[1].experts)
+    with pytest.raises(error, match="mi355x experts|pack_bank"):
+        hf.pack_experts(model)
+    for block in model:
+        assert sorted(n for n, _ in block.experts.named_parameters()) == ["down_proj", "gate_up_proj"]
+        assert not list(block.experts.buffers())
+    model[1] = SparseMoeBlock(64, 3, 2, 64).bfloat16()
+    assert hf.pack_experts(model) == 3
+    assert not any(list(b.experts.parameters()) for b in model)
+
+
+def test_a_bank_elsewhere_keeps_a_model_as_it_is(monkeypatch):
+    model = nn.ModuleList(SparseMoeBlock(64, 3, 2, 64).bfloat16() for _ in range(2))
+    with pytest.raises(RuntimeError, match="GPU only"):
+        hf.pack_experts(model)
+    assert all(len(list(b.experts.parameters())) == 2 for b in model)
