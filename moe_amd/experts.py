@@ -143,6 +143,7 @@ def check_packable(bank: nn.Module) -> None:
     if shape2 != (E, H, I2 // 2):
         raise ValueError(f"pack_bank: gate_up_proj {shape1} and down_proj {shape2}, expected "
                          "[E, 2I, H] and [E, H, I]")
+    ops.check_bank4_size("pack_bank", E, H, I2 // 2)
 
 
 def pack_bank(bank: nn.Module) -> nn.Module:

@@ -1109,6 +1109,21 @@ def packed_bank(name: str, x: torch.Tensor, gate_up_proj: Packed4, down_proj: Pa
     return bank, E, H, I2 // 2
 
 
+BANK4_MAX_EXPERTS = 16384
+BANK4_MAX_FEATURES = 1 << 22    # H and I
+BANK4_MAX_CODES = 1 << 31       # bytes of an expert's codes, exclusive
+
+
+def check_bank4_size(name: str, E: int, H: int, I: int) -> None:
+    """Raises for a bank that moe_amd_experts4 takes with no number of tokens."""
+    codes = max(math.prod(_pack4_shapes(s)[0]) for s in ((2 * I, H), (H, I)))
+    if not 1 <= E <= BANK4_MAX_EXPERTS or not 0 < H <= BANK4_MAX_FEATURES \
+            or not 0 < I <= BANK4_MAX_FEATURES or codes >= BANK4_MAX_CODES:
+        raise NotImplementedError(
+            f"{name}: E={E}, H={H}, I={I}; a bank in 4 bits has up to {BANK4_MAX_EXPERTS} "
+            f"experts, {BANK4_MAX_FEATURES} features and 2 GB of an expert's codes")
+
+
 def _bank4_inputs(name: str, x, gate_up_proj, down_proj, *others):
     """packed_bank, contiguous, and the rest of the checks of a C entry on it."""
     bank, E, H, I = packed_bank(name, x, gate_up_proj, down_proj)

@@ -6,7 +6,8 @@ import pytest
 import torch
 from torch import nn
 
-from moe_amd import hf, ops
+from moe_amd import _lib, hf, ops
+from moe_amd.experts import pack_bank
 from moe_amd.layer import SparseMoeBlock, moe_layer
 from test_pack4 import _pack_on_cpu, _packed
 
@@ -18,6 +19,14 @@ def test_neither_or_both_weights_are_packed():
     for router in ("softmax", "sigmoid"):
         with pytest.raises(TypeError, match="both be in 4 bits"):
             moe_layer(x, wr, torch.zeros(3, 128, 64, dtype=BF), _packed(3, 64, 64), 2, router=router)
+
+
+def _bank(shape1, shape2):
+    """A bank of bf16 weights that take no memory."""
+    bank = nn.Module()
+    for name, shape in (("gate_up_proj", shape1), ("down_proj", shape2)):
+        setattr(bank, name, nn.Parameter(torch.zeros(1, 1, 1, dtype=BF).expand(shape)))
+    return bank
 
 
 @pytest.mark.parametrize("spoil,error", [
@@ -47,3 +56,20 @@ def test_a_bank_elsewhere_keeps_a_model_as_it_is(monkeypatch):
     with pytest.raises(RuntimeError, match="GPU only"):
         hf.pack_experts(model)
     assert all(len(list(b.experts.parameters())) == 2 for b in model)
+
+
+@pytest.mark.parametrize("E,H,I", [(16385, 64, 64), (1, (1 << 22) + 64, 64), (1, 64, (1 << 22) + 64),
+                                   (2, 1 << 16, 1 << 16)])
+def test_banks_that_no_call_takes_are_not_packed(built_lib, monkeypatch, E, H, I):
+    _pack_on_cpu(monkeypatch)
+    assert _lib.load().moe_amd_experts4_workspace_size(1, E, 1, H, I) == 0
+    bank = _bank((E, 2 * I, H), (E, H, I))
+    with pytest.raises(NotImplementedError, match="pack_bank"):
+        pack_bank(bank)
+    assert bank.gate_up_proj.shape == (E, 2 * I, H)
+
+
+def test_the_largest_banks_are(built_lib):
+    for E, H, I in ((16384, 64, 64), (1, 1 << 22, 64), (1, 64, 1 << 22), (1, 1 << 16, (1 << 15) - 64)):
+        assert _lib.load().moe_amd_experts4_workspace_size(1, E, 1, H, I) > 0
+        ops.check_bank4_size("test", E, H, I)
