@@ -467,7 +467,9 @@ int moe_amd_unpack4(const void* q, const void* scale, int64_t batch, int64_t n, 
  * block's largest finite one, and within 2^-39 of that below; out [T,H] bf16, sums in
  * fp32.  Sentinel rows are not written and contribute
  * nothing.  H and I multiples of 64, S < 2^29, T H 2 < 2^31, an expert's codes
- * below 2 GB; codes and scales 16-byte aligned. */
+ * below 2 GB; codes and scales 16-byte aligned.  The arguments are those of the exact
+ * entries: `offsets` of the two products is the permutation's and must not be null, though
+ * they find an expert's rows in tile_plan. */
 int moe_amd_gemm_gate_up_swiglu4(const void* hidden_states, const int32_t* row_src, int top_k,
                                  const int32_t* offsets, const void* tile_plan,
                                  const void* gate_up_q, const void* gate_up_scale, int64_t T,

@@ -131,7 +131,7 @@ int check(const void* x, int dtype, int64_t batch, int64_t n, int64_t k, const v
               "%s: batch=%lld n=%lld k=%lld too large", who, (long long)batch, (long long)n,
               (long long)k);
   if (batch == 0 || n == 0 || k == 0) return MOE_OK;
-  // (the number of tiles is below 2^50 / 4 here)
+  // (a matrix has at most 2^27 by 2^24 tiles here)
   MOE_REQUIRE(pack4_tiles(n, k) <= ((int64_t)1 << 40) / batch, MOE_ERR_UNSUPPORTED,
               "%s: batch=%lld n=%lld k=%lld too large", who, (long long)batch, (long long)n,
               (long long)k);
