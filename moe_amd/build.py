@@ -31,8 +31,8 @@ HIPFLAGS = [
 
 # Flags of single sources.  gemm4: a tile goes to one of four main loops, a branch that
 # all lanes take alike; made structured all the same, it keeps what the loops share in
-# two copies, of which 17 to 45 registers spill (gate and up of 16384 tokens: 694 us, and
-# 622 without; no register spills then).
+# two copies, of which 49 to 427 registers spill (gate and up of 16384 tokens, one box: 2490 us,
+# and 677 without; no register spills then).
 SOURCE_FLAGS = {
     "gemm4.hip": ["-mllvm", "-structurizecfg-skip-uniform-regions=1"],
 }

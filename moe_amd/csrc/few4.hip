@@ -20,7 +20,11 @@
 // complete in order.
 //
 // H = 2048, E = 128, K = 8, I = 768: 22 us for one token, 75 for 64 (gate/up 5.8 TB/s,
-// down 4.4); E = 1792: 183 us (6.5 and 5.6 TB/s).  few.hip: 23, 215 and 620.
+// down 4.4); E = 1792: 181 us (6.5 and 5.6 TB/s).  few.hip: 23, 215 and 620.
+// The tokens stay in registers up to H = 2048 and I = 768 (kGateUpTiles, kDownTiles); beyond,
+// they are loaded anew for each tile row: 64 tokens at H = 4096 take gate/up to 4.7 TB/s,
+// at I = 1024 down to 2.5, and the whole call (routing given) 141 and 114 us, where the
+// grouped products of gemm4.hip take 122 and 100.
 //
 // Sums are fp32; act is rounded to bf16, the next product's operand type, once
 // (not at all for up to 16 rows of 12288 values together: kSmallRows, kSmallValues); y

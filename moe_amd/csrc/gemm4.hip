@@ -32,15 +32,17 @@
 // largest, a column 2^12 times its neighbours leaves those 5e-2 off.)  Each output is
 // rounded once.
 //
-// Measured (gate/up, down, combine; H 2048, I 768, top 8 of 128 experts):
-//   16384 tokens  645 us (1.28 PF), 350 us (1.18 PF), 100 us (6.0 TB/s); a plain bf16
-//                 product reaches 1.4 to 1.6 PF on this card: bound by the matrix
-//                 units.  The epilogues are 8% and 19% of that; the rest are the
+// Measured (gate/up, down, combine; H 2048, I 768, top 8 of 128 experts; medians, ranges
+// are boxes):
+//   16384 tokens  646 to 676 us (1.28 to 1.22 PF), 349 to 369 us (1.18 to 1.12 PF), 99 us
+//                 (6.1 TB/s); a plain bf16 product reaches 1.4 to 1.6 PF on this card.  The
+//                 matrix units are busy 70 and 60% of the cycles, at the 1.8 GHz that the
+//                 power leaves: the epilogues are 8% and 19% of the time; the rest are the
 //                 conversions' issue slots and each expert's last, partial tile
-//    1021 tokens  60 us, 38 us, 9 us: 320 MB of weights and 64 rows an expert, so
-//                 that both bounds are near (3.6 TB/s, 0.86 PF)
-// and 2048 tokens on 1792 experts (9 rows each): 480 us, 298 us, 14 us, bound by the
-// 4.5 GB of weights (6.2 and 5.0 TB/s).
+//    1021 tokens  58 to 72 us, 37 to 45 us, 8 us: 320 MB of weights and 64 rows an expert, so
+//                 that both bounds are near (3.6 TB/s, 0.85 PF)
+// and 2048 tokens on 1792 experts (9 rows each): 475 to 492 us, 292 to 302 us, 14 us, bound by
+// the 4.5 GB of weights (6.2 and 5.0 TB/s).
 //
 // Reference: transformers/integrations/moe.py:377-478.
 #include "common.h"
@@ -703,22 +705,25 @@ int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, int b, hipStr
   return check_launch(who);
 }
 
-// Row tiles by the mean rows of an expert (us at 2048 columns, I 768, top 8; few: 64
-// rows, four waves; many: 128 rows, four waves for gate and up, eight, which read a row
-// half as often, for down: its contraction is short):
-//   mean rows, experts  8, 128  32, 128  48, 128  64, 128  128, 128  512, 128  1024, 128  9, 1792
-//   gate/up  few            39       47       69       78       104       371        713     524
-//            many           41       46       56       60       118       388        682     557
-//   down     few            23       27       33       42        60       216        414     313
-//            many           24       28       34       38        65       204        382     309
+// Row tiles by the mean rows of an expert (us at 2048 columns, I 768, top 8, three banks by
+// turns; few: 64 rows, four waves; many: 128 rows, four waves for gate and up, eight, which
+// read a row half as often, for down: its contraction is short):
+//   mean rows, experts  8, 128  32, 128  40, 128  48, 128  64, 128  128, 128  512, 128  1024, 128  9, 1792
+//   gate/up  few            40       49       54       62       79       121       385        716     524
+//            many           42       49       56       61       68       125       370        684     567
+//   down     few            23       28       32       35       41        68       221        419     314
+//            many           25       30       34       37       43        71       210        373     306
 // and many down's columns want to be a whole number of 512: where 256 do as well and the
 // rest is more than a ninth, few (3000 tokens on 32 experts, top 6, I 320, 576 columns:
-// 26.2 and 15.6; 8192 on 64, top 4, I 512, 1280 columns: 58.9 and 49.3).
+// 24.0 and 14.6; 8192 on 64, top 4, I 512, 1280 columns: 64.8 and 54.2).
 // Few rows take half the registers, so that three workgroups share a CU where two do
 // of many, which read the weights half as often.
 // Few rows stream the codes of a bank that the memory-side cache cannot hold: 2048
-// tokens on 1792 experts 517 and 309 us become 480 and 297, while with 300 on 128 the
+// tokens on 1792 experts 524 and 314 us become 487 and 302, while with 300 on 128 the
 // same bank's next call takes 45 and 26 us where it finds a part of it there in 41 and 23.
+// The host knows the mean over all experts, not the counts: where all 2048 tokens go to
+// 8, 16, 64 or 256 of the 1792 experts, gate/up and down take 99 + 57, 103 + 63, 113 + 68 and
+// 151 + 85 us, the best of the three forms 84 + 50, 98 + 55, 107 + 63 and 138 + 81.
 constexpr int64_t kMemoryCache = 256ll << 20;
 template <bool GATE>
 int launch4(Gemm4Args& a, int64_t S, int E, const void* tile_plan, hipStream_t st, const char* who) {

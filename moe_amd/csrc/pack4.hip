@@ -7,7 +7,8 @@
 // or 128 consecutive bytes and a wave's 64 codes words are 256 bytes.
 // Values to pack come by non-temporal loads: sixteen matrices [1536, 2048] of fp32 take
 // 41 us (5.5 TB/s; 56 us otherwise).  Unpacked ones are stored as usual: 35 us (6.6
-// TB/s; 80 us by non-temporal stores).
+// TB/s; 80 us by non-temporal stores).  128 matrices, beyond the memory-side cache: fp32
+// 359 and 485 us (5.1 and 3.8 TB/s), bf16 268 and 277 us (3.8 and 3.7 TB/s).
 #include "common.h"
 #include "pack4.h"
 

@@ -11,7 +11,7 @@ routed expert's weights once; ``SparseMoeBlock.few_tokens`` and
 They may be captured in a HIP graph.
 
 A bank in 4 bits (``ops.Packed4`` for both of gate_up_proj and down_proj; bf16 hidden
-states) is streamed as it is, a fifth to a quarter of the bytes.
+states) is streamed as it is, 0.27 of the bytes.
 """
 from __future__ import annotations
 
