@@ -12,7 +12,7 @@
 // one workgroup), 8 at 16384, skewed routing up to 10, where the general form's kernels take
 // 13.5; past it counting all ids in every workgroup costs more than two launches.
 // E = 1792: 8, 10 and 11 us, the general form 26.  (Calls one after another, the ids in the
-// L2; 12 us at 8168 and 22 at E = 1792, 16384 between products that fill it.)
+// L2; 8.6 us at 8168 and 16.5 at E = 1792, 16384 between products that fill it.)
 //
 // General, three launches (23 us at S = 524288, E = 128, where seven took 41):
 //   hist        one wave per 256-entry chunk, LDS atomics -> per-chunk
@@ -405,8 +405,9 @@ __global__ __launch_bounds__(64 * kWaves) void tail_kernel(
 }
 
 // The small form: 2 blocks and one for each 1024 entries, of 1024 threads, see the head of
-// the file.  MANY: more than kManyRows entries, of which many may be one expert's.  LDS: counters [E+1] of all entries, in the upper halves of the scatter's blocks
-// of those before the block's (S < 2^16), and there its waves' ((w, e) at w * (E + 1) + e).
+// the file.  MANY: more than kManyRows entries, of which many may be one expert's.  LDS:
+// counters [E+1] of all entries, with those before the block's in their upper halves where
+// it scatters (S < 2^16), and there its waves' counters ((w, e) at w * (E + 1) + e).
 constexpr int kSmallWaves = 16;
 constexpr int kSmallChunk = 64 * kSmallWaves;
 constexpr int kOwnRows = 512;  // MANY: an expert's tiles by one thread, of more rows by a wave
@@ -559,7 +560,8 @@ constexpr size_t kTailScratch = 512 * sizeof(int);
 
 // Rows up to which the small form is taken, and the LDS it needs.
 constexpr int kSmallRows = 16384;
-// The form for many of them above (us for 128 experts, even routing and all to one):
+// Above kManyRows the form for many of them (us for 128 experts, even routing and all to one;
+// between 4096 and 8168 the one gains up to 1 us of even routing, the other 4 to 11 of skew):
 //   rows      4104        6000        8168        16384
 //   few   5.4, 11.4   5.7, 15.4   6.4, 18.2   7.7, 31.9
 //   many  6.4,  6.9   6.4,  6.9   6.4,  6.9   7.8,  8.3
@@ -627,7 +629,7 @@ int permute_run(const int64_t* topk_index, int64_t S, int E, void* workspace,
                 hipGetErrorString(err));
     const int blocks = S == 0 ? 1 : (int)((S + kSmallChunk - 1) / kSmallChunk);
     kernel<<<2 + blocks, 1024, small_lds(E), st>>>(topk_index, (int)S, E, counts, offsets, row_src,
-                                                   slot, tile_starts, info0, info1, info2, sched);
+                                             slot, tile_starts, info0, info1, info2, sched);
     return check_launch(who);
   }
   const int64_t nch = (S + kChunk - 1) / kChunk;
