@@ -483,7 +483,8 @@ int moe_amd_combine16(const void* y, const void* y_scale, const int32_t* slot,
 
 /* All of it with a caller's routing topk_index, topk_weights [T,K]: moe_amd_permute,
  * the two products and the combine, in a 16-byte aligned workspace of
- * moe_amd_experts4_workspace_size bytes (0: sizes that the call refuses).  Ids outside
+ * moe_amd_experts4_workspace_size bytes (0: sizes that the call refuses, more than 10239
+ * experts among them).  Ids outside
  * [0, E) contribute nothing. */
 size_t moe_amd_experts4_workspace_size(int64_t T, int E, int K, int H, int I);
 int moe_amd_experts4(const void* hidden_states, const int64_t* topk_index, const void* topk_weights,

@@ -79,6 +79,9 @@ static inline size_t plan_bytes(int64_t S, int E) {
   return plan_sched_offset(S, E) + align_up((size_t)(kSchedQueueInts + kSchedStartInts + E) * 4, 16);
 }
 
+// The most experts of a permutation: the counters of its four waves in 160 KB of LDS.
+constexpr int kPermuteExperts = 160 * 1024 / (4 * 4) - 1;
+
 // True for a null or 16-byte aligned pointer (the vector paths' requirement).
 static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 

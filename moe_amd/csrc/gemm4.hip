@@ -760,7 +760,7 @@ Layout4 layout4(int64_t S, int E, int H, int I) {
 }
 
 int check_experts4(int64_t T, int K, int E, int H, int I, const char* who) {
-  MOE_REQUIRE(T >= 0 && K >= 1 && E <= 16384, MOE_ERR_ARG, "%s: T=%lld, K=%d or E=%d out of range",
+  MOE_REQUIRE(T >= 0 && K >= 1 && E <= kPermuteExperts, MOE_ERR_ARG, "%s: T=%lld, K=%d or E=%d out of range",
               who, (long long)T, K, E);
   MOE_REQUIRE(T < (int64_t)1 << 31, MOE_ERR_UNSUPPORTED, "%s: T=%lld too large", who, (long long)T);
   const int rc = check4(T * K, E, H, I, who);

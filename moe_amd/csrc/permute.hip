@@ -612,7 +612,8 @@ int permute_run(const int64_t* topk_index, int64_t S, int E, void* workspace,
   MOE_REQUIRE(workspace && workspace_bytes >= need, MOE_ERR_WORKSPACE,
               "%s: workspace %zu bytes < %zu needed", who, workspace_bytes, need);
   const size_t lds = (size_t)kWaves * (E + 1) * sizeof(int);
-  MOE_REQUIRE(lds <= 160 * 1024, MOE_ERR_ARG, "%s: E=%d needs too much LDS", who, E);
+  static_assert(kWaves * (kPermuteExperts + 1) * sizeof(int) <= 160 * 1024, "LDS");
+  MOE_REQUIRE(E <= kPermuteExperts, MOE_ERR_ARG, "%s: E=%d needs too much LDS", who, E);
   const size_t tail_lds = lds > kTailScratch ? lds : kTailScratch;
   hipStream_t st = (hipStream_t)stream;
   int* tile_starts = (int*)tile_plan;

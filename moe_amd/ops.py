@@ -1109,7 +1109,7 @@ def packed_bank(name: str, x: torch.Tensor, gate_up_proj: Packed4, down_proj: Pa
     return bank, E, H, I2 // 2
 
 
-BANK4_MAX_EXPERTS = 16384
+BANK4_MAX_EXPERTS = 10239       # the permutation's
 BANK4_MAX_FEATURES = 1 << 22    # H and I
 BANK4_MAX_CODES = 1 << 31       # bytes of an expert's codes, exclusive
 

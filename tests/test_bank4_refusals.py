@@ -58,7 +58,7 @@ def test_a_bank_elsewhere_keeps_a_model_as_it_is(monkeypatch):
     assert all(len(list(b.experts.parameters())) == 2 for b in model)
 
 
-@pytest.mark.parametrize("E,H,I", [(16385, 64, 64), (1, (1 << 22) + 64, 64), (1, 64, (1 << 22) + 64),
+@pytest.mark.parametrize("E,H,I", [(10240, 64, 64), (1, (1 << 22) + 64, 64), (1, 64, (1 << 22) + 64),
                                    (2, 1 << 16, 1 << 16)])
 def test_banks_that_no_call_takes_are_not_packed(built_lib, monkeypatch, E, H, I):
     _pack_on_cpu(monkeypatch)
@@ -70,6 +70,6 @@ def test_banks_that_no_call_takes_are_not_packed(built_lib, monkeypatch, E, H, I
 
 
 def test_the_largest_banks_are(built_lib):
-    for E, H, I in ((16384, 64, 64), (1, 1 << 22, 64), (1, 64, 1 << 22), (1, 1 << 16, (1 << 15) - 64)):
+    for E, H, I in ((10239, 64, 64), (1, 1 << 22, 64), (1, 64, 1 << 22), (1, 1 << 16, (1 << 15) - 64)):
         assert _lib.load().moe_amd_experts4_workspace_size(1, E, 1, H, I) > 0
         ops.check_bank4_size("test", E, H, I)

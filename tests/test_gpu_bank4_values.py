@@ -191,3 +191,19 @@ def test_acts_beyond_bf16(T):
         out = few.experts_forward_few(x[:1].expand(n, H), idx[:1].expand(n, 1), w[:1].expand(n, 1),
                                       b1, b2).float()
         assert torch.equal(out, (sign * torch.inf).expand(n, H)), n
+
+
+def test_the_most_experts():
+    """What the workspace's size allows, the call takes: 10239 experts, and not one more."""
+    g = _gen(3)
+    E, H, I, T, K = 10239, 64, 64, 600, 2
+    b1, b2 = _banks(g, E, H, I)
+    x, w = torch.randn(T, H, generator=g, device=DEV, dtype=BF), torch.rand(T, K, device=DEV)
+    idx = torch.randint(0, 40, (T, K), generator=g, device=DEV) * 257 % E
+    idx[:, 1] = torch.where(idx[:, 1] == idx[:, 0], E - 1, idx[:, 1])
+    out = experts_forward(x, idx, w, b1.packed, b2.packed)
+    assert distance(out, layer(x, idx, w, b1, b2, True)) < LIMIT
+    more = [ops.Packed4(p.q[:1].expand(E + 1, *p.q.shape[1:]), p.scale[:1].expand(E + 1, *p.scale.shape[1:]),
+                        (E + 1, *p.shape[1:]), BF) for p in (b1.packed, b2.packed)]
+    with pytest.raises(RuntimeError, match="E=10240"):
+        experts_forward(x, idx, w, *more)
